@@ -502,6 +502,76 @@ int ts_rope_kv_write(void* qkv, int64_t qkv_stride, const int64_t* positions,
 int ts_silu_mul(const void* gu, int64_t gu_stride, void* out, int64_t out_stride,
                 int64_t num_tokens, int32_t intermediate, void* stream);
 
+/*
+ * The 8-bit paged cache of one layer: k_cache / v_cache int8 codes [num_blocks, num_kv_heads, 16,
+ * head_dim] contiguous, k_scale / v_scale fp32 [num_blocks, num_kv_heads] contiguous; a code stands
+ * for code * scale (scales >= 0). It takes half the bytes of the fp16 cache (plus 8 bytes for each
+ * block and KV head). The reference has no such cache; the step's metadata is the same.
+ *
+ * ts_kv_write_int8: the step's new rows into the blocks that they fall in. The rows
+ * query_start_loc[b] .. query_start_loc[b + 1] - 1 of the flat batch are sequence b's last ones:
+ * positions seq_lens[b] - n .. seq_lens[b] - 1 (negative positions are skipped), in the blocks that
+ * its table names. For every block touched, per KV head, K and V apart:
+ *   scale' = max(scale if the block holds earlier rows of the sequence, max|new rows| / 127)
+ *   code'  = rint(code * (scale / scale')) of the earlier rows when scale' > scale
+ *   code   = rint(row / scale') of the new rows                       (fp32, ties to even)
+ * A block whose row 0 is written starts anew; rows past the sequence's end keep their codes. New
+ * rows that are not finite make scale' NaN (and their codes 0). Blocks are owned by one wavefront
+ * each, so no two sequences of a call may write into the same block (their rows would race; no
+ * access leaves the cache). Block ids outside [0, num_blocks) and blocks past max_blocks_per_seq
+ * are skipped. max_query_len shapes the launch only: a bound below the real one is slower, not
+ * wrong. k / v rows fp16, aligned to 16 bytes (8 at head_dim 32, 4 at head_dim 16); head_dim 16,
+ * 32, 64, 128 or 256.
+ *
+ * ts_rope_kv_write_int8: the same for the k and v heads of qkv [T, (H + 2 KVH) D], k rotated first
+ * (rotate-half RoPE by the fp32 tables, computed in 64 bits and rounded to fp32), with the rotated q
+ * rows, rounded once, in q_out [T, H, D] (contiguous); qkv is not written. Rows 16-byte aligned.
+ * positions[t] outside [0, max_position) use the table's nearest row.
+ */
+int ts_kv_write_int8(const void* k, const void* v, int64_t k_stride_t, int64_t k_stride_h,
+                     int64_t v_stride_t, int64_t v_stride_h, void* k_cache, void* v_cache,
+                     float* k_scale, float* v_scale, int64_t num_blocks,
+                     const int32_t* block_tables, int64_t bt_stride, int32_t max_blocks_per_seq,
+                     const int32_t* seq_lens, const int32_t* query_start_loc, int32_t num_seqs,
+                     int32_t num_decode, int32_t max_query_len, int64_t num_tokens,
+                     int32_t num_kv_heads, int32_t head_dim, void* stream);
+
+int ts_rope_kv_write_int8(const void* qkv, int64_t qkv_stride, const int64_t* positions,
+                          const float* cos_table, const float* sin_table, int64_t max_position,
+                          void* q_out, void* k_cache, void* v_cache, float* k_scale, float* v_scale,
+                          int64_t num_blocks, const int32_t* block_tables, int64_t bt_stride,
+                          int32_t max_blocks_per_seq, const int32_t* seq_lens,
+                          const int32_t* query_start_loc, int32_t num_seqs, int32_t num_decode,
+                          int32_t max_query_len, int64_t num_tokens, int32_t num_heads,
+                          int32_t num_kv_heads, int32_t head_dim, void* stream);
+
+/*
+ * Attention over an 8-bit paged cache: the contract of ts_paged_attention (decode rows
+ * [0, num_decode), one query row each; then the query_start_loc rows of the other sequences under
+ * the bottom-right causal mask) with K and V read as code * scale. Products are taken on the codes
+ * in fp16 (exact) with fp32 sums; scores, softmax statistics and outputs are fp32, P is rounded to
+ * fp16 before the P.V product. Rows that see no token are zeros; a row that sees a block whose K or
+ * V scale is not finite is NaN. A decode row's result does not depend on the rest of the batch
+ * given max_seq_len. The host bounds shape the launch only: bounds below the batch's real values
+ * are slower, not wrong. head_dim 16, 32, 64, 128 or 256, any number of query heads per KV head; q
+ * rows 16-byte aligned, scale > 0. Workspace: the queried size, 256-byte aligned (may be 0).
+ */
+size_t ts_paged_attention_int8_workspace_bytes(int32_t num_seqs, int32_t num_decode,
+                                               int32_t max_query_len, int32_t max_seq_len,
+                                               int32_t max_prefill_seq_len, int32_t num_heads,
+                                               int32_t num_kv_heads, int32_t head_dim,
+                                               int32_t cu_count);
+
+int ts_paged_attention_int8(const void* q, int64_t q_stride_t, int64_t q_stride_h, void* out,
+                            int64_t out_stride_t, int64_t num_tokens, const void* k_cache,
+                            const void* v_cache, const float* k_scale, const float* v_scale,
+                            int64_t num_blocks, const int32_t* block_tables, int64_t bt_stride,
+                            int32_t max_blocks_per_seq, const int32_t* seq_lens,
+                            const int32_t* query_start_loc, int32_t num_seqs, int32_t num_decode,
+                            int32_t max_query_len, int32_t max_seq_len, int32_t max_prefill_seq_len,
+                            int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, float scale,
+                            void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

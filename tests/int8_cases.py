@@ -1,0 +1,62 @@
+"""Batches over an 8-bit paged cache for the tests: seeded inputs on the host, and their tensors."""
+
+from __future__ import annotations
+
+import numpy as np
+import torch
+
+from turingserve_amd.metadata import AttentionMetadata
+
+BLOCK = 16
+HEADS = [(4, 2, 16), (6, 2, 32), (14, 2, 64), (12, 2, 128), (8, 8, 64), (34, 2, 64), (4, 1, 256)]
+
+
+class Case:
+    """items: (cached, new) tokens of each sequence, decode rows first. The cache is filled with
+    seeded codes and scales everywhere, also where no sequence has tokens yet."""
+
+    def __init__(self, heads, items, num_decode=0, seed=0, spare=3, k_size=1.0, tail_rows=0):
+        self.H, self.KVH, self.D = heads
+        self.items, self.num_decode = items, num_decode
+        rng = np.random.default_rng(seed)
+        need = [-(-(c + n) // BLOCK) for c, n in items]
+        self.NB = sum(need) + 1 + spare
+        ids = rng.permutation(self.NB - 1)[:sum(need)] + 1
+        self.tables = np.zeros((len(items), max(1, max(need))), np.int32)
+        at = 0
+        for b, w in enumerate(need):
+            self.tables[b, :w] = ids[at:at + w]
+            at += w
+        self.lens = np.array([c + n for c, n in items], np.int32)
+        self.starts = np.concatenate([[0], np.cumsum([n for _, n in items])]).astype(np.int32)
+        self.T = int(self.starts[-1]) + tail_rows
+        self.pos = np.concatenate([np.arange(c, c + n) for c, n in items]
+                                  + [np.zeros(tail_rows, np.int64)]).astype(np.int64)
+        self.qkv = rng.standard_normal((self.T, (self.H + 2 * self.KVH) * self.D)).astype(np.float16)
+        shape = (2, self.NB, self.KVH)
+        self.codes = rng.integers(-127, 128, (*shape, BLOCK, self.D)).astype(np.int8)
+        self.scales = np.exp(rng.normal(-4.0, 0.7, shape)).astype(np.float32)
+        self.scales[0] *= k_size
+        self.scale = self.D ** -0.5
+
+    def split(self):
+        x = self.qkv.reshape(self.T, self.H + 2 * self.KVH, self.D)
+        return x[:, :self.H], x[:, self.H:self.H + self.KVH], x[:, self.H + self.KVH:]
+
+    def on(self, device):
+        """(qkv, q, k, v views, (k_cache, v_cache, k_scale, v_scale), meta) as tensors."""
+        t = lambda a: torch.from_numpy(a).to(device)
+        qkv = t(self.qkv)
+        x = qkv.view(self.T, self.H + 2 * self.KVH, self.D)
+        codes, scales = t(self.codes.copy()), t(self.scales.copy())
+        return (qkv, x[:, :self.H], x[:, self.H:self.H + self.KVH], x[:, self.H + self.KVH:],
+                (codes[0], codes[1], scales[0], scales[1]), self.meta(device))
+
+    def meta(self, device, **changes):
+        t = lambda a: torch.from_numpy(a).to(device)
+        n = np.diff(self.starts)
+        f = dict(query_start_loc=t(self.starts), seq_lens=t(self.lens), block_tables=t(self.tables),
+                 slot_mapping=torch.full((self.T,), -1, dtype=torch.int64, device=device),
+                 num_decode=self.num_decode, max_query_len=int(n.max()), max_seq_len=int(self.lens.max()),
+                 max_prefill_seq_len=int(self.lens[self.num_decode:].max(initial=0)))
+        return AttentionMetadata(**{**f, **changes})

@@ -98,6 +98,16 @@ SIGNATURES = {
     "ts_rope_kv_write": (ctypes.c_int, [_p, _i64, _p, _p, _p, _i64, _i64, _i32, _i32, _i32, _p,
                                         _p, _i64, _p, _p]),
     "ts_silu_mul": (ctypes.c_int, [_p, _i64, _p, _i64, _i64, _i32, _p]),
+    "ts_kv_write_int8": (ctypes.c_int, [_p, _p, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _i64, _p,
+                                        _i64, _i32, _p, _p, _i32, _i32, _i32, _i64, _i32, _i32,
+                                        _p]),
+    "ts_rope_kv_write_int8": (ctypes.c_int, [_p, _i64, _p, _p, _p, _i64, _p, _p, _p, _p, _p, _i64,
+                                             _p, _i64, _i32, _p, _p, _i32, _i32, _i32, _i64, _i32,
+                                             _i32, _i32, _p]),
+    "ts_paged_attention_int8_workspace_bytes": (_sz, [_i32] * 9),
+    "ts_paged_attention_int8": (ctypes.c_int, [_p, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _p, _i64,
+                                               _p, _i64, _i32, _p, _p, _i32, _i32, _i32, _i32, _i32,
+                                               _i32, _i32, _i32, _f32, _p, _sz, _p]),
 }
 
 # The measurement-only probes library (include/turingserve_probes.h): not part of the product ABI.

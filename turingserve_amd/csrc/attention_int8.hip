@@ -1,0 +1,182 @@
+// Entry points of the attention over the 8-bit paged cache: decode rows, then prompt rows.
+#include "prefill_int8.h"
+
+namespace ts {
+
+constexpr int kI8PrefillWaves = 4;
+constexpr int kI8PrefillRows = 32 * kI8PrefillWaves;
+constexpr int kI8MinSteps = 4;           // 64-token steps that a prefill split is worth
+constexpr int kI8MaxPrefillSplits = 16;
+
+// Launch shape and scratch of a batch, from the host's bounds.
+struct Int8Plan {
+  int max_splits;                        // decode: splits of the longest sequence
+  int tiles, splits;                     // prefill: per (sequence, KV head)
+  size_t dec_o, dec_ml, pre_o, pre_ml;   // offsets of the partials
+  size_t bytes;
+};
+
+static size_t take(size_t& at, size_t bytes) {
+  const size_t here = at;
+  at += (bytes + 255) / 256 * 256;
+  return here;
+}
+
+static Int8Plan int8_plan(int num_seqs, int num_decode, int max_query_len, int max_seq_len,
+                          int max_prefill_seq_len, int H, int KVH, int D, int cus) {
+  Int8Plan pl = {};
+  size_t at = 0;
+  const int64_t nb = ((int64_t)(max_seq_len > 0 ? max_seq_len : 0) + kBlockSize - 1) / kBlockSize;
+  pl.max_splits = i8_splits((int)nb, kI8MaxSplits);
+  if (num_decode > 0 && pl.max_splits > 1) {
+    const size_t rows = (size_t)num_decode * H * pl.max_splits;
+    pl.dec_o = take(at, rows * D * sizeof(float));
+    pl.dec_ml = take(at, rows * 2 * sizeof(float));
+  }
+  const int P = num_seqs - num_decode;
+  pl.tiles = pl.splits = 1;
+  if (P > 0) {
+    const int64_t rows = (int64_t)(max_query_len > 0 ? max_query_len : 1) * (H / KVH);
+    const int64_t tiles = (rows + kI8PrefillRows - 1) / kI8PrefillRows;
+    pl.tiles = (int)(tiles < (1 << 20) ? tiles : (1 << 20));
+    const int seq = max_prefill_seq_len > 0 ? max_prefill_seq_len : max_seq_len;
+    const int steps = (seq > 0 ? seq - 1 : 0) / kI8Keys + 1;
+    // Two workgroups fit a CU; fewer tiles than that are cut along the keys.
+    const int64_t groups = (int64_t)P * pl.tiles * KVH;
+    int64_t n = (2 * (int64_t)cus + groups - 1) / groups;
+    if (n > steps / kI8MinSteps) n = steps / kI8MinSteps;
+    if (n > kI8MaxPrefillSplits) n = kI8MaxPrefillSplits;
+    pl.splits = n < 1 ? 1 : (int)n;
+    if (pl.splits > 1) {
+      const size_t r = (size_t)groups * pl.splits * kI8PrefillRows;
+      pl.pre_o = take(at, r * D * sizeof(float));
+      pl.pre_ml = take(at, r * 2 * sizeof(float));
+    }
+  }
+  pl.bytes = at;
+  return pl;
+}
+
+static bool int8_head_dim(int D) { return D == 16 || D == 32 || D == 64 || D == 128 || D == 256; }
+
+template <int D>
+static int launch_decode(const Int8DecodeArgs& a, int cus, hipStream_t s) {
+  // Every split of the batch, at most four workgroups a CU; the rest go round.
+  const int64_t units = (int64_t)a.num_seqs * a.max_splits * a.kvh * a.head_tiles;
+  const int64_t cap = 4 * (int64_t)cus;
+  decode_int8_kernel<D><<<(unsigned)(units < cap ? units : cap), kI8Threads, 0, s>>>(a);
+  if (a.max_splits > 1) decode_int8_merge_kernel<D><<<dim3(a.num_seqs, a.heads), kWave, 0, s>>>(a);
+  return check_launch("paged_attention_int8");
+}
+
+template <int D>
+static int launch_prefill(const Int8PrefillArgs& p, unsigned grid, hipStream_t s) {
+  prefill_int8_kernel<D, kI8PrefillWaves><<<grid, kI8PrefillWaves * kWave, 0, s>>>(p);
+  if (p.splits > 1) {
+    const unsigned merge = grid / p.splits * (kI8PrefillRows / (256 / (D / 4)));
+    prefill_int8_merge_kernel<D, kI8PrefillRows><<<merge, 256, 0, s>>>(p);
+  }
+  return check_launch("paged_attention_int8");
+}
+
+}  // namespace ts
+
+using namespace ts;
+
+extern "C" size_t ts_paged_attention_int8_workspace_bytes(int32_t num_seqs, int32_t num_decode,
+                                                          int32_t max_query_len, int32_t max_seq_len,
+                                                          int32_t max_prefill_seq_len,
+                                                          int32_t num_heads, int32_t num_kv_heads,
+                                                          int32_t head_dim, int32_t cu_count) {
+  if (num_seqs <= 0 || num_decode < 0 || num_decode > num_seqs || num_kv_heads <= 0 ||
+      num_heads < num_kv_heads || num_heads % num_kv_heads != 0 || !int8_head_dim(head_dim))
+    return 0;
+  return int8_plan(num_seqs, num_decode, max_query_len, max_seq_len, max_prefill_seq_len, num_heads,
+                   num_kv_heads, head_dim, cu_count > 0 ? cu_count : 256).bytes;
+}
+
+extern "C" int ts_paged_attention_int8(const void* q, int64_t q_stride_t, int64_t q_stride_h, void* out,
+                                       int64_t out_stride_t, int64_t num_tokens, const void* k_cache,
+                                       const void* v_cache, const float* k_scale, const float* v_scale,
+                                       int64_t num_blocks, const int32_t* block_tables,
+                                       int64_t bt_stride, int32_t max_blocks_per_seq,
+                                       const int32_t* seq_lens, const int32_t* query_start_loc,
+                                       int32_t num_seqs, int32_t num_decode, int32_t max_query_len,
+                                       int32_t max_seq_len, int32_t max_prefill_seq_len,
+                                       int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                       float scale, void* workspace, size_t workspace_bytes,
+                                       void* stream) {
+  ts::clear_error();
+  TS_REQUIRE(num_seqs >= 0 && num_decode >= 0 && num_decode <= num_seqs && num_decode <= num_tokens,
+             TS_ERR_INVALID_ARG, "paged_attention_int8: num_seqs=%d num_decode=%d num_tokens=%lld",
+             num_seqs, num_decode, (long long)num_tokens);
+  if (num_seqs == 0 || num_tokens == 0) return TS_OK;
+  TS_REQUIRE(q && out && k_cache && v_cache && k_scale && v_scale && block_tables && seq_lens &&
+                 query_start_loc,
+             TS_ERR_INVALID_ARG, "paged_attention_int8: null pointer argument");
+  TS_REQUIRE(int8_head_dim(head_dim), TS_ERR_UNSUPPORTED,
+             "paged_attention_int8: head_dim %d (16, 32, 64, 128, 256)", head_dim);
+  TS_REQUIRE(num_kv_heads > 0 && num_heads > 0 && num_heads % num_kv_heads == 0, TS_ERR_INVALID_ARG,
+             "paged_attention_int8: %d heads over %d KV heads", num_heads, num_kv_heads);
+  TS_REQUIRE(num_blocks > 0 && max_blocks_per_seq > 0 && bt_stride >= max_blocks_per_seq,
+             TS_ERR_INVALID_ARG, "paged_attention_int8: num_blocks=%lld max_blocks_per_seq=%d bt_stride=%lld",
+             (long long)num_blocks, max_blocks_per_seq, (long long)bt_stride);
+  TS_REQUIRE(q_stride_t % 8 == 0 && q_stride_h % 8 == 0 && q_stride_t >= 0 && q_stride_h >= 0 &&
+                 out_stride_t % 4 == 0 && out_stride_t >= (int64_t)num_heads * head_dim &&
+                 aligned(q, 16) && aligned(out, 8) && aligned(k_cache, 16) && aligned(v_cache, 16) &&
+                 aligned(k_scale, 4) && aligned(v_scale, 4),
+             TS_ERR_INVALID_ARG, "paged_attention_int8: misaligned q / out / caches");
+  TS_REQUIRE(scale > 0.f && scale < INFINITY, TS_ERR_INVALID_ARG,
+             "paged_attention_int8: scale must be positive and finite");
+  int cus = 0;
+  int status = device_cu_count(stream, &cus);
+  if (status != TS_OK) return status;
+  const Int8Plan pl = int8_plan(num_seqs, num_decode, max_query_len, max_seq_len, max_prefill_seq_len,
+                                num_heads, num_kv_heads, head_dim, cus);
+  TS_REQUIRE(pl.bytes == 0 || (workspace && workspace_bytes >= pl.bytes && aligned(workspace, 256)),
+             TS_ERR_WORKSPACE, "paged_attention_int8: workspace of %zu bytes, %zu needed", workspace_bytes,
+             pl.bytes);
+  char* ws = static_cast<char*>(workspace);
+  const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  Int8DecodeArgs a = {};
+  a.q = static_cast<const half_t*>(q), a.q_st = q_stride_t, a.q_sh = q_stride_h;
+  a.out = static_cast<half_t*>(out), a.out_st = out_stride_t;
+  a.kc = static_cast<const int8_t*>(k_cache), a.vc = static_cast<const int8_t*>(v_cache);
+  a.ks = k_scale, a.vs = v_scale, a.num_blocks = num_blocks;
+  a.block_tables = block_tables, a.bt_stride = bt_stride, a.max_blocks = max_blocks_per_seq;
+  a.seq_lens = seq_lens, a.heads = num_heads, a.kvh = num_kv_heads;
+  a.group = num_heads / num_kv_heads, a.head_tiles = (a.group + 15) / 16;
+  a.sl2 = scale * 1.44269504088896340736f;
+  if (num_decode > 0) {
+    a.num_seqs = num_decode, a.max_splits = pl.max_splits;
+    a.part_o = reinterpret_cast<float*>(ws + pl.dec_o);
+    a.part_ml = reinterpret_cast<float*>(ws + pl.dec_ml);
+    switch (head_dim) {
+      case 16: status = launch_decode<16>(a, cus, s); break;
+      case 32: status = launch_decode<32>(a, cus, s); break;
+      case 64: status = launch_decode<64>(a, cus, s); break;
+      case 128: status = launch_decode<128>(a, cus, s); break;
+      default: status = launch_decode<256>(a, cus, s); break;
+    }
+    if (status != TS_OK) return status;
+  }
+  if (num_seqs > num_decode) {
+    Int8PrefillArgs p = {};
+    p.a = a;
+    p.a.part_o = reinterpret_cast<float*>(ws + pl.pre_o);
+    p.a.part_ml = reinterpret_cast<float*>(ws + pl.pre_ml);
+    p.qsl = query_start_loc, p.num_tokens = num_tokens;
+    p.num_seqs = num_seqs, p.first = num_decode, p.tiles = pl.tiles, p.splits = pl.splits;
+    const int64_t grid = (int64_t)(num_seqs - num_decode) * pl.tiles * num_kv_heads * pl.splits;
+    TS_REQUIRE(grid * kI8PrefillRows < (1ll << 31), TS_ERR_UNSUPPORTED,
+               "paged_attention_int8: %lld workgroups", (long long)grid);
+    switch (head_dim) {
+      case 16: status = launch_prefill<16>(p, (unsigned)grid, s); break;
+      case 32: status = launch_prefill<32>(p, (unsigned)grid, s); break;
+      case 64: status = launch_prefill<64>(p, (unsigned)grid, s); break;
+      case 128: status = launch_prefill<128>(p, (unsigned)grid, s); break;
+      default: status = launch_prefill<256>(p, (unsigned)grid, s); break;
+    }
+  }
+  return status;
+}

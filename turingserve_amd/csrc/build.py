@@ -24,7 +24,7 @@ LIB_PATH = os.path.join(LIB_DIR, "libturingserve_hip.so")
 PROBES_PATH = os.path.join(LIB_DIR, "libturingserve_probes.so")
 BUILD_DIR = os.path.join(HERE, "_build")
 SOURCES = ["capi.hip", "kv_write.hip", "decode.hip", "prefill.hip", "ragged.hip", "w8a16.hip",
-           "small_ops.hip", "metadata.hip"]
+           "small_ops.hip", "metadata.hip", "kv_write_int8.hip", "attention_int8.hip"]
 PROBE_SOURCES = ["probes.hip"]
 ARCH = "gfx950"
 
@@ -42,6 +42,7 @@ SOURCE_FLAGS = {
     "decode.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "ragged.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "attention_int8.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 
 

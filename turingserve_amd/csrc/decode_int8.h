@@ -1,0 +1,428 @@
+// Decode attention over the 8-bit paged cache: one query row per sequence.
+//
+//   s_j = scale * ks[blk(j)] * (q . code_k[j]),  out = sum_j softmax(s)_j * vs[blk(j)] * code_v[j]
+//
+// One workgroup of four wavefronts takes one split of one sequence's blocks for one KV head (and up
+// to 16 of its query heads, the rows of an MFMA tile): every code is read once for the whole group
+// of heads. The four wavefronts take pairs of blocks in turn with a running maximum and sum each,
+// meet once at the end in LDS, and either write the row or leave a partial (m, l, O) for the merge
+// launch.
+#pragma once
+
+#include "int8_kv.h"
+
+namespace ts {
+
+constexpr int kI8Waves = 4;
+constexpr int kI8Threads = kI8Waves * kWave;
+constexpr int kI8SplitBlocks = 16;     // blocks of a split, as long as kI8MaxSplits suffice
+constexpr int kI8MaxSplits = 64;
+constexpr float kI8Rescale = 8.f;      // a row's reference moves when a score passes it by 2^8
+
+// Splits of a sequence of nb blocks, at most `most` (the partials that the workspace holds for a
+// row, from the host's bound on the lengths): from its own length, so that a row's result does not
+// depend on the rest of the batch.
+__host__ __device__ inline int i8_splits(int nb, int most) {
+  const int n = (nb + kI8SplitBlocks - 1) / kI8SplitBlocks;
+  return n < 1 ? 1 : (n > most ? most : n);
+}
+
+struct Int8DecodeArgs {
+  const half_t* q;
+  int64_t q_st, q_sh;
+  half_t* out;
+  int64_t out_st;
+  const int8_t *kc, *vc;
+  const float *ks, *vs;
+  int64_t num_blocks;
+  const int32_t* block_tables;
+  int64_t bt_stride;
+  int max_blocks;
+  const int32_t* seq_lens;
+  int num_seqs, heads, kvh, group, head_tiles;   // group = heads / kvh, head_tiles = ceil(group / 16)
+  float sl2;                                     // scale * log2(e)
+  int max_splits;                                // partials per row in the workspace
+  float *part_o, *part_ml;                       // [S, H, max_splits, D], [S, H, max_splits, 2]
+};
+
+// Tokens of a sequence that its table holds.
+__device__ __forceinline__ int i8_kv_len(int len, int max_blocks) {
+  const int64_t most = (int64_t)max_blocks * kBlockSize;
+  return len < 0 ? 0 : (len > most ? (int)most : len);
+}
+
+// A block with a scale that is not finite makes the scores of its visible tokens NaN, and its V
+// scale 0: tokens which a row does not see stay out of it (0 * NaN would not).
+__device__ __forceinline__ void i8_poison(float& ks, float& vs) {
+  if (!(fabsf(ks) < INFINITY && fabsf(vs) < INFINITY)) ks = __builtin_nanf(""), vs = 0.f;
+}
+
+template <int D>
+struct I8Pair {
+  // K: lane (c, g) holds codes of token c; V: tokens 4 g + r, dims VW c .. VW c + VW - 1.
+  static constexpr int KW = D >= 64 ? D / 16 : (D == 32 ? 2 : 1);   // words of K per block and lane
+  static constexpr int VW = D / 16;
+  static constexpr int VWORDS = (VW + 3) / 4;
+  uint32_t k[2][KW], v[2][4][VWORDS];
+};
+
+template <int D>
+__device__ __forceinline__ void i8_load_k(const int8_t* base, int c, int g, uint32_t (&k)[I8Pair<D>::KW]) {
+  if constexpr (D >= 64) {
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) {
+      const uint4_t x = ld<uint4_t>(base + c * D + 64 * i + 16 * g);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) k[4 * i + w] = x[w];
+    }
+  } else if constexpr (D == 32) {
+    const int2_t x = ld<int2_t>(base + c * D + 8 * g);
+    k[0] = x[0], k[1] = x[1];
+  } else {
+    k[0] = ld<uint32_t>(base + c * D + 4 * g);
+  }
+}
+
+template <int D>
+__device__ __forceinline__ void i8_load_v(const int8_t* base, int c, int g,
+                                          uint32_t (&v)[4][I8Pair<D>::VWORDS]) {
+  constexpr int VW = I8Pair<D>::VW;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int8_t* p = base + (4 * g + r) * D + VW * c;
+    if constexpr (VW == 16) {
+      const uint4_t x = ld<uint4_t>(p);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) v[r][w] = x[w];
+    } else if constexpr (VW == 8) {
+      const int2_t x = ld<int2_t>(p);
+      v[r][0] = x[0], v[r][1] = x[1];
+    } else if constexpr (VW == 4) {
+      v[r][0] = ld<uint32_t>(p);
+    } else if constexpr (VW == 2) {
+      v[r][0] = ld<uint16_t>(p);
+    } else {
+      v[r][0] = ld<uint8_t>(p);
+    }
+  }
+}
+
+// q as the B operand of S^T = K . Q^T, in the order of dims in which i8_load_k lays K out.
+template <int D>
+struct I8Query {
+  static constexpr int N = D >= 32 ? D / 32 : 1;
+  half8_t x[N];
+};
+
+template <int D>
+__device__ __forceinline__ void i8_load_q(const half_t* row, int g, bool real, I8Query<D>& q) {
+  const half8_t zero = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < I8Query<D>::N; ++i) q.x[i] = zero;
+  if (!real) return;
+  if constexpr (D >= 64) {
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) q.x[i] = ld<half8_t>(row + 64 * (i / 2) + 16 * g + 8 * (i % 2));
+  } else if constexpr (D == 32) {
+    q.x[0] = ld<half8_t>(row + 8 * g);
+  } else {
+    const half4_t t = ld<half4_t>(row + 4 * g);
+    q.x[0] = {t[0], t[1], t[2], t[3], 0, 0, 0, 0};
+  }
+}
+
+template <int D>
+__device__ __forceinline__ float4_t i8_scores(const uint32_t (&k)[I8Pair<D>::KW], const I8Query<D>& q) {
+  float4_t s = {0.f, 0.f, 0.f, 0.f};
+  if constexpr (D >= 32) {
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) s = mfma16x16x32(codes8(k[2 * i], k[2 * i + 1]), q.x[i], s);
+  } else {
+    const uint32_t u = k[0] ^ 0x80808080u;
+    const half2_t a = codes01(u), b = codes23(u);
+    s = mfma16x16x16(half4_t{a[0], a[1], b[0], b[1]}, lo4(q.x[0]), s);
+  }
+  return s;
+}
+
+// V^T operand of output tile t (dims VW i + t): tokens 4 g .. 4 g + 3 of block a, then of block b.
+template <int D, int t>
+__device__ __forceinline__ half8_t i8_vt(const uint32_t (&v)[2][4][I8Pair<D>::VWORDS]) {
+  constexpr int w = t / 4, q = t % 4;
+  const half2_t a = column2<q>(v[0][0][w], v[0][1][w]), b = column2<q>(v[0][2][w], v[0][3][w]);
+  const half2_t c = column2<q>(v[1][0][w], v[1][1][w]), d = column2<q>(v[1][2][w], v[1][3][w]);
+  return {a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+template <int D, int t = 0>
+__device__ __forceinline__ void i8_pv(float4_t (&o)[D / 16], const uint32_t (&v)[2][4][I8Pair<D>::VWORDS],
+                                      half8_t p, float alpha) {
+  if constexpr (t < D / 16) {
+    o[t] = mfma16x16x32(i8_vt<D, t>(v), p, o[t] * alpha);
+    i8_pv<D, t + 1>(o, v, p, alpha);
+  }
+}
+
+// The state of one wavefront's 16 rows: O^T in units of the V scale `vref`.
+template <int D>
+struct I8State {
+  float m, l;
+  float4_t o[D / 16];
+};
+
+// One pair of blocks (tokens t0 .. t0 + 31 of the sequence for a, b next to each other): fk / fv
+// the blocks' K factor (scale * log2 e * ks) and V factor (vs / vref).
+template <int D>
+__device__ __forceinline__ void i8_step(I8State<D>& st, const I8Pair<D>& x, const I8Query<D>& q, float fka,
+                                        float fkb, float fva, float fvb, int ta, int tb, int len, int g) {
+  float4_t sa = i8_scores<D>(x.k[0], q), sb = i8_scores<D>(x.k[1], q);
+  sa *= fka;
+  sb *= fkb;
+  if (tb + kBlockSize > len || ta + kBlockSize > len) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      sa[r] = ta + 4 * g + r < len ? sa[r] : -INFINITY;
+      sb[r] = tb + 4 * g + r < len ? sb[r] : -INFINITY;
+    }
+  }
+  const float top = rows_max(vmax(vmax(vmax(sa[0], sa[1]), vmax(sa[2], sa[3])),
+                                  vmax(vmax(sb[0], sb[1]), vmax(sb[2], sb[3]))));
+  // !(<=): a NaN score (a block whose scale is NaN) moves the reference to NaN and stays
+  const bool move = !(top <= st.m + kI8Rescale);
+  float alpha = 1.f;
+  if (__ballot(move)) {
+    alpha = move ? fast_exp2(st.m - top) : 1.f;            // m = -inf: 0
+    st.l *= alpha;
+    st.m = move ? top : st.m;
+  }
+  const float neg = st.m == -INFINITY ? 0.f : -st.m;
+  float pa[4], pb[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) pa[r] = fast_exp2(sa[r] + neg), pb[r] = fast_exp2(sb[r] + neg);
+  st.l += ((pa[0] + pa[1]) + (pa[2] + pa[3])) + ((pb[0] + pb[1]) + (pb[2] + pb[3]));
+  half8_t p;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) p[r] = (half_t)(pa[r] * fva), p[4 + r] = (half_t)(pb[r] * fvb);
+  // Codes left past the end are finite, and p is 0 there.
+  i8_pv<D>(st.o, x.v, p, alpha);
+}
+
+// One split [b0, b1) of a sequence's blocks by one wavefront (of kI8Waves). Blocks are taken 64
+// at a time: lane i holds block i's id and scales, and the V scale that P is measured against is
+// the largest so far (rounding P * vs / vref to fp16 then loses only what is far below the
+// block with the largest V).
+template <int D>
+__device__ __forceinline__ void i8_split(const Int8DecodeArgs& a, I8State<D>& st, float& vref,
+                                         const I8Query<D>& q, int b, int h, int b0, int b1, int len,
+                                         int wave) {
+  const int lane = threadIdx.x % kWave, c = lane % 16, g = lane / 16;
+  const int32_t* table = a.block_tables + b * a.bt_stride;
+  const int64_t block_bytes = (int64_t)kBlockSize * D;
+  for (int lo = b0; lo < b1; lo += kWave) {
+    const int n = min(b1 - lo, kWave);
+    int blk = 0;
+    float ks = 0.f, vs = 0.f;
+    if (lane < n) {
+      blk = clamp_block(table[lo + lane], a.num_blocks);
+      ks = a.ks[(int64_t)blk * a.kvh + h];
+      vs = a.vs[(int64_t)blk * a.kvh + h];
+      i8_poison(ks, vs);
+    }
+    float top = fmaxf(vs, 0.f);
+#pragma unroll
+    for (int m = 1; m < kWave; m <<= 1) top = fmaxf(top, shfl_xor(top, m));
+    if (top > vref) {
+      const float f = vref / top;
+      vref = top;
+#pragma unroll
+      for (int t = 0; t < D / 16; ++t) st.o[t] *= f;
+    }
+    const float inv = vref > 0.f ? 1.f / vref : 0.f;
+    ks *= a.sl2;
+    vs *= inv;
+
+    auto lane_int = [&](int v, int i) { return __builtin_amdgcn_readlane(v, i); };
+    auto lane_f = [&](float v, int i) {
+      return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), i));
+    };
+    auto load = [&](I8Pair<D>& x, int i) {                 // blocks i, i + 1 of the 64
+      const int j = min(i + 1, n - 1);
+      const int64_t ua = ((int64_t)lane_int(blk, i) * a.kvh + h) * block_bytes;
+      const int64_t ub = ((int64_t)lane_int(blk, j) * a.kvh + h) * block_bytes;
+      i8_load_k<D>(a.kc + ua, c, g, x.k[0]);
+      i8_load_k<D>(a.kc + ub, c, g, x.k[1]);
+      i8_load_v<D>(a.vc + ua, c, g, x.v[0]);
+      i8_load_v<D>(a.vc + ub, c, g, x.v[1]);
+    };
+    auto step = [&](I8Pair<D>& x, int i) {
+      const int j = min(i + 1, n - 1);
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int w = 0; w < I8Pair<D>::VWORDS; ++w) x.v[u][r][w] ^= 0x80808080u;
+      // with an odd count the last pair's second block is its first, wholly past the end
+      const int ta = (lo + i) * kBlockSize;
+      const int tb = i + 1 < n ? ta + kBlockSize : len;
+      i8_step<D>(st, x, q, lane_f(ks, i), lane_f(ks, j), lane_f(vs, i), lane_f(vs, j), ta, tb,
+                 len, g);
+    };
+    constexpr int STEP = 2 * kI8Waves;
+    I8Pair<D> x, y;
+    int i = 2 * wave;
+    if (i < n) load(x, i);
+    while (i < n) {
+      if (i + STEP < n) load(y, i + STEP);
+      step(x, i);
+      i += STEP;
+      if (i >= n) break;
+      if (i + STEP < n) load(x, i + STEP);
+      step(y, i);
+      i += STEP;
+    }
+  }
+}
+
+// The four wavefronts' states meet in LDS; the row (or its partial) is written.
+template <int D>
+__device__ __forceinline__ void i8_finish(const Int8DecodeArgs& a, I8State<D>& st, float vref, int b,
+                                          int head0, int rows, int split, int splits, int wave,
+                                          float* s_o, float* s_ml) {
+  constexpr int VW = D / 16;
+  const int lane = threadIdx.x % kWave, c = lane % 16, g = lane / 16;
+  const float l = rows_sum(st.l);
+  __syncthreads();                                         // the last item's reads of LDS
+  if (c < rows) {
+    float* dst = s_o + (wave * 16 + c) * D;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int t = 0; t < VW; ++t) dst[VW * (4 * g + r) + t] = st.o[t][r];
+    if (g == 0) {
+      s_ml[2 * (wave * 16 + c)] = st.m;
+      s_ml[2 * (wave * 16 + c) + 1] = l;
+    }
+  }
+  __syncthreads();
+  for (int u = threadIdx.x; u < rows * (D / 4); u += kI8Threads) {
+    const int row = u / (D / 4), d = u % (D / 4) * 4;
+    float m[kI8Waves], top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kI8Waves; ++w) m[w] = s_ml[2 * (w * 16 + row)], top = vmax(top, m[w]);
+    float sum = 0.f;
+    float4_t o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < kI8Waves; ++w) {
+      const float f = m[w] == -INFINITY ? 0.f : fast_exp2(m[w] - top);
+      sum += f * s_ml[2 * (w * 16 + row) + 1];
+      o += ld<float4_t>(s_o + (w * 16 + row) * D + d) * f;
+    }
+    const int64_t h = head0 + row;
+    if (splits == 1) {
+      const float f = sum == 0.f ? 0.f : vref / sum;       // no visible key: zeros
+      ts::st<half4_t>(a.out + b * a.out_st + h * D + d, to_half4(o * f));
+    } else {
+      const int64_t at = ((int64_t)b * a.heads + h) * a.max_splits + split;
+      ts::st<float4_t>(a.part_o + at * D + d, o * vref);
+      if (d == 0) {
+        a.part_ml[2 * at] = top;
+        a.part_ml[2 * at + 1] = sum;
+      }
+    }
+  }
+}
+
+// Item `item` of the batch's splits, numbered densely over the sequences: its sequence, split and
+// split count. Every wavefront looks it up for itself, 64 sequences at a time.
+__device__ __forceinline__ bool i8_find(const Int8DecodeArgs& a, int item, int& b, int& split, int& splits,
+                                        int& len) {
+  const int lane = threadIdx.x % kWave;
+  int base = 0;
+  for (int s0 = 0; s0 < a.num_seqs; s0 += kWave) {
+    int n = 0, kv = 0;
+    if (s0 + lane < a.num_seqs) {
+      kv = i8_kv_len(a.seq_lens[s0 + lane], a.max_blocks);
+      n = i8_splits((kv + kBlockSize - 1) / kBlockSize, a.max_splits);
+    }
+    int sum = n;
+#pragma unroll
+    for (int m = 1; m < kWave; m <<= 1) {
+      const int up = __shfl_up(sum, m, kWave);
+      sum += lane >= m ? up : 0;
+    }
+    const uint64_t past = __ballot(base + sum > item);
+    if (past) {
+      const int i = __ffsll((unsigned long long)past) - 1;
+      b = s0 + i;
+      splits = __builtin_amdgcn_readlane(n, i);
+      split = item - (base + __builtin_amdgcn_readlane(sum, i) - splits);
+      len = __builtin_amdgcn_readlane(kv, i);
+      return true;
+    }
+    base += __builtin_amdgcn_readlane(sum, kWave - 1);
+  }
+  return false;
+}
+
+template <int D>
+struct I8DecodeLds {
+  float o[kI8Waves * 16 * D];
+  float ml[2 * kI8Waves * 16];
+};
+
+template <int D>
+__global__ void __launch_bounds__(kI8Threads) decode_int8_kernel(Int8DecodeArgs a) {
+  __shared__ __align__(16) I8DecodeLds<D> lds;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int lane = threadIdx.x % kWave, c = lane % 16, g = lane / 16;
+  const int tiles = a.kvh * a.head_tiles;
+  for (int64_t u = blockIdx.x;; u += gridDim.x) {
+    const int64_t item = u / tiles;
+    const int tile = (int)(u % tiles);
+    int b, split, splits, len;
+    if (item > INT32_MAX || !i8_find(a, (int)item, b, split, splits, len)) return;
+    const int h = tile / a.head_tiles, r0 = tile % a.head_tiles * 16;
+    const int head0 = h * a.group + r0, rows = min(a.group - r0, 16);
+    I8Query<D> q;
+    i8_load_q<D>(a.q + b * a.q_st + (int64_t)(head0 + c) * a.q_sh, g, c < rows, q);
+    I8State<D> st;
+    st.m = -INFINITY, st.l = 0.f;
+#pragma unroll
+    for (int t = 0; t < D / 16; ++t) st.o[t] = {0.f, 0.f, 0.f, 0.f};
+    float vref = 0.f;
+    const int nb = (len + kBlockSize - 1) / kBlockSize;
+    const int b0 = (int)((int64_t)nb * split / splits), b1 = (int)((int64_t)nb * (split + 1) / splits);
+    i8_split<D>(a, st, vref, q, b, h, b0, b1, len, wave);
+    i8_finish<D>(a, st, vref, b, head0, rows, split, splits, wave, lds.o, lds.ml);
+  }
+}
+
+// Rows of sequences with more than one split: one workgroup per (sequence, head).
+template <int D>
+__global__ void __launch_bounds__(kWave) decode_int8_merge_kernel(Int8DecodeArgs a) {
+  const int b = blockIdx.x, h = blockIdx.y, lane = threadIdx.x;
+  const int len = i8_kv_len(table_entry(a.seq_lens + b), a.max_blocks);
+  const int splits = i8_splits((len + kBlockSize - 1) / kBlockSize, a.max_splits);
+  if (splits == 1) return;
+  const int64_t row = ((int64_t)b * a.heads + h) * a.max_splits;
+  // lane i: split i's weight
+  float m = -INFINITY, l = 0.f;
+  if (lane < splits) m = a.part_ml[2 * (row + lane)], l = a.part_ml[2 * (row + lane) + 1];
+  float top = m;
+#pragma unroll
+  for (int k = 1; k < kWave; k <<= 1) top = vmax(top, shfl_xor(top, k));
+  const float f = m == -INFINITY ? 0.f : fast_exp2(m - top);
+  float sum = f * l;
+#pragma unroll
+  for (int k = 1; k < kWave; k <<= 1) sum += shfl_xor(sum, k);
+  const float inv = 1.f / sum;
+  for (int d0 = 0; d0 < D; d0 += kWave) {                  // every lane: each holds a weight
+    const int d = min(d0 + lane, D - 1);
+    float o = 0.f;
+    for (int i = 0; i < splits; ++i) o += a.part_o[(row + i) * D + d] * __shfl(f, i, kWave);
+    if (d0 + lane < D) a.out[b * a.out_st + (int64_t)h * D + d] = (half_t)(o * inv);
+  }
+}
+
+}  // namespace ts

@@ -1,0 +1,47 @@
+// The 8-bit paged cache shared by its write and attention kernels: int8 codes
+// [num_blocks, KVH, 16, D] with one fp32 scale per (block, KV head), [num_blocks, KVH]; a code
+// stands for code * scale.
+//
+// Codes become fp16 exactly in registers: u = code + 128 (the sign bit flipped) under the high
+// byte 0x64 is the fp16 number 1024 + u, and subtracting 1152 leaves the code (every integer up to
+// 2048 is an fp16 number, so nothing rounds).
+#pragma once
+
+#include "common.h"
+
+namespace ts {
+
+constexpr float kCodeMax = 127.f;
+
+__device__ __forceinline__ half2_t as_half2(uint32_t w) { return __builtin_bit_cast(half2_t, w); }
+
+// 1024 + u (two packed) -> the codes.
+__device__ __forceinline__ half2_t unbias(uint32_t w) {
+  const half2_t off = {(half_t)1152.f, (half_t)1152.f};
+  return as_half2(w) - off;
+}
+
+// Codes 0, 1 and 2, 3 of a word (sign bits flipped already) as packed fp16.
+__device__ __forceinline__ half2_t codes01(uint32_t u) {
+  return unbias(__builtin_amdgcn_perm(0x64646464u, u, 0x04010400u));
+}
+__device__ __forceinline__ half2_t codes23(uint32_t u) {
+  return unbias(__builtin_amdgcn_perm(0x64646464u, u, 0x04030402u));
+}
+
+// Eight consecutive codes (two words) as an MFMA operand.
+__device__ __forceinline__ half8_t codes8(uint32_t w0, uint32_t w1) {
+  w0 ^= 0x80808080u;
+  w1 ^= 0x80808080u;
+  const half2_t a = codes01(w0), b = codes23(w0), c = codes01(w1), d = codes23(w1);
+  return {a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// Code `q` of each of two words (sign bits flipped already) as packed fp16: a column of the
+// rows that the words come from.
+template <int q>
+__device__ __forceinline__ half2_t column2(uint32_t row0, uint32_t row1) {
+  return unbias(__builtin_amdgcn_perm(row1, row0, 0x0c040c00u + q * 0x00010001u) | 0x64006400u);
+}
+
+}  // namespace ts

@@ -4,7 +4,8 @@ Restates the parts of the reference's engine that shape the kernels' inputs: a b
 that never hands out the null block 0 (kv/block_allocator.py:16-62), continuous batching with
 decodes scheduled first and prompts prefilled in chunks under a token budget
 (scheduler/scheduler.py:65-130), an input builder per step (host or device) and graph replay of
-pure-decode steps (runner/model_runner.py:20-28). Sampling is greedy argmax.
+pure-decode steps (runner/model_runner.py:20-28). Sampling is greedy argmax. kv_cache_dtype
+"int8" keeps K and V as 8-bit codes with a scale for each block and KV head.
 """
 
 from __future__ import annotations
@@ -56,9 +57,9 @@ class Request:
 class GreedyEngine:
     def __init__(self, model, num_blocks: int, max_num_batched_tokens: int = 256,
                  max_num_seqs: int = 32, max_model_len: int = 1024, graph_sizes=(),
-                 device_metadata: bool = False) -> None:
+                 device_metadata: bool = False, kv_cache_dtype: str = "fp16") -> None:
         self.model = model
-        self.kv = model.new_kv_cache(num_blocks)
+        self.kv = model.new_kv_cache(num_blocks, kv_cache_dtype)
         self.alloc = BlockAllocator(num_blocks)
         self.budget = max_num_batched_tokens
         self.max_seqs = max_num_seqs

@@ -21,6 +21,7 @@ import numpy as np
 import torch
 
 from turingserve_amd.metadata import AttentionMetadata, BatchItem, _arena_bytes, _carve
+from turingserve_amd.quant import Int8KVCache
 
 
 class StaticDecodeBatch:
@@ -84,7 +85,7 @@ class DecodeGraphs:
     """Pure-decode steps captured once per batch size of `sizes` and replayed with the step's rows
     written into the static batch."""
 
-    def __init__(self, model, kv_cache: torch.Tensor, sizes, max_blocks_per_seq: int,
+    def __init__(self, model, kv_cache: torch.Tensor | Int8KVCache, sizes, max_blocks_per_seq: int,
                  max_model_len: int) -> None:
         self.model, self.kv_cache = model, kv_cache
         self.ladder = sorted(set(int(s) for s in sizes))

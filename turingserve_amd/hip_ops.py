@@ -25,7 +25,8 @@ __all__ = ["kv_write", "paged_attention", "linear", "lm_head_int8", "logits_int8
            "decode_attention_v1", "decode_attention_v2", "decode_attention_v3",
            "prefill_attention", "rmsnorm", "rmsnorm_residual", "rope_", "silu_mul", "w8a16_glu",
            "gate_up_silu", "rope_kv_write_", "decode_kv_write_attention",
-           "decode_rope_kv_write_attention"]
+           "decode_rope_kv_write_attention", "kv_write_int8", "rope_kv_write_int8",
+           "paged_attention_int8"]
 
 DEFAULT_PARTITION = 0            # v3 split size when the caller names none: 0 = own-length
 
@@ -708,4 +709,122 @@ def silu_mul(gu: torch.Tensor) -> torch.Tensor:
     out = torch.empty(T, inter, dtype=gu.dtype, device=gu.device)
     N.check(N.lib().ts_silu_mul(_ptr(gu), gu.stride(0), _ptr(out), out.stride(0), T, inter,
                                 _stream(gu)), "silu_mul")
+    return out
+
+
+# ------------------------------------------------------------------------------------------
+# The 8-bit paged cache: int8 codes with a scale for each block and KV head
+# ------------------------------------------------------------------------------------------
+def _int8_args(what: str, k_cache, v_cache, k_scale, v_scale, meta, device) -> tuple:
+    """Checks of the cache and the step's metadata; (NB, KVH, D, block tables, seq_lens,
+    query_start_loc, table stride)."""
+    shape = k_cache.shape
+    if len(shape) != 4 or shape[2] != 16 or shape != v_cache.shape:
+        raise ValueError(f"{what}: caches must be [num_blocks, KVH, 16, D], got {tuple(shape)}")
+    _require(k_cache.dtype == torch.int8 and v_cache.dtype == torch.int8 and
+             k_cache.is_contiguous() and v_cache.is_contiguous(),
+             "{}: caches must be contiguous int8", what)
+    NB, KVH, _, D = shape
+    for s in (k_scale, v_scale):
+        _require(s.dtype == torch.float32 and s.shape == (NB, KVH) and s.is_contiguous(),
+                 "{}: scales must be contiguous fp32 [num_blocks, KVH]", what)
+    bt = meta.block_tables
+    if bt.dtype != torch.int32 or bt.stride(1) != 1:
+        bt = bt.to(torch.int32).contiguous()
+    sl, qsl = _i32(meta.seq_lens), _i32(meta.query_start_loc)
+    B = sl.shape[0]
+    _require(bt.shape[0] >= B and qsl.shape[0] >= B + 1 and 0 <= meta.num_decode <= B,
+             "{}: metadata of {} sequences", what, B)
+    for t in (k_cache, v_cache, k_scale, v_scale, bt, sl, qsl):
+        _require(t.device == device, "{}: every tensor must live on the same GPU", what)
+    return NB, KVH, D, bt, sl, qsl, bt.stride(0) if bt.shape[0] > 1 else bt.shape[1]
+
+
+def kv_write_int8(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                  k_scale: torch.Tensor, v_scale: torch.Tensor, meta) -> None:
+    """The step's new rows k, v [T, KVH, D] (strided views of qkv allowed) into an 8-bit paged
+    cache: codes [NB, KVH, 16, D] int8, scales [NB, KVH] fp32, a code standing for code * scale.
+    A block's scale becomes max(scale of the rows already there, max|new rows| / 127); rows there
+    are requantised when it grows, and a block whose row 0 is written starts anew. The rows of
+    sequence b (query_start_loc[b] .. [b + 1]) are its last ones (positions up to seq_lens[b] - 1)
+    and lie where its block table says; slot_mapping is not read. Rows that are not finite make
+    their block's scale NaN. No two sequences of a step may write into one block."""
+    T, KVH, D = k.shape
+    if T == 0:
+        return
+    _check_gpu(k, v)
+    NB, ckvh, cd, bt, sl, qsl, bt_st = _int8_args("kv_write_int8", k_cache, v_cache, k_scale, v_scale,
+                                                  meta, k.device)
+    _require(v.shape == k.shape and v.device == k.device and ckvh == KVH and cd == D,
+             "kv_write_int8: shape mismatch")
+    _require(k.dtype == torch.float16 and v.dtype == torch.float16 and k.stride(2) == 1 and
+             v.stride(2) == 1, "kv_write_int8: k, v must be fp16 with unit stride over D")
+    N.check(N.lib().ts_kv_write_int8(
+        _ptr(k), _ptr(v), k.stride(0), k.stride(1), v.stride(0), v.stride(1), _ptr(k_cache),
+        _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), NB, _ptr(bt), bt_st, bt.shape[1], _ptr(sl),
+        _ptr(qsl), sl.shape[0], meta.num_decode, int(meta.max_query_len), T, KVH, D, _stream(k)),
+        "kv_write_int8")
+
+
+def rope_kv_write_int8(qkv: torch.Tensor, positions: torch.Tensor, cos: torch.Tensor,
+                       sin: torch.Tensor, H: int, KVH: int, D: int, k_cache: torch.Tensor,
+                       v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                       meta) -> torch.Tensor:
+    """kv_write_int8 of qkv's k and v heads with k rotated on the way (rotate-half RoPE by the
+    fp32 tables cos / sin [max_len, D / 2]), in one launch with the rotation of q, which is
+    returned as [T, H, D]; qkv [T, (H + 2 KVH) D] is left as it is. Rotations are computed wider
+    than fp16 and rounded once: q to fp16, k straight to its code."""
+    _check_gpu(qkv, positions, cos, sin)
+    T = qkv.shape[0]
+    _require(qkv.dim() == 2 and qkv.stride(1) == 1 and qkv.dtype == torch.float16 and
+             qkv.shape[1] >= (H + 2 * KVH) * D,
+             "rope_kv_write_int8: qkv must be fp16 [T, (H + 2 KVH) D]")
+    q = torch.empty(T, H, D, dtype=qkv.dtype, device=qkv.device)
+    if T == 0:
+        return q
+    NB, ckvh, cd, bt, sl, qsl, bt_st = _int8_args("rope_kv_write_int8", k_cache, v_cache, k_scale,
+                                                  v_scale, meta, qkv.device)
+    _require(ckvh == KVH and cd == D, "rope_kv_write_int8: cache shape mismatch")
+    _require(cos.dtype == torch.float32 and sin.dtype == torch.float32 and cos.is_contiguous()
+             and sin.is_contiguous() and cos.shape == sin.shape and cos.dim() == 2 and
+             cos.shape[1] == D // 2,
+             "rope_kv_write_int8: tables must be contiguous fp32 [max_len, D / 2]")
+    _require(positions.shape[0] >= T and positions.device == qkv.device == cos.device == sin.device,
+             "rope_kv_write_int8: positions shorter than qkv, or tensors of several devices")
+    pos = positions if (positions.dtype == torch.int64 and positions.is_contiguous()) \
+        else positions.to(torch.int64).contiguous()
+    N.check(N.lib().ts_rope_kv_write_int8(
+        _ptr(qkv), qkv.stride(0) if T > 1 else qkv.shape[1], _ptr(pos), _ptr(cos), _ptr(sin),
+        cos.shape[0], _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), NB,
+        _ptr(bt), bt_st, bt.shape[1], _ptr(sl), _ptr(qsl), sl.shape[0], meta.num_decode,
+        int(meta.max_query_len), T, H, KVH, D, _stream(qkv)), "rope_kv_write_int8")
+    return q
+
+
+def paged_attention_int8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                         k_scale: torch.Tensor, v_scale: torch.Tensor, meta,
+                         scale: float) -> torch.Tensor:
+    """paged_attention over an 8-bit cache (see kv_write_int8): q [T, H, D] -> [T, H*D], one row
+    for each of the first num_decode sequences, the rows of query_start_loc for the others under
+    the bottom-right causal mask. A row that sees a block whose scale is not finite is NaN; a row
+    that sees no token is zeros."""
+    T, H, D = q.shape
+    out = torch.empty(T, H * D, dtype=q.dtype, device=q.device)
+    if T == 0:
+        return out
+    _check_gpu(q)
+    NB, KVH, cd, bt, sl, qsl, bt_st = _int8_args("paged_attention_int8", k_cache, v_cache, k_scale,
+                                                 v_scale, meta, q.device)
+    _require(cd == D and q.stride(2) == 1 and q.dtype == torch.float16,
+             "paged_attention_int8: q must be fp16 [T, H, D] with unit stride over D")
+    B, S = sl.shape[0], meta.num_decode
+    bounds = (int(meta.max_query_len), int(meta.max_seq_len), _prefill_seq_bound(meta))
+    ws_bytes = N.lib().ts_paged_attention_int8_workspace_bytes(B, S, *bounds, H, KVH, D,
+                                                               N.cu_count(q.device.index or 0))
+    ws = _workspace(ws_bytes, q.device)
+    N.check(N.lib().ts_paged_attention_int8(
+        _ptr(q), q.stride(0) if T > 1 else H * D, q.stride(1) if H > 1 else D, _ptr(out), H * D, T,
+        _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), NB, _ptr(bt), bt_st, bt.shape[1],
+        _ptr(sl), _ptr(qsl), B, S, *bounds, H, KVH, D, float(scale), _ptr(ws), ws_bytes, _stream(q)),
+        "paged_attention_int8")
     return out

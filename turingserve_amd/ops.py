@@ -18,7 +18,8 @@ def _reference() -> SimpleNamespace:
         name="reference", rmsnorm=r.rmsnorm, rmsnorm_residual=r.rmsnorm_residual,
         silu_mul=r.silu_mul, rope_=r.rope_, linear=r.linear, kv_write=r.kv_write,
         paged_attention=r.paged_attention, dense_causal_attention=r.dense_causal_attention,
-        attention_with_mask=r.attention_with_mask)
+        attention_with_mask=r.attention_with_mask, kv_write_int8=r.kv_write_int8,
+        rope_kv_write_int8=r.rope_kv_write_int8, paged_attention_int8=r.paged_attention_int8)
 
 
 def _hip() -> SimpleNamespace:
@@ -43,6 +44,9 @@ def _hip() -> SimpleNamespace:
     ns.decode_rope_kv_write_attention = h.decode_rope_kv_write_attention
     ns.decode_split_map = h.decode_split_map
     ns.linear_rope_kv_write = h.linear_rope_kv_write
+    ns.kv_write_int8 = h.kv_write_int8
+    ns.rope_kv_write_int8 = h.rope_kv_write_int8
+    ns.paged_attention_int8 = h.paged_attention_int8
     return ns
 
 

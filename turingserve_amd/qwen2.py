@@ -14,7 +14,7 @@ from dataclasses import dataclass
 
 import torch
 
-from turingserve_amd.quant import LinearWeight, quantize
+from turingserve_amd.quant import Int8KVCache, LinearWeight, quantize
 
 
 @dataclass(frozen=True)
@@ -180,8 +180,16 @@ class Qwen2Model:
         """Decoder layer `index` from its normed input x to the MLP activation: qkv, RoPE, the
         K/V write into kv_cache[index], attention, o_proj with post_attention_layernorm, and
         silu(gate) * up; returns (the input of down_proj, residual). split_map: the step's
-        decode split map (fused decode only), shared by every layer."""
+        decode split map (fused decode only), shared by every layer. An Int8KVCache takes the
+        8-bit write and attention instead."""
         c, ops, lw = self.cfg, self.ops, self.w.layers[index]
+        if isinstance(kv_cache, Int8KVCache):
+            cache = kv_cache.layer(index)
+            q = ops.rope_kv_write_int8(ops.linear(x, lw.qkv_proj), positions, self.cos, self.sin,
+                                       c.num_heads, c.num_kv_heads, c.head_dim, *cache, meta)
+            a = ops.paged_attention_int8(q, *cache, meta, self.scale)
+            x, residual = self._project_norm(a, lw.o_proj, residual, lw.post_attention_norm)
+            return self._mlp_act(x, lw), residual
         k_cache, v_cache = kv_cache[index, 0], kv_cache[index, 1]
         H, KVH, D = c.num_heads, c.num_kv_heads, c.head_dim
         a = None
@@ -225,14 +233,16 @@ class Qwen2Model:
 
     @torch.inference_mode()
     def forward(self, input_ids, positions, meta, kv_cache):
-        """kv_cache [L, 2, num_blocks, KVH, 16, D] -> final normed hidden rows [T, hidden].
+        """kv_cache [L, 2, num_blocks, KVH, 16, D], or an Int8KVCache -> final normed hidden rows
+        [T, hidden].
         The same chain as layer_forward over every layer and the final norm, with each layer's
         down_proj taken together with the norm that consumes it (the next input_layernorm, or
         the final norm): the same values, without a separate split-K reduction launch."""
         c, layers = self.cfg, self.w.layers
         fused = self.pure_decode(meta, input_ids.shape[0])
         # one decode split map per step, read by every layer's fused decode launch
-        build_map = getattr(self.ops, "decode_split_map", None) if fused else None
+        build_map = (getattr(self.ops, "decode_split_map", None)
+                     if fused and not isinstance(kv_cache, Int8KVCache) else None)
         split_map = (build_map(meta, c.num_heads, c.num_kv_heads, c.head_dim, kv_cache.shape[2],
                                kv_cache.device) if build_map is not None else None)
         h = self.w.embed_tokens[input_ids]
@@ -257,7 +267,12 @@ class Qwen2Model:
             return self.ops.lm_head_int8(h, *head).float()
         return (h @ self.w.embed_tokens.T).float()
 
-    def new_kv_cache(self, num_blocks: int) -> torch.Tensor:
+    def new_kv_cache(self, num_blocks: int, dtype: str = "fp16") -> torch.Tensor | Int8KVCache:
+        """dtype "fp16" (the activations' type) or "int8" (Int8KVCache: half the bytes)."""
         c = self.cfg
+        if dtype == "int8":
+            return Int8KVCache.new(c.num_layers, num_blocks, c.num_kv_heads, c.head_dim, self.device)
+        if dtype != "fp16":
+            raise ValueError(f"unknown KV cache dtype {dtype!r}")
         return torch.zeros(c.num_layers, 2, num_blocks, c.num_kv_heads, 16, c.head_dim,
                            dtype=self.dtype, device=self.device)

@@ -116,3 +116,70 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         vv = v_cache[blocks].permute(0, 2, 1, 3).reshape(nb * 16, KVH, D)[:seq_len]
         out[qs:qe] = attention_with_mask(q[qs:qe], kk, vv, scale)
     return out
+
+
+def kv_write_int8(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                  k_scale: torch.Tensor, v_scale: torch.Tensor, meta) -> None:
+    """Twin of the quantising write into an 8-bit paged cache (codes [NB, KVH, 16, D] int8, scales
+    [NB, KVH] fp32), a block at a time. k, v [T, KVH, D] in any floating type."""
+    qsl, tables = meta.query_start_loc.tolist(), meta.block_tables.tolist()
+    for b, length in enumerate(meta.seq_lens.tolist()):
+        start = length - (qsl[b + 1] - qsl[b])
+        for j in range(max(start, 0) // 16, -(-length // 16)):
+            if j >= len(tables[b]) or not 0 <= tables[b][j] < k_cache.shape[0]:
+                continue
+            lo, hi = max(start, 16 * j), min(length, 16 * (j + 1))
+            rows = slice(qsl[b] + lo - start, qsl[b] + hi - start)
+            for x, codes, scales in ((k, k_cache, k_scale), (v, v_cache, v_scale)):
+                _write_block(x[rows].transpose(0, 1).float(), codes[tables[b][j]],
+                             scales[tables[b][j]], max(lo, 0) - 16 * j)
+
+
+def _write_block(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, at: int) -> None:
+    """Rows x [KVH, n, D] fp32 into rows at .. at + n - 1 of one block, in place."""
+    was = scales.clone() if at > 0 else torch.zeros_like(scales)
+    top = x.abs().amax((1, 2))
+    scale = torch.maximum(was, top / torch.full_like(top, 127.0))
+    scale = torch.where(torch.isfinite(top), scale, torch.nan)
+    for h, (old, new) in enumerate(zip(was.tolist(), scale.tolist())):
+        if new > old:
+            codes[h, :at] = torch.round(codes[h, :at].float() * (was[h] / scale[h])).to(torch.int8)
+        codes[h, at:at + x.shape[1]] = \
+            torch.round(x[h] / scale[h]).clamp(-127, 127).to(torch.int8) if new > 0 else 0
+    scales.copy_(scale)
+
+
+def rope_kv_write_int8(qkv: torch.Tensor, positions: torch.Tensor, cos: torch.Tensor,
+                       sin: torch.Tensor, H: int, KVH: int, D: int, k_cache: torch.Tensor,
+                       v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                       meta) -> torch.Tensor:
+    """Twin: rotate-half RoPE of q (returned, [T, H, D], rounded once) and k (rounded to fp32), then
+    kv_write_int8 of the rotated k and of v."""
+    T, half = qkv.shape[0], D // 2
+    pos = positions[:T].clamp(0, cos.shape[0] - 1)
+    c, s = cos[pos].double()[:, None], sin[pos].double()[:, None]
+    x = qkv[:, :(H + 2 * KVH) * D].view(T, H + 2 * KVH, D)
+    x1, x2 = x[:, :H + KVH, :half].double(), x[:, :H + KVH, half:].double()
+    qk = torch.cat([x1 * c - x2 * s, x2 * c + x1 * s], dim=-1).float()
+    kv_write_int8(qk[:, H:], x[:, H + KVH:], k_cache, v_cache, k_scale, v_scale, meta)
+    return qk[:, :H].to(qkv.dtype)
+
+
+def paged_attention_int8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                         k_scale: torch.Tensor, v_scale: torch.Tensor, meta,
+                         scale: float) -> torch.Tensor:
+    """Twin: the sequences' blocks as fp32 values, then attention_with_mask; rows of sequences with
+    seq_len 0 stay 0."""
+    T, H, D = q.shape
+    KVH = k_cache.shape[1]
+    out = torch.zeros(T, H * D, dtype=q.dtype, device=q.device)
+    qsl = meta.query_start_loc.tolist()
+    for b, seq_len in enumerate(meta.seq_lens.tolist()):
+        qs, qe = qsl[b], qsl[b + 1]
+        if seq_len == 0 or qe == qs:
+            continue
+        blocks = meta.block_tables[b, :-(-seq_len // 16)].long()
+        kk, vv = ((c[blocks].float() * s[blocks][:, :, None, None]).permute(0, 2, 1, 3)
+                  .reshape(-1, KVH, D)[:seq_len] for c, s in ((k_cache, k_scale), (v_cache, v_scale)))
+        out[qs:qe] = attention_with_mask(q[qs:qe], kk, vv, scale)
+    return out
