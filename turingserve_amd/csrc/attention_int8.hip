@@ -61,11 +61,11 @@ static bool int8_head_dim(int D) { return D == 16 || D == 32 || D == 64 || D == 
 
 template <int D>
 static int launch_decode(const Int8DecodeArgs& a, int cus, hipStream_t s) {
-  // Every split of the batch, at most four workgroups a CU; the rest go round.
+  // Every split of the batch, at most as many workgroups as the CUs hold; the rest go round.
   const int64_t units = (int64_t)a.num_seqs * a.max_splits * a.kvh * a.head_tiles;
-  const int64_t cap = 4 * (int64_t)cus;
+  const int64_t cap = (int64_t)i8_decode_groups(D) * cus;
   decode_int8_kernel<D><<<(unsigned)(units < cap ? units : cap), kI8Threads, 0, s>>>(a);
-  if (a.max_splits > 1) decode_int8_merge_kernel<D><<<dim3(a.num_seqs, a.heads), kWave, 0, s>>>(a);
+  if (a.max_splits > 1) decode_int8_merge_kernel<D><<<dim3(a.num_seqs, a.heads), kI8Threads, 0, s>>>(a);
   return check_launch("paged_attention_int8");
 }
 

@@ -45,6 +45,32 @@ struct Int8DecodeArgs {
   float *part_o, *part_ml;                       // [S, H, max_splits, D], [S, H, max_splits, 2]
 };
 
+// Wavefront scans on the VALU (DPP row shifts, then the rows' last lanes broadcast on): a step costs
+// a few cycles where a shuffle through the LDS unit costs over a hundred, and both scans stand in
+// front of a workgroup's first K/V request.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int i8_dpp(int v) {             // 0 where no lane moves in
+  return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ int i8_scan(int v) {            // inclusive sums
+  v += i8_dpp<0x111, 0xf>(v);
+  v += i8_dpp<0x112, 0xf>(v);
+  v += i8_dpp<0x114, 0xf>(v);
+  v += i8_dpp<0x118, 0xf>(v);
+  v += i8_dpp<0x142, 0xa>(v);
+  return v + i8_dpp<0x143, 0xc>(v);
+}
+__device__ __forceinline__ float i8_most(float x) {        // the largest of 64 values >= 0
+  int v = __float_as_int(x);
+  v = max(v, i8_dpp<0x111, 0xf>(v));
+  v = max(v, i8_dpp<0x112, 0xf>(v));
+  v = max(v, i8_dpp<0x114, 0xf>(v));
+  v = max(v, i8_dpp<0x118, 0xf>(v));
+  v = max(v, i8_dpp<0x142, 0xa>(v));
+  v = max(v, i8_dpp<0x143, 0xc>(v));
+  return __int_as_float(__builtin_amdgcn_readlane(v, kWave - 1));
+}
+
 // Tokens of a sequence that its table holds.
 __device__ __forceinline__ int i8_kv_len(int len, int max_blocks) {
   const int64_t most = (int64_t)max_blocks * kBlockSize;
@@ -228,19 +254,7 @@ __device__ __forceinline__ void i8_split(const Int8DecodeArgs& a, I8State<D>& st
       vs = a.vs[(int64_t)blk * a.kvh + h];
       i8_poison(ks, vs);
     }
-    float top = fmaxf(vs, 0.f);
-#pragma unroll
-    for (int m = 1; m < kWave; m <<= 1) top = fmaxf(top, shfl_xor(top, m));
-    if (top > vref) {
-      const float f = vref / top;
-      vref = top;
-#pragma unroll
-      for (int t = 0; t < D / 16; ++t) st.o[t] *= f;
-    }
-    const float inv = vref > 0.f ? 1.f / vref : 0.f;
-    ks *= a.sl2;
-    vs *= inv;
-
+    // the first two pairs are requested behind the scales and before they are waited for
     auto lane_int = [&](int v, int i) { return __builtin_amdgcn_readlane(v, i); };
     auto lane_f = [&](float v, int i) {
       return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), i));
@@ -272,17 +286,38 @@ __device__ __forceinline__ void i8_split(const Int8DecodeArgs& a, I8State<D>& st
     I8Pair<D> x, y;
     int i = 2 * wave;
     if (i < n) load(x, i);
-    while (i < n) {
-      if (i + STEP < n) load(y, i + STEP);
+    if (i + STEP < n) load(y, i + STEP);
+    const float top = i8_most(fmaxf(vs, 0.f));
+    if (top > vref) {
+      const float f = vref / top;
+      vref = top;
+#pragma unroll
+      for (int t = 0; t < D / 16; ++t) st.o[t] *= f;
+    }
+    const float inv = vref > 0.f ? 1.f / vref : 0.f;
+    ks *= a.sl2;
+    vs *= inv;
+
+    if (i >= n) continue;
+    while (true) {
       step(x, i);
+      if (i + 2 * STEP < n) load(x, i + 2 * STEP);
       i += STEP;
       if (i >= n) break;
-      if (i + STEP < n) load(x, i + STEP);
       step(y, i);
+      if (i + 2 * STEP < n) load(y, i + 2 * STEP);
       i += STEP;
+      if (i >= n) break;
     }
   }
 }
+
+template <int D>
+struct I8DecodeLds {
+  static constexpr int ROW = D + 4;      // floats of a row: rows start on different banks
+  float o[kI8Waves * 16 * ROW];
+  float ml[2 * kI8Waves * 16];
+};
 
 // The four wavefronts' states meet in LDS; the row (or its partial) is written.
 template <int D>
@@ -294,7 +329,7 @@ __device__ __forceinline__ void i8_finish(const Int8DecodeArgs& a, I8State<D>& s
   const float l = rows_sum(st.l);
   __syncthreads();                                         // the last item's reads of LDS
   if (c < rows) {
-    float* dst = s_o + (wave * 16 + c) * D;
+    float* dst = s_o + (wave * 16 + c) * I8DecodeLds<D>::ROW;
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
@@ -316,7 +351,7 @@ __device__ __forceinline__ void i8_finish(const Int8DecodeArgs& a, I8State<D>& s
     for (int w = 0; w < kI8Waves; ++w) {
       const float f = m[w] == -INFINITY ? 0.f : fast_exp2(m[w] - top);
       sum += f * s_ml[2 * (w * 16 + row) + 1];
-      o += ld<float4_t>(s_o + (w * 16 + row) * D + d) * f;
+      o += ld<float4_t>(s_o + (w * 16 + row) * I8DecodeLds<D>::ROW + d) * f;
     }
     const int64_t h = head0 + row;
     if (splits == 1) {
@@ -345,12 +380,7 @@ __device__ __forceinline__ bool i8_find(const Int8DecodeArgs& a, int item, int& 
       kv = i8_kv_len(a.seq_lens[s0 + lane], a.max_blocks);
       n = i8_splits((kv + kBlockSize - 1) / kBlockSize, a.max_splits);
     }
-    int sum = n;
-#pragma unroll
-    for (int m = 1; m < kWave; m <<= 1) {
-      const int up = __shfl_up(sum, m, kWave);
-      sum += lane >= m ? up : 0;
-    }
+    const int sum = i8_scan(n);
     const uint64_t past = __ballot(base + sum > item);
     if (past) {
       const int i = __ffsll((unsigned long long)past) - 1;
@@ -365,14 +395,11 @@ __device__ __forceinline__ bool i8_find(const Int8DecodeArgs& a, int item, int& 
   return false;
 }
 
-template <int D>
-struct I8DecodeLds {
-  float o[kI8Waves * 16 * D];
-  float ml[2 * kI8Waves * 16];
-};
+// Workgroups that a CU holds at once, by registers.
+constexpr int i8_decode_groups(int D) { return D > 128 ? 1 : (D == 128 ? 3 : 4); }
 
 template <int D>
-__global__ void __launch_bounds__(kI8Threads) decode_int8_kernel(Int8DecodeArgs a) {
+__global__ void __launch_bounds__(kI8Threads, i8_decode_groups(D)) decode_int8_kernel(Int8DecodeArgs a) {
   __shared__ __align__(16) I8DecodeLds<D> lds;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int lane = threadIdx.x % kWave, c = lane % 16, g = lane / 16;
@@ -398,31 +425,49 @@ __global__ void __launch_bounds__(kI8Threads) decode_int8_kernel(Int8DecodeArgs 
   }
 }
 
-// Rows of sequences with more than one split: one workgroup per (sequence, head).
+// Rows of sequences with more than one split: one workgroup per (sequence, head), D / 4 threads a
+// partial. The first partial of each thread and every split's (m, l) are requested before the
+// sequence's length is known (they lie in the workspace whatever it is), the others at once after
+// it.
 template <int D>
-__global__ void __launch_bounds__(kWave) decode_int8_merge_kernel(Int8DecodeArgs a) {
-  const int b = blockIdx.x, h = blockIdx.y, lane = threadIdx.x;
+__global__ void __launch_bounds__(kI8Threads) decode_int8_merge_kernel(Int8DecodeArgs a) {
+  constexpr int PER_ROW = D / 4, GROUPS = kI8Threads / PER_ROW;
+  constexpr int N = (kI8MaxSplits + GROUPS - 1) / GROUPS;
+  __shared__ __align__(16) float s_o[GROUPS][D];
+  const int b = blockIdx.x, h = blockIdx.y, lane = threadIdx.x % kWave;
+  const int group = threadIdx.x / PER_ROW, d = threadIdx.x % PER_ROW * 4;
+  const int64_t row = ((int64_t)b * a.heads + h) * a.max_splits;
+  const float* part = a.part_o + row * D + d;
+  const float2_t ml = ld<float2_t>(a.part_ml + 2 * (row + min(lane, a.max_splits - 1)));
+  float4_t x[N];
+  x[0] = ld<float4_t>(part + (int64_t)min(group, a.max_splits - 1) * D);
   const int len = i8_kv_len(table_entry(a.seq_lens + b), a.max_blocks);
   const int splits = i8_splits((len + kBlockSize - 1) / kBlockSize, a.max_splits);
   if (splits == 1) return;
-  const int64_t row = ((int64_t)b * a.heads + h) * a.max_splits;
+#pragma unroll
+  for (int i = 1; i < N; ++i)
+    if (group + i * GROUPS < splits) x[i] = ld<float4_t>(part + (int64_t)(group + i * GROUPS) * D);
   // lane i: split i's weight
-  float m = -INFINITY, l = 0.f;
-  if (lane < splits) m = a.part_ml[2 * (row + lane)], l = a.part_ml[2 * (row + lane) + 1];
+  const float m = lane < splits ? ml[0] : -INFINITY;
   float top = m;
 #pragma unroll
   for (int k = 1; k < kWave; k <<= 1) top = vmax(top, shfl_xor(top, k));
   const float f = m == -INFINITY ? 0.f : fast_exp2(m - top);
-  float sum = f * l;
+  float sum = lane < splits ? f * ml[1] : 0.f;
 #pragma unroll
   for (int k = 1; k < kWave; k <<= 1) sum += shfl_xor(sum, k);
-  const float inv = 1.f / sum;
-  for (int d0 = 0; d0 < D; d0 += kWave) {                  // every lane: each holds a weight
-    const int d = min(d0 + lane, D - 1);
-    float o = 0.f;
-    for (int i = 0; i < splits; ++i) o += a.part_o[(row + i) * D + d] * __shfl(f, i, kWave);
-    if (d0 + lane < D) a.out[b * a.out_st + (int64_t)h * D + d] = (half_t)(o * inv);
+  float4_t o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float w = __shfl(f, min(group + i * GROUPS, kWave - 1), kWave);
+    if (group + i * GROUPS < splits) o += x[i] * w;
   }
+  st<float4_t>(&s_o[group][d], o);
+  __syncthreads();
+  if (threadIdx.x >= PER_ROW) return;
+  const int most = min(splits, GROUPS);
+  for (int i = 1; i < most; ++i) o += ld<float4_t>(&s_o[i][d]);
+  st<half4_t>(a.out + b * a.out_st + (int64_t)h * D + d, to_half4(o * (1.f / sum)));
 }
 
 }  // namespace ts

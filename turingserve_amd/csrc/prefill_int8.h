@@ -204,8 +204,7 @@ __global__ void __launch_bounds__(WAVES* kWave, D >= 256 ? 1 : 2) prefill_int8_k
       float top = 0.f;
 #pragma unroll
       for (int i = 0; i < kI8Window; i += kWave) top = fmaxf(top, lds.vs[i + lane]);
-#pragma unroll
-      for (int k = 1; k < kWave; k <<= 1) top = fmaxf(top, shfl_xor(top, k));
+      top = i8_most(top);
       if (top > vref) {
         const float f = vref / top;
         vref = top;
