@@ -93,7 +93,8 @@ def paged_attention(q, codes, scales, tables, seq_lens, starts, scale: float):
 
     * the score of a token is a dot product of D terms in fp32, times two fp32 factors: off by at
       most (D + 4) 2^-24 reach; the exponent's argument and the exponential add 4 * 2^-24 * reach
-      and 2^-22; call the sum e. Weights are then off by a factor within 1 +- 2 e (numerator and
+      and 2^-22, the ratio of a block's V scale to the largest, which may pass through a base-2
+      logarithm of at most 30, another 2^-19; call the sum e. Weights are then off by a factor within 1 +- 2 e (numerator and
       sum);
     * a weight is rounded to fp16 relative to a running reference that the row's largest weight is
       never below: 2^-11 of it, or 2^-25 (half a subnormal step) of the largest V value;
@@ -109,7 +110,7 @@ def paged_attention(q, codes, scales, tables, seq_lens, starts, scale: float):
         k, v = (values(c, s, tables[b], held) for c, s in zip(codes, scales))
         seen = np.clip(np.arange(lo, hi) - lo + length - (hi - lo) + 1, 0, held)
         o, w, r = attention(q[lo:hi].astype(np.float64), k, v, seen, scale)
-        e = (D + 8) * 2.0 ** -24 * r[:, :, None] + 2.0 ** -22
+        e = (D + 8) * 2.0 ** -24 * r[:, :, None] + 2.0 ** -22 + 2.0 ** -19
         top = np.abs(v).max() if held else 0.0
         lim = ((2.0 ** -11 + 2 * e + held * 2.0 ** -23) * w + held * 2.0 ** -25 * top
                + 2.0 ** -11 * np.abs(o) + 2.0 ** -25)

@@ -3,15 +3,13 @@
 
 namespace ts {
 
-constexpr int kI8PrefillWaves = 4;
-constexpr int kI8PrefillRows = 32 * kI8PrefillWaves;
-constexpr int kI8MinSteps = 4;           // 64-token steps that a prefill split is worth
-constexpr int kI8MaxPrefillSplits = 16;
+// Wavefronts of a prefill workgroup; a CU holds one by registers.
+constexpr int i8_prefill_waves(int D) { return D > 128 ? 4 : 8; }
 
 // Launch shape and scratch of a batch, from the host's bounds.
 struct Int8Plan {
   int max_splits;                        // decode: splits of the longest sequence
-  int tiles, splits;                     // prefill: per (sequence, KV head)
+  int tiles, groups;                     // prefill: tiles of a chunk, workgroups
   size_t dec_o, dec_ml, pre_o, pre_ml;   // offsets of the partials
   size_t bytes;
 };
@@ -34,24 +32,17 @@ static Int8Plan int8_plan(int num_seqs, int num_decode, int max_query_len, int m
     pl.dec_ml = take(at, rows * 2 * sizeof(float));
   }
   const int P = num_seqs - num_decode;
-  pl.tiles = pl.splits = 1;
   if (P > 0) {
+    const int tile_rows = 32 * i8_prefill_waves(D);
     const int64_t rows = (int64_t)(max_query_len > 0 ? max_query_len : 1) * (H / KVH);
-    const int64_t tiles = (rows + kI8PrefillRows - 1) / kI8PrefillRows;
-    pl.tiles = (int)(tiles < (1 << 20) ? tiles : (1 << 20));
+    pl.tiles = (int)((rows + tile_rows - 1) / tile_rows);
     const int seq = max_prefill_seq_len > 0 ? max_prefill_seq_len : max_seq_len;
-    const int steps = (seq > 0 ? seq - 1 : 0) / kI8Keys + 1;
-    // Two workgroups fit a CU; fewer tiles than that are cut along the keys.
-    const int64_t groups = (int64_t)P * pl.tiles * KVH;
-    int64_t n = (2 * (int64_t)cus + groups - 1) / groups;
-    if (n > steps / kI8MinSteps) n = steps / kI8MinSteps;
-    if (n > kI8MaxPrefillSplits) n = kI8MaxPrefillSplits;
-    pl.splits = n < 1 ? 1 : (int)n;
-    if (pl.splits > 1) {
-      const size_t r = (size_t)groups * pl.splits * kI8PrefillRows;
-      pl.pre_o = take(at, r * D * sizeof(float));
-      pl.pre_ml = take(at, r * 2 * sizeof(float));
-    }
+    const int64_t steps = (int64_t)P * pl.tiles * KVH * ((seq > 0 ? seq - 1 : 0) / kI8Keys + 1);
+    const int64_t most = cus;
+    pl.groups = (int)(steps / kI8MinShare < most ? (steps < kI8MinShare ? 1 : steps / kI8MinShare) : most);
+    const size_t r = (size_t)2 * pl.groups * tile_rows;
+    pl.pre_o = take(at, r * D * sizeof(float));
+    pl.pre_ml = take(at, r * 2 * sizeof(float));
   }
   pl.bytes = at;
   return pl;
@@ -70,11 +61,13 @@ static int launch_decode(const Int8DecodeArgs& a, int cus, hipStream_t s) {
 }
 
 template <int D>
-static int launch_prefill(const Int8PrefillArgs& p, unsigned grid, hipStream_t s) {
-  prefill_int8_kernel<D, kI8PrefillWaves><<<grid, kI8PrefillWaves * kWave, 0, s>>>(p);
-  if (p.splits > 1) {
-    const unsigned merge = grid / p.splits * (kI8PrefillRows / (256 / (D / 4)));
-    prefill_int8_merge_kernel<D, kI8PrefillRows><<<merge, 256, 0, s>>>(p);
+static int launch_prefill(const Int8PrefillArgs& p, hipStream_t s) {
+  constexpr int WAVES = i8_prefill_waves(D), ROWS = 32 * WAVES;
+  prefill_int8_kernel<D, WAVES><<<p.groups, WAVES * kWave, 0, s>>>(p);
+  if (p.groups > 1) {
+    const unsigned merge =
+        (unsigned)((p.num_seqs - p.first) * p.tiles * p.a.kvh * (ROWS / kI8MergeRows));
+    prefill_int8_merge_kernel<D, ROWS><<<merge, 256, 0, s>>>(p);
   }
   return check_launch("paged_attention_int8");
 }
@@ -166,16 +159,17 @@ extern "C" int ts_paged_attention_int8(const void* q, int64_t q_stride_t, int64_
     p.a.part_o = reinterpret_cast<float*>(ws + pl.pre_o);
     p.a.part_ml = reinterpret_cast<float*>(ws + pl.pre_ml);
     p.qsl = query_start_loc, p.num_tokens = num_tokens;
-    p.num_seqs = num_seqs, p.first = num_decode, p.tiles = pl.tiles, p.splits = pl.splits;
-    const int64_t grid = (int64_t)(num_seqs - num_decode) * pl.tiles * num_kv_heads * pl.splits;
-    TS_REQUIRE(grid * kI8PrefillRows < (1ll << 31), TS_ERR_UNSUPPORTED,
-               "paged_attention_int8: %lld workgroups", (long long)grid);
+    p.num_seqs = num_seqs, p.first = num_decode, p.tiles = pl.tiles, p.groups = pl.groups;
+    const int64_t rows = (int64_t)(num_seqs - num_decode) * pl.tiles * 32 * i8_prefill_waves(head_dim);
+    TS_REQUIRE(rows * num_heads < (1ll << 31) && num_tokens * (num_heads / num_kv_heads) < (1ll << 31),
+               TS_ERR_UNSUPPORTED, "paged_attention_int8: %lld tokens in chunks of up to %d",
+               (long long)num_tokens, max_query_len);
     switch (head_dim) {
-      case 16: status = launch_prefill<16>(p, (unsigned)grid, s); break;
-      case 32: status = launch_prefill<32>(p, (unsigned)grid, s); break;
-      case 64: status = launch_prefill<64>(p, (unsigned)grid, s); break;
-      case 128: status = launch_prefill<128>(p, (unsigned)grid, s); break;
-      default: status = launch_prefill<256>(p, (unsigned)grid, s); break;
+      case 16: status = launch_prefill<16>(p, s); break;
+      case 32: status = launch_prefill<32>(p, s); break;
+      case 64: status = launch_prefill<64>(p, s); break;
+      case 128: status = launch_prefill<128>(p, s); break;
+      default: status = launch_prefill<256>(p, s); break;
     }
   }
   return status;
