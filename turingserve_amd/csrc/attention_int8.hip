@@ -3,9 +3,6 @@
 
 namespace ts {
 
-// Wavefronts of a prefill workgroup; a CU holds one by registers.
-constexpr int i8_prefill_waves(int D) { return D > 128 ? 4 : 8; }
-
 // Launch shape and scratch of a batch, from the host's bounds.
 struct Int8Plan {
   int max_splits;                        // decode: splits of the longest sequence
@@ -63,7 +60,7 @@ static int launch_decode(const Int8DecodeArgs& a, int cus, hipStream_t s) {
 template <int D>
 static int launch_prefill(const Int8PrefillArgs& p, hipStream_t s) {
   constexpr int WAVES = i8_prefill_waves(D), ROWS = 32 * WAVES;
-  prefill_int8_kernel<D, WAVES><<<p.groups, WAVES * kWave, 0, s>>>(p);
+  prefill_int8_kernel<D><<<p.groups, WAVES * kWave, 0, s>>>(p);
   if (p.groups > 1) {
     const unsigned merge =
         (unsigned)((p.num_seqs - p.first) * p.tiles * p.a.kvh * (ROWS / kI8MergeRows));
@@ -160,8 +157,10 @@ extern "C" int ts_paged_attention_int8(const void* q, int64_t q_stride_t, int64_
     p.a.part_ml = reinterpret_cast<float*>(ws + pl.pre_ml);
     p.qsl = query_start_loc, p.num_tokens = num_tokens;
     p.num_seqs = num_seqs, p.first = num_decode, p.tiles = pl.tiles, p.groups = pl.groups;
-    const int64_t rows = (int64_t)(num_seqs - num_decode) * pl.tiles * 32 * i8_prefill_waves(head_dim);
-    TS_REQUIRE(rows * num_heads < (1ll << 31) && num_tokens * (num_heads / num_kv_heads) < (1ll << 31),
+    // the kernels count rows and steps in 31 bits
+    const int64_t units = (int64_t)(num_seqs - num_decode) * pl.tiles * num_kv_heads;
+    TS_REQUIRE(units * (max_blocks_per_seq / kI8StepBlocks + 2) < (1ll << 31) && units * 256 < (1ll << 31) &&
+                   num_tokens * (num_heads / num_kv_heads) < (1ll << 30),
                TS_ERR_UNSUPPORTED, "paged_attention_int8: %lld tokens in chunks of up to %d",
                (long long)num_tokens, max_query_len);
     switch (head_dim) {

@@ -16,24 +16,25 @@ constexpr float kCodeMax = 127.f;
 __device__ __forceinline__ half2_t as_half2(uint32_t w) { return __builtin_bit_cast(half2_t, w); }
 
 // 1024 + u (two packed) -> the codes.
-__device__ __forceinline__ half2_t unbias(uint32_t w) {
-  const half2_t off = {(half_t)1152.f, (half_t)1152.f};
+__device__ __forceinline__ half2_t unbias(uint32_t w, half2_t off = {(half_t)1152.f, (half_t)1152.f}) {
   return as_half2(w) - off;
 }
 
 // Codes 0, 1 and 2, 3 of a word (sign bits flipped already) as packed fp16.
-__device__ __forceinline__ half2_t codes01(uint32_t u) {
-  return unbias(__builtin_amdgcn_perm(0x64646464u, u, 0x04010400u));
+__device__ __forceinline__ half2_t codes01(uint32_t u, half2_t off = {(half_t)1152.f, (half_t)1152.f}) {
+  return unbias(__builtin_amdgcn_perm(0x64646464u, u, 0x04010400u), off);
 }
-__device__ __forceinline__ half2_t codes23(uint32_t u) {
-  return unbias(__builtin_amdgcn_perm(0x64646464u, u, 0x04030402u));
+__device__ __forceinline__ half2_t codes23(uint32_t u, half2_t off = {(half_t)1152.f, (half_t)1152.f}) {
+  return unbias(__builtin_amdgcn_perm(0x64646464u, u, 0x04030402u), off);
 }
 
-// Eight consecutive codes (two words) as an MFMA operand.
-__device__ __forceinline__ half8_t codes8(uint32_t w0, uint32_t w1) {
+// Eight consecutive codes (two words) as an MFMA operand; off: 1152, or NaN for codes that mean
+// nothing.
+__device__ __forceinline__ half8_t codes8(uint32_t w0, uint32_t w1,
+                                          half2_t off = {(half_t)1152.f, (half_t)1152.f}) {
   w0 ^= 0x80808080u;
   w1 ^= 0x80808080u;
-  const half2_t a = codes01(w0), b = codes23(w0), c = codes01(w1), d = codes23(w1);
+  const half2_t a = codes01(w0, off), b = codes23(w0, off), c = codes01(w1, off), d = codes23(w1, off);
   return {a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 

@@ -77,47 +77,46 @@ struct I8PrefillLds {
   static constexpr int NV = D > 128 ? 2 : 3;               // (what fits)
   __align__(16) half_t k[2][I8Tile<D>::HALVES], v[NV][I8Tile<D>::HALVES];
   int n[kI8Kept * kWave], scan[kI8Kept * kWave];           // the walk's kept pairs
-  int blk[kI8Window];
+  int blk[kI8Window];                                      // the sign bit: a scale is not finite
   __align__(16) float fk[kI8Window + 4], vs[kI8Window];        // scale * log2 e * ks; log2(vs / vref)
   __align__(16) float back[kI8Window];                     // vref / vs
-  bool bad[kI8Window + 4];                                 // a scale is not finite
 };
 
-// Rows of one sequence's chunk.
+// Rows of one sequence's chunk. (The entry point refuses batches whose rows times heads or steps
+// pass 31 bits.)
 struct I8Chunk {
-  int64_t q0, start;                     // its first flat row, that row's position
+  int q0, start;                         // its first flat row, that row's position
   int n, kv;                             // rows, tokens in the cache
 };
 
 __device__ __forceinline__ I8Chunk i8_chunk(const Int8PrefillArgs& p, int b) {
-  const int64_t q0 = p.qsl[b], q1 = p.qsl[b + 1];
-  const int len = p.a.seq_lens[b];
+  const int q0 = p.qsl[b], q1 = p.qsl[b + 1], len = p.a.seq_lens[b];
   I8Chunk k;
   k.q0 = q0;
-  k.n = q0 < 0 || q1 <= q0 || q1 > p.num_tokens ? 0 : (int)(q1 - q0);
+  k.n = q0 < 0 || q1 <= q0 || q1 > p.num_tokens ? 0 : q1 - q0;
   k.kv = i8_kv_len(len, p.a.max_blocks);
-  k.start = (int64_t)len - k.n;
+  k.start = max(len, 0) - k.n;
   return k;
 }
 
 // Tokens that a row of a chunk sees.
-__device__ __forceinline__ int i8_sees(const I8Chunk& k, int64_t token) {
-  return (int)max((int64_t)0, min((int64_t)k.kv, k.start + token + 1));
+__device__ __forceinline__ int i8_sees(const I8Chunk& k, int token) {
+  return max(0, min(k.kv, k.start + token + 1));
 }
 
 // Steps of tile t of a chunk: one at least, so that somebody writes the rows.
 template <int ROWS>
 __device__ __forceinline__ int i8_steps(const I8Chunk& k, int group, int t) {
-  const int64_t rows = (int64_t)k.n * group;
-  if ((int64_t)t * ROWS >= rows) return 0;
-  const int sees = i8_sees(k, (int)(min(rows, (int64_t)(t + 1) * ROWS) - 1) / group);
+  const int rows = k.n * group;
+  if (t * ROWS >= rows) return 0;
+  const int sees = i8_sees(k, (min(rows, (t + 1) * ROWS) - 1) / group);
   return max(1, (sees + kI8Keys - 1) / kI8Keys);
 }
 
 // Where the batch's steps lie: pairs (sequence, tile) in order, each with all its KV heads.
 struct I8Place {
   int pair, steps;
-  int64_t before;                        // steps of the pairs before it, for one KV head
+  int before;                            // steps of the pairs before it, for one KV head
 };
 
 // The pairs' steps, a pair a lane: the first kI8Kept * 64 pairs are kept, further ones are worked out
@@ -125,7 +124,7 @@ struct I8Place {
 template <int ROWS>
 struct I8Walk {
   int n[kI8Kept], scan[kI8Kept];         // steps, and their sums from the first lane of the 64
-  int64_t total;                         // of all pairs, for one KV head
+  int total;                             // of all pairs, for one KV head
 
   static __device__ __forceinline__ int steps(const Int8PrefillArgs& p, int pair) {
     if (pair >= (p.num_seqs - p.first) * p.tiles) return 0;
@@ -162,7 +161,7 @@ struct I8Walk {
       scan[i] = ls[i * kWave + threadIdx.x % kWave];
     }
   }
-  static __device__ __forceinline__ bool in(int n, int scan, int base, int64_t sum, int64_t at, I8Place& place) {
+  static __device__ __forceinline__ bool in(int n, int scan, int base, int sum, int at, I8Place& place) {
     const uint64_t past = __ballot(sum + scan > at);
     if (!past) return false;
     const int i = __ffsll((unsigned long long)past) - 1;
@@ -172,10 +171,10 @@ struct I8Walk {
     return true;
   }
   // The pair that step `at` (below total) falls in.
-  __device__ __forceinline__ I8Place find(const Int8PrefillArgs& p, int64_t at) const {
+  __device__ __forceinline__ I8Place find(const Int8PrefillArgs& p, int at) const {
     const int lane = threadIdx.x % kWave;
     I8Place place;
-    int64_t sum = 0;
+    int sum = 0;
 #pragma unroll
     for (int i = 0; i < kI8Kept; ++i) {
       if (in(n[i], scan[i], i * kWave, sum, at, place)) return place;
@@ -188,9 +187,9 @@ struct I8Walk {
     }
   }
   // Steps of the pairs before `pair`.
-  __device__ __forceinline__ int64_t before(const Int8PrefillArgs& p, int pair) const {
+  __device__ __forceinline__ int before(const Int8PrefillArgs& p, int pair) const {
     const int lane = threadIdx.x % kWave;
-    int64_t sum = 0;
+    int sum = 0;
 #pragma unroll
     for (int i = 0; i < kI8Kept; ++i) {
       const int last = pair - 1 - i * kWave;               // lane of the last pair before it
@@ -204,10 +203,22 @@ struct I8Walk {
   }
 };
 
-// Workgroups that share `total` steps.
-__device__ __forceinline__ int64_t i8_shares(int64_t total, int groups) {
-  return max((int64_t)1, min((int64_t)groups, total / kI8MinShare));
-}
+// `total` steps shared over workgroups: share w is [begin(w), begin(w + 1)), the first `more` of
+// them one step longer.
+struct I8Shares {
+  int count, each, more;
+  __device__ __forceinline__ I8Shares(int total, int groups) {
+    count = max(1, min(groups, total / kI8MinShare));
+    each = (int)((unsigned)total / (unsigned)count);
+    more = total - each * count;
+  }
+  __device__ __forceinline__ int begin(int w) const { return w * each + min(w, more); }
+  __device__ __forceinline__ int of(int step) const {      // the share that a step belongs to
+    const int longer = more * (each + 1);
+    return step < longer ? (int)((unsigned)step / (unsigned)(each + 1))
+                         : more + (int)((unsigned)(step - longer) / (unsigned)each);
+  }
+};
 
 // The codes of a step that one thread widens: units of 16 codes of a K row, and of 4 tokens x 4
 // dims of V; 4 D of each in a step. Unit u belongs to block u / D of the step.
@@ -216,29 +227,37 @@ struct I8Stage {
   static constexpr int UNITS = 4 * D;
   static constexpr int N = (UNITS + THREADS - 1) / THREADS;
   static constexpr bool ALL = UNITS % THREADS == 0;        // every thread has N units
+  static constexpr bool UNIFORM = D >= kWave;              // a wavefront's unit lies in one block
   uint4_t k[N];
   uint32_t v[N][4];
+  half2_t off[N];                                          // what the codes of K are off by
 
   static __device__ __forceinline__ int unit(int i) { return threadIdx.x + i * THREADS; }
-  static __device__ __forceinline__ int64_t base(const Int8DecodeArgs& a, const I8PrefillLds<D>& lds, int w0,
-                                                 int last, int h, int u) {
-    return ((int64_t)lds.blk[min(w0 + u / D, last)] * a.kvh + h) * (kBlockSize * D);
+  // The ids of blocks w0 .. w0 + 3 of the window (the last real one again past the end).
+  static __device__ __forceinline__ void ids(const I8PrefillLds<D>& lds, int w0, int last, int (&id)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) id[i] = lds.blk[min(w0 + min(unit(i), UNITS - 1) / D, last)];
   }
-  // Requests blocks w0 .. w0 + 3 of the window (the last real one again past the end).
-  __device__ __forceinline__ void request_k(const Int8DecodeArgs& a, const I8PrefillLds<D>& lds, int w0,
-                                            int last, int h) {
+  static __device__ __forceinline__ int64_t base(const Int8DecodeArgs& a, int id, int h) {
+    int blk = id & 0x7fffffff;
+    if (UNIFORM) blk = __builtin_amdgcn_readfirstlane(blk);
+    return ((int64_t)blk * a.kvh + h) * (kBlockSize * D);
+  }
+  __device__ __forceinline__ void request_k(const Int8DecodeArgs& a, const int (&id)[N], int h) {
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      if (ALL || unit(i) < UNITS)
-        k[i] = ld<uint4_t>(a.kc + base(a, lds, w0, last, h, unit(i)) + 16 * (unit(i) % D));
+      if (ALL || unit(i) < UNITS) {
+        k[i] = ld<uint4_t>(a.kc + base(a, id[i], h) + 16 * (unit(i) % D));
+        const half_t o = id[i] < 0 ? (half_t)__builtin_nanf("") : (half_t)1152.f;
+        off[i] = {o, o};
+      }
   }
-  __device__ __forceinline__ void request_v(const Int8DecodeArgs& a, const I8PrefillLds<D>& lds, int w0,
-                                            int last, int h) {
+  __device__ __forceinline__ void request_v(const Int8DecodeArgs& a, const int (&id)[N], int h) {
 #pragma unroll
     for (int i = 0; i < N; ++i)
       if (ALL || unit(i) < UNITS) {
         const int in = unit(i) % D;                        // 4 tokens at 4 (in / (D / 4)), 4 dims
-        const int8_t* p = a.vc + base(a, lds, w0, last, h, unit(i)) + 4 * (in / (D / 4)) * D + 4 * (in % (D / 4));
+        const int8_t* p = a.vc + base(a, id[i], h) + (4 * (in / (D / 4)) * D + 4 * (in % (D / 4)));
 #pragma unroll
         for (int r = 0; r < 4; ++r) v[i][r] = ld<uint32_t>(p + r * D);
       }
@@ -248,8 +267,8 @@ struct I8Stage {
     for (int i = 0; i < N; ++i)
       if (ALL || unit(i) < UNITS) {
         const int key = unit(i) / (D / 16), chunk = 2 * (unit(i) % (D / 16));
-        st<half8_t>(tile + I8Tile<D>::k_at(key, chunk), codes8(k[i][0], k[i][1]));
-        st<half8_t>(tile + I8Tile<D>::k_at(key, chunk + 1), codes8(k[i][2], k[i][3]));
+        st<half8_t>(tile + I8Tile<D>::k_at(key, chunk), codes8(k[i][0], k[i][1], off[i]));
+        st<half8_t>(tile + I8Tile<D>::k_at(key, chunk + 1), codes8(k[i][2], k[i][3], off[i]));
       }
   }
   template <int q>
@@ -275,81 +294,108 @@ struct I8Stage {
   }
 };
 
-// The rows of one wavefront: q as MFMA operand, O^T, each lane's reference and partial sum, and the
-// operands' places in their tiles.
+// The 32 rows of one wavefront: q as MFMA operand, O^T, each lane's reference and partial sum, and
+// the operands' places in LDS.
 template <int D>
 struct I8Rows {
   static constexpr int DT = (D + 31) / 32;                 // output tiles of 32 dims
-  static constexpr int NQ = D / 16, NP = 2 * DT;           // MFMAs of 32 tokens: K . Q^T, V^T . P^T
-  static constexpr int ALL = 2 * NQ + 2 * NP, AHEAD = 4;   // of a step; operands requested ahead
-  half8_t q[D / 16];
+  static constexpr int NQ = D / 16, NP = 2 * DT;           // operands of 32 tokens: K, V^T
+  static constexpr int ALL = 2 * NQ + 2 * NP, AHEAD = 5;   // of a step; requested ahead
+  half8_t q[NQ];
   float16_t o[DT];
   float m, l, alpha;
   bool moved;                                              // alpha has not reached o yet
-  int kat[NQ], vat[4];
+  int kat, vat[4];                                         // (chunks of a K row: kat ^ 16 i)
 
   // Operand j of a step: V of the last step's last 32 tokens, K of the next step, V of this step's
   // first 32 tokens (block by block, so that consecutive MFMAs add to different tiles).
   __device__ __forceinline__ half8_t operand(const half_t* vp, const half_t* kn, const half_t* vc, int j) const {
     if (j < NP) return ld<half8_t>(vp + vat[2 + j / DT] + (j % DT) * 32 * kI8Keys);
     j -= NP;
-    if (j < 2 * NQ) return ld<half8_t>(kn + kat[j % NQ] + (j / NQ) * 32 * D);
+    if (j < 2 * NQ) return ld<half8_t>(kn + (kat ^ 16 * (j % NQ)) + (j / NQ) * 32 * D);
     j -= 2 * NQ;
     return ld<half8_t>(vc + vat[j / DT] + (j % DT) * 32 * kI8Keys);
   }
 };
-
-// Scores j * 16 / N .. of one 32-token tile to P' (blocks `blk`, `blk` + 1) and the row's sum.
-template <int N>
-__device__ __forceinline__ void i8_exp(float& l, const float16_t& s, int j, float fk0, float fk1, float off0,
-                                       float off1, float back0, float back1, float& sum, half8_t& p0,
-                                       half8_t& p1) {
-#pragma unroll
-  for (int e = j * 16 / N; e < (j + 1) * 16 / N; ++e) {
-    const float x = fast_exp2(fmaf(s[e], e < 8 ? fk0 : fk1, e < 8 ? off0 : off1));
-    sum = e % 8 == 0 ? x : sum + x;
-    if (e < 8) p0[e] = (half_t)x; else p1[e - 8] = (half_t)x;
-    if (e % 8 == 7) l = fmaf(sum, e < 8 ? back0 : back1, l);
-  }
-}
 
 // Keeps a value's computation where it stands: without it the exponentials sink past the MFMAs they
 // are meant to run beside, down to the block that uses them.
 template <typename T>
 __device__ __forceinline__ void i8_pin(T& v) { asm volatile("" : "+v"(v)); }
 
+// The exponentials of a step's 32 scores per lane, a few at a time: P' in fp16 and the row's sum. In
+// call j of N, the products of the j-th share are formed, the exponentials of the share before it
+// taken, and the share before that summed and rounded, so that nothing waits for the result in
+// front of it. Calls N and N + 1 finish.
+struct I8Exp {
+  float t[32], x[32], sum[4][2];
+  template <int N>
+  __device__ __forceinline__ void share(int j, const float16_t (&s)[2], const float4_t& fk, const float (&off)[4],
+                                        const float4_t& back, float& l, half8_t (&p)[4]) {
+    constexpr int PER = 32 / N;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int e = (j - 2) * PER + i, b = e / 8;          // summed
+      if (e < 0 || e >= 32) continue;
+      sum[b][e % 2] = e % 8 < 2 ? x[e] : sum[b][e % 2] + x[e];
+      i8_pin(sum[b][e % 2]);
+      p[b][e % 8] = (half_t)x[e];
+      if (e % 8 == 7) {
+        l = fmaf(sum[b][0] + sum[b][1], back[b], l);
+        i8_pin(l), i8_pin(p[b]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int e = (j - 1) * PER + i;
+      if (e >= 0 && e < 32) x[e] = fast_exp2(t[e]), i8_pin(x[e]);
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int e = j * PER + i;
+      if (e < 32) t[e] = fmaf(s[e / 16][e % 16], fk[e / 8], off[e / 8]), i8_pin(t[e]);
+    }
+  }
+};
+
 // One step of a wavefront. Its scores stand in sc (tokens 0-31, 32-63), P' of the last step's
-// second half in pr[2], pr[3]; the next step's scores replace them. Four phases, each a run of MFMAs beside a share of the vector work:
+// second half in pr[2], pr[3]; the next step's scores replace them. Four phases, each a run of MFMAs
+// beside a share of the vector work:
 //   P'(sc[0])  beside  O += V P' of the last step's second half
 //   P'(sc[1])  beside  sc[0] = K . Q^T of the next step
 //   staging    beside  sc[1] = K . Q^T of the next step
 //   maxima of the next scores  beside  O += V P' of this step's first half
-// so that no second set of scores is needed (the registers of two wavefronts a SIMD). The order is
+// so that no second set of scores is needed (two wavefronts share a SIMD's registers). The order is
 // pinned, MFMA by MFMA: left to itself the compiler sets MFMAs and exponentials one after the other.
-// Returns the row's largest next score.
+// The workgroup meets behind the third phase: what the fourth reads is written two steps later.
+// Returns each row's largest next score.
 template <int D, typename Mask, typename Work>
 __device__ __forceinline__ float i8_step64(I8Rows<D>& w, const half_t* vp, const half_t* kn, const half_t* vc,
                                            float16_t (&sc)[2], half8_t (&pr)[4], const float* fkp,
-                                           const float* fvp, const float* backp, Mask mask, Work work) {
+                                           const float* fvp, const float* backp, const float* fknp, Mask mask,
+                                           Work work) {
   typedef I8Rows<D> R;
   constexpr int NQ = R::NQ, NP = R::NP, AHEAD = R::AHEAD;
   half8_t op[AHEAD];
+  const float4_t fk = ld<float4_t>(fkp), fv = ld<float4_t>(fvp);
 #pragma unroll
   for (int j = 0; j < AHEAD; ++j) op[j] = w.operand(vp, kn, vc, j);
+  const float4_t back = ld<float4_t>(backp);
   auto next = [&](int j) {                                 // operand j, and the request of a later one
     const half8_t x = op[j % AHEAD];
     if (j + AHEAD < R::ALL) op[j % AHEAD] = w.operand(vp, kn, vc, j + AHEAD);
     return x;
   };
-  const float4_t fk = ld<float4_t>(fkp), fv = ld<float4_t>(fvp), back = ld<float4_t>(backp);
   const float neg = w.m == -INFINITY ? 0.f : -w.m;
-  const float off0 = neg + fv[0], off1 = neg + fv[1], off2 = neg + fv[2], off3 = neg + fv[3];
-  float sum;
+  const float off[4] = {neg + fv[0], neg + fv[1], neg + fv[2], neg + fv[3]};
+  work(0);                                                 // global requests
+  // exponentials: NP + NQ shares beside the first two phases' MFMAs where both have as many
+  constexpr int N = 2 * (NP < NQ ? NP : NQ);
+  I8Exp ex;
 #pragma unroll
   for (int j = 0; j < NP; ++j) {
     w.o[j % R::DT] = mfma_i8(next(j), pr[2 + j / R::DT], w.o[j % R::DT]);
-    i8_exp<NP>(w.l, sc[0], j, fk[0], fk[1], off0, off1, back[0], back[1], sum, pr[0], pr[1]);
-    if (j == NP - 1) i8_pin(pr[0]), i8_pin(pr[1]), i8_pin(w.l);
+    if (j < N / 2) ex.share<N>(j, sc, fk, off, back, w.l, pr);
     __builtin_amdgcn_sched_barrier(0);
   }
   if (w.moved) {
@@ -363,28 +409,33 @@ __device__ __forceinline__ float i8_step64(I8Rows<D>& w, const half_t* vp, const
 #pragma unroll
   for (int j = 0; j < NQ; ++j) {
     sc[0] = mfma_i8(next(NP + j), w.q[j], j == 0 ? zero : sc[0]);
-    i8_exp<NQ>(w.l, sc[1], j, fk[2], fk[3], off2, off3, back[2], back[3], sum, pr[2], pr[3]);
-    if (j == NQ - 1) i8_pin(pr[2]), i8_pin(pr[3]), i8_pin(w.l);
+    if (j < N / 2) ex.share<N>(N / 2 + j, sc, fk, off, back, w.l, pr);
     __builtin_amdgcn_sched_barrier(0);
   }
 #pragma unroll
   for (int j = 0; j < NQ; ++j) {
     sc[1] = mfma_i8(next(NP + NQ + j), w.q[j], j == 0 ? zero : sc[1]);
-    if (j == 0) work(0);
-    if (j == NQ / 2) work(1);
+    if (j < 2) ex.share<N>(N + j, sc, fk, off, back, w.l, pr);
+    if (NQ < 2) ex.share<N>(N + 1, sc, fk, off, back, w.l, pr);
+    if (j == NQ / 4) work(1);                              // K of a later step to LDS
+    if (j == NQ / 2) work(2);                              // V
     __builtin_amdgcn_sched_barrier(0);
   }
+  const float4_t fkn = ld<float4_t>(fknp);
   mask(sc);
+  __syncthreads();
   float top[4];
 #pragma unroll
   for (int j = 0; j < NP; ++j) {
     w.o[j % R::DT] = mfma_i8(next(NP + 2 * NQ + j), pr[j / R::DT], w.o[j % R::DT]);
 #pragma unroll
-    for (int e = j * 32 / NP; e < (j + 1) * 32 / NP; ++e)
-      top[e / 8] = e % 8 == 0 ? sc[e / 16][e % 16] : vmax(top[e / 8], sc[e / 16][e % 16]);
+    for (int i = j * 32 / NP; i < (j + 1) * 32 / NP; ++i) {
+      const int b = i / 2 % 4, e = i / 8 * 2 + i % 2;      // two scores of each block in turn
+      const float x = sc[b / 2][8 * (b % 2) + e];
+      top[b] = e == 0 ? x : vmax(top[b], x);
+    }
     __builtin_amdgcn_sched_barrier(0);
   }
-  const float4_t fkn = ld<float4_t>(fkp + 4);
   return vmax(vmax(top[0] * fkn[0], top[1] * fkn[1]), vmax(top[2] * fkn[2], top[3] * fkn[3]));
 }
 
@@ -406,29 +457,25 @@ __device__ __forceinline__ void i8_reference(I8Rows<D>& w, float best) {
 // One tile's steps [s0, s1) by the workgroup.
 template <int D, int WAVES>
 __device__ __forceinline__ void i8_piece(const Int8PrefillArgs& p, I8PrefillLds<D>& lds, const I8Chunk& k,
-                                         int b, int tile, int h, int s0, int s1, bool whole, int64_t slot) {
-  constexpr int THREADS = WAVES * kWave, ROWS = 32 * WAVES;
-  constexpr int DT = (D + 31) / 32;                        // output tiles of 32 dims
+                                         int b, int tile, int h, int s0, int s1, bool whole, int slot) {
+  typedef I8Rows<D> R;
+  typedef I8Stage<D, WAVES * kWave> S;
+  constexpr int DT = R::DT, THREADS = WAVES * kWave, ROWS = 32 * WAVES, NV = I8PrefillLds<D>::NV;
   const Int8DecodeArgs& a = p.a;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int lane = threadIdx.x % kWave, c = lane % 32, hh = lane / 32;
-  const int64_t rows = (int64_t)k.n * a.group, wrow = (int64_t)tile * ROWS + 32 * wave, row = wrow + c;
-  const bool real = row < rows;
-  const int token = real ? (int)row / a.group : 0;
-  const int head = h * a.group + (real ? (int)row % a.group : 0);
-  const int vis = real ? i8_sees(k, token) : 0;
+  const int rows = k.n * a.group, wrow = tile * ROWS + 32 * wave;
+  const int row = min(wrow + c, rows - 1);                 // (rows past the last one stand in for it)
+  const int token = row / a.group, head = h * a.group + row % a.group, vis = i8_sees(k, token);
   // rows ascend in tokens: the wavefront's first row sees least
-  const int least = wrow < rows ? i8_sees(k, (int)wrow / a.group) : 0;
-  const int sees = i8_sees(k, (int)(min(rows, (int64_t)(tile + 1) * ROWS) - 1) / a.group);
+  const int least = i8_sees(k, min(wrow, rows - 1) / a.group);
+  const int sees = i8_sees(k, (min(rows, (tile + 1) * ROWS) - 1) / a.group);
   const int nb = (sees + kBlockSize - 1) / kBlockSize;     // blocks that the tile sees
-
-  I8Rows<D> w;
-  const half_t* qrow = a.q + (k.q0 + token) * a.q_st + (int64_t)head * a.q_sh;
+  R w;
+  const half_t* qrow = a.q + (int64_t)(k.q0 + token) * a.q_st + (int64_t)head * a.q_sh;
 #pragma unroll
-  for (int i = 0; i < D / 16; ++i) {
-    w.q[i] = ld<half8_t>(qrow + 16 * i + 8 * hh);
-    w.kat[i] = I8Tile<D>::k_at(c, 2 * i + hh);
-  }
+  for (int i = 0; i < D / 16; ++i) w.q[i] = ld<half8_t>(qrow + 16 * i + 8 * hh);
+  w.kat = I8Tile<D>::k_at(c, hh);
 #pragma unroll
   for (int i = 0; i < 4; ++i) w.vat[i] = I8Tile<D>::v_at(D < 32 ? c % D : c, i, hh);
 #pragma unroll
@@ -438,56 +485,42 @@ __device__ __forceinline__ void i8_piece(const Int8PrefillArgs& p, I8PrefillLds<
   w.m = -INFINITY, w.l = 0.f, w.alpha = 1.f, w.moved = false;
   float vref = 0.f;
 
-  I8Stage<D, THREADS> stage;
   s1 = min(s1, (nb + kI8StepBlocks - 1) / kI8StepBlocks);  // (nothing visible: no step)
   for (int w0 = s0; w0 < s1; w0 += kI8Window / kI8StepBlocks) {
     // a window of the sequence's blocks: ids, scales
     const int n = min(s1 - w0, kI8Window / kI8StepBlocks);
     const int blocks = min(nb - w0 * kI8StepBlocks, n * kI8StepBlocks), last = blocks - 1;
     __syncthreads();                                       // the last window's and piece's reads
-    constexpr int PER = (kI8Window + THREADS - 1) / THREADS;
-    int blk[PER];
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int at = threadIdx.x + i * THREADS;
-      blk[i] = at < blocks ? clamp_block(a.block_tables[b * a.bt_stride + w0 * kI8StepBlocks + at], a.num_blocks) : 0;
-      if (at < kI8Window) lds.blk[at] = blk[i];
-    }
-    __syncthreads();
-    float ks[PER], vs[PER];
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const bool there = threadIdx.x + i * THREADS < blocks;
-      ks[i] = there ? a.ks[(int64_t)blk[i] * a.kvh + h] : 0.f;
-      vs[i] = there ? a.vs[(int64_t)blk[i] * a.kvh + h] : 0.f;
-    }
-    I8Stage<D, THREADS> early;                             // K of the window's second step
-    stage.request_k(a, lds, 0, last, h);
-    early.request_k(a, lds, kI8StepBlocks, last, h);
-    stage.request_v(a, lds, 0, last, h);
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int at = threadIdx.x + i * THREADS;
-      i8_poison(ks[i], vs[i]);
-      // A K factor of 0 or NaN would leave hidden tokens (-inf) NaN: scores of a factor as small as
-      // the least one are 0, and those of blocks without finite scales become NaN in the mask.
-      const float f = ks[i] * a.sl2;
-      if (at < kI8Window) {
-        lds.fk[at] = f > kI8LeastFactor ? f : kI8LeastFactor;
-        lds.vs[at] = vs[i];
-        lds.bad[at] = f != f;
+    for (int i = threadIdx.x; i < kI8Window; i += THREADS) {
+      int blk = 0;
+      float ks = 0.f, vs = 0.f;
+      if (i < blocks) {
+        blk = clamp_block(a.block_tables[b * a.bt_stride + w0 * kI8StepBlocks + i], a.num_blocks);
+        ks = a.ks[(int64_t)blk * a.kvh + h];
+        vs = a.vs[(int64_t)blk * a.kvh + h];
+        i8_poison(ks, vs);
       }
+      // A K factor of 0 or NaN would leave hidden tokens (-inf) NaN: scores of a factor as small as
+      // the least one are 0, and the codes of blocks without finite scales are staged as NaN.
+      const float f = ks * a.sl2;
+      lds.blk[i] = f == f ? blk : blk | (int)0x80000000;
+      lds.fk[i] = f > kI8LeastFactor ? f : kI8LeastFactor;
+      lds.vs[i] = vs;
     }
     __syncthreads();
+    // K of step i + 2 and V of step i + 1 are requested in step i - 1 and go to LDS in step i.
+    S now, later;
+    int id[S::N], idv[S::N];
+    S::ids(lds, 0, last, idv);
+    now.request_k(a, idv, h);
+    later.request_v(a, idv, h);
+    S::ids(lds, kI8StepBlocks, last, idv);
+    later.request_k(a, idv, h);
+    S::ids(lds, 2 * kI8StepBlocks, last, id);
     float top = 0.f;
-    bool some = false;
 #pragma unroll
-    for (int i = 0; i < kI8Window; i += kWave) {
-      top = fmaxf(top, lds.vs[i + lane]);
-      some = some || lds.bad[i + lane];
-    }
+    for (int i = 0; i < kI8Window; i += kWave) top = fmaxf(top, lds.vs[i + lane]);
     top = i8_most(top);
-    const bool bad = __ballot(some) != 0;
     if (top > vref) {
       const float f = vref / top;
       vref = top;
@@ -500,73 +533,57 @@ __device__ __forceinline__ void i8_piece(const Int8PrefillArgs& p, I8PrefillLds<
       lds.vs[i] = f;
       lds.back[i] = fast_exp2(-f);
     }
-    stage.place_k(lds.k[0]);
-    early.place_k(lds.k[1]);
-    stage.place_v(lds.v[0]);
+    now.place_k(lds.k[0]);
+    for (int i = threadIdx.x; i < I8Tile<D>::HALVES / 8; i += THREADS)
+      st<half8_t>(lds.v[1] + 8 * i, half8_t{0, 0, 0, 0, 0, 0, 0, 0});
     __syncthreads();
 
-    // Step i reads K of step i + 1 in k[(i + 1) % 2] and V of steps i - 1 and i in two of three
-    // tiles; meanwhile K of step i + 2 and V of step i + 1 go to tiles whose last readers were in
-    // step i - 1.
-    auto mask = [&](float16_t (&x)[2], int step) {
-      if (bad || (step + 1) * kI8Keys > least) {
-        const int key0 = step * kI8Keys + 4 * hh;
+    // Step i reads K of step i + 1 in k[(i + 1) % 2] and V of steps i - 1 and i; meanwhile K of step
+    // i + 2 and V of step i + 1 go to tiles whose last readers were in step i - 1. The first of them,
+    // step -1, has hidden scores only (and V codes of 0): it is there for the scores
+    // of step 0. The loop has no branch but the mask's and the reference's: past the window's end
+    // the last blocks are staged again, and the scores of the step behind it are not used.
+    float16_t sc[2];
+    half8_t pr[4];
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
+    for (int i = 0; i < 16; ++i) sc[0][i] = sc[1][i] = -INFINITY;
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            x[kt][i] = key0 + 32 * kt + 8 * (i / 4) + i % 4 < vis ? x[kt][i] : -INFINITY;
-        if (bad)
+    for (int e = 0; e < 8; ++e) pr[2][e] = pr[3][e] = (half_t)0.f;
+    int v0 = 1, v1 = 0, v2 = NV - 1;                       // V of this step, the next, the last one
+    for (int i = -1; i < n; ++i) {
+      auto work = [&](int part) {
+        if (part == 0) {                                   // (idv: of step i + 2, id: of step i + 3)
+          now = later;
+          later.request_v(a, idv, h);
+          later.request_k(a, id, h);
+#pragma unroll
+          for (int e = 0; e < S::N; ++e) idv[e] = id[e];
+          S::ids(lds, (i + 4) * kI8StepBlocks, last, id);
+        }
+        if (part == 1) now.place_k(lds.k[i & 1]);
+        if (part == 2) now.place_v(lds.v[v1]);
+      };
+      auto mask = [&](float16_t (&x)[2]) {
+        const int step = w0 + i + 1;
+        if ((step + 1) * kI8Keys > least) {
+          const int key0 = step * kI8Keys + 4 * hh;
 #pragma unroll
           for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-              if (lds.bad[(step - w0) * kI8StepBlocks + 2 * kt + i / 8] && x[kt][i] != -INFINITY)
-                x[kt][i] = __builtin_nanf("");
-      }
-    };
-    float16_t sc[2];
-    half8_t pr[4];
-    {
-      constexpr int NQ = I8Rows<D>::NQ;
-      float16_t zero;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) zero[i] = 0.f;
-#pragma unroll
-      for (int j = 0; j < 2 * NQ; ++j)
-        sc[j / NQ] = mfma_i8(ld<half8_t>(lds.k[0] + w.kat[j % NQ] + j / NQ * 32 * D), w.q[j % NQ],
-                             j % NQ == 0 ? zero : sc[j / NQ]);
-      mask(sc, w0);
-      const float4_t fk = ld<float4_t>(lds.fk);
-      float t[4];
-#pragma unroll
-      for (int e = 0; e < 32; ++e) t[e / 8] = e % 8 == 0 ? sc[e / 16][e % 16] : vmax(t[e / 8], sc[e / 16][e % 16]);
-      i8_reference<D>(w, vmax(vmax(t[0] * fk[0], t[1] * fk[1]), vmax(t[2] * fk[2], t[3] * fk[3])));
-      // no step before the first: its P' is 0, beside finite codes
-#pragma unroll
-      for (int e = 0; e < 8; ++e) pr[2][e] = pr[3][e] = (half_t)0.f;
-    }
-    // The loop has no branch but the mask's and the reference's: past the window's end the last
-    // blocks are staged again, and the scores of the step behind it are computed and not used.
-    constexpr int NV = I8PrefillLds<D>::NV;
-    int v0 = 0, v1 = 1, v2 = NV - 1;                       // V of this step, the next, the last one
-    for (int i = 0; i < n; ++i) {
-      stage.request_k(a, lds, (i + 2) * kI8StepBlocks, last, h);
-      stage.request_v(a, lds, (i + 1) * kI8StepBlocks, last, h);
-      auto work = [&](int part) {
-        if (part == 0) stage.place_k(lds.k[i & 1]); else stage.place_v(lds.v[v1]);
+            for (int e = 0; e < 16; ++e)
+              x[kt][e] = key0 + 32 * kt + 8 * (e / 4) + e % 4 < vis ? x[kt][e] : -INFINITY;
+        }
       };
-      auto masked = [&](float16_t (&x)[2]) { mask(x, w0 + i + 1); };
-      const int wb = i * kI8StepBlocks;
-      const float best = i8_step64<D>(w, lds.v[i == 0 ? v0 : v2], lds.k[(i + 1) & 1], lds.v[v0], sc, pr,
-                                      lds.fk + wb, lds.vs + wb, lds.back + wb, masked, work);
+      const int wb = max(i, 0) * kI8StepBlocks;
+      const half_t *vc = lds.v[v0], *vp = lds.v[i < 0 ? v0 : v2];
+      const float best = i8_step64<D>(w, vp, lds.k[(i + 1) & 1], vc, sc, pr, lds.fk + wb, lds.vs + wb,
+                                      lds.back + wb, lds.fk + (i + 1) * kI8StepBlocks, mask, work);
       i8_reference<D>(w, i + 1 < n ? best : w.m);          // (its own reference moves none, also a NaN)
-      __syncthreads();
       const int v = v2;
       v2 = v0, v0 = v1, v1 = NV == 2 ? v2 : v;
     }
 #pragma unroll
-    for (int j = 0; j < I8Rows<D>::NP; ++j)                // the last step's second half
+    for (int j = 0; j < R::NP; ++j)                        // the last step's second half
       w.o[j % DT] = mfma_i8(ld<half8_t>(lds.v[v2] + w.vat[2 + j / DT] + j % DT * 32 * kI8Keys), pr[2 + j / DT],
                             w.o[j % DT]);
   }
@@ -574,44 +591,42 @@ __device__ __forceinline__ void i8_piece(const Int8PrefillArgs& p, I8PrefillLds<
   // lanes c and c + 32 hold the two halves of row c's sum
   const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(w.l), __float_as_uint(w.l), false, false);
   const float l = __uint_as_float(both[0]) + __uint_as_float(both[1]);
-  if (!real) return;
-  if (whole) {
-    const float f = l == 0.f ? 0.f : vref / l;             // nothing visible: zeros
-    half_t* dst = a.out + (k.q0 + token) * a.out_st + (int64_t)head * D;
+  if (wrow + c >= rows) return;
+  const int64_t at = (int64_t)slot * ROWS + 32 * wave + c;
+  if (!whole && hh == 0) st<float2_t>(a.part_ml + 2 * at, float2_t{w.m, l});
+  const float f = !whole ? vref : l == 0.f ? 0.f : vref / l;   // nothing visible: zeros
+  half_t* dst = a.out + (int64_t)(k.q0 + token) * a.out_st + (int64_t)head * D;
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
+  for (int t = 0; t < DT; ++t)
 #pragma unroll
-      for (int i = 0; i < 16; i += 4) {
-        const int d = 32 * dt + 8 * (i / 4) + 4 * hh;
-        if (D < 32 && d >= D) break;
-        st<half4_t>(dst + d, to_half4(float4_t{w.o[dt][i], w.o[dt][i + 1], w.o[dt][i + 2], w.o[dt][i + 3]} * f));
-      }
-  } else {
-    const int64_t at = slot * ROWS + 32 * wave + c;
-    if (hh == 0) st<float2_t>(a.part_ml + 2 * at, float2_t{w.m, l});
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-      for (int i = 0; i < 16; i += 4) {
-        const int d = 32 * dt + 8 * (i / 4) + 4 * hh;
-        if (D < 32 && d >= D) break;
-        st<float4_t>(a.part_o + at * D + d,
-                     float4_t{w.o[dt][i], w.o[dt][i + 1], w.o[dt][i + 2], w.o[dt][i + 3]} * vref);
-      }
-  }
+    for (int i = 0; i < 16; i += 4) {
+      const int d = 32 * t + 8 * (i / 4) + 4 * hh;
+      if (D < 32 && d >= D) break;
+      const float4_t x = float4_t{w.o[t][i], w.o[t][i + 1], w.o[t][i + 2], w.o[t][i + 3]} * f;
+      if (whole)
+        st<half4_t>(dst + d, to_half4(x));
+      else
+        st<float4_t>(a.part_o + at * D + d, x);
+    }
 }
 
-template <int D, int WAVES>
-__global__ void __launch_bounds__(WAVES* kWave, D >= 256 ? 1 : 2) prefill_int8_kernel(Int8PrefillArgs p) {
-  constexpr int ROWS = 32 * WAVES;
+// Wavefronts of a workgroup; a CU holds one by registers.
+constexpr int i8_prefill_waves(int D) { return D > 128 ? 4 : 8; }
+
+template <int D>
+__global__ void __launch_bounds__(i8_prefill_waves(D) * kWave, D > 128 ? 1 : 2)
+prefill_int8_kernel(Int8PrefillArgs p) {
+  constexpr int WAVES = i8_prefill_waves(D), ROWS = 32 * WAVES;
   __shared__ __align__(16) I8PrefillLds<D> lds;
   const Int8DecodeArgs& a = p.a;
-  int64_t at, hi;
+  int at, hi;
   {
     const I8Walk<ROWS> walk(p);
-    const int64_t total = walk.total * a.kvh, shares = i8_shares(total, p.groups);
-    if (blockIdx.x >= shares || total == 0) return;
-    at = total * blockIdx.x / shares, hi = total * (blockIdx.x + 1) / shares;
+    const int total = walk.total * a.kvh;
+    if (total == 0) return;
+    const I8Shares shares(total, p.groups);
+    if ((int)blockIdx.x >= shares.count) return;
+    at = shares.begin(blockIdx.x), hi = shares.begin(blockIdx.x + 1);
     if (threadIdx.x < kWave) walk.save(lds.n, lds.scan);
     __syncthreads();
   }
@@ -619,18 +634,17 @@ __global__ void __launch_bounds__(WAVES* kWave, D >= 256 ? 1 : 2) prefill_int8_k
   for (bool extra = false; extra || at < hi;) {
     int s0 = 0, s1, steps;
     if (!extra) {
-      const I8Place place = I8Walk<ROWS>(lds.n, lds.scan).find(p, at / a.kvh);
-      const int64_t in = at - place.before * a.kvh;
+      const I8Place place = I8Walk<ROWS>(lds.n, lds.scan).find(p, (int)((unsigned)at / (unsigned)a.kvh));
+      const unsigned in = at - place.before * a.kvh;
       steps = place.steps;
-      h = (int)(in / steps), s0 = (int)(in % steps);
-      s1 = (int)min((int64_t)steps, s0 + (hi - at));
+      h = (int)(in / (unsigned)steps), s0 = (int)(in % (unsigned)steps);
+      s1 = min(steps, s0 + (hi - at));
       b = p.first + place.pair / p.tiles, tile = place.pair % p.tiles;
       at += s1 - s0;
     }
     const I8Chunk k = i8_chunk(p, b);
     if (extra) s1 = steps = i8_steps<ROWS>(k, a.group, tile);
-    i8_piece<D, WAVES>(p, lds, k, b, tile, h, s0, s1, s0 == 0 && s1 == steps,
-                       2 * (int64_t)blockIdx.x + (s0 == 0));
+    i8_piece<D, WAVES>(p, lds, k, b, tile, h, s0, s1, s0 == 0 && s1 == steps, 2 * blockIdx.x + (s0 == 0));
     // Tiles past the host's bound on the rows follow, whole, the first step of the last tile that it
     // allows for.
     extra = (extra || (tile == p.tiles - 1 && s0 == 0)) && i8_steps<ROWS>(k, a.group, tile + 1) > 0;
@@ -644,32 +658,31 @@ template <int D, int ROWS>
 __global__ void __launch_bounds__(256) prefill_int8_merge_kernel(Int8PrefillArgs p) {
   constexpr int PER = 256 / (D / 4), N = 4;                // rows at a time, partials requested at once
   const Int8DecodeArgs& a = p.a;
-  const int64_t unit = blockIdx.x / (ROWS / kI8MergeRows);
+  const int unit = blockIdx.x / (ROWS / kI8MergeRows);
   const int row0 = (int)(blockIdx.x % (ROWS / kI8MergeRows)) * kI8MergeRows;
-  const int h = (int)(unit % a.kvh), pair = (int)(unit / a.kvh);
+  const int h = unit % a.kvh, pair = unit / a.kvh;
   const int b = p.first + pair / p.tiles, tile = pair % p.tiles;
   const I8Chunk k = i8_chunk(p, b);
-  const int64_t rows = (int64_t)k.n * a.group;
-  if ((int64_t)tile * ROWS + row0 >= rows) return;
+  const int rows = k.n * a.group;
+  if (tile * ROWS + row0 >= rows) return;
   const I8Walk<ROWS> walk(p);
   const int steps = i8_steps<ROWS>(k, a.group, tile);
-  const int64_t total = walk.total * a.kvh, shares = i8_shares(total, p.groups);
-  const int64_t g0 = walk.before(p, pair) * a.kvh + (int64_t)h * steps, g1 = g0 + steps;
-  // share w begins at total * w / shares: the last one that begins at or before a step
-  const int64_t first = ((g0 + 1) * shares - 1) / total, last = (g1 * shares - 1) / total;
+  const I8Shares shares(walk.total * a.kvh, p.groups);
+  const int g0 = walk.before(p, pair) * a.kvh + h * steps;
+  const int first = shares.of(g0), last = shares.of(g0 + steps - 1);
   if (first == last) return;                               // one workgroup wrote it
   const int d = threadIdx.x % (D / 4) * 4;
   for (int in = row0 + threadIdx.x / (D / 4); in < row0 + kI8MergeRows; in += PER) {
-    const int64_t row = (int64_t)tile * ROWS + in;
+    const int row = tile * ROWS + in;
     if (row >= rows) return;
     float top = -INFINITY, sum = 0.f;
     float4_t o = {0.f, 0.f, 0.f, 0.f};
-    for (int64_t i0 = first; i0 <= last; i0 += N) {
+    for (int i0 = first; i0 <= last; i0 += N) {
       float2_t ml[N];
       float4_t x[N];
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const int64_t at = (2 * min(i0 + i, last) + (i0 + i == first)) * ROWS + in;
+        const int64_t at = (int64_t)(2 * min(i0 + i, last) + (i0 + i == first)) * ROWS + in;
         ml[i] = ld<float2_t>(a.part_ml + 2 * at);
         x[i] = ld<float4_t>(a.part_o + at * D + d);
       }
@@ -689,8 +702,8 @@ __global__ void __launch_bounds__(256) prefill_int8_merge_kernel(Int8PrefillArgs
       }
     }
     const float f = sum == 0.f ? 0.f : 1.f / sum;
-    const int token = (int)row / a.group, head = h * a.group + (int)row % a.group;
-    st<half4_t>(a.out + (k.q0 + token) * a.out_st + (int64_t)head * D + d, to_half4(o * f));
+    const int token = row / a.group, head = h * a.group + row % a.group;
+    st<half4_t>(a.out + (int64_t)(k.q0 + token) * a.out_st + (int64_t)head * D + d, to_half4(o * f));
   }
 }
 
