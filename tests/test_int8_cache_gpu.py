@@ -299,6 +299,44 @@ def test_prefill_matches_the_oracle(heads):
         assert_rows(H.paged_attention_int8(q, *cache, m, c.scale), c, f"prefill {heads} {bounds}")
 
 
+VERIFY = [(0, 5), (1, 5), (12, 3), (300, 5), (2047, 4), (9, 1), (255, 2), (5000, 5), (4094, 5)]
+
+
+@pytest.mark.parametrize("heads", HEADS)
+def test_a_few_rows_per_sequence(heads):
+    """The rows of a speculative step: up to five a sequence, beside decode rows."""
+    c = Case(heads, [(100, 1), (0, 1)] + VERIFY, num_decode=2, seed=30)
+    c.lens[3] = 3                                    # five rows, three positions
+    _, q, _, _, cache, meta = c.on(DEV)
+    out = H.paged_attention_int8(q, *cache, meta, c.scale)
+    assert_rows(out, c, f"verify {heads}")
+    assert not out[int(c.starts[3]):int(c.starts[3]) + 2].any()
+    for bounds in (dict(max_query_len=2), dict(max_seq_len=100, max_prefill_seq_len=0),
+                   dict(max_query_len=200), dict(num_decode=0)):
+        m = dataclasses.replace(meta, **bounds)
+        assert_rows(H.paged_attention_int8(q, *cache, m, c.scale), c, f"verify {heads} {bounds}")
+
+
+@pytest.mark.parametrize("side", [0, 1])
+def test_a_few_rows_around_a_block_without_a_finite_scale(side):
+    """Rows before the block are right, rows that see it NaN, also where later blocks are hidden."""
+    c = Case((14, 2, 64), [(317, 40), (30, 36)], seed=31)
+    c.scales[side, c.tables[0, 20], 1] = np.nan      # tokens 320 .. 335
+    c.scales[side, c.tables[1, 3], 1] = np.nan       # tokens 48 .. 63
+    _, q, _, _, cache, meta = c.on(DEV)
+    clean = np.nan_to_num(c.scales, nan=0.0)
+    hit = np.zeros((c.T, c.H), bool)
+    hit[3:40, 7:] = True                             # positions 320 and later of the first
+    hit[40 + 18:, 7:] = True                         # 48 and later of the second
+    for bound in (40, 4):                            # the chunk kernel; tiles of 16 rows, unsplit
+        out = H.paged_attention_int8(q, *cache, dataclasses.replace(meta, max_query_len=bound), c.scale)
+        got = out.cpu().numpy().reshape(c.T, c.H, c.D)
+        assert np.isnan(got[hit]).all() and np.isfinite(got[~hit]).all(), bound
+        ref, lim = O.paged_attention(c.split()[0], c.codes, clean, c.tables, c.lens, c.starts, c.scale)
+        ok = ~np.repeat(hit, c.D, axis=1).reshape(c.T, -1)
+        assert (np.abs(out.double().cpu().numpy() - ref) <= lim)[ok].all(), bound
+
+
 @pytest.mark.parametrize("heads", [(12, 2, 128), (14, 2, 64)])
 def test_prefill_over_a_long_prefix(heads):
     """More blocks than are looked up at once, and split along the keys."""

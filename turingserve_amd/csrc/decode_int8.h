@@ -1,10 +1,12 @@
-// Decode attention over the 8-bit paged cache: one query row per sequence.
+// Attention of one or a few query rows per sequence over the 8-bit paged cache (decode rows, the
+// rows of a speculative step).
 //
 //   s_j = scale * ks[blk(j)] * (q . code_k[j]),  out = sum_j softmax(s)_j * vs[blk(j)] * code_v[j]
 //
-// One workgroup of four wavefronts takes one split of one sequence's blocks for one KV head (and up
-// to 16 of its query heads, the rows of an MFMA tile): every code is read once for the whole group
-// of heads. The four wavefronts take pairs of blocks in turn with a running maximum and sum each,
+// The rows of a sequence for one KV head, row = token * group + head, stand in tiles of 16 (the rows
+// of an MFMA tile); row i's token sees the first seq_len - n + token + 1 tokens. One workgroup of
+// four wavefronts takes one split of the sequence's blocks for one tile: every code is read once for
+// a whole group of heads. The four wavefronts take pairs of blocks in turn with a running maximum and sum each,
 // meet once at the end in LDS, and either write the row or leave a partial (m, l, O) for the merge
 // launch.
 #pragma once
@@ -22,8 +24,8 @@ constexpr float kI8Rescale = 8.f;      // a row's reference moves when a score p
 // Splits of a sequence of nb blocks, at most `most` (the partials that the workspace holds for a
 // row, from the host's bound on the lengths): from its own length, so that a row's result does not
 // depend on the rest of the batch.
-__host__ __device__ inline int i8_splits(int nb, int most) {
-  const int n = (nb + kI8SplitBlocks - 1) / kI8SplitBlocks;
+__host__ __device__ inline int i8_splits(int nb, int most, int each = kI8SplitBlocks) {
+  const int n = (nb + each - 1) / each;
   return n < 1 ? 1 : (n > most ? most : n);
 }
 
@@ -38,12 +40,45 @@ struct Int8DecodeArgs {
   const int32_t* block_tables;
   int64_t bt_stride;
   int max_blocks;
-  const int32_t* seq_lens;
-  int num_seqs, heads, kvh, group, head_tiles;   // group = heads / kvh, head_tiles = ceil(group / 16)
+  const int32_t *seq_lens, *qsl;
+  int64_t num_tokens;
+  int num_seqs, num_decode;                      // sequences; the first num_decode have one row each
+  int heads, kvh, group;                         // group = heads / kvh
   float sl2;                                     // scale * log2(e)
-  int max_splits;                                // partials per row in the workspace
-  float *part_o, *part_ml;                       // [S, H, max_splits, D], [S, H, max_splits, 2]
+  int row_slots, max_splits;                     // rows per (sequence, KV head), splits of the partials
+  float *part_o, *part_ml;                       // [S, KVH, row_slots, max_splits, D], [.., 2]
 };
+
+// The rows of a sequence.
+struct I8Seq {
+  int q0, n, kv, start;                          // first flat row, rows, tokens, position of row q0
+};
+__device__ __forceinline__ int i8_kv_len(int len, int max_blocks);
+
+__device__ __forceinline__ I8Seq i8_seq(const Int8DecodeArgs& a, int b) {
+  I8Seq s;
+  const int len = a.seq_lens[b];
+  s.q0 = b, s.n = 1;
+  if (b >= a.num_decode) {
+    const int q0 = a.qsl[b], q1 = a.qsl[b + 1];
+    s.q0 = q0;
+    s.n = q0 < 0 || q1 <= q0 || q1 > a.num_tokens ? 0 : q1 - q0;
+  }
+  s.kv = i8_kv_len(len, a.max_blocks);
+  s.start = max(len, 0) - s.n;
+  return s;
+}
+
+// Splits of a sequence's blocks: longer ones where several tiles of rows share them, one where its
+// rows pass what the workspace holds.
+__device__ __forceinline__ int i8_splits(const Int8DecodeArgs& a, const I8Seq& s);
+
+__device__ __forceinline__ int i8_splits(const Int8DecodeArgs& a, const I8Seq& s) {
+  const int rows = s.n * a.group, tiles = (rows + 15) / 16;
+  if (rows > a.row_slots) return 1;
+  const int each = s.n == 1 ? kI8SplitBlocks : kI8SplitBlocks * tiles;
+  return i8_splits((s.kv + kBlockSize - 1) / kBlockSize, a.max_splits, each);
+}
 
 // Wavefront scans on the VALU (DPP row shifts, then the rows' last lanes broadcast on): a step costs
 // a few cycles where a shuffle through the LDS unit costs over a hundred, and both scans stand in
@@ -196,30 +231,33 @@ struct I8State {
   float4_t o[D / 16];
 };
 
-// One pair of blocks (tokens t0 .. t0 + 31 of the sequence for a, b next to each other): fk / fv
-// the blocks' K factor (scale * log2 e * ks) and V factor (vs / vref).
+// One pair of blocks (tokens ta .. and tb .. of the sequence): fk / fv the blocks' K factor (scale *
+// log2 e * ks) and V factor (vs / vref). A row sees the tokens below `vis`, all rows of the tile those
+// below `least`.
 template <int D>
 __device__ __forceinline__ void i8_step(I8State<D>& st, const I8Pair<D>& x, const I8Query<D>& q, float fka,
-                                        float fkb, float fva, float fvb, int ta, int tb, int len, int g) {
+                                        float fkb, float fva, float fvb, int ta, int tb, int vis, int least,
+                                        int g) {
   float4_t sa = i8_scores<D>(x.k[0], q), sb = i8_scores<D>(x.k[1], q);
   sa *= fka;
   sb *= fkb;
-  if (tb + kBlockSize > len || ta + kBlockSize > len) {
+  if (tb + kBlockSize > least || ta + kBlockSize > least) {
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      sa[r] = ta + 4 * g + r < len ? sa[r] : -INFINITY;
-      sb[r] = tb + 4 * g + r < len ? sb[r] : -INFINITY;
+      sa[r] = ta + 4 * g + r < vis ? sa[r] : -INFINITY;
+      sb[r] = tb + 4 * g + r < vis ? sb[r] : -INFINITY;
     }
   }
   const float top = rows_max(vmax(vmax(vmax(sa[0], sa[1]), vmax(sa[2], sa[3])),
                                   vmax(vmax(sb[0], sb[1]), vmax(sb[2], sb[3]))));
-  // !(<=): a NaN score (a block whose scale is NaN) moves the reference to NaN and stays
+  // !(<=): a NaN score (a block whose scale is NaN) moves the reference to NaN, where it stays
   const bool move = !(top <= st.m + kI8Rescale);
   float alpha = 1.f;
   if (__ballot(move)) {
-    alpha = move ? fast_exp2(st.m - top) : 1.f;            // m = -inf: 0
+    const float to = vmax(st.m, top);
+    alpha = move ? fast_exp2(st.m - to) : 1.f;             // m = -inf: 0
     st.l *= alpha;
-    st.m = move ? top : st.m;
+    st.m = move ? to : st.m;
   }
   const float neg = st.m == -INFINITY ? 0.f : -st.m;
   float pa[4], pb[4];
@@ -240,7 +278,7 @@ __device__ __forceinline__ void i8_step(I8State<D>& st, const I8Pair<D>& x, cons
 template <int D>
 __device__ __forceinline__ void i8_split(const Int8DecodeArgs& a, I8State<D>& st, float& vref,
                                          const I8Query<D>& q, int b, int h, int b0, int b1, int len,
-                                         int wave) {
+                                         int vis, int least, int wave) {
   const int lane = threadIdx.x % kWave, c = lane % 16, g = lane / 16;
   const int32_t* table = a.block_tables + b * a.bt_stride;
   const int64_t block_bytes = (int64_t)kBlockSize * D;
@@ -280,7 +318,7 @@ __device__ __forceinline__ void i8_split(const Int8DecodeArgs& a, I8State<D>& st
       const int ta = (lo + i) * kBlockSize;
       const int tb = i + 1 < n ? ta + kBlockSize : len;
       i8_step<D>(st, x, q, lane_f(ks, i), lane_f(ks, j), lane_f(vs, i), lane_f(vs, j), ta, tb,
-                 len, g);
+                 vis, least, g);
     };
     constexpr int STEP = 2 * kI8Waves;
     I8Pair<D> x, y;
@@ -321,8 +359,8 @@ struct I8DecodeLds {
 
 // The four wavefronts' states meet in LDS; the row (or its partial) is written.
 template <int D>
-__device__ __forceinline__ void i8_finish(const Int8DecodeArgs& a, I8State<D>& st, float vref, int b,
-                                          int head0, int rows, int split, int splits, int wave,
+__device__ __forceinline__ void i8_finish(const Int8DecodeArgs& a, I8State<D>& st, float vref, int b, int h,
+                                          int q0, int row0, int rows, int split, int splits, int wave,
                                           float* s_o, float* s_ml) {
   constexpr int VW = D / 16;
   const int lane = threadIdx.x % kWave, c = lane % 16, g = lane / 16;
@@ -353,12 +391,12 @@ __device__ __forceinline__ void i8_finish(const Int8DecodeArgs& a, I8State<D>& s
       sum += f * s_ml[2 * (w * 16 + row) + 1];
       o += ld<float4_t>(s_o + (w * 16 + row) * I8DecodeLds<D>::ROW + d) * f;
     }
-    const int64_t h = head0 + row;
     if (splits == 1) {
       const float f = sum == 0.f ? 0.f : vref / sum;       // no visible key: zeros
-      ts::st<half4_t>(a.out + b * a.out_st + h * D + d, to_half4(o * f));
+      const int token = (row0 + row) / a.group, head = h * a.group + (row0 + row) % a.group;
+      ts::st<half4_t>(a.out + (int64_t)(q0 + token) * a.out_st + (int64_t)head * D + d, to_half4(o * f));
     } else {
-      const int64_t at = ((int64_t)b * a.heads + h) * a.max_splits + split;
+      const int64_t at = (((int64_t)b * a.kvh + h) * a.row_slots + row0 + row) * a.max_splits + split;
       ts::st<float4_t>(a.part_o + at * D + d, o * vref);
       if (d == 0) {
         a.part_ml[2 * at] = top;
@@ -368,26 +406,34 @@ __device__ __forceinline__ void i8_finish(const Int8DecodeArgs& a, I8State<D>& s
   }
 }
 
-// Item `item` of the batch's splits, numbered densely over the sequences: its sequence, split and
-// split count. Every wavefront looks it up for itself, 64 sequences at a time.
-__device__ __forceinline__ bool i8_find(const Int8DecodeArgs& a, int item, int& b, int& split, int& splits,
-                                        int& len) {
+// Item `item` of the batch's (split, row tile) pairs, numbered densely over the sequences. Every
+// wavefront looks it up for itself, 64 sequences at a time.
+struct I8Item {
+  int b, split, splits, tile;
+  I8Seq seq;
+};
+
+__device__ __forceinline__ bool i8_find(const Int8DecodeArgs& a, int item, I8Item& x) {
   const int lane = threadIdx.x % kWave;
   int base = 0;
   for (int s0 = 0; s0 < a.num_seqs; s0 += kWave) {
-    int n = 0, kv = 0;
+    int splits = 1, tiles = 0;
+    I8Seq s = {};
     if (s0 + lane < a.num_seqs) {
-      kv = i8_kv_len(a.seq_lens[s0 + lane], a.max_blocks);
-      n = i8_splits((kv + kBlockSize - 1) / kBlockSize, a.max_splits);
+      s = i8_seq(a, s0 + lane);
+      splits = i8_splits(a, s);
+      tiles = (s.n * a.group + 15) / 16;
     }
-    const int sum = i8_scan(n);
+    const int n = splits * tiles, sum = i8_scan(n);
     const uint64_t past = __ballot(base + sum > item);
     if (past) {
       const int i = __ffsll((unsigned long long)past) - 1;
-      b = s0 + i;
-      splits = __builtin_amdgcn_readlane(n, i);
-      split = item - (base + __builtin_amdgcn_readlane(sum, i) - splits);
-      len = __builtin_amdgcn_readlane(kv, i);
+      auto of = [&](int v) { return __builtin_amdgcn_readlane(v, i); };
+      x.b = s0 + i;
+      x.splits = of(splits);
+      const unsigned in = item - (base + of(sum) - of(n)), t = of(tiles);
+      x.split = (int)(t == 1 ? in : in / t), x.tile = (int)(in - x.split * t);
+      x.seq = {of(s.q0), of(s.n), of(s.kv), of(s.start)};
       return true;
     }
     base += __builtin_amdgcn_readlane(sum, kWave - 1);
@@ -403,71 +449,86 @@ __global__ void __launch_bounds__(kI8Threads, i8_decode_groups(D)) decode_int8_k
   __shared__ __align__(16) I8DecodeLds<D> lds;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int lane = threadIdx.x % kWave, c = lane % 16, g = lane / 16;
-  const int tiles = a.kvh * a.head_tiles;
   for (int64_t u = blockIdx.x;; u += gridDim.x) {
-    const int64_t item = u / tiles;
-    const int tile = (int)(u % tiles);
-    int b, split, splits, len;
-    if (item > INT32_MAX || !i8_find(a, (int)item, b, split, splits, len)) return;
-    const int h = tile / a.head_tiles, r0 = tile % a.head_tiles * 16;
-    const int head0 = h * a.group + r0, rows = min(a.group - r0, 16);
+    const int64_t item = u / (unsigned)a.kvh;
+    const int h = (int)(u - item * a.kvh);
+    I8Item x;
+    if (item > INT32_MAX || !i8_find(a, (int)item, x)) return;
+    const int row0 = 16 * x.tile, rows = min(x.seq.n * a.group - row0, 16), kv = x.seq.kv;
+    const int row = row0 + min(c, rows - 1), token = row / a.group;
+    const int vis = min(kv, max(0, x.seq.start + token + 1));
+    const int least = min(kv, max(0, x.seq.start + row0 / a.group + 1));
     I8Query<D> q;
-    i8_load_q<D>(a.q + b * a.q_st + (int64_t)(head0 + c) * a.q_sh, g, c < rows, q);
+    i8_load_q<D>(a.q + (int64_t)(x.seq.q0 + token) * a.q_st + (int64_t)(h * a.group + row - token * a.group) * a.q_sh,
+                 g, c < rows, q);
     I8State<D> st;
     st.m = -INFINITY, st.l = 0.f;
 #pragma unroll
     for (int t = 0; t < D / 16; ++t) st.o[t] = {0.f, 0.f, 0.f, 0.f};
     float vref = 0.f;
-    const int nb = (len + kBlockSize - 1) / kBlockSize;
-    const int b0 = (int)((int64_t)nb * split / splits), b1 = (int)((int64_t)nb * (split + 1) / splits);
-    i8_split<D>(a, st, vref, q, b, h, b0, b1, len, wave);
-    i8_finish<D>(a, st, vref, b, head0, rows, split, splits, wave, lds.o, lds.ml);
+    const int nb = (kv + kBlockSize - 1) / kBlockSize;
+    const int b0 = (int)((unsigned)(nb * x.split) / (unsigned)x.splits);
+    const int b1 = (int)((unsigned)(nb * (x.split + 1)) / (unsigned)x.splits);
+    i8_split<D>(a, st, vref, q, x.b, h, b0, b1, kv, vis, least, wave);
+    i8_finish<D>(a, st, vref, x.b, h, x.seq.q0, row0, rows, x.split, x.splits, wave, lds.o, lds.ml);
   }
 }
 
-// Rows of sequences with more than one split: one workgroup per (sequence, head), D / 4 threads a
-// partial. The first partial of each thread and every split's (m, l) are requested before the
-// sequence's length is known (they lie in the workspace whatever it is), the others at once after
-// it.
+// Rows of sequences with more than one split: one wavefront a row, D / 4 lanes a partial. Each lane's
+// first partial and every split's (m, l) are requested before the sequence's length is known (they
+// lie in the workspace whatever it is), the others at once after it. (A workgroup a row, its eight
+// groups meeting in LDS, took twice as long at 2240 rows of a few splits: 10.5 us.)
 template <int D>
 __global__ void __launch_bounds__(kI8Threads) decode_int8_merge_kernel(Int8DecodeArgs a) {
-  constexpr int PER_ROW = D / 4, GROUPS = kI8Threads / PER_ROW;
-  constexpr int N = (kI8MaxSplits + GROUPS - 1) / GROUPS;
-  __shared__ __align__(16) float s_o[GROUPS][D];
-  const int b = blockIdx.x, h = blockIdx.y, lane = threadIdx.x % kWave;
-  const int group = threadIdx.x / PER_ROW, d = threadIdx.x % PER_ROW * 4;
-  const int64_t row = ((int64_t)b * a.heads + h) * a.max_splits;
+  constexpr int PER_ROW = D / 4, GROUPS = kWave / PER_ROW;
+  constexpr int N = 64 / GROUPS < 16 ? 64 / GROUPS : 16;   // partials of a lane at a time
+  const int b = blockIdx.y, lane = threadIdx.x % kWave;
+  const int slot = blockIdx.x * kI8Waves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int h = slot / a.row_slots, r = slot - h * a.row_slots;
+  if (h >= a.kvh) return;
+  const int group = lane / PER_ROW, d = lane % PER_ROW * 4;
+  const int64_t row = (((int64_t)b * a.kvh + h) * a.row_slots + r) * a.max_splits;
   const float* part = a.part_o + row * D + d;
   const float2_t ml = ld<float2_t>(a.part_ml + 2 * (row + min(lane, a.max_splits - 1)));
   float4_t x[N];
   x[0] = ld<float4_t>(part + (int64_t)min(group, a.max_splits - 1) * D);
-  const int len = i8_kv_len(table_entry(a.seq_lens + b), a.max_blocks);
-  const int splits = i8_splits((len + kBlockSize - 1) / kBlockSize, a.max_splits);
-  if (splits == 1) return;
-#pragma unroll
-  for (int i = 1; i < N; ++i)
-    if (group + i * GROUPS < splits) x[i] = ld<float4_t>(part + (int64_t)(group + i * GROUPS) * D);
+  const I8Seq seq = i8_seq(a, b);
+  const int splits = i8_splits(a, seq);
+  if (splits == 1 || r >= seq.n * a.group) return;
   // lane i: split i's weight
   const float m = lane < splits ? ml[0] : -INFINITY;
-  float top = m;
-#pragma unroll
-  for (int k = 1; k < kWave; k <<= 1) top = vmax(top, shfl_xor(top, k));
-  const float f = m == -INFINITY ? 0.f : fast_exp2(m - top);
-  float sum = lane < splits ? f * ml[1] : 0.f;
-#pragma unroll
-  for (int k = 1; k < kWave; k <<= 1) sum += shfl_xor(sum, k);
   float4_t o = {0.f, 0.f, 0.f, 0.f};
+  float f = 0.f, sum = 0.f;
+  for (int i0 = 0; i0 < splits; i0 += N * GROUPS) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const float w = __shfl(f, min(group + i * GROUPS, kWave - 1), kWave);
-    if (group + i * GROUPS < splits) o += x[i] * w;
+    for (int i = 0; i < N; ++i) {
+      const int k = i0 + group + i * GROUPS;
+      if ((i > 0 || i0 > 0) && k < splits) x[i] = ld<float4_t>(part + (int64_t)k * D);
+    }
+    if (i0 == 0) {
+      float top = m;
+#pragma unroll
+      for (int k = 1; k < kWave; k <<= 1) top = vmax(top, shfl_xor(top, k));
+      f = m == -INFINITY ? 0.f : fast_exp2(m - top);
+      sum = lane < splits ? f * ml[1] : 0.f;
+#pragma unroll
+      for (int k = 1; k < kWave; k <<= 1) sum += shfl_xor(sum, k);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int k = i0 + group + i * GROUPS;
+      const float w = __shfl(f, min(k, kWave - 1), kWave);
+      if (k < splits) o += x[i] * w;
+    }
   }
-  st<float4_t>(&s_o[group][d], o);
-  __syncthreads();
-  if (threadIdx.x >= PER_ROW) return;
-  const int most = min(splits, GROUPS);
-  for (int i = 1; i < most; ++i) o += ld<float4_t>(&s_o[i][d]);
-  st<half4_t>(a.out + b * a.out_st + (int64_t)h * D + d, to_half4(o * (1.f / sum)));
+#pragma unroll
+  for (int k = PER_ROW; k < kWave; k <<= 1)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] += shfl_xor(o[e], k);
+  if (group > 0) return;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;          // (nothing visible)
+  const int token = r / a.group, head = h * a.group + r - token * a.group;
+  st<half4_t>(a.out + (int64_t)(seq.q0 + token) * a.out_st + (int64_t)head * D + d, to_half4(o * inv));
 }
 
 }  // namespace ts

@@ -45,8 +45,6 @@ struct I8Const {
 
 struct Int8PrefillArgs {
   Int8DecodeArgs a;                      // (part_o, part_ml: two partials of a tile per workgroup)
-  const int32_t* qsl;
-  int64_t num_tokens;
   int num_seqs, first;                   // sequences first .. num_seqs - 1
   int tiles;                             // of the longest chunk by the host's bound
   int groups;                            // workgroups of the main launch
@@ -90,10 +88,10 @@ struct I8Chunk {
 };
 
 __device__ __forceinline__ I8Chunk i8_chunk(const Int8PrefillArgs& p, int b) {
-  const int q0 = p.qsl[b], q1 = p.qsl[b + 1], len = p.a.seq_lens[b];
+  const int q0 = p.a.qsl[b], q1 = p.a.qsl[b + 1], len = p.a.seq_lens[b];
   I8Chunk k;
   k.q0 = q0;
-  k.n = q0 < 0 || q1 <= q0 || q1 > p.num_tokens ? 0 : q1 - q0;
+  k.n = q0 < 0 || q1 <= q0 || q1 > p.a.num_tokens ? 0 : q1 - q0;
   k.kv = i8_kv_len(len, p.a.max_blocks);
   k.start = max(len, 0) - k.n;
   return k;
@@ -448,9 +446,10 @@ __device__ __forceinline__ void i8_reference(I8Rows<D>& w, float best) {
   const bool move = !(best <= w.m + kI8Rescale);           // NaN moves it too
   w.moved = __ballot(move) != 0;
   if (w.moved) {
-    w.alpha = move ? fast_exp2(w.m - best) : 1.f;
+    const float to = vmax(w.m, best);                      // (a NaN stays)
+    w.alpha = move ? fast_exp2(w.m - to) : 1.f;
     w.l *= w.alpha;
-    w.m = move ? best : w.m;
+    w.m = move ? to : w.m;
   }
 }
 
