@@ -224,7 +224,7 @@ __device__ __forceinline__ void i8_pv(float4_t (&o)[D / 16], const uint32_t (&v)
   }
 }
 
-// The state of one wavefront's 16 rows: O^T in units of the V scale `vref`.
+// The state of one wavefront's 16 rows: O^T in units of kColumnUnit times the V scale `vref`.
 template <int D>
 struct I8State {
   float m, l;
@@ -392,12 +392,12 @@ __device__ __forceinline__ void i8_finish(const Int8DecodeArgs& a, I8State<D>& s
       o += ld<float4_t>(s_o + (w * 16 + row) * I8DecodeLds<D>::ROW + d) * f;
     }
     if (splits == 1) {
-      const float f = sum == 0.f ? 0.f : vref / sum;       // no visible key: zeros
+      const float f = sum == 0.f ? 0.f : kColumnUnit * vref / sum;   // no visible key: zeros
       const int token = (row0 + row) / a.group, head = h * a.group + (row0 + row) % a.group;
       ts::st<half4_t>(a.out + (int64_t)(q0 + token) * a.out_st + (int64_t)head * D + d, to_half4(o * f));
     } else {
       const int64_t at = (((int64_t)b * a.kvh + h) * a.row_slots + row0 + row) * a.max_splits + split;
-      ts::st<float4_t>(a.part_o + at * D + d, o * vref);
+      ts::st<float4_t>(a.part_o + at * D + d, o * (kColumnUnit * vref));
       if (d == 0) {
         a.part_ml[2 * at] = top;
         a.part_ml[2 * at + 1] = sum;

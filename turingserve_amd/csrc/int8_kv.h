@@ -38,11 +38,15 @@ __device__ __forceinline__ half8_t codes8(uint32_t w0, uint32_t w1,
   return {a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// Code `q` of each of two words (sign bits flipped already) as packed fp16: a column of the
-// rows that the words come from.
+// Code `q` of each of two words (sign bits flipped already) as packed fp16, in units of
+// 1 / kColumnUnit: a column of the rows that the words come from. u alone in a half is the fp16
+// subnormal u 2^-24; times 2^15 minus 1/4 it is (u - 128) 2^-9, exactly, in one packed instruction.
+constexpr float kColumnUnit = 512.f;
 template <int q>
 __device__ __forceinline__ half2_t column2(uint32_t row0, uint32_t row1) {
-  return unbias(__builtin_amdgcn_perm(row1, row0, 0x0c040c00u + q * 0x00010001u) | 0x64006400u);
+  const half2_t up = {(half_t)32768.f, (half_t)32768.f}, off = {(half_t)-0.25f, (half_t)-0.25f};
+  return __builtin_elementwise_fma(as_half2(__builtin_amdgcn_perm(row1, row0, 0x0c040c00u + q * 0x00010001u)),
+                                   up, off);
 }
 
 }  // namespace ts

@@ -72,8 +72,7 @@ struct I8Tile {
 
 template <int D>
 struct I8PrefillLds {
-  static constexpr int NV = D > 128 ? 2 : 3;               // (what fits)
-  __align__(16) half_t k[2][I8Tile<D>::HALVES], v[NV][I8Tile<D>::HALVES];
+  __align__(16) half_t k[2][I8Tile<D>::HALVES], v[2][I8Tile<D>::HALVES];
   int n[kI8Kept * kWave], scan[kI8Kept * kWave];           // the walk's kept pairs
   int blk[kI8Window];                                      // the sign bit: a scale is not finite
   __align__(16) float fk[kI8Window + 4], vs[kI8Window];        // scale * log2 e * ks; log2(vs / vref)
@@ -298,7 +297,7 @@ template <int D>
 struct I8Rows {
   static constexpr int DT = (D + 31) / 32;                 // output tiles of 32 dims
   static constexpr int NQ = D / 16, NP = 2 * DT;           // operands of 32 tokens: K, V^T
-  static constexpr int ALL = 2 * NQ + 2 * NP, AHEAD = 5;   // of a step; requested ahead
+  static constexpr int ALL = 2 * NQ + 2 * NP, AHEAD = 4;   // of a step; requested ahead
   half8_t q[NQ];
   float16_t o[DT];
   float m, l, alpha;
@@ -362,11 +361,12 @@ struct I8Exp {
 //   P'(sc[0])  beside  O += V P' of the last step's second half
 //   P'(sc[1])  beside  sc[0] = K . Q^T of the next step
 //   staging    beside  sc[1] = K . Q^T of the next step
-//   maxima of the next scores  beside  O += V P' of this step's first half
+//   maxima of the next scores, more staging  beside  O += V P' of this step's first half
 // so that no second set of scores is needed (two wavefronts share a SIMD's registers). The order is
 // pinned, MFMA by MFMA: left to itself the compiler sets MFMAs and exponentials one after the other.
-// The workgroup meets behind the third phase: what the fourth reads is written two steps later.
-// Returns each row's largest next score.
+// The workgroup meets between the third phase and the fourth: K is staged before, over what the
+// step before read, and V behind it, over what the first phase read. Returns each row's largest
+// next score.
 template <int D, typename Mask, typename Work>
 __device__ __forceinline__ float i8_step64(I8Rows<D>& w, const half_t* vp, const half_t* kn, const half_t* vc,
                                            float16_t (&sc)[2], half8_t (&pr)[4], const float* fkp,
@@ -400,7 +400,6 @@ __device__ __forceinline__ float i8_step64(I8Rows<D>& w, const half_t* vp, const
 #pragma unroll
     for (int i = 0; i < R::DT; ++i) w.o[i] *= w.alpha;
   }
-  if constexpr (I8PrefillLds<D>::NV == 2) __syncthreads();  // V of the last step is staged over
   float16_t zero;
 #pragma unroll
   for (int i = 0; i < 16; ++i) zero[i] = 0.f;
@@ -416,7 +415,6 @@ __device__ __forceinline__ float i8_step64(I8Rows<D>& w, const half_t* vp, const
     if (j < 2) ex.share<N>(N + j, sc, fk, off, back, w.l, pr);
     if (NQ < 2) ex.share<N>(N + 1, sc, fk, off, back, w.l, pr);
     if (j == NQ / 4) work(1);                              // K of a later step to LDS
-    if (j == NQ / 2) work(2);                              // V
     __builtin_amdgcn_sched_barrier(0);
   }
   const float4_t fkn = ld<float4_t>(fknp);
@@ -432,6 +430,7 @@ __device__ __forceinline__ float i8_step64(I8Rows<D>& w, const half_t* vp, const
       const float x = sc[b / 2][8 * (b % 2) + e];
       top[b] = e == 0 ? x : vmax(top[b], x);
     }
+    if (j == NP / 2) work(2);                              // V
     __builtin_amdgcn_sched_barrier(0);
   }
   return vmax(vmax(top[0] * fkn[0], top[1] * fkn[1]), vmax(top[2] * fkn[2], top[3] * fkn[3]));
@@ -459,7 +458,7 @@ __device__ __forceinline__ void i8_piece(const Int8PrefillArgs& p, I8PrefillLds<
                                          int b, int tile, int h, int s0, int s1, bool whole, int slot) {
   typedef I8Rows<D> R;
   typedef I8Stage<D, WAVES * kWave> S;
-  constexpr int DT = R::DT, THREADS = WAVES * kWave, ROWS = 32 * WAVES, NV = I8PrefillLds<D>::NV;
+  constexpr int DT = R::DT, THREADS = WAVES * kWave, ROWS = 32 * WAVES;
   const Int8DecodeArgs& a = p.a;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int lane = threadIdx.x % kWave, c = lane % 32, hh = lane / 32;
@@ -471,9 +470,6 @@ __device__ __forceinline__ void i8_piece(const Int8PrefillArgs& p, I8PrefillLds<
   const int sees = i8_sees(k, (min(rows, (tile + 1) * ROWS) - 1) / a.group);
   const int nb = (sees + kBlockSize - 1) / kBlockSize;     // blocks that the tile sees
   R w;
-  const half_t* qrow = a.q + (int64_t)(k.q0 + token) * a.q_st + (int64_t)head * a.q_sh;
-#pragma unroll
-  for (int i = 0; i < D / 16; ++i) w.q[i] = ld<half8_t>(qrow + 16 * i + 8 * hh);
   w.kat = I8Tile<D>::k_at(c, hh);
 #pragma unroll
   for (int i = 0; i < 4; ++i) w.vat[i] = I8Tile<D>::v_at(D < 32 ? c % D : c, i, hh);
@@ -490,32 +486,42 @@ __device__ __forceinline__ void i8_piece(const Int8PrefillArgs& p, I8PrefillLds<
     const int n = min(s1 - w0, kI8Window / kI8StepBlocks);
     const int blocks = min(nb - w0 * kI8StepBlocks, n * kI8StepBlocks), last = blocks - 1;
     __syncthreads();                                       // the last window's and piece's reads
-    for (int i = threadIdx.x; i < kI8Window; i += THREADS) {
-      int blk = 0;
+    constexpr int PER = (kI8Window + THREADS - 1) / THREADS;
+    int blk[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int at = threadIdx.x + i * THREADS;
+      blk[i] = at < blocks ? clamp_block(a.block_tables[b * a.bt_stride + w0 * kI8StepBlocks + at], a.num_blocks) : 0;
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int at = threadIdx.x + i * THREADS;
       float ks = 0.f, vs = 0.f;
-      if (i < blocks) {
-        blk = clamp_block(a.block_tables[b * a.bt_stride + w0 * kI8StepBlocks + i], a.num_blocks);
-        ks = a.ks[(int64_t)blk * a.kvh + h];
-        vs = a.vs[(int64_t)blk * a.kvh + h];
+      if (at < blocks) {
+        ks = a.ks[(int64_t)blk[i] * a.kvh + h];
+        vs = a.vs[(int64_t)blk[i] * a.kvh + h];
         i8_poison(ks, vs);
       }
       // A K factor of 0 or NaN would leave hidden tokens (-inf) NaN: scores of a factor as small as
       // the least one are 0, and the codes of blocks without finite scales are staged as NaN.
       const float f = ks * a.sl2;
-      lds.blk[i] = f == f ? blk : blk | (int)0x80000000;
-      lds.fk[i] = f > kI8LeastFactor ? f : kI8LeastFactor;
-      lds.vs[i] = vs;
+      if (at < kI8Window) {
+        lds.blk[at] = f == f ? blk[i] : blk[i] | (int)0x80000000;
+        lds.fk[at] = f > kI8LeastFactor ? f : kI8LeastFactor;
+        lds.vs[at] = vs;
+      }
     }
     __syncthreads();
-    // K of step i + 2 and V of step i + 1 are requested in step i - 1 and go to LDS in step i.
-    S now, later;
-    int id[S::N], idv[S::N];
-    S::ids(lds, 0, last, idv);
-    now.request_k(a, idv, h);
-    later.request_v(a, idv, h);
-    S::ids(lds, kI8StepBlocks, last, idv);
-    later.request_k(a, idv, h);
-    S::ids(lds, 2 * kI8StepBlocks, last, id);
+    S stage;
+    int id0[S::N], id1[S::N], id2[S::N];                   // of the next step, the second, the third
+    S::ids(lds, 0, last, id0);
+    S::ids(lds, kI8StepBlocks, last, id1);
+    stage.request_k(a, id0, h);
+    if (w0 == s0) {                                        // q behind what the first scores wait for
+      const half_t* qrow = a.q + (int64_t)(k.q0 + token) * a.q_st + (int64_t)head * a.q_sh;
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) w.q[i] = ld<half8_t>(qrow + 16 * i + 8 * hh);
+    }
     float top = 0.f;
 #pragma unroll
     for (int i = 0; i < kI8Window; i += kWave) top = fmaxf(top, lds.vs[i + lane]);
@@ -532,40 +538,37 @@ __device__ __forceinline__ void i8_piece(const Int8PrefillArgs& p, I8PrefillLds<
       lds.vs[i] = f;
       lds.back[i] = fast_exp2(-f);
     }
-    now.place_k(lds.k[0]);
-    for (int i = threadIdx.x; i < I8Tile<D>::HALVES / 8; i += THREADS)
-      st<half8_t>(lds.v[1] + 8 * i, half8_t{0, 0, 0, 0, 0, 0, 0, 0});
+    stage.place_k(lds.k[0]);
+    for (int i = threadIdx.x; i < 2 * I8Tile<D>::HALVES / 8; i += THREADS)
+      st<half8_t>(lds.v[0] + 8 * i, half8_t{0, 0, 0, 0, 0, 0, 0, 0});
     __syncthreads();
 
-    // Step i reads K of step i + 1 in k[(i + 1) % 2] and V of steps i - 1 and i; meanwhile K of step
-    // i + 2 and V of step i + 1 go to tiles whose last readers were in step i - 1. The first of them,
-    // step -1, has hidden scores only (and V codes of 0): it is there for the scores
-    // of step 0. The loop has no branch but the mask's and the reference's: past the window's end
-    // the last blocks are staged again, and the scores of the step behind it are not used.
+    // Step i reads K of step i + 1 in k[(i + 1) % 2], V of steps i - 1 and i in v[(i - 1) % 2] and
+    // v[i % 2], and stages K of step i + 2 and V of step i + 1. The first of them, step -1, has hidden
+    // scores only (and V codes of 0): it is there for the scores of step 0. The loop has no branch
+    // but the mask's and the reference's: past the window's end the last blocks are staged again,
+    // and the scores of the step behind it are not used.
     float16_t sc[2];
     half8_t pr[4];
 #pragma unroll
     for (int i = 0; i < 16; ++i) sc[0][i] = sc[1][i] = -INFINITY;
 #pragma unroll
     for (int e = 0; e < 8; ++e) pr[2][e] = pr[3][e] = (half_t)0.f;
-    int v0 = 1, v1 = 0, v2 = NV - 1;                       // V of this step, the next, the last one
-    for (int i = -1; i < n; ++i) {
+    auto step = [&](auto parity, int i) {
+      constexpr int P = decltype(parity)::value;           // i % 2
       auto work = [&](int part) {
-        if (part == 0) {                                   // (idv: of step i + 2, id: of step i + 3)
-          now = later;
-          later.request_v(a, idv, h);
-          later.request_k(a, id, h);
-#pragma unroll
-          for (int e = 0; e < S::N; ++e) idv[e] = id[e];
-          S::ids(lds, (i + 4) * kI8StepBlocks, last, id);
+        if (part == 0) {
+          stage.request_k(a, id1, h);
+          stage.request_v(a, id0, h);
+          S::ids(lds, (i + 3) * kI8StepBlocks, last, id2);
         }
-        if (part == 1) now.place_k(lds.k[i & 1]);
-        if (part == 2) now.place_v(lds.v[v1]);
+        if (part == 1) stage.place_k(lds.k[P]);
+        if (part == 2) stage.place_v(lds.v[1 - P]);
       };
       auto mask = [&](float16_t (&x)[2]) {
-        const int step = w0 + i + 1;
-        if ((step + 1) * kI8Keys > least) {
-          const int key0 = step * kI8Keys + 4 * hh;
+        const int at = w0 + i + 1;
+        if ((at + 1) * kI8Keys > least) {
+          const int key0 = at * kI8Keys + 4 * hh;
 #pragma unroll
           for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
@@ -574,17 +577,20 @@ __device__ __forceinline__ void i8_piece(const Int8PrefillArgs& p, I8PrefillLds<
         }
       };
       const int wb = max(i, 0) * kI8StepBlocks;
-      const half_t *vc = lds.v[v0], *vp = lds.v[i < 0 ? v0 : v2];
-      const float best = i8_step64<D>(w, vp, lds.k[(i + 1) & 1], vc, sc, pr, lds.fk + wb, lds.vs + wb,
+      const float best = i8_step64<D>(w, lds.v[1 - P], lds.k[1 - P], lds.v[P], sc, pr, lds.fk + wb, lds.vs + wb,
                                       lds.back + wb, lds.fk + (i + 1) * kI8StepBlocks, mask, work);
       i8_reference<D>(w, i + 1 < n ? best : w.m);          // (its own reference moves none, also a NaN)
-      const int v = v2;
-      v2 = v0, v0 = v1, v1 = NV == 2 ? v2 : v;
-    }
 #pragma unroll
-    for (int j = 0; j < R::NP; ++j)                        // the last step's second half
-      w.o[j % DT] = mfma_i8(ld<half8_t>(lds.v[v2] + w.vat[2 + j / DT] + j % DT * 32 * kI8Keys), pr[2 + j / DT],
-                            w.o[j % DT]);
+      for (int e = 0; e < S::N; ++e) id0[e] = id1[e], id1[e] = id2[e];
+    };
+    for (int i = -1; i < n; i += 2) {
+      step(I8Const<1>(), i);
+      if (i + 1 < n) step(I8Const<0>(), i + 1);
+    }
+    const half_t* vl = lds.v[(n - 1) & 1];                 // the last step's second half
+#pragma unroll
+    for (int j = 0; j < R::NP; ++j)
+      w.o[j % DT] = mfma_i8(ld<half8_t>(vl + w.vat[2 + j / DT] + j % DT * 32 * kI8Keys), pr[2 + j / DT], w.o[j % DT]);
   }
 
   // lanes c and c + 32 hold the two halves of row c's sum
@@ -593,6 +599,7 @@ __device__ __forceinline__ void i8_piece(const Int8PrefillArgs& p, I8PrefillLds<
   if (wrow + c >= rows) return;
   const int64_t at = (int64_t)slot * ROWS + 32 * wave + c;
   if (!whole && hh == 0) st<float2_t>(a.part_ml + 2 * at, float2_t{w.m, l});
+  vref *= kColumnUnit;
   const float f = !whole ? vref : l == 0.f ? 0.f : vref / l;   // nothing visible: zeros
   half_t* dst = a.out + (int64_t)(k.q0 + token) * a.out_st + (int64_t)head * D;
 #pragma unroll
@@ -619,6 +626,7 @@ prefill_int8_kernel(Int8PrefillArgs p) {
   __shared__ __align__(16) I8PrefillLds<D> lds;
   const Int8DecodeArgs& a = p.a;
   int at, hi;
+  I8Place place;
   {
     const I8Walk<ROWS> walk(p);
     const int total = walk.total * a.kvh;
@@ -626,14 +634,15 @@ prefill_int8_kernel(Int8PrefillArgs p) {
     const I8Shares shares(total, p.groups);
     if ((int)blockIdx.x >= shares.count) return;
     at = shares.begin(blockIdx.x), hi = shares.begin(blockIdx.x + 1);
+    place = walk.find(p, (int)((unsigned)at / (unsigned)a.kvh));
     if (threadIdx.x < kWave) walk.save(lds.n, lds.scan);
-    __syncthreads();
   }
   int b = 0, h = 0, tile = 0;
-  for (bool extra = false; extra || at < hi;) {
+  for (bool extra = false, more = false; extra || at < hi;) {
     int s0 = 0, s1, steps;
     if (!extra) {
-      const I8Place place = I8Walk<ROWS>(lds.n, lds.scan).find(p, (int)((unsigned)at / (unsigned)a.kvh));
+      if (more) place = I8Walk<ROWS>(lds.n, lds.scan).find(p, (int)((unsigned)at / (unsigned)a.kvh));
+      more = true;                                         // (i8_piece meets between the save and this)
       const unsigned in = at - place.before * a.kvh;
       steps = place.steps;
       h = (int)(in / (unsigned)steps), s0 = (int)(in % (unsigned)steps);
@@ -652,7 +661,7 @@ prefill_int8_kernel(Int8PrefillArgs p) {
 }
 
 // Tiles that several workgroups share: D / 4 threads a row, 32 rows a workgroup.
-constexpr int kI8MergeRows = 32;
+constexpr int kI8MergeRows = 16;
 template <int D, int ROWS>
 __global__ void __launch_bounds__(256) prefill_int8_merge_kernel(Int8PrefillArgs p) {
   constexpr int PER = 256 / (D / 4), N = 4;                // rows at a time, partials requested at once
