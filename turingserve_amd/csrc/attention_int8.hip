@@ -3,14 +3,18 @@
 
 namespace ts {
 
-// Rows per (sequence, KV head) up to which a chunk is taken in the decode kernel's tiles of 16 rows,
-// each of which reads the sequence's codes anew.
+// Chunks that the decode kernel takes, in tiles of 16 rows each of which reads the sequence's codes
+// anew: those of few rows, and those whose tiles and pairs of blocks are few and whose sequences are
+// short enough to be taken in one split.
 constexpr int kI8ShortRows = 64;
+constexpr int64_t kI8SmallWork = 32768;  // (tile, pair of blocks) steps
+constexpr int kI8SmallSeq = 1024;
 
 // Launch shape and scratch of a batch, from the host's bounds.
 struct Int8Plan {
   int small;                             // sequences that the decode kernel takes: the first ones
-  int row_slots, max_splits;             // its rows per (sequence, KV head), splits of the longest
+  int row_slots, max_splits;             // a chunk's partial rows per KV head, splits of the longest
+  int64_t slots;                         // rows with partials
   int tiles, groups;                     // prefill: tiles of a chunk, workgroups
   size_t dec_o, dec_ml, pre_o, pre_ml;   // offsets of the partials
   size_t bytes;
@@ -29,23 +33,27 @@ static Int8Plan int8_plan(int num_seqs, int num_decode, int max_query_len, int m
   const int64_t nb = ((int64_t)(max_seq_len > 0 ? max_seq_len : 0) + kBlockSize - 1) / kBlockSize;
   const int G = H / KVH;
   const int64_t chunk_rows = (int64_t)(max_query_len > 0 ? max_query_len : 1) * G;
-  const bool all = num_decode == num_seqs || chunk_rows <= kI8ShortRows;
+  const int64_t P = num_seqs - num_decode;
+  const int seq = max_prefill_seq_len > 0 ? max_prefill_seq_len : max_seq_len > 0 ? max_seq_len : 1;
+  const int64_t work = P * KVH * ((chunk_rows + 15) / 16) * ((seq + 31) / 32);
+  const bool all = P == 0 || chunk_rows <= kI8ShortRows || (seq <= kI8SmallSeq && work <= kI8SmallWork);
   pl.small = all ? num_seqs : num_decode;
-  pl.row_slots = all && num_decode < num_seqs ? (int)chunk_rows : G;
+  pl.row_slots = (int)(chunk_rows < kI8ShortRows ? chunk_rows : kI8ShortRows);
+  if (pl.row_slots < G) pl.row_slots = G;
   pl.max_splits = i8_splits((int)nb, kI8MaxSplits);
   if (pl.small > 0 && pl.max_splits > 1) {
-    const size_t rows = (size_t)pl.small * KVH * pl.row_slots * pl.max_splits;
+    pl.slots = (int64_t)num_decode * H + (pl.small - num_decode) * (int64_t)KVH * pl.row_slots;
+    const size_t rows = (size_t)pl.slots * pl.max_splits;
     pl.dec_o = take(at, rows * D * sizeof(float));
     pl.dec_ml = take(at, rows * 2 * sizeof(float));
   }
-  const int P = num_seqs - pl.small;
-  if (P > 0) {
+  if (!all) {
     const int tile_rows = 32 * i8_prefill_waves(D);
     pl.tiles = (int)((chunk_rows + tile_rows - 1) / tile_rows);
-    const int seq = max_prefill_seq_len > 0 ? max_prefill_seq_len : max_seq_len;
-    const int64_t steps = (int64_t)P * pl.tiles * KVH * ((seq > 0 ? seq - 1 : 0) / kI8Keys + 1);
-    const int64_t most = cus;
-    pl.groups = (int)(steps / kI8MinShare < most ? (steps < kI8MinShare ? 1 : steps / kI8MinShare) : most);
+    const int64_t steps = P * pl.tiles * KVH * ((seq - 1) / kI8Keys + 1);
+    const int64_t cost = steps + P * pl.tiles * KVH * kI8TileCost;
+    const int64_t most = (int64_t)i8_prefill_groups(D) * cus;
+    pl.groups = (int)(cost / kI8MinShare < most ? (cost < kI8MinShare ? 1 : cost / kI8MinShare) : most);
     const size_t r = (size_t)2 * pl.groups * tile_rows;
     pl.pre_o = take(at, r * D * sizeof(float));
     pl.pre_ml = take(at, r * 2 * sizeof(float));
@@ -59,13 +67,14 @@ static bool int8_head_dim(int D) { return D == 16 || D == 32 || D == 64 || D == 
 template <int D>
 static int launch_decode(const Int8DecodeArgs& a, int cus, hipStream_t s) {
   // Every split of the batch, at most as many workgroups as the CUs hold; the rest go round.
-  const int64_t tiles = (a.row_slots + 15) / 16;
-  const int64_t units = (int64_t)a.num_seqs * a.max_splits * a.kvh * tiles;
+  const int64_t most = a.num_seqs > a.num_decode ? INT32_MAX : (int64_t)a.num_decode * a.max_splits;
+  const int64_t units = most * a.kvh * ((a.group + 15) / 16);
   const int64_t cap = (int64_t)i8_decode_groups(D) * cus;
   decode_int8_kernel<D><<<(unsigned)(units < cap ? units : cap), kI8Threads, 0, s>>>(a);
   if (a.max_splits > 1) {
-    const dim3 merge((a.kvh * a.row_slots + kI8Waves - 1) / kI8Waves, a.num_seqs);
-    decode_int8_merge_kernel<D><<<merge, kI8Threads, 0, s>>>(a);
+    const int64_t slots = (int64_t)a.num_decode * a.heads +
+                          (int64_t)(a.num_seqs - a.num_decode) * a.kvh * a.row_slots;
+    decode_int8_merge_kernel<D><<<(unsigned)((slots + kI8Waves - 1) / kI8Waves), kI8Threads, 0, s>>>(a);
   }
   return check_launch("paged_attention_int8");
 }
@@ -148,14 +157,15 @@ extern "C" int ts_paged_attention_int8(const void* q, int64_t q_stride_t, int64_
   a.ks = k_scale, a.vs = v_scale, a.num_blocks = num_blocks;
   a.block_tables = block_tables, a.bt_stride = bt_stride, a.max_blocks = max_blocks_per_seq;
   a.seq_lens = seq_lens, a.heads = num_heads, a.kvh = num_kv_heads;
+  a.by_kvh = I8Div::by(num_kv_heads), a.by_group = I8Div::by(num_heads / num_kv_heads);
   a.group = num_heads / num_kv_heads, a.qsl = query_start_loc, a.num_tokens = num_tokens;
   a.sl2 = scale * 1.44269504088896340736f;
   // the kernels count rows in 31 bits
-  TS_REQUIRE(num_tokens * a.group < (1ll << 30) && pl.small < (1 << 16), TS_ERR_UNSUPPORTED,
+  TS_REQUIRE(num_tokens * a.group < (1ll << 30) && pl.slots < (1ll << 30), TS_ERR_UNSUPPORTED,
              "paged_attention_int8: %lld tokens of %d sequences", (long long)num_tokens, num_seqs);
   if (pl.small > 0) {
     a.num_seqs = pl.small, a.num_decode = num_decode;
-    a.row_slots = pl.row_slots, a.max_splits = pl.max_splits;
+    a.row_slots = pl.row_slots, a.max_splits = pl.max_splits, a.by_slots = I8Div::by(pl.row_slots);
     a.part_o = reinterpret_cast<float*>(ws + pl.dec_o);
     a.part_ml = reinterpret_cast<float*>(ws + pl.dec_ml);
     switch (head_dim) {
@@ -173,9 +183,10 @@ extern "C" int ts_paged_attention_int8(const void* q, int64_t q_stride_t, int64_
     p.a.part_o = reinterpret_cast<float*>(ws + pl.pre_o);
     p.a.part_ml = reinterpret_cast<float*>(ws + pl.pre_ml);
     p.num_seqs = num_seqs, p.first = pl.small, p.tiles = pl.tiles, p.groups = pl.groups;
+    p.by_tiles = I8Div::by(pl.tiles);
     // ... and steps
     const int64_t units = (int64_t)(num_seqs - pl.small) * pl.tiles * num_kv_heads;
-    TS_REQUIRE(units * (max_blocks_per_seq / kI8StepBlocks + 2) < (1ll << 31) && units * 256 < (1ll << 31),
+    TS_REQUIRE(units * (max_blocks_per_seq / kI8StepBlocks + 2 + kI8TileCost) < (1ll << 31) && units * 256 < (1ll << 31),
                TS_ERR_UNSUPPORTED, "paged_attention_int8: %lld tokens in chunks of up to %d",
                (long long)num_tokens, max_query_len);
     switch (head_dim) {

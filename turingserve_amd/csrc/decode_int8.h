@@ -29,6 +29,22 @@ __host__ __device__ inline int i8_splits(int nb, int most, int each = kI8SplitBl
   return n < 1 ? 1 : (n > most ? most : n);
 }
 
+// Division of 0 <= x < 2^31 by a number that the host knows: x * mul >> 32 >> shift, with mul =
+// ceil(2^(31 + l) / d) and shift = l - 1 for 2^(l - 1) < d <= 2^l, which is exact there.
+struct I8Div {
+  unsigned mul;
+  int shift;                             // -1: by 1
+  __host__ __device__ static I8Div by(int d) {
+    if (d <= 1) return {0, -1};
+    int l = 1;
+    while ((1ll << l) < d) ++l;
+    return {(unsigned)(((1ull << (31 + l)) + d - 1) / d), l - 1};
+  }
+  __device__ __forceinline__ int operator()(int x) const {
+    return shift < 0 ? x : (int)(__umulhi((unsigned)x, mul) >> shift);
+  }
+};
+
 struct Int8DecodeArgs {
   const half_t* q;
   int64_t q_st, q_sh;
@@ -44,9 +60,12 @@ struct Int8DecodeArgs {
   int64_t num_tokens;
   int num_seqs, num_decode;                      // sequences; the first num_decode have one row each
   int heads, kvh, group;                         // group = heads / kvh
+  I8Div by_kvh, by_group, by_slots;
   float sl2;                                     // scale * log2(e)
-  int row_slots, max_splits;                     // rows per (sequence, KV head), splits of the partials
-  float *part_o, *part_ml;                       // [S, KVH, row_slots, max_splits, D], [.., 2]
+  // Partials [slots, max_splits, D] and (m, l) [slots, max_splits, 2]: group slots per (sequence, KV
+  // head) of the first num_decode sequences, then row_slots for the others.
+  int row_slots, max_splits;
+  float *part_o, *part_ml;
 };
 
 // The rows of a sequence.
@@ -67,6 +86,13 @@ __device__ __forceinline__ I8Seq i8_seq(const Int8DecodeArgs& a, int b) {
   s.kv = i8_kv_len(len, a.max_blocks);
   s.start = max(len, 0) - s.n;
   return s;
+}
+
+// The partials' slot of a row.
+__device__ __forceinline__ int64_t i8_slot(const Int8DecodeArgs& a, int b, int h, int row) {
+  return b < a.num_decode
+             ? (int64_t)(b * a.kvh + h) * a.group + row
+             : (int64_t)a.num_decode * a.heads + (int64_t)((b - a.num_decode) * a.kvh + h) * a.row_slots + row;
 }
 
 // Splits of a sequence's blocks: longer ones where several tiles of rows share them, one where its
@@ -393,10 +419,10 @@ __device__ __forceinline__ void i8_finish(const Int8DecodeArgs& a, I8State<D>& s
     }
     if (splits == 1) {
       const float f = sum == 0.f ? 0.f : kColumnUnit * vref / sum;   // no visible key: zeros
-      const int token = (row0 + row) / a.group, head = h * a.group + (row0 + row) % a.group;
+      const int token = a.by_group(row0 + row), head = h * a.group + row0 + row - token * a.group;
       ts::st<half4_t>(a.out + (int64_t)(q0 + token) * a.out_st + (int64_t)head * D + d, to_half4(o * f));
     } else {
-      const int64_t at = (((int64_t)b * a.kvh + h) * a.row_slots + row0 + row) * a.max_splits + split;
+      const int64_t at = i8_slot(a, b, h, row0 + row) * a.max_splits + split;
       ts::st<float4_t>(a.part_o + at * D + d, o * (kColumnUnit * vref));
       if (d == 0) {
         a.part_ml[2 * at] = top;
@@ -450,14 +476,14 @@ __global__ void __launch_bounds__(kI8Threads, i8_decode_groups(D)) decode_int8_k
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int lane = threadIdx.x % kWave, c = lane % 16, g = lane / 16;
   for (int64_t u = blockIdx.x;; u += gridDim.x) {
-    const int64_t item = u / (unsigned)a.kvh;
-    const int h = (int)(u - item * a.kvh);
+    if (u > INT32_MAX) return;
+    const int item = a.by_kvh((int)u), h = (int)u - item * a.kvh;
     I8Item x;
-    if (item > INT32_MAX || !i8_find(a, (int)item, x)) return;
+    if (!i8_find(a, item, x)) return;
     const int row0 = 16 * x.tile, rows = min(x.seq.n * a.group - row0, 16), kv = x.seq.kv;
-    const int row = row0 + min(c, rows - 1), token = row / a.group;
+    const int row = row0 + min(c, rows - 1), token = a.by_group(row);
     const int vis = min(kv, max(0, x.seq.start + token + 1));
-    const int least = min(kv, max(0, x.seq.start + row0 / a.group + 1));
+    const int least = min(kv, max(0, x.seq.start + a.by_group(row0) + 1));
     I8Query<D> q;
     i8_load_q<D>(a.q + (int64_t)(x.seq.q0 + token) * a.q_st + (int64_t)(h * a.group + row - token * a.group) * a.q_sh,
                  g, c < rows, q);
@@ -482,12 +508,15 @@ template <int D>
 __global__ void __launch_bounds__(kI8Threads) decode_int8_merge_kernel(Int8DecodeArgs a) {
   constexpr int PER_ROW = D / 4, GROUPS = kWave / PER_ROW;
   constexpr int N = 64 / GROUPS < 16 ? 64 / GROUPS : 16;   // partials of a lane at a time
-  const int b = blockIdx.y, lane = threadIdx.x % kWave;
+  const int lane = threadIdx.x % kWave;
   const int slot = blockIdx.x * kI8Waves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int h = slot / a.row_slots, r = slot - h * a.row_slots;
-  if (h >= a.kvh) return;
+  const int behind = slot - a.num_decode * a.heads;        // of the sequences past num_decode
+  const int unit = behind < 0 ? a.by_group(slot) : a.by_slots(behind);
+  const int r = behind < 0 ? slot - unit * a.group : behind - unit * a.row_slots;
+  const int seq0 = a.by_kvh(unit), h = unit - seq0 * a.kvh, b = behind < 0 ? seq0 : a.num_decode + seq0;
+  if (b >= a.num_seqs) return;
   const int group = lane / PER_ROW, d = lane % PER_ROW * 4;
-  const int64_t row = (((int64_t)b * a.kvh + h) * a.row_slots + r) * a.max_splits;
+  const int64_t row = (int64_t)slot * a.max_splits;
   const float* part = a.part_o + row * D + d;
   const float2_t ml = ld<float2_t>(a.part_ml + 2 * (row + min(lane, a.max_splits - 1)));
   float4_t x[N];
@@ -527,7 +556,7 @@ __global__ void __launch_bounds__(kI8Threads) decode_int8_merge_kernel(Int8Decod
     for (int e = 0; e < 4; ++e) o[e] += shfl_xor(o[e], k);
   if (group > 0) return;
   const float inv = sum == 0.f ? 0.f : 1.f / sum;          // (nothing visible)
-  const int token = r / a.group, head = h * a.group + r - token * a.group;
+  const int token = a.by_group(r), head = h * a.group + r - token * a.group;
   st<half4_t>(a.out + (int64_t)(seq.q0 + token) * a.out_st + (int64_t)head * D + d, to_half4(o * inv));
 }
 

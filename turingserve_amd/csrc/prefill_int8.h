@@ -33,7 +33,7 @@ typedef float float16_t __attribute__((ext_vector_type(16)));
 constexpr int kI8Keys = 64;              // tokens of a step
 constexpr int kI8StepBlocks = kI8Keys / kBlockSize;
 constexpr int kI8Window = 256;           // blocks whose ids and scales are held in LDS at a time
-constexpr int kI8MinShare = 4;           // steps that a workgroup is worth
+constexpr int kI8MinShare = 8;           // steps (and tiles' costs) that a workgroup is worth
 constexpr float kI8LeastRatio = -30.f;   // log2 of the least V scale ratio
 constexpr float kI8LeastFactor = 1e-30f;
 constexpr int kI8Kept = 4;               // times 64 pairs (sequence, tile) whose steps are kept
@@ -47,6 +47,7 @@ struct Int8PrefillArgs {
   Int8DecodeArgs a;                      // (part_o, part_ml: two partials of a tile per workgroup)
   int num_seqs, first;                   // sequences first .. num_seqs - 1
   int tiles;                             // of the longest chunk by the host's bound
+  I8Div by_tiles;
   int groups;                            // workgroups of the main launch
 };
 
@@ -101,13 +102,19 @@ __device__ __forceinline__ int i8_sees(const I8Chunk& k, int token) {
   return max(0, min(k.kv, k.start + token + 1));
 }
 
-// Steps of tile t of a chunk: one at least, so that somebody writes the rows.
+// A tile counts as kI8TileCost steps more than it has: what its start costs (the sequence's lookup,
+// q, the first blocks' ids, scales and codes, one after the other: 11 to 15 thousand cycles beside 2.8
+// thousand a step at head_dim 64). Steps of a share that fall on them are nobody's.
+constexpr int kI8TileCost = 4;
+
+// What tile t of a chunk counts for: its steps (one at least, so that somebody writes the rows) behind
+// kI8TileCost.
 template <int ROWS>
-__device__ __forceinline__ int i8_steps(const I8Chunk& k, int group, int t) {
-  const int rows = k.n * group;
+__device__ __forceinline__ int i8_steps(const Int8DecodeArgs& a, const I8Chunk& k, int t) {
+  const int rows = k.n * a.group;
   if (t * ROWS >= rows) return 0;
-  const int sees = i8_sees(k, (min(rows, (t + 1) * ROWS) - 1) / group);
-  return max(1, (sees + kI8Keys - 1) / kI8Keys);
+  const int sees = i8_sees(k, a.by_group(min(rows, (t + 1) * ROWS) - 1));
+  return kI8TileCost + max(1, (sees + kI8Keys - 1) / kI8Keys);
 }
 
 // Where the batch's steps lie: pairs (sequence, tile) in order, each with all its KV heads.
@@ -125,7 +132,8 @@ struct I8Walk {
 
   static __device__ __forceinline__ int steps(const Int8PrefillArgs& p, int pair) {
     if (pair >= (p.num_seqs - p.first) * p.tiles) return 0;
-    return i8_steps<ROWS>(i8_chunk(p, p.first + pair / p.tiles), p.a.group, pair % p.tiles);
+    const int seq = p.by_tiles(pair);
+    return i8_steps<ROWS>(p.a, i8_chunk(p, p.first + seq), pair - seq * p.tiles);
   }
   __device__ __forceinline__ I8Walk(const Int8PrefillArgs& p) {
     const int lane = threadIdx.x % kWave, pairs = (p.num_seqs - p.first) * p.tiles;
@@ -249,14 +257,14 @@ struct I8Stage {
         off[i] = {o, o};
       }
   }
-  __device__ __forceinline__ void request_v(const Int8DecodeArgs& a, const int (&id)[N], int h) {
+  // Row r of the 4 tokens (one at a time, so that they stand between other work).
+  __device__ __forceinline__ void request_v(const Int8DecodeArgs& a, const int (&id)[N], int h, int r) {
 #pragma unroll
     for (int i = 0; i < N; ++i)
       if (ALL || unit(i) < UNITS) {
         const int in = unit(i) % D;                        // 4 tokens at 4 (in / (D / 4)), 4 dims
         const int8_t* p = a.vc + base(a, id[i], h) + (4 * (in / (D / 4)) * D + 4 * (in % (D / 4)));
-#pragma unroll
-        for (int r = 0; r < 4; ++r) v[i][r] = ld<uint32_t>(p + r * D);
+        v[i][r] = ld<uint32_t>(p + r * D);
       }
   }
   __device__ __forceinline__ void place_k(half_t* tile) const {
@@ -364,9 +372,9 @@ struct I8Exp {
 //   maxima of the next scores, more staging  beside  O += V P' of this step's first half
 // so that no second set of scores is needed (two wavefronts share a SIMD's registers). The order is
 // pinned, MFMA by MFMA: left to itself the compiler sets MFMAs and exponentials one after the other.
-// The workgroup meets between the third phase and the fourth: K is staged before, over what the
-// step before read, and V behind it, over what the first phase read. Returns each row's largest
-// next score.
+// The workgroup meets behind the first phase, with no LDS read under way: what the step before staged
+// (K in its third phase, V in its fourth) is read behind that, and this step stages over what was
+// read before it. Returns each row's largest next score.
 template <int D, typename Mask, typename Work>
 __device__ __forceinline__ float i8_step64(I8Rows<D>& w, const half_t* vp, const half_t* kn, const half_t* vc,
                                            float16_t (&sc)[2], half8_t (&pr)[4], const float* fkp,
@@ -377,25 +385,29 @@ __device__ __forceinline__ float i8_step64(I8Rows<D>& w, const half_t* vp, const
   half8_t op[AHEAD];
   const float4_t fk = ld<float4_t>(fkp), fv = ld<float4_t>(fvp);
 #pragma unroll
-  for (int j = 0; j < AHEAD; ++j) op[j] = w.operand(vp, kn, vc, j);
+  for (int j = 0; j < AHEAD && j < NP; ++j) op[j] = w.operand(vp, kn, vc, j);
   const float4_t back = ld<float4_t>(backp);
-  auto next = [&](int j) {                                 // operand j, and the request of a later one
+  // Operand j, and the request of a later one below `end`. (The ring starts anew behind the barrier.)
+  auto next = [&](int j, int end) {
     const half8_t x = op[j % AHEAD];
-    if (j + AHEAD < R::ALL) op[j % AHEAD] = w.operand(vp, kn, vc, j + AHEAD);
+    if (j + AHEAD < end) op[j % AHEAD] = w.operand(vp, kn, vc, j + AHEAD);
     return x;
   };
   const float neg = w.m == -INFINITY ? 0.f : -w.m;
   const float off[4] = {neg + fv[0], neg + fv[1], neg + fv[2], neg + fv[3]};
-  work(0);                                                 // global requests
   // exponentials: NP + NQ shares beside the first two phases' MFMAs where both have as many
   constexpr int N = 2 * (NP < NQ ? NP : NQ);
   I8Exp ex;
 #pragma unroll
   for (int j = 0; j < NP; ++j) {
-    w.o[j % R::DT] = mfma_i8(next(j), pr[2 + j / R::DT], w.o[j % R::DT]);
+    w.o[j % R::DT] = mfma_i8(next(j, NP), pr[2 + j / R::DT], w.o[j % R::DT]);
     if (j < N / 2) ex.share<N>(j, sc, fk, off, back, w.l, pr);
+    if (j == 0) work(0);                                   // requests of K, V to come
     __builtin_amdgcn_sched_barrier(0);
   }
+  __syncthreads();
+#pragma unroll
+  for (int j = NP; j < NP + AHEAD; ++j) op[j % AHEAD] = w.operand(vp, kn, vc, j);
   if (w.moved) {
 #pragma unroll
     for (int i = 0; i < R::DT; ++i) w.o[i] *= w.alpha;
@@ -405,13 +417,14 @@ __device__ __forceinline__ float i8_step64(I8Rows<D>& w, const half_t* vp, const
   for (int i = 0; i < 16; ++i) zero[i] = 0.f;
 #pragma unroll
   for (int j = 0; j < NQ; ++j) {
-    sc[0] = mfma_i8(next(NP + j), w.q[j], j == 0 ? zero : sc[0]);
+    sc[0] = mfma_i8(next(NP + j, R::ALL), w.q[j], j == 0 ? zero : sc[0]);
     if (j < N / 2) ex.share<N>(N / 2 + j, sc, fk, off, back, w.l, pr);
+    for (int v = j * 4 / NQ; v < (j + 1) * 4 / NQ; ++v) work(3 + v);
     __builtin_amdgcn_sched_barrier(0);
   }
 #pragma unroll
   for (int j = 0; j < NQ; ++j) {
-    sc[1] = mfma_i8(next(NP + NQ + j), w.q[j], j == 0 ? zero : sc[1]);
+    sc[1] = mfma_i8(next(NP + NQ + j, R::ALL), w.q[j], j == 0 ? zero : sc[1]);
     if (j < 2) ex.share<N>(N + j, sc, fk, off, back, w.l, pr);
     if (NQ < 2) ex.share<N>(N + 1, sc, fk, off, back, w.l, pr);
     if (j == NQ / 4) work(1);                              // K of a later step to LDS
@@ -419,11 +432,10 @@ __device__ __forceinline__ float i8_step64(I8Rows<D>& w, const half_t* vp, const
   }
   const float4_t fkn = ld<float4_t>(fknp);
   mask(sc);
-  __syncthreads();
   float top[4];
 #pragma unroll
   for (int j = 0; j < NP; ++j) {
-    w.o[j % R::DT] = mfma_i8(next(NP + 2 * NQ + j), pr[j / R::DT], w.o[j % R::DT]);
+    w.o[j % R::DT] = mfma_i8(next(NP + 2 * NQ + j, R::ALL), pr[j / R::DT], w.o[j % R::DT]);
 #pragma unroll
     for (int i = j * 32 / NP; i < (j + 1) * 32 / NP; ++i) {
       const int b = i / 2 % 4, e = i / 8 * 2 + i % 2;      // two scores of each block in turn
@@ -464,10 +476,10 @@ __device__ __forceinline__ void i8_piece(const Int8PrefillArgs& p, I8PrefillLds<
   const int lane = threadIdx.x % kWave, c = lane % 32, hh = lane / 32;
   const int rows = k.n * a.group, wrow = tile * ROWS + 32 * wave;
   const int row = min(wrow + c, rows - 1);                 // (rows past the last one stand in for it)
-  const int token = row / a.group, head = h * a.group + row % a.group, vis = i8_sees(k, token);
+  const int token = a.by_group(row), head = h * a.group + row - token * a.group, vis = i8_sees(k, token);
   // rows ascend in tokens: the wavefront's first row sees least
-  const int least = i8_sees(k, min(wrow, rows - 1) / a.group);
-  const int sees = i8_sees(k, (min(rows, (tile + 1) * ROWS) - 1) / a.group);
+  const int least = i8_sees(k, a.by_group(min(wrow, rows - 1)));
+  const int sees = i8_sees(k, a.by_group(min(rows, (tile + 1) * ROWS) - 1));
   const int nb = (sees + kBlockSize - 1) / kBlockSize;     // blocks that the tile sees
   R w;
   w.kat = I8Tile<D>::k_at(c, hh);
@@ -559,9 +571,9 @@ __device__ __forceinline__ void i8_piece(const Int8PrefillArgs& p, I8PrefillLds<
       auto work = [&](int part) {
         if (part == 0) {
           stage.request_k(a, id1, h);
-          stage.request_v(a, id0, h);
           S::ids(lds, (i + 3) * kI8StepBlocks, last, id2);
         }
+        if (part >= 3) stage.request_v(a, id0, h, part - 3);
         if (part == 1) stage.place_k(lds.k[P]);
         if (part == 2) stage.place_v(lds.v[1 - P]);
       };
@@ -616,8 +628,12 @@ __device__ __forceinline__ void i8_piece(const Int8PrefillArgs& p, I8PrefillLds<
     }
 }
 
-// Wavefronts of a workgroup; a CU holds one by registers.
-constexpr int i8_prefill_waves(int D) { return D > 128 ? 4 : 8; }
+// Wavefronts of a workgroup, and the workgroups that a CU holds by registers. At head_dim 128 eight
+// wavefronts stage a step together (85 us at 2048 rows on 4096 cached, 12/2 heads; two workgroups of
+// four 102 us); at 64 and below a step's codes are one unit a thread for four (27 us against 40 at
+// five chunks of 90 to 1100 rows, 14/2 heads).
+constexpr int i8_prefill_waves(int D) { return D == 128 ? 8 : 4; }
+constexpr int i8_prefill_groups(int D) { return D > 128 ? 1 : 8 / i8_prefill_waves(D); }
 
 template <int D>
 __global__ void __launch_bounds__(i8_prefill_waves(D) * kWave, D > 128 ? 1 : 2)
@@ -634,28 +650,30 @@ prefill_int8_kernel(Int8PrefillArgs p) {
     const I8Shares shares(total, p.groups);
     if ((int)blockIdx.x >= shares.count) return;
     at = shares.begin(blockIdx.x), hi = shares.begin(blockIdx.x + 1);
-    place = walk.find(p, (int)((unsigned)at / (unsigned)a.kvh));
+    place = walk.find(p, a.by_kvh(at));
     if (threadIdx.x < kWave) walk.save(lds.n, lds.scan);
   }
   int b = 0, h = 0, tile = 0;
   for (bool extra = false, more = false; extra || at < hi;) {
     int s0 = 0, s1, steps;
     if (!extra) {
-      if (more) place = I8Walk<ROWS>(lds.n, lds.scan).find(p, (int)((unsigned)at / (unsigned)a.kvh));
-      more = true;                                         // (i8_piece meets between the save and this)
+      if (more) place = I8Walk<ROWS>(lds.n, lds.scan).find(p, a.by_kvh(at));
+      if (!more) __syncthreads();                          // (saved)
+      more = true;
       const unsigned in = at - place.before * a.kvh;
-      steps = place.steps;
-      h = (int)(in / (unsigned)steps), s0 = (int)(in % (unsigned)steps);
-      s1 = min(steps, s0 + (hi - at));
-      b = p.first + place.pair / p.tiles, tile = place.pair % p.tiles;
-      at += s1 - s0;
+      h = (int)(in / (unsigned)place.steps);
+      const int c0 = (int)in - h * place.steps, c1 = min(place.steps, c0 + (hi - at));
+      b = p.by_tiles(place.pair), tile = place.pair - b * p.tiles, b += p.first;
+      at += c1 - c0;
+      steps = place.steps - kI8TileCost, s0 = max(0, c0 - kI8TileCost), s1 = c1 - kI8TileCost;
+      if (s1 <= s0) continue;
     }
     const I8Chunk k = i8_chunk(p, b);
-    if (extra) s1 = steps = i8_steps<ROWS>(k, a.group, tile);
+    if (extra) s1 = steps = i8_steps<ROWS>(a, k, tile) - kI8TileCost;
     i8_piece<D, WAVES>(p, lds, k, b, tile, h, s0, s1, s0 == 0 && s1 == steps, 2 * blockIdx.x + (s0 == 0));
     // Tiles past the host's bound on the rows follow, whole, the first step of the last tile that it
     // allows for.
-    extra = (extra || (tile == p.tiles - 1 && s0 == 0)) && i8_steps<ROWS>(k, a.group, tile + 1) > 0;
+    extra = (extra || (tile == p.tiles - 1 && s0 == 0)) && i8_steps<ROWS>(a, k, tile + 1) > 0;
     if (extra) ++tile;
   }
 }
@@ -668,16 +686,16 @@ __global__ void __launch_bounds__(256) prefill_int8_merge_kernel(Int8PrefillArgs
   const Int8DecodeArgs& a = p.a;
   const int unit = blockIdx.x / (ROWS / kI8MergeRows);
   const int row0 = (int)(blockIdx.x % (ROWS / kI8MergeRows)) * kI8MergeRows;
-  const int h = unit % a.kvh, pair = unit / a.kvh;
-  const int b = p.first + pair / p.tiles, tile = pair % p.tiles;
+  const int pair = a.by_kvh(unit), h = unit - pair * a.kvh;
+  const int seq = p.by_tiles(pair), b = p.first + seq, tile = pair - seq * p.tiles;
   const I8Chunk k = i8_chunk(p, b);
   const int rows = k.n * a.group;
   if (tile * ROWS + row0 >= rows) return;
   const I8Walk<ROWS> walk(p);
-  const int steps = i8_steps<ROWS>(k, a.group, tile);
+  const int steps = i8_steps<ROWS>(a, k, tile);
   const I8Shares shares(walk.total * a.kvh, p.groups);
   const int g0 = walk.before(p, pair) * a.kvh + h * steps;
-  const int first = shares.of(g0), last = shares.of(g0 + steps - 1);
+  const int first = shares.of(g0 + kI8TileCost), last = shares.of(g0 + steps - 1);
   if (first == last) return;                               // one workgroup wrote it
   const int d = threadIdx.x % (D / 4) * 4;
   for (int in = row0 + threadIdx.x / (D / 4); in < row0 + kI8MergeRows; in += PER) {
@@ -710,7 +728,7 @@ __global__ void __launch_bounds__(256) prefill_int8_merge_kernel(Int8PrefillArgs
       }
     }
     const float f = sum == 0.f ? 0.f : 1.f / sum;
-    const int token = row / a.group, head = h * a.group + row % a.group;
+    const int token = a.by_group(row), head = h * a.group + row - token * a.group;
     st<half4_t>(a.out + (int64_t)(k.q0 + token) * a.out_st + (int64_t)head * D + d, to_half4(o * f));
   }
 }
