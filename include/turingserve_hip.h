@@ -516,12 +516,12 @@ int ts_silu_mul(const void* gu, int64_t gu_stride, void* out, int64_t out_stride
  *   code'  = rint(code * (scale / scale')) of the earlier rows when scale' > scale
  *   code   = rint(row / scale') of the new rows                       (fp32, ties to even)
  * A block whose row 0 is written starts anew; rows past the sequence's end keep their codes. New
- * rows that are not finite make scale' NaN (and their codes 0). Blocks are owned by one wavefront
+ * rows that are not finite make scale' NaN (and their codes 0). Blocks are owned by one workgroup
  * each, so no two sequences of a call may write into the same block (their rows would race; no
  * access leaves the cache). Block ids outside [0, num_blocks) and blocks past max_blocks_per_seq
  * are skipped. max_query_len shapes the launch only: a bound below the real one is slower, not
- * wrong. k / v rows fp16, aligned to 16 bytes (8 at head_dim 32, 4 at head_dim 16); head_dim 16,
- * 32, 64, 128 or 256.
+ * wrong. k / v rows fp16, aligned to head_dim / 16 bytes (2 at least); head_dim 16, 32, 64, 128 or
+ * 256.
  *
  * ts_rope_kv_write_int8: the same for the k and v heads of qkv [T, (H + 2 KVH) D], k rotated first
  * (rotate-half RoPE by the fp32 tables, computed in 64 bits and rounded to fp32), with the rotated q

@@ -116,7 +116,7 @@ odd = ctypes.c_void_p(258)
     (_write, dict(D=96), N.TS_ERR_UNSUPPORTED, "head_dim 96"),
     (_write, dict(bts=3), N.TS_ERR_INVALID_ARG, "bt_stride"),
     (_write, dict(mb=0), N.TS_ERR_INVALID_ARG, "max_blocks"),
-    (_write, dict(kst=68), N.TS_ERR_INVALID_ARG, "aligned"),
+    (_write, dict(kst=67), N.TS_ERR_INVALID_ARG, "aligned"),
     (_write, dict(k=odd), N.TS_ERR_INVALID_ARG, "aligned"),
     (_write, dict(vc=odd), N.TS_ERR_INVALID_ARG, "aligned"),
     (_write, dict(seqs=1 << 30, mq=1 << 20), N.TS_ERR_UNSUPPORTED, "workgroups"),

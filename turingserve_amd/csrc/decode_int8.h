@@ -106,32 +106,6 @@ __device__ __forceinline__ int i8_splits(const Int8DecodeArgs& a, const I8Seq& s
   return i8_splits((s.kv + kBlockSize - 1) / kBlockSize, a.max_splits, each);
 }
 
-// Wavefront scans on the VALU (DPP row shifts, then the rows' last lanes broadcast on): a step costs
-// a few cycles where a shuffle through the LDS unit costs over a hundred, and both scans stand in
-// front of a workgroup's first K/V request.
-template <int CTRL, int ROWS>
-__device__ __forceinline__ int i8_dpp(int v) {             // 0 where no lane moves in
-  return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
-}
-__device__ __forceinline__ int i8_scan(int v) {            // inclusive sums
-  v += i8_dpp<0x111, 0xf>(v);
-  v += i8_dpp<0x112, 0xf>(v);
-  v += i8_dpp<0x114, 0xf>(v);
-  v += i8_dpp<0x118, 0xf>(v);
-  v += i8_dpp<0x142, 0xa>(v);
-  return v + i8_dpp<0x143, 0xc>(v);
-}
-__device__ __forceinline__ float i8_most(float x) {        // the largest of 64 values >= 0
-  int v = __float_as_int(x);
-  v = max(v, i8_dpp<0x111, 0xf>(v));
-  v = max(v, i8_dpp<0x112, 0xf>(v));
-  v = max(v, i8_dpp<0x114, 0xf>(v));
-  v = max(v, i8_dpp<0x118, 0xf>(v));
-  v = max(v, i8_dpp<0x142, 0xa>(v));
-  v = max(v, i8_dpp<0x143, 0xc>(v));
-  return __int_as_float(__builtin_amdgcn_readlane(v, kWave - 1));
-}
-
 // Tokens of a sequence that its table holds.
 __device__ __forceinline__ int i8_kv_len(int len, int max_blocks) {
   const int64_t most = (int64_t)max_blocks * kBlockSize;

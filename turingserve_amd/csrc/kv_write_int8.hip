@@ -8,9 +8,12 @@
 // the sequence's end keep their codes. A row that is not finite makes its block's scale NaN, so
 // that whatever attends to the block comes out NaN and nothing finite is made up.
 //
-// One wavefront owns one (block, KV head, K or V): it holds the whole block in registers (four
-// lanes a row), so the maximum, the scale and every row's rewrite need no other wavefront and the
-// result does not depend on the order of anything. A sequence's blocks are found from the step's
+// One workgroup owns one (block, KV head, K or V): it holds the whole block in registers (sixteen
+// lanes a row; a single new row, as a decode step appends, over D / 2 threads), so the maximum, the
+// scale and every row's rewrite need no other workgroup and the result does not depend on the order
+// of anything. A launch is bound by its chain of dependent loads (lengths, then block id, rows and
+// positions, then codes, scale and angles), so each link asks for everything it can before it waits.
+// A sequence's blocks are found from the step's
 // metadata (query_start_loc, seq_lens, block tables), not from slots: the rows of a block then lie
 // together and its owner knows them without a search. The rest of the grid (RoPE form) rotates q.
 #include <float.h>
@@ -20,20 +23,18 @@
 
 namespace ts {
 
-constexpr int kWriteWaves = 4;
+constexpr int kWriteThreads = 256;
 
-// A lane's share of a row: D / 4 elements in pieces of VEC, piece p at element (4 p + s) * VEC.
-// The pieces of the first half of a row and their rotation partners in the second half belong to
-// the same lane.
+// A thread's share of a row: VEC elements of its first half and their rotation partners in the
+// second. Sixteen lanes hold a row (eight at head_dim 16, the others then nothing).
 template <int D>
 struct RowShare {
-  static constexpr int VEC = D >= 64 ? 8 : D / 8;
-  static constexpr int PIECES = D / (4 * VEC);
+  static constexpr int VEC = D >= 32 ? D / 32 : 1;
+  static constexpr int LANES = D / (2 * VEC);
   typedef _Float16 Halves __attribute__((ext_vector_type(VEC)));
   typedef int8_t Codes __attribute__((ext_vector_type(VEC)));
   typedef float Floats __attribute__((ext_vector_type(VEC)));
 };
-
 struct Int8WriteArgs {
   const half_t *k, *v;                    // rows of the step (k, v heads)
   int64_t k_st, k_sh, v_st, v_sh;
@@ -44,7 +45,7 @@ struct Int8WriteArgs {
   int64_t bt_stride;
   int max_blocks;
   const int32_t *seq_lens, *qsl;
-  int num_seqs, num_decode, chunk_slots;  // slots (wavefront groups) of a sequence past num_decode
+  int num_seqs, num_decode, chunk_slots;  // slots (workgroups a unit) of a sequence past num_decode
   int64_t num_tokens;
   int kvh;
   // RoPE form
@@ -58,112 +59,164 @@ struct Int8WriteArgs {
   int64_t kv_groups;                      // workgroups before the first q workgroup
 };
 
-// Rotation of a K row in 64 bits, rounded once to 32: a row's code is decided by the quotient's
+// Rotation of a pair of K in 64 bits, rounded once to 32: a row's code is decided by the quotient's
 // last bits, and the products (11 x 24 bits) are exact here.
-template <int D, typename V>
-__device__ __forceinline__ void rotate_k(V& lo, V& hi, const float* cp, const float* sp) {
-#pragma unroll
-  for (int e = 0; e < RowShare<D>::VEC; ++e) {
-    const double c = cp[e], s = sp[e], a = lo[e], b = hi[e];
-    lo[e] = (float)fma(-b, s, a * c);
-    hi[e] = (float)fma(a, s, b * c);
-  }
+__device__ __forceinline__ void rotate_k(float& lo, float& hi, float cos, float sin) {
+  const double c = cos, s = sin, a = lo, b = hi;
+  lo = (float)fma(-b, s, a * c);
+  hi = (float)fma(a, s, b * c);
 }
+
+// The largest |value| of the wavefront; a NaN's bits are above every number's.
+__device__ __forceinline__ float largest(float x) { return i8_most(fabsf(x)); }
+__device__ __forceinline__ float larger(float a, float b) {
+  return __int_as_float(max(__float_as_int(fabsf(a)), __float_as_int(fabsf(b))));
+}
+
+// The block's new scale. NaN where a new value or the old scale is not finite.
+__device__ __forceinline__ float grown(float was, float top) {
+  return top <= FLT_MAX ? vmax(was, top / kCodeMax) : __builtin_nanf("");
+}
+
+// rint(x / scale) for |x| <= 127 scale, by a reciprocal where that decides it: x * rcp is within
+// 127 * 2^-22 of the quotient, so it rounds alike unless it lies that close to a half. `near` is set
+// where the division has to be made.
+__device__ __forceinline__ float code_of(float x, float rcp, bool& near) {
+  const float y = x * rcp, c = rintf(y);
+  near = near || fabsf(fabsf(y - c) - 0.5f) < 1.f / 16384.f;
+  return c;
+}
+__device__ __forceinline__ float exact_code(float x, float scale) {
+  return fminf(fmaxf(rintf(x / scale), -kCodeMax), kCodeMax);
+}
+
+// Both segments of a thread's share of row r of a block.
+template <int D>
+struct RowCodes {
+  typedef RowShare<D> R;
+  typename R::Codes a, b;
+  __device__ __forceinline__ void load(const int8_t* block, int r, int s) {
+    a = ld<typename R::Codes>(block + r * D + s * R::VEC);
+    b = ld<typename R::Codes>(block + r * D + s * R::VEC + D / 2);
+  }
+  __device__ __forceinline__ void store(int8_t* block, int r, int s) const {
+    st(block + r * D + s * R::VEC, a);
+    st(block + r * D + s * R::VEC + D / 2, b);
+  }
+};
 
 template <int D, bool ROPE, bool IS_K>
-__device__ __forceinline__ void write_block(const Int8WriteArgs& a, int b, int j, int64_t blk, int first,
-                                            int len, int64_t row0, int h) {
+__device__ __forceinline__ void write_block(const Int8WriteArgs& a, int j, int64_t blk, int first, int len,
+                                            int64_t row0, int h, float* s_top) {
   typedef RowShare<D> R;
-  const int lane = threadIdx.x % kWave, r = lane >> 2, s = lane & 3;
+  constexpr bool TURN = ROPE && IS_K;
+  const int tid = threadIdx.x, r = tid >> 4, s = tid & 15;
+  const bool lane = s < R::LANES;
   const int lo = first > 16 * j ? first - 16 * j : 0;      // rows [0, lo) stand there already
   const int hi = min(len - 16 * j, 16);                    // rows [lo, hi) are new
-  const bool fresh = r >= lo && r < hi, old = r < lo;
-  const int64_t t = row0 + 16 * j + r;                     // flat row of a new row
   const int64_t unit = blk * a.kvh + h;
-  int8_t* dst = (IS_K ? a.kc : a.vc) + (unit * kBlockSize + r) * D;
+  int8_t* block = (IS_K ? a.kc : a.vc) + unit * kBlockSize * D;
   float* scale = (IS_K ? a.ks : a.vs) + unit;
-
-  typename R::Floats x[R::PIECES];
-  typename R::Codes code[R::PIECES];
-#pragma unroll
-  for (int p = 0; p < R::PIECES; ++p)
-#pragma unroll
-    for (int e = 0; e < R::VEC; ++e) x[p][e] = 0.f;
-  if (fresh) {
-    const half_t* src = IS_K ? a.k + t * a.k_st + h * a.k_sh : a.v + t * a.v_st + h * a.v_sh;
-#pragma unroll
-    for (int p = 0; p < R::PIECES; ++p) {
-      const typename R::Halves y = ld<typename R::Halves>(src + (4 * p + s) * R::VEC);
-#pragma unroll
-      for (int e = 0; e < R::VEC; ++e) x[p][e] = (float)y[e];
-    }
-    if (ROPE && IS_K) {
-      const int64_t pos = rope_row(a.positions[t], a.max_pos) * (D / 2);
-#pragma unroll
-      for (int p = 0; p < R::PIECES / 2; ++p) {
-        const int at = (4 * p + s) * R::VEC;
-        rotate_k<D>(x[p], x[p + R::PIECES / 2], a.cos_t + pos + at, a.sin_t + pos + at);
-      }
-    }
-  } else if (old) {
-#pragma unroll
-    for (int p = 0; p < R::PIECES; ++p) code[p] = ld<typename R::Codes>(dst + (4 * p + s) * R::VEC);
-  }
+  const half_t* rows = IS_K ? a.k + h * a.k_sh : a.v + h * a.v_sh;
+  const int64_t st_t = IS_K ? a.k_st : a.v_st;
+  const bool old = lane && r < lo;
   const float was = lo > 0 ? *scale : 0.f;
+  RowCodes<D> kept;
+  if (old) kept.load(block, r, s);
 
+  const bool single = hi - lo == 1;
+  RowCodes<D> code;
+  float x1 = 0.f, y1 = 0.f;                                // a single row: one pair a thread
+  typename R::Floats x, y;
+  bool fresh;
   float top = 0.f;
+  if (single) {
+    fresh = tid < D / 2;
+    if (fresh) {
+      const int64_t t = row0 + 16 * j + lo;
+      x1 = (float)rows[t * st_t + tid], y1 = (float)rows[t * st_t + tid + D / 2];
+      if (TURN) {
+        const int64_t pos = rope_row(a.positions[t], a.max_pos) * (D / 2);
+        rotate_k(x1, y1, a.cos_t[pos + tid], a.sin_t[pos + tid]);
+      }
+      top = larger(x1, y1);
+    }
+  } else {
+    fresh = lane && r >= lo && r < hi;
+    if (fresh) {
+      const int64_t t = row0 + 16 * j + r;
+      const typename R::Halves u = ld<typename R::Halves>(rows + t * st_t + s * R::VEC);
+      const typename R::Halves v = ld<typename R::Halves>(rows + t * st_t + s * R::VEC + D / 2);
 #pragma unroll
-  for (int p = 0; p < R::PIECES; ++p)
+      for (int e = 0; e < R::VEC; ++e) x[e] = (float)u[e], y[e] = (float)v[e];
+      if (TURN) {
+        const int64_t pos = rope_row(a.positions[t], a.max_pos) * (D / 2) + s * R::VEC;
+        const typename R::Floats c = ld<typename R::Floats>(a.cos_t + pos);
+        const typename R::Floats n = ld<typename R::Floats>(a.sin_t + pos);
 #pragma unroll
-    for (int e = 0; e < R::VEC; ++e) top = vmax(top, fabsf(x[p][e]));   // NaN stays NaN
+        for (int e = 0; e < R::VEC; ++e) {
+          float f = x[e], g = y[e];
+          rotate_k(f, g, c[e], n[e]);
+          x[e] = f, y[e] = g;
+        }
+      }
 #pragma unroll
-  for (int m = 1; m < kWave; m <<= 1) top = vmax(top, shfl_xor(top, m));
-  const float now = top <= FLT_MAX ? vmax(was, top / kCodeMax) : __builtin_nanf("");
-
-  if (old && now > was) {                                  // false where the scale is NaN
-    const float ratio = was / now;
-#pragma unroll
-    for (int p = 0; p < R::PIECES; ++p) {
-#pragma unroll
-      for (int e = 0; e < R::VEC; ++e) code[p][e] = (int8_t)(int)rintf((float)code[p][e] * ratio);
-      st(dst + (4 * p + s) * R::VEC, code[p]);
+      for (int e = 0; e < R::VEC; ++e) top = larger(top, larger(x[e], y[e]));
     }
   }
-  if (fresh) {
+  top = largest(top);
+  if (tid % kWave == 0) s_top[tid / kWave] = top;
+  __syncthreads();
+  const float now = grown(was, larger(larger(s_top[0], s_top[1]), larger(s_top[2], s_top[3])));
+
+  if (fresh && single) {
+    int8_t* dst = block + lo * D + tid;
+    dst[0] = now > 0.f ? (int8_t)(int)exact_code(x1, now) : (int8_t)0;
+    dst[D / 2] = now > 0.f ? (int8_t)(int)exact_code(y1, now) : (int8_t)0;
+  } else if (fresh) {
+    const float rcp = now >= FLT_MIN ? 1.f / now : 0.f;    // (scales below the normal numbers divide)
+    bool near = !(now >= FLT_MIN);
 #pragma unroll
-    for (int p = 0; p < R::PIECES; ++p) {
+    for (int e = 0; e < R::VEC; ++e) {
+      code.a[e] = (int8_t)(int)code_of(x[e], rcp, near);
+      code.b[e] = (int8_t)(int)code_of(y[e], rcp, near);
+    }
+    if (near) {
 #pragma unroll
       for (int e = 0; e < R::VEC; ++e) {
-        const float y = now > 0.f ? rintf(x[p][e] / now) : 0.f;
-        code[p][e] = (int8_t)(int)fminf(fmaxf(y, -kCodeMax), kCodeMax);
+        code.a[e] = now > 0.f ? (int8_t)(int)exact_code(x[e], now) : (int8_t)0;
+        code.b[e] = now > 0.f ? (int8_t)(int)exact_code(y[e], now) : (int8_t)0;
       }
-      st(dst + (4 * p + s) * R::VEC, code[p]);
     }
+    code.store(block, r, s);
   }
-  if (lane == 0) *scale = now;
+  if (old && now > was) {                                  // (not where the scale is NaN)
+    const float ratio = was / now;
+#pragma unroll
+    for (int e = 0; e < R::VEC; ++e) {
+      kept.a[e] = (int8_t)(int)rintf((float)kept.a[e] * ratio);
+      kept.b[e] = (int8_t)(int)rintf((float)kept.b[e] * ratio);
+    }
+    kept.store(block, r, s);
+  }
+  if (tid == 0) *scale = now;
 }
 
-// Grid: kv_groups workgroups for the K/V blocks (slot-major, units of one wavefront each: a
-// sequence's first num_decode rows have one slot, the others chunk_slots), then, in the RoPE form,
-// one per four (16-row tile, q head) pairs. A sequence with more blocks than slots goes through
-// them in steps of its slots, so the host's bound on the rows decides the speed only.
+// Grid: kv_groups workgroups for the K/V blocks (slot-major, 2 KVH units a slot: a sequence's first
+// num_decode rows have one slot, the others chunk_slots), then, in the RoPE form, one for every 16
+// rows of a q head. A sequence with more blocks than slots goes through them in steps of its slots,
+// so the host's bound on the rows decides the speed only.
 template <int D, bool ROPE>
-__global__ void __launch_bounds__(kWriteWaves * kWave) kv_write_int8_kernel(Int8WriteArgs a) {
+__global__ void __launch_bounds__(kWriteThreads) kv_write_int8_kernel(Int8WriteArgs a) {
   typedef RowShare<D> R;
-  const int lane = threadIdx.x % kWave;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  __shared__ float s_top[2][kWriteThreads / kWave];        // of two blocks in turn
   if (!ROPE || blockIdx.x < a.kv_groups) {
     const int units = 2 * a.kvh;
-    const int64_t u = (int64_t)blockIdx.x * kWriteWaves + wave;
-    const int64_t slot = u / units;
-    const int unit = (int)(u % units);
-    int b, at, step;
-    if (slot < a.num_decode) {
-      b = (int)slot, at = 0, step = 1;
-    } else {
-      const int64_t rest = slot - a.num_decode;
-      b = a.num_decode + (int)(rest / a.chunk_slots), at = (int)(rest % a.chunk_slots);
-      step = a.chunk_slots;
+    const int slot = (int)(blockIdx.x / (unsigned)units), unit = (int)(blockIdx.x - slot * units);
+    int b = slot, at = 0, step = 1;
+    if (slot >= a.num_decode) {
+      const int rest = slot - a.num_decode, q = (int)((unsigned)rest / (unsigned)a.chunk_slots);
+      b = a.num_decode + q, at = rest - q * a.chunk_slots, step = a.chunk_slots;
     }
     if (b >= a.num_seqs) return;
     const int len = table_entry(a.seq_lens + b);
@@ -171,46 +224,46 @@ __global__ void __launch_bounds__(kWriteWaves * kWave) kv_write_int8_kernel(Int8
     if (len <= 0 || q0 < 0 || q1 <= q0 || q1 > a.num_tokens) return;
     const int64_t start = (int64_t)len - (q1 - q0);        // position of the sequence's row q0
     const int first = start > 0 ? (int)start : 0;
+    int turn = 0;
     for (int j = first / kBlockSize + at; j <= (len - 1) / kBlockSize && j < a.max_blocks; j += step) {
       const int64_t blk = table_entry(a.block_tables + b * a.bt_stride + j);
       if (blk < 0 || blk >= a.num_blocks) continue;
       if (unit < a.kvh)
-        write_block<D, ROPE, true>(a, b, j, blk, first, len, q0 - start, unit);
+        write_block<D, ROPE, true>(a, j, blk, first, len, q0 - start, unit, s_top[turn]);
       else
-        write_block<D, ROPE, false>(a, b, j, blk, first, len, q0 - start, unit - a.kvh);
+        write_block<D, ROPE, false>(a, j, blk, first, len, q0 - start, unit - a.kvh, s_top[turn]);
+      turn ^= 1;
     }
   } else if constexpr (ROPE) {
-    const int64_t u = ((int64_t)blockIdx.x - a.kv_groups) * kWriteWaves + wave;
-    const int h = (int)(u % a.heads);
-    const int64_t t = (u / a.heads) * 16 + (lane >> 2);
-    if (t >= a.num_tokens) return;
-    const int s = lane & 3;
-    const int64_t pos = rope_row(a.positions[t], a.max_pos) * (D / 2);
+    const int64_t u = blockIdx.x - a.kv_groups;
+    const int64_t tile = u / a.heads;
+    const int h = (int)(u - tile * a.heads), s = threadIdx.x & 15;
+    const int64_t t = tile * 16 + (threadIdx.x >> 4);
+    if (t >= a.num_tokens || s >= R::LANES) return;
+    const int at = s * R::VEC;
     const half_t* src = a.q + t * a.q_st + (int64_t)h * D;
     half_t* dst = a.q_out + (t * a.heads + h) * D;
+    typename R::Halves x = ld<typename R::Halves>(src + at), y = ld<typename R::Halves>(src + D / 2 + at);
+    const int64_t pos = rope_row(a.positions[t], a.max_pos) * (D / 2) + at;
+    const typename R::Floats c = ld<typename R::Floats>(a.cos_t + pos);
+    const typename R::Floats n = ld<typename R::Floats>(a.sin_t + pos);
 #pragma unroll
-    for (int p = 0; p < R::PIECES / 2; ++p) {
-      const int at = (4 * p + s) * R::VEC;
-      typename R::Halves x = ld<typename R::Halves>(src + at), y = ld<typename R::Halves>(src + D / 2 + at);
-#pragma unroll
-      for (int e = 0; e < R::VEC; ++e) {                   // in fp32, rounded once
-        const float c = a.cos_t[pos + at + e], n = a.sin_t[pos + at + e];
-        const float f = (float)x[e], g = (float)y[e];
-        x[e] = (half_t)fmaf(-g, n, f * c);
-        y[e] = (half_t)fmaf(f, n, g * c);
-      }
-      st(dst + at, x);
-      st(dst + D / 2 + at, y);
+    for (int e = 0; e < R::VEC; ++e) {                     // in fp32, rounded once
+      const float f = (float)x[e], g = (float)y[e];
+      x[e] = (half_t)fmaf(-g, n[e], f * c[e]);
+      y[e] = (half_t)fmaf(f, n[e], g * c[e]);
     }
+    st(dst + at, x);
+    st(dst + D / 2 + at, y);
   }
 }
 
 template <int D>
 int launch_write(const Int8WriteArgs& a, bool rope, unsigned grid, hipStream_t s) {
   if (rope)
-    kv_write_int8_kernel<D, true><<<grid, kWriteWaves * kWave, 0, s>>>(a);
+    kv_write_int8_kernel<D, true><<<grid, kWriteThreads, 0, s>>>(a);
   else
-    kv_write_int8_kernel<D, false><<<grid, kWriteWaves * kWave, 0, s>>>(a);
+    kv_write_int8_kernel<D, false><<<grid, kWriteThreads, 0, s>>>(a);
   return check_launch(rope ? "rope_kv_write_int8" : "kv_write_int8");
 }
 
@@ -228,7 +281,7 @@ static int write_int8(Int8WriteArgs a, bool rope, int D, int max_query_len, cons
              (long long)a.bt_stride, max_query_len);
   TS_REQUIRE(D == 16 || D == 32 || D == 64 || D == 128 || D == 256, TS_ERR_UNSUPPORTED,
              "%s: head_dim %d (16, 32, 64, 128, 256)", what, D);
-  const int vec = D >= 64 ? 8 : D / 8;                     // elements of one load
+  const int vec = D >= 32 ? D / 32 : 1;                    // elements of one load
   TS_REQUIRE(a.k_st >= 0 && a.k_sh >= 0 && a.v_st >= 0 && a.v_sh >= 0 && a.k_st % vec == 0 &&
                  a.k_sh % vec == 0 && a.v_st % vec == 0 && a.v_sh % vec == 0 &&
                  aligned(a.k, 2 * vec) && aligned(a.v, 2 * vec),
@@ -238,9 +291,8 @@ static int write_int8(Int8WriteArgs a, bool rope, int D, int max_query_len, cons
   // One sequence of max_query_len rows falls in at most this many blocks.
   a.chunk_slots = (int)(((int64_t)max_query_len + 14) / kBlockSize + 1);
   const int64_t slots = a.num_decode + (int64_t)(a.num_seqs - a.num_decode) * a.chunk_slots;
-  a.kv_groups = (slots * 2 * a.kvh + kWriteWaves - 1) / kWriteWaves;
-  const int64_t q_units = rope ? (a.num_tokens + 15) / 16 * a.heads : 0;
-  const int64_t grid = a.kv_groups + (q_units + kWriteWaves - 1) / kWriteWaves;
+  a.kv_groups = slots * 2 * a.kvh;
+  const int64_t grid = a.kv_groups + (rope ? (a.num_tokens + 15) / 16 * a.heads : 0);
   if (grid == 0) return TS_OK;
   TS_REQUIRE(grid < (1ll << 31), TS_ERR_UNSUPPORTED, "%s: %lld workgroups", what, (long long)grid);
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
