@@ -132,6 +132,7 @@ odd = ctypes.c_void_p(258)
     (_attend, dict(D=80), N.TS_ERR_UNSUPPORTED, "head_dim 80"),
     (_attend, dict(h=3, kvh=2), N.TS_ERR_INVALID_ARG, "heads"),
     (_attend, dict(nb=0), N.TS_ERR_INVALID_ARG, "num_blocks"),
+    (_attend, dict(mb=(1 << 26) + 1, bts=1 << 27), N.TS_ERR_INVALID_ARG, "max_blocks"),
     (_attend, dict(qst=130), N.TS_ERR_INVALID_ARG, "misaligned"),
     (_attend, dict(ost=64), N.TS_ERR_INVALID_ARG, "misaligned"),
     (_attend, dict(q=odd), N.TS_ERR_INVALID_ARG, "misaligned"),
@@ -151,6 +152,10 @@ def test_empty_calls_and_workspace_sizes():
     long = size(4, 4, 1, 32768, 0, 12, 2, 128, 256)
     assert long >= 4 * 12 * 64 * (128 + 2) * 4
     assert size(8, 8, 1, 32768, 0, 12, 2, 128, 256) > long
+    # chunks of several tiles of 16 rows leave no more partials than one tile, but for a split a tile
+    tile = 16 * 64 * (128 + 2) * 4 * 4
+    assert tile <= size(4, 0, 16, 32768, 32768, 8, 8, 128, 256) / 8 < 1.01 * tile
+    assert tile <= size(4, 0, 128, 32768, 32768, 8, 8, 128, 256) / 8 < 1.15 * tile
 
 
 def test_python_wrappers_refuse():

@@ -317,6 +317,22 @@ def test_a_few_rows_per_sequence(heads):
         assert_rows(H.paged_attention_int8(q, *cache, m, c.scale), c, f"verify {heads} {bounds}")
 
 
+@pytest.mark.parametrize("heads", HEADS)
+def test_short_chunks_beside_long_prefixes(heads):
+    """Up to 21 rows a sequence: several tiles of 16 rows whose splits are merged, with as many
+    partials in the workspace as one tile has."""
+    items = [(4200, 16), (300, 21), (2047, 9), (20000, 12), (0, 21), (100, 1), (33, 20)]
+    c = Case(heads, [(1500, 1)] + items, num_decode=1, seed=32)
+    _, q, _, _, cache, meta = c.on(DEV)
+    out = H.paged_attention_int8(q, *cache, meta, c.scale)
+    assert_rows(out, c, f"short chunks {heads}")
+    # host bounds below the batch's own leave fewer partials: fewer splits
+    for bounds in (dict(max_query_len=3), dict(max_query_len=8, max_seq_len=900, max_prefill_seq_len=900),
+                   dict(max_query_len=1, max_seq_len=20100, max_prefill_seq_len=20100)):
+        m = dataclasses.replace(meta, **bounds)
+        assert_rows(H.paged_attention_int8(q, *cache, m, c.scale), c, f"short chunks {heads} {bounds}")
+
+
 @pytest.mark.parametrize("side", [0, 1])
 def test_a_few_rows_around_a_block_without_a_finite_scale(side):
     """Rows before the block are right, rows that see it NaN, also where later blocks are hidden."""
@@ -357,16 +373,19 @@ def test_mixed_batch(heads):
     H.kv_write_int8(k, v, *cache, meta)
     want = oracle_write(c)
     assert_cache(cache, want)
-    out = H.paged_attention_int8(q, *cache, meta, c.scale)
-    assert_rows(out, c, f"mixed {heads}", cache=want)
-    assert not out[1].any() and not out[int(c.starts[5])].any()
+    for bound in (777, 30000):                       # tiles of 16 rows, the prompt kernel
+        out = H.paged_attention_int8(q, *cache, dataclasses.replace(meta, max_prefill_seq_len=bound), c.scale)
+        assert_rows(out, c, f"mixed {heads} {bound}", cache=want)
+        assert not out[1].any() and not out[int(c.starts[5])].any()
 
 
 def test_table_shorter_than_the_sequence():
     c = Case((14, 2, 64), [(299, 1), (50, 200)], num_decode=1, seed=20)
     c.tables = np.ascontiguousarray(c.tables[:, :8])          # 128 tokens of 300 and 250
     _, q, _, _, cache, meta = c.on(DEV)
-    assert_rows(H.paged_attention_int8(q, *cache, meta, c.scale), c)
+    for bound in (300, 30000):
+        m = dataclasses.replace(meta, max_prefill_seq_len=bound)
+        assert_rows(H.paged_attention_int8(q, *cache, m, c.scale), c, f"{bound}")
 
 
 def test_foreign_block_ids_read_block_zero():
@@ -375,14 +394,16 @@ def test_foreign_block_ids_read_block_zero():
     bad = meta.block_tables.clone()
     bad[0, 2], bad[1, 3] = c.NB + 100, -5
     c.tables[0, 2] = c.tables[1, 3] = 0
-    m = dataclasses.replace(meta, block_tables=bad)
-    assert_rows(H.paged_attention_int8(q, *cache, m, c.scale), c)
+    for bound in (100, 30000):
+        m = dataclasses.replace(meta, block_tables=bad, max_prefill_seq_len=bound)
+        assert_rows(H.paged_attention_int8(q, *cache, m, c.scale), c, f"{bound}")
 
 
 @pytest.mark.parametrize("heads", [(12, 2, 128), (14, 2, 64)])
 @pytest.mark.parametrize("side", [0, 1])
 @pytest.mark.parametrize("bad", [np.nan, np.inf])
-def test_blocks_without_a_finite_scale(heads, side, bad):
+@pytest.mark.parametrize("bound", [501, 30000])      # tiles of 16 rows, the prompt kernel
+def test_blocks_without_a_finite_scale(heads, side, bad, bound):
     """Rows that see a token of such a block are NaN, rows before it (and other sequences) are not;
     blocks past a sequence's end have no say."""
     c = Case(heads, [(100, 1), (500, 1), (5, 150), (0, 40)], num_decode=2, seed=22)
@@ -391,6 +412,7 @@ def test_blocks_without_a_finite_scale(heads, side, bad):
     unused = sorted(set(range(c.NB)) - set(c.tables.ravel().tolist()))
     c.scales[:, unused] = np.nan
     _, q, _, _, cache, meta = c.on(DEV)
+    meta = dataclasses.replace(meta, max_prefill_seq_len=bound)
     out = H.paged_attention_int8(q, *cache, meta, c.scale)
     clean = np.nan_to_num(c.scales, nan=0.0, posinf=0.0)
     got = out.cpu().numpy().reshape(c.T, c.H, c.D)

@@ -4,17 +4,22 @@
 namespace ts {
 
 // Chunks that the decode kernel takes, in tiles of 16 rows each of which reads the sequence's codes
-// anew: those of few rows, and those whose tiles and pairs of blocks are few and whose sequences are
-// short enough to be taken in one split.
-constexpr int kI8ShortRows = 64;
-constexpr int64_t kI8SmallWork = 32768;  // (tile, pair of blocks) steps
-constexpr int kI8SmallSeq = 1024;
+// anew. Us a call here and in the prefill kernel, D = 128, 12/2 heads:
+//   rows per KV head up to kI8ShortRows (their splits are merged): 16 chunks of 8 tokens on 4096 cached
+//   31.6 / 37.7, one of 21 on 8192 23.5 / 34.0, 16 of 21 on 4096 41.9 / 42.3; above it, one chunk of
+//   42 on 4096 35.9 / 33.3, 16 of 32 57.4 / 46.9;
+//   otherwise sequences up to kI8SmallSeq tokens, each tile's in one piece, of kI8SmallWork (tile, pair
+//   of blocks) steps at most: 4 chunks of 128 on 2048 34.6 / 40.8, 16 of 128 on 512 35.4 / 41.5; above
+//   them 16 of 64 on 2048 51.7 / 44.6, 4 of 512 on 1024 53.3 / 44.1, one of 64 on 4096 35.7 / 33.7.
+constexpr int kI8ShortRows = 128;
+constexpr int kI8SmallSeq = 2048;
+constexpr int64_t kI8SmallWork = 32768;
 
 // Launch shape and scratch of a batch, from the host's bounds.
 struct Int8Plan {
   int small;                             // sequences that the decode kernel takes: the first ones
-  int row_slots, max_splits;             // a chunk's partial rows per KV head, splits of the longest
-  int64_t slots;                         // rows with partials
+  int row_slots, max_splits;             // a chunk's rows per KV head that are merged, splits of the longest
+  int chunk_parts;                       // a chunk's partials per KV head
   int tiles, groups;                     // prefill: tiles of a chunk, workgroups
   size_t dec_o, dec_ml, pre_o, pre_ml;   // offsets of the partials
   size_t bytes;
@@ -41,9 +46,12 @@ static Int8Plan int8_plan(int num_seqs, int num_decode, int max_query_len, int m
   pl.row_slots = (int)(chunk_rows < kI8ShortRows ? chunk_rows : kI8ShortRows);
   if (pl.row_slots < G) pl.row_slots = G;
   pl.max_splits = i8_splits((int)nb, kI8MaxSplits);
+  const int row_tiles = (pl.row_slots + 15) / 16;
+  pl.chunk_parts = row_tiles == 1 ? pl.row_slots * pl.max_splits : 16 * (pl.max_splits + row_tiles);
+  if (pl.chunk_parts < G * pl.max_splits) pl.chunk_parts = G * pl.max_splits;   // (chunks of one row)
   if (pl.small > 0 && pl.max_splits > 1) {
-    pl.slots = (int64_t)num_decode * H + (pl.small - num_decode) * (int64_t)KVH * pl.row_slots;
-    const size_t rows = (size_t)pl.slots * pl.max_splits;
+    const size_t rows = (size_t)num_decode * H * pl.max_splits +
+                        (size_t)(pl.small - num_decode) * KVH * pl.chunk_parts;
     pl.dec_o = take(at, rows * D * sizeof(float));
     pl.dec_ml = take(at, rows * 2 * sizeof(float));
   }
@@ -62,20 +70,22 @@ static Int8Plan int8_plan(int num_seqs, int num_decode, int max_query_len, int m
   return pl;
 }
 
+// Rows that the decode kernel's merge goes over.
+static int64_t merge_rows(const Int8Plan& pl, int num_decode, int H, int KVH) {
+  return (int64_t)num_decode * H + (int64_t)(pl.small - num_decode) * KVH * pl.row_slots;
+}
+
 static bool int8_head_dim(int D) { return D == 16 || D == 32 || D == 64 || D == 128 || D == 256; }
 
 template <int D>
-static int launch_decode(const Int8DecodeArgs& a, int cus, hipStream_t s) {
+static int launch_decode(const Int8DecodeArgs& a, int64_t rows, int cus, hipStream_t s) {
   // Every split of the batch, at most as many workgroups as the CUs hold; the rest go round.
   const int64_t most = a.num_seqs > a.num_decode ? INT32_MAX : (int64_t)a.num_decode * a.max_splits;
   const int64_t units = most * a.kvh * ((a.group + 15) / 16);
   const int64_t cap = (int64_t)i8_decode_groups(D) * cus;
   decode_int8_kernel<D><<<(unsigned)(units < cap ? units : cap), kI8Threads, 0, s>>>(a);
-  if (a.max_splits > 1) {
-    const int64_t slots = (int64_t)a.num_decode * a.heads +
-                          (int64_t)(a.num_seqs - a.num_decode) * a.kvh * a.row_slots;
-    decode_int8_merge_kernel<D><<<(unsigned)((slots + kI8Waves - 1) / kI8Waves), kI8Threads, 0, s>>>(a);
-  }
+  if (a.max_splits > 1)
+    decode_int8_merge_kernel<D><<<(unsigned)((rows + kI8Waves - 1) / kI8Waves), kI8Threads, 0, s>>>(a);
   return check_launch("paged_attention_int8");
 }
 
@@ -130,7 +140,9 @@ extern "C" int ts_paged_attention_int8(const void* q, int64_t q_stride_t, int64_
              "paged_attention_int8: head_dim %d (16, 32, 64, 128, 256)", head_dim);
   TS_REQUIRE(num_kv_heads > 0 && num_heads > 0 && num_heads % num_kv_heads == 0, TS_ERR_INVALID_ARG,
              "paged_attention_int8: %d heads over %d KV heads", num_heads, num_kv_heads);
-  TS_REQUIRE(num_blocks > 0 && max_blocks_per_seq > 0 && bt_stride >= max_blocks_per_seq,
+  // (a sequence's tokens are counted in 31 bits)
+  TS_REQUIRE(num_blocks > 0 && max_blocks_per_seq > 0 && max_blocks_per_seq <= 1 << 26 &&
+                 bt_stride >= max_blocks_per_seq,
              TS_ERR_INVALID_ARG, "paged_attention_int8: num_blocks=%lld max_blocks_per_seq=%d bt_stride=%lld",
              (long long)num_blocks, max_blocks_per_seq, (long long)bt_stride);
   TS_REQUIRE(q_stride_t % 8 == 0 && q_stride_h % 8 == 0 && q_stride_t >= 0 && q_stride_h >= 0 &&
@@ -160,20 +172,26 @@ extern "C" int ts_paged_attention_int8(const void* q, int64_t q_stride_t, int64_
   a.by_kvh = I8Div::by(num_kv_heads), a.by_group = I8Div::by(num_heads / num_kv_heads);
   a.group = num_heads / num_kv_heads, a.qsl = query_start_loc, a.num_tokens = num_tokens;
   a.sl2 = scale * 1.44269504088896340736f;
-  // the kernels count rows in 31 bits
-  TS_REQUIRE(num_tokens * a.group < (1ll << 30) && pl.slots < (1ll << 30), TS_ERR_UNSUPPORTED,
-             "paged_attention_int8: %lld tokens of %d sequences", (long long)num_tokens, num_seqs);
+  // the kernels count rows in 31 bits, and steps
+  const int64_t units = (int64_t)(num_seqs - pl.small) * pl.tiles * num_kv_heads;
+  TS_REQUIRE(num_tokens * a.group < (1ll << 30) && merge_rows(pl, num_decode, num_heads, num_kv_heads) < (1ll << 30) &&
+                 units * (max_blocks_per_seq / kI8StepBlocks + 2 + kI8TileCost) < (1ll << 31) &&
+                 units * 256 < (1ll << 31),
+             TS_ERR_UNSUPPORTED, "paged_attention_int8: %lld tokens of %d sequences in chunks of up to %d",
+             (long long)num_tokens, num_seqs, max_query_len);
   if (pl.small > 0) {
     a.num_seqs = pl.small, a.num_decode = num_decode;
-    a.row_slots = pl.row_slots, a.max_splits = pl.max_splits, a.by_slots = I8Div::by(pl.row_slots);
+    a.row_slots = pl.row_slots, a.max_splits = pl.max_splits, a.chunk_parts = pl.chunk_parts;
+    a.by_slots = I8Div::by(pl.row_slots);
     a.part_o = reinterpret_cast<float*>(ws + pl.dec_o);
     a.part_ml = reinterpret_cast<float*>(ws + pl.dec_ml);
+    const int64_t rows = merge_rows(pl, num_decode, num_heads, num_kv_heads);
     switch (head_dim) {
-      case 16: status = launch_decode<16>(a, cus, s); break;
-      case 32: status = launch_decode<32>(a, cus, s); break;
-      case 64: status = launch_decode<64>(a, cus, s); break;
-      case 128: status = launch_decode<128>(a, cus, s); break;
-      default: status = launch_decode<256>(a, cus, s); break;
+      case 16: status = launch_decode<16>(a, rows, cus, s); break;
+      case 32: status = launch_decode<32>(a, rows, cus, s); break;
+      case 64: status = launch_decode<64>(a, rows, cus, s); break;
+      case 128: status = launch_decode<128>(a, rows, cus, s); break;
+      default: status = launch_decode<256>(a, rows, cus, s); break;
     }
     if (status != TS_OK) return status;
   }
@@ -184,11 +202,6 @@ extern "C" int ts_paged_attention_int8(const void* q, int64_t q_stride_t, int64_
     p.a.part_ml = reinterpret_cast<float*>(ws + pl.pre_ml);
     p.num_seqs = num_seqs, p.first = pl.small, p.tiles = pl.tiles, p.groups = pl.groups;
     p.by_tiles = I8Div::by(pl.tiles);
-    // ... and steps
-    const int64_t units = (int64_t)(num_seqs - pl.small) * pl.tiles * num_kv_heads;
-    TS_REQUIRE(units * (max_blocks_per_seq / kI8StepBlocks + 2 + kI8TileCost) < (1ll << 31) && units * 256 < (1ll << 31),
-               TS_ERR_UNSUPPORTED, "paged_attention_int8: %lld tokens in chunks of up to %d",
-               (long long)num_tokens, max_query_len);
     switch (head_dim) {
       case 16: status = launch_prefill<16>(p, s); break;
       case 32: status = launch_prefill<32>(p, s); break;

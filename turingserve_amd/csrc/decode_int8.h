@@ -62,9 +62,10 @@ struct Int8DecodeArgs {
   int heads, kvh, group;                         // group = heads / kvh
   I8Div by_kvh, by_group, by_slots;
   float sl2;                                     // scale * log2(e)
-  // Partials [slots, max_splits, D] and (m, l) [slots, max_splits, 2]: group slots per (sequence, KV
-  // head) of the first num_decode sequences, then row_slots for the others.
-  int row_slots, max_splits;
+  // Partials, D floats each and (m, l): max_splits for each row of the first num_decode sequences, then
+  // chunk_parts for each (sequence, KV head) of the others, whose rows have as many as they have
+  // splits (merged where they are row_slots rows at most).
+  int row_slots, max_splits, chunk_parts;
   float *part_o, *part_ml;
 };
 
@@ -88,22 +89,24 @@ __device__ __forceinline__ I8Seq i8_seq(const Int8DecodeArgs& a, int b) {
   return s;
 }
 
-// The partials' slot of a row.
-__device__ __forceinline__ int64_t i8_slot(const Int8DecodeArgs& a, int b, int h, int row) {
-  return b < a.num_decode
-             ? (int64_t)(b * a.kvh + h) * a.group + row
-             : (int64_t)a.num_decode * a.heads + (int64_t)((b - a.num_decode) * a.kvh + h) * a.row_slots + row;
+// Splits of a sequence's blocks: longer ones where several tiles of rows share them, so that its
+// partials stay those of one tile. (chunk_parts holds them within the host's bounds; past those the
+// splits are fewer, one where its rows pass row_slots.)
+__device__ __forceinline__ int i8_splits(const Int8DecodeArgs& a, const I8Seq& s, bool decode) {
+  const int rows = s.n * a.group, nb = (s.kv + kBlockSize - 1) / kBlockSize;
+  if (decode) return i8_splits(nb, a.max_splits);
+  if (rows > a.row_slots) return 1;
+  const int tiles = s.n == 1 ? 1 : (rows + 15) / 16;
+  const int n = i8_splits(nb, min(a.max_splits, kI8MaxSplits / tiles), kI8SplitBlocks * tiles);
+  return max(1, min(n, (int)((unsigned)a.chunk_parts / (unsigned)max(rows, 1))));
 }
 
-// Splits of a sequence's blocks: longer ones where several tiles of rows share them, one where its
-// rows pass what the workspace holds.
-__device__ __forceinline__ int i8_splits(const Int8DecodeArgs& a, const I8Seq& s);
-
-__device__ __forceinline__ int i8_splits(const Int8DecodeArgs& a, const I8Seq& s) {
-  const int rows = s.n * a.group, tiles = (rows + 15) / 16;
-  if (rows > a.row_slots) return 1;
-  const int each = s.n == 1 ? kI8SplitBlocks : kI8SplitBlocks * tiles;
-  return i8_splits((s.kv + kBlockSize - 1) / kBlockSize, a.max_splits, each);
+// The first partial of a row.
+__device__ __forceinline__ int64_t i8_partial(const Int8DecodeArgs& a, int b, int h, int row, int splits) {
+  return b < a.num_decode
+             ? ((int64_t)(b * a.kvh + h) * a.group + row) * a.max_splits
+             : (int64_t)a.num_decode * a.heads * a.max_splits +
+                   (int64_t)((b - a.num_decode) * a.kvh + h) * a.chunk_parts + row * splits;
 }
 
 // Tokens of a sequence that its table holds.
@@ -396,7 +399,7 @@ __device__ __forceinline__ void i8_finish(const Int8DecodeArgs& a, I8State<D>& s
       const int token = a.by_group(row0 + row), head = h * a.group + row0 + row - token * a.group;
       ts::st<half4_t>(a.out + (int64_t)(q0 + token) * a.out_st + (int64_t)head * D + d, to_half4(o * f));
     } else {
-      const int64_t at = i8_slot(a, b, h, row0 + row) * a.max_splits + split;
+      const int64_t at = i8_partial(a, b, h, row0 + row, splits) + split;
       ts::st<float4_t>(a.part_o + at * D + d, o * (kColumnUnit * vref));
       if (d == 0) {
         a.part_ml[2 * at] = top;
@@ -421,7 +424,7 @@ __device__ __forceinline__ bool i8_find(const Int8DecodeArgs& a, int item, I8Ite
     I8Seq s = {};
     if (s0 + lane < a.num_seqs) {
       s = i8_seq(a, s0 + lane);
-      splits = i8_splits(a, s);
+      splits = i8_splits(a, s, s0 + lane < a.num_decode);
       tiles = (s.n * a.group + 15) / 16;
     }
     const int n = splits * tiles, sum = i8_scan(n);
@@ -474,10 +477,10 @@ __global__ void __launch_bounds__(kI8Threads, i8_decode_groups(D)) decode_int8_k
   }
 }
 
-// Rows of sequences with more than one split: one wavefront a row, D / 4 lanes a partial. Each lane's
-// first partial and every split's (m, l) are requested before the sequence's length is known (they
-// lie in the workspace whatever it is), the others at once after it. (A workgroup a row, its eight
-// groups meeting in LDS, took twice as long at 2240 rows of a few splits: 10.5 us.)
+// Rows of sequences with more than one split: one wavefront a row, D / 4 lanes a partial. A decode
+// row's first partials and every split's (m, l) are requested before the sequence's length is known
+// (they lie in the workspace whatever it is), the others at once after it. (A workgroup a row, its
+// eight groups meeting in LDS, took twice as long at 2240 rows of a few splits: 10.5 us.)
 template <int D>
 __global__ void __launch_bounds__(kI8Threads) decode_int8_merge_kernel(Int8DecodeArgs a) {
   constexpr int PER_ROW = D / 4, GROUPS = kWave / PER_ROW;
@@ -490,14 +493,19 @@ __global__ void __launch_bounds__(kI8Threads) decode_int8_merge_kernel(Int8Decod
   const int seq0 = a.by_kvh(unit), h = unit - seq0 * a.kvh, b = behind < 0 ? seq0 : a.num_decode + seq0;
   if (b >= a.num_seqs) return;
   const int group = lane / PER_ROW, d = lane % PER_ROW * 4;
-  const int64_t row = (int64_t)slot * a.max_splits;
-  const float* part = a.part_o + row * D + d;
-  const float2_t ml = ld<float2_t>(a.part_ml + 2 * (row + min(lane, a.max_splits - 1)));
+  float2_t ml;
   float4_t x[N];
-  x[0] = ld<float4_t>(part + (int64_t)min(group, a.max_splits - 1) * D);
+  auto request = [&](int64_t row, int n) {                 // its first partials, all its (m, l)
+    ml = ld<float2_t>(a.part_ml + 2 * (row + min(lane, n - 1)));
+    x[0] = ld<float4_t>(a.part_o + (row + min(group, n - 1)) * D + d);
+  };
+  if (behind < 0) request((int64_t)slot * a.max_splits, a.max_splits);
   const I8Seq seq = i8_seq(a, b);
-  const int splits = i8_splits(a, seq);
+  const int splits = i8_splits(a, seq, behind < 0);
   if (splits == 1 || r >= seq.n * a.group) return;
+  const int64_t row = i8_partial(a, b, h, r, splits);
+  const float* part = a.part_o + row * D + d;
+  if (behind >= 0) request(row, splits);
   // lane i: split i's weight
   const float m = lane < splits ? ml[0] : -INFINITY;
   float4_t o = {0.f, 0.f, 0.f, 0.f};
