@@ -282,6 +282,25 @@ def test_scales_of_very_different_size():
 
 
 # ------------------------------------------------------------------------------------- prefill
+@pytest.mark.parametrize("heads", [(4, 2, 16), (14, 2, 64)])
+def test_one_long_prompt_among_many_short_ones(heads):
+    """More sequences than a lookup holds at once, their blocks and tiles numbered across them: the
+    write (also with the host's bound far below the long one), both kernels' attention."""
+    items = [(9, 1), (700, 1)] + [(i % 37, 1 + i % 5) for i in range(75)] + [(40, 2500)] + \
+        [(i % 50, 1 + i % 30) for i in range(90)]
+    c = Case(heads, items, num_decode=2, seed=33)
+    c.lens[10] = 0                                   # a chunk without positions
+    _, q, k, v, cache, meta = c.on(DEV)
+    want = oracle_write(c)
+    for bound in (2500, 1, 90):
+        mine = tuple(t.clone() for t in cache)
+        H.kv_write_int8(k, v, *mine, dataclasses.replace(meta, max_query_len=bound))
+        assert_cache(mine, want, f"{bound}")
+    for bounds in (dict(), dict(max_query_len=8), dict(max_query_len=3, max_prefill_seq_len=60)):
+        m = dataclasses.replace(meta, **bounds)
+        assert_rows(H.paged_attention_int8(q, *mine, m, c.scale), c, f"{bounds}", cache=want)
+
+
 PREFILL = [(0, 1), (0, 15), (15, 16), (37, 16), (1000, 17), (0, 300), (16, 530), (63, 65), (4000, 5)]
 
 

@@ -20,8 +20,9 @@ struct Int8Plan {
   int small;                             // sequences that the decode kernel takes: the first ones
   int row_slots, max_splits;             // a chunk's rows per KV head that are merged, splits of the longest
   int chunk_parts;                       // a chunk's partials per KV head
-  int tiles, groups;                     // prefill: tiles of a chunk, workgroups
+  int groups;                            // prefill: workgroups
   size_t dec_o, dec_ml, pre_o, pre_ml;   // offsets of the partials
+  size_t joints;
   size_t bytes;
 };
 
@@ -57,14 +58,14 @@ static Int8Plan int8_plan(int num_seqs, int num_decode, int max_query_len, int m
   }
   if (!all) {
     const int tile_rows = 32 * i8_prefill_waves(D);
-    pl.tiles = (int)((chunk_rows + tile_rows - 1) / tile_rows);
-    const int64_t steps = P * pl.tiles * KVH * ((seq - 1) / kI8Keys + 1);
-    const int64_t cost = steps + P * pl.tiles * KVH * kI8TileCost;
+    const int64_t tiles = P * KVH * ((chunk_rows + tile_rows - 1) / tile_rows);
+    const int64_t cost = tiles * ((seq - 1) / kI8Keys + 1 + kI8TileCost);
     const int64_t most = (int64_t)i8_prefill_groups(D) * cus;
     pl.groups = (int)(cost / kI8MinShare < most ? (cost < kI8MinShare ? 1 : cost / kI8MinShare) : most);
     const size_t r = (size_t)2 * pl.groups * tile_rows;
     pl.pre_o = take(at, r * D * sizeof(float));
     pl.pre_ml = take(at, r * 2 * sizeof(float));
+    pl.joints = take(at, pl.groups * sizeof(I8Joint));
   }
   pl.bytes = at;
   return pl;
@@ -93,11 +94,8 @@ template <int D>
 static int launch_prefill(const Int8PrefillArgs& p, hipStream_t s) {
   constexpr int WAVES = i8_prefill_waves(D), ROWS = 32 * WAVES;
   prefill_int8_kernel<D><<<p.groups, WAVES * kWave, 0, s>>>(p);
-  if (p.groups > 1) {
-    const unsigned merge =
-        (unsigned)((p.num_seqs - p.first) * p.tiles * p.a.kvh * (ROWS / kI8MergeRows));
-    prefill_int8_merge_kernel<D, ROWS><<<merge, 256, 0, s>>>(p);
-  }
+  if (p.groups > 1)
+    prefill_int8_merge_kernel<D, ROWS><<<(p.groups - 1) * (ROWS / kI8MergeRows), 256, 0, s>>>(p);
   return check_launch("paged_attention_int8");
 }
 
@@ -172,13 +170,16 @@ extern "C" int ts_paged_attention_int8(const void* q, int64_t q_stride_t, int64_
   a.by_kvh = I8Div::by(num_kv_heads), a.by_group = I8Div::by(num_heads / num_kv_heads);
   a.group = num_heads / num_kv_heads, a.qsl = query_start_loc, a.num_tokens = num_tokens;
   a.sl2 = scale * 1.44269504088896340736f;
-  // the kernels count rows in 31 bits, and steps
-  const int64_t units = (int64_t)(num_seqs - pl.small) * pl.tiles * num_kv_heads;
+  // The kernels count rows in 31 bits, and steps: those of at most `tiles` tiles, each of which sees
+  // what its table holds before the chunk and the chunk (the last term: the rounded rate).
+  const int tile_rows = 32 * i8_prefill_waves(head_dim);
+  const int64_t one = num_tokens * a.group / tile_rows + 1, tiles = one + num_seqs - pl.small;
+  const int64_t steps = kI8TileCost + 4 + (max_blocks_per_seq + (num_tokens + 2 * tile_rows) / kBlockSize) /
+                        kI8StepBlocks + one / 4096;
   TS_REQUIRE(num_tokens * a.group < (1ll << 30) && merge_rows(pl, num_decode, num_heads, num_kv_heads) < (1ll << 30) &&
-                 units * (max_blocks_per_seq / kI8StepBlocks + 2 + kI8TileCost) < (1ll << 31) &&
-                 units * 256 < (1ll << 31),
-             TS_ERR_UNSUPPORTED, "paged_attention_int8: %lld tokens of %d sequences in chunks of up to %d",
-             (long long)num_tokens, num_seqs, max_query_len);
+                 (pl.small == num_seqs || tiles * steps * num_kv_heads < (1ll << 31)),
+             TS_ERR_UNSUPPORTED, "paged_attention_int8: %lld tokens of %d sequences over tables of %d blocks",
+             (long long)num_tokens, num_seqs, max_blocks_per_seq);
   if (pl.small > 0) {
     a.num_seqs = pl.small, a.num_decode = num_decode;
     a.row_slots = pl.row_slots, a.max_splits = pl.max_splits, a.chunk_parts = pl.chunk_parts;
@@ -200,8 +201,9 @@ extern "C" int ts_paged_attention_int8(const void* q, int64_t q_stride_t, int64_
     p.a = a;
     p.a.part_o = reinterpret_cast<float*>(ws + pl.pre_o);
     p.a.part_ml = reinterpret_cast<float*>(ws + pl.pre_ml);
-    p.num_seqs = num_seqs, p.first = pl.small, p.tiles = pl.tiles, p.groups = pl.groups;
-    p.by_tiles = I8Div::by(pl.tiles);
+    p.joints = reinterpret_cast<I8Joint*>(ws + pl.joints);
+    p.num_seqs = num_seqs, p.first = pl.small, p.groups = pl.groups;
+    p.rate = i8_rate(32 * i8_prefill_waves(head_dim), a.group);
     switch (head_dim) {
       case 16: status = launch_prefill<16>(p, s); break;
       case 32: status = launch_prefill<32>(p, s); break;

@@ -437,7 +437,7 @@ __device__ __forceinline__ bool i8_find(const Int8DecodeArgs& a, int item, I8Ite
       const unsigned in = item - (base + of(sum) - of(n)), t = of(tiles);
       x.split = (int)(t == 1 ? in : in / t), x.tile = (int)(in - x.split * t);
       x.seq = {of(s.q0), of(s.n), of(s.kv), of(s.start)};
-      return true;
+      return x.split < x.splits;                           // (only lengths past 31 bits could have it)
     }
     base += __builtin_amdgcn_readlane(sum, kWave - 1);
   }

@@ -45,7 +45,7 @@ struct Int8WriteArgs {
   int64_t bt_stride;
   int max_blocks;
   const int32_t *seq_lens, *qsl;
-  int num_seqs, num_decode, chunk_slots;  // slots (workgroups a unit) of a sequence past num_decode
+  int num_seqs, num_decode, chunk_slots;  // workgroups a unit for the blocks of sequences past num_decode
   int64_t num_tokens;
   int kvh;
   // RoPE form
@@ -73,7 +73,7 @@ __device__ __forceinline__ float larger(float a, float b) {
   return __int_as_float(max(__float_as_int(fabsf(a)), __float_as_int(fabsf(b))));
 }
 
-// The block's new scale. NaN where a new value or the old scale is not finite.
+// The block's new scale: NaN where a new value is not finite; one that is not finite stays so.
 __device__ __forceinline__ float grown(float was, float top) {
   return top <= FLT_MAX ? vmax(was, top / kCodeMax) : __builtin_nanf("");
 }
@@ -202,10 +202,56 @@ __device__ __forceinline__ void write_block(const Int8WriteArgs& a, int j, int64
   if (tid == 0) *scale = now;
 }
 
-// Grid: kv_groups workgroups for the K/V blocks (slot-major, 2 KVH units a slot: a sequence's first
-// num_decode rows have one slot, the others chunk_slots), then, in the RoPE form, one for every 16
-// rows of a q head. A sequence with more blocks than slots goes through them in steps of its slots,
-// so the host's bound on the rows decides the speed only.
+// A sequence of the step: its rows' positions and the blocks that they fall in.
+struct WriteSeq {
+  int len, first;                         // tokens after the step, position of its first row in the cache
+  int64_t row0;                           // flat row of position 0
+  int j0, blocks;                         // its first block, blocks (0: nothing to write)
+};
+
+__device__ __forceinline__ WriteSeq write_seq(const Int8WriteArgs& a, int len, int64_t q0, int64_t q1) {
+  WriteSeq s = {};
+  if (len <= 0 || q0 < 0 || q1 <= q0 || q1 > a.num_tokens) return s;
+  const int64_t start = (int64_t)len - (q1 - q0);          // position of row q0
+  s.len = len, s.first = start > 0 ? (int)start : 0, s.row0 = q0 - start;
+  s.j0 = s.first / kBlockSize;
+  s.blocks = max(0, min((len - 1) / kBlockSize, a.max_blocks - 1) - s.j0 + 1);
+  return s;
+}
+
+// Block `item` of the sequences past num_decode, numbered densely over them: every wavefront looks it
+// up for itself, a sequence a lane, 64 at a time. (With as many workgroups a sequence as the longest
+// chunk has blocks, 31 prompts of 100 tokens beside one of 8192 took 44 us, 128 of them 158.)
+__device__ __forceinline__ bool write_find(const Int8WriteArgs& a, int item, int& b, int& j, WriteSeq& s) {
+  const int lane = threadIdx.x % kWave;
+  int base = 0;
+  for (int first = a.num_decode; first < a.num_seqs; first += kWave) {
+    WriteSeq x = {};
+    int q0 = 0;
+    if (first + lane < a.num_seqs) {
+      q0 = a.qsl[first + lane];
+      x = write_seq(a, a.seq_lens[first + lane], q0, a.qsl[first + lane + 1]);
+    }
+    const int sum = i8_scan(x.blocks);
+    const uint64_t past = __ballot(base + sum > item);
+    if (past) {
+      const int i = __ffsll((unsigned long long)past) - 1;
+      auto of = [&](int v) { return __builtin_amdgcn_readlane(v, i); };
+      b = first + i;
+      s.len = of(x.len), s.first = of(x.first), s.j0 = of(x.j0), s.blocks = of(x.blocks);
+      s.row0 = (int64_t)of(q0) - of((int)(q0 - x.row0));   // (the start, an int)
+      const int at = item - (base + of(sum) - s.blocks);
+      j = s.j0 + at;
+      return at >= 0 && at < s.blocks;
+    }
+    base += __builtin_amdgcn_readlane(sum, kWave - 1);
+  }
+  return false;
+}
+
+// Grid: kv_groups workgroups for the K/V blocks (2 KVH units a block: one a decode row, then
+// chunk_slots for the blocks of the other sequences, in turn where they are more), then, in the RoPE
+// form, one for every 16 rows of a q head. The host's bound on the rows decides the speed only.
 template <int D, bool ROPE>
 __global__ void __launch_bounds__(kWriteThreads) kv_write_int8_kernel(Int8WriteArgs a) {
   typedef RowShare<D> R;
@@ -213,26 +259,26 @@ __global__ void __launch_bounds__(kWriteThreads) kv_write_int8_kernel(Int8WriteA
   if (!ROPE || blockIdx.x < a.kv_groups) {
     const int units = 2 * a.kvh;
     const int slot = (int)(blockIdx.x / (unsigned)units), unit = (int)(blockIdx.x - slot * units);
-    int b = slot, at = 0, step = 1;
-    if (slot >= a.num_decode) {
-      const int rest = slot - a.num_decode, q = (int)((unsigned)rest / (unsigned)a.chunk_slots);
-      b = a.num_decode + q, at = rest - q * a.chunk_slots, step = a.chunk_slots;
-    }
-    if (b >= a.num_seqs) return;
-    const int len = table_entry(a.seq_lens + b);
-    const int64_t q0 = table_entry(a.qsl + b), q1 = table_entry(a.qsl + b + 1);
-    if (len <= 0 || q0 < 0 || q1 <= q0 || q1 > a.num_tokens) return;
-    const int64_t start = (int64_t)len - (q1 - q0);        // position of the sequence's row q0
-    const int first = start > 0 ? (int)start : 0;
     int turn = 0;
-    for (int j = first / kBlockSize + at; j <= (len - 1) / kBlockSize && j < a.max_blocks; j += step) {
+    auto write = [&](const WriteSeq& s, int b, int j) {
       const int64_t blk = table_entry(a.block_tables + b * a.bt_stride + j);
-      if (blk < 0 || blk >= a.num_blocks) continue;
+      if (blk < 0 || blk >= a.num_blocks) return;
       if (unit < a.kvh)
-        write_block<D, ROPE, true>(a, j, blk, first, len, q0 - start, unit, s_top[turn]);
+        write_block<D, ROPE, true>(a, j, blk, s.first, s.len, s.row0, unit, s_top[turn]);
       else
-        write_block<D, ROPE, false>(a, j, blk, first, len, q0 - start, unit - a.kvh, s_top[turn]);
+        write_block<D, ROPE, false>(a, j, blk, s.first, s.len, s.row0, unit - a.kvh, s_top[turn]);
       turn ^= 1;
+    };
+    if (slot < a.num_decode) {
+      const WriteSeq s = write_seq(a, table_entry(a.seq_lens + slot), table_entry(a.qsl + slot),
+                                   table_entry(a.qsl + slot + 1));
+      for (int j = s.j0; j < s.j0 + s.blocks; ++j) write(s, slot, j);
+    } else {
+      WriteSeq s;
+      int b, j;
+      for (int64_t item = slot - a.num_decode; item <= INT32_MAX && write_find(a, (int)item, b, j, s);
+           item += a.chunk_slots)
+        write(s, b, j);
     }
   } else if constexpr (ROPE) {
     const int64_t u = blockIdx.x - a.kv_groups;
@@ -288,13 +334,15 @@ static int write_int8(Int8WriteArgs a, bool rope, int D, int max_query_len, cons
              TS_ERR_INVALID_ARG, "%s: k and v rows must be %d-byte aligned", what, 2 * vec);
   TS_REQUIRE(aligned(a.kc, 16) && aligned(a.vc, 16) && aligned(a.ks, 4) && aligned(a.vs, 4),
              TS_ERR_INVALID_ARG, "%s: caches must be 16-byte aligned", what);
-  // One sequence of max_query_len rows falls in at most this many blocks.
-  a.chunk_slots = (int)(((int64_t)max_query_len + 14) / kBlockSize + 1);
-  const int64_t slots = a.num_decode + (int64_t)(a.num_seqs - a.num_decode) * a.chunk_slots;
-  a.kv_groups = slots * 2 * a.kvh;
+  // n rows fall in at most (n + 14) / 16 + 1 blocks: less than n / 16 + 2.
+  const int64_t chunks = a.num_seqs - a.num_decode, each = ((int64_t)max_query_len + 14) / kBlockSize + 1;
+  const int64_t blocks = a.num_tokens / kBlockSize + 2 * chunks;
+  const int64_t chunk_slots = chunks * each < blocks ? chunks * each : blocks;
+  a.kv_groups = (a.num_decode + chunk_slots) * 2 * a.kvh;
   const int64_t grid = a.kv_groups + (rope ? (a.num_tokens + 15) / 16 * a.heads : 0);
   if (grid == 0) return TS_OK;
   TS_REQUIRE(grid < (1ll << 31), TS_ERR_UNSUPPORTED, "%s: %lld workgroups", what, (long long)grid);
+  a.chunk_slots = (int)chunk_slots;
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   switch (D) {
     case 16: return launch_write<16>(a, rope, (unsigned)grid, s);

@@ -21,7 +21,9 @@
 // The batch's steps (of every sequence, tile and KV head, in that order) are shared evenly over
 // the launched workgroups. Where a share begins or ends inside a tile, its part of the tile is left
 // as a partial (m, l, O in fp32) for the merge launch; a workgroup leaves two at most. Every
-// workgroup works the shares out for itself from the sequences' lengths.
+// workgroup works the shares out for itself from the sequences' lengths, a sequence a lane: the steps
+// of a sequence's first t tiles have a closed form, so a batch of one long and many short prompts
+// costs what its rows cost.
 #pragma once
 
 #include "decode_int8.h"
@@ -33,22 +35,31 @@ typedef float float16_t __attribute__((ext_vector_type(16)));
 constexpr int kI8Keys = 64;              // tokens of a step
 constexpr int kI8StepBlocks = kI8Keys / kBlockSize;
 constexpr int kI8Window = 256;           // blocks whose ids and scales are held in LDS at a time
-constexpr int kI8MinShare = 8;           // steps (and tiles' costs) that a workgroup is worth
+constexpr int kI8MinShare = 6;           // steps (and tiles' costs) that a workgroup is worth: 4, 6, 8 and 16 are
+                                         // 31.4, 31.7, 31.8 and 33 us at five chunks of 90 to 1100 rows
 constexpr float kI8LeastRatio = -30.f;   // log2 of the least V scale ratio
 constexpr float kI8LeastFactor = 1e-30f;
-constexpr int kI8Kept = 4;               // times 64 pairs (sequence, tile) whose steps are kept
 
 template <int N>
 struct I8Const {
   static constexpr int value = N;
 };
 
+// What the merge launch does about the beginning of a share (left by the share's workgroup, so that
+// the merge need not look the tile up): the tile's rows and the shares that its partials come from,
+// where it is the first one inside the tile.
+struct I8Joint {
+  int first, last;                       // equal: nothing
+  int q0, rows, row0, h;                 // the chunk's first flat row and rows per KV head, the tile's first
+  int pad[2];
+};
+
 struct Int8PrefillArgs {
   Int8DecodeArgs a;                      // (part_o, part_ml: two partials of a tile per workgroup)
+  I8Joint* joints;                       // one for each workgroup
   int num_seqs, first;                   // sequences first .. num_seqs - 1
-  int tiles;                             // of the longest chunk by the host's bound
-  I8Div by_tiles;
   int groups;                            // workgroups of the main launch
+  int rate;                              // i8_rate
 };
 
 __device__ __forceinline__ float16_t mfma_i8(half8_t a, half8_t b, float16_t c) {
@@ -74,7 +85,7 @@ struct I8Tile {
 template <int D>
 struct I8PrefillLds {
   __align__(16) half_t k[2][I8Tile<D>::HALVES], v[2][I8Tile<D>::HALVES];
-  int n[kI8Kept * kWave], scan[kI8Kept * kWave];           // the walk's kept pairs
+  int walk[5][kWave];                                      // I8Walk
   int blk[kI8Window];                                      // the sign bit: a scale is not finite
   __align__(16) float fk[kI8Window + 4], vs[kI8Window];        // scale * log2 e * ks; log2(vs / vref)
   __align__(16) float back[kI8Window];                     // vref / vs
@@ -102,109 +113,106 @@ __device__ __forceinline__ int i8_sees(const I8Chunk& k, int token) {
   return max(0, min(k.kv, k.start + token + 1));
 }
 
-// A tile counts as kI8TileCost steps more than it has: what its start costs (the sequence's lookup,
-// q, the first blocks' ids, scales and codes, one after the other: 11 to 15 thousand cycles beside 2.8
-// thousand a step at head_dim 64). Steps of a share that fall on them are nobody's.
-constexpr int kI8TileCost = 4;
-
-// What tile t of a chunk counts for: its steps (one at least, so that somebody writes the rows) behind
-// kI8TileCost.
+// The steps of a tile that sees `sees` tokens (one at least, so that somebody writes its rows).
 template <int ROWS>
 __device__ __forceinline__ int i8_steps(const Int8DecodeArgs& a, const I8Chunk& k, int t) {
-  const int rows = k.n * a.group;
-  if (t * ROWS >= rows) return 0;
-  const int sees = i8_sees(k, a.by_group(min(rows, (t + 1) * ROWS) - 1));
-  return kI8TileCost + max(1, (sees + kI8Keys - 1) / kI8Keys);
+  const int sees = i8_sees(k, a.by_group(min(k.n * a.group, (t + 1) * ROWS) - 1));
+  return max(1, (sees + kI8Keys - 1) / kI8Keys);
 }
 
-// Where the batch's steps lie: pairs (sequence, tile) in order, each with all its KV heads.
+// What a tile counts for: kI8TileCost for its start (the sequence's lookup, q, the first blocks' ids,
+// scales and codes, one after the other: 11 to 15 thousand cycles beside 2.8 thousand a step at
+// head_dim 64), then its steps, then what makes the sum over a sequence's first t tiles
+//   C(t) = t (kI8TileCost + 2) + floor((t start + t (t + 1) / 2 ROWS / group) / 64):
+// C(t + 1) - C(t) > kI8TileCost + 1 + (start + (t + 1) ROWS / group) / 64, and tile t sees at most
+// start + ((t + 1) ROWS - 1) / group + 1 tokens, whose steps are fewer than the sum's last two terms.
+// Steps of a share that fall on a tile's start or behind its last one are nobody's. (At
+// 2048 rows on 4096 cached, 12/2 heads of 128, and five chunks of 90 to 1100, 14/2 heads of 64: 96.0 and
+// 32.1 us with kI8TileCost 3, 94.4 and 31.8 with 5, 94.8 and 31.7 with 7.)
+constexpr int kI8TileCost = 5;
+// ROWS / (2 group) of a step's 64 tokens in units of 2^-12, rounded up.
+constexpr int i8_rate(int rows, int group) { return (32 * rows + group - 1) / group; }
+
+__device__ __forceinline__ int i8_cost(const Int8PrefillArgs& p, int start, int t) {
+  return t * (kI8TileCost + 2) + (int)(((int64_t)t * ((int64_t)start << 6) + (int64_t)t * (t + 1) * p.rate) >> 12);
+}
+
+// Where the batch's steps lie: tiles in order, each with all its KV heads.
 struct I8Place {
-  int pair, steps;
-  int before;                            // steps of the pairs before it, for one KV head
+  I8Chunk k;
+  int seq, tile, cost;
+  int before;                            // what the tiles before it count for, for one KV head
 };
 
-// The pairs' steps, a pair a lane: the first kI8Kept * 64 pairs are kept, further ones are worked out
-// again where they are asked for. Every wavefront for itself.
+// The sequences' costs, a sequence a lane: the first 64 are kept, further ones are worked out again
+// where they are asked for. Every wavefront for itself.
 template <int ROWS>
 struct I8Walk {
-  int n[kI8Kept], scan[kI8Kept];         // steps, and their sums from the first lane of the 64
-  int total;                             // of all pairs, for one KV head
+  I8Chunk k;
+  int scan;                              // sums of the costs from the first lane of the 64
+  int total;                             // of all sequences, for one KV head
 
-  static __device__ __forceinline__ int steps(const Int8PrefillArgs& p, int pair) {
-    if (pair >= (p.num_seqs - p.first) * p.tiles) return 0;
-    const int seq = p.by_tiles(pair);
-    return i8_steps<ROWS>(p.a, i8_chunk(p, p.first + seq), pair - seq * p.tiles);
+  static __device__ __forceinline__ int tiles(const Int8PrefillArgs& p, int n) {
+    return (n * p.a.group + ROWS - 1) / ROWS;
+  }
+  static __device__ __forceinline__ int start(const I8Chunk& k) { return max(0, min(k.start, k.kv)); }
+  // This lane's sequence of those from `first` on.
+  static __device__ __forceinline__ int cost(const Int8PrefillArgs& p, int first, I8Chunk& k) {
+    const int b = first + threadIdx.x % kWave;
+    k = {};
+    if (b < p.num_seqs) k = i8_chunk(p, b);
+    return i8_cost(p, start(k), tiles(p, k.n));
   }
   __device__ __forceinline__ I8Walk(const Int8PrefillArgs& p) {
-    const int lane = threadIdx.x % kWave, pairs = (p.num_seqs - p.first) * p.tiles;
-    total = 0;
-#pragma unroll
-    for (int i = 0; i < kI8Kept; ++i) {
-      n[i] = scan[i] = 0;
-      if (i * kWave < pairs) n[i] = steps(p, i * kWave + lane);
-    }
-#pragma unroll
-    for (int i = 0; i < kI8Kept; ++i) {
-      if (i * kWave < pairs) scan[i] = i8_scan(n[i]);
-      total += __builtin_amdgcn_readlane(scan[i], kWave - 1);
-    }
-    for (int base = kI8Kept * kWave; base < pairs; base += kWave)
-      total += __builtin_amdgcn_readlane(i8_scan(steps(p, base + lane)), kWave - 1);
+    scan = i8_scan(cost(p, p.first, k));
+    total = __builtin_amdgcn_readlane(scan, kWave - 1);
+    I8Chunk x;
+    for (int first = p.first + kWave; first < p.num_seqs; first += kWave)
+      total += __builtin_amdgcn_readlane(i8_scan(cost(p, first, x)), kWave - 1);
   }
   // Kept in LDS while a tile needs the registers.
-  __device__ __forceinline__ void save(int* ln, int* ls) const {
-#pragma unroll
-    for (int i = 0; i < kI8Kept; ++i) {
-      ln[i * kWave + threadIdx.x % kWave] = n[i];
-      ls[i * kWave + threadIdx.x % kWave] = scan[i];
-    }
+  __device__ __forceinline__ void save(int (*to)[kWave]) const {
+    const int lane = threadIdx.x % kWave;
+    to[0][lane] = k.q0, to[1][lane] = k.start, to[2][lane] = k.n, to[3][lane] = k.kv, to[4][lane] = scan;
   }
-  __device__ __forceinline__ I8Walk(const int* ln, const int* ls) {
-#pragma unroll
-    for (int i = 0; i < kI8Kept; ++i) {
-      n[i] = ln[i * kWave + threadIdx.x % kWave];
-      scan[i] = ls[i * kWave + threadIdx.x % kWave];
-    }
+  __device__ __forceinline__ I8Walk(const int (*from)[kWave]) {
+    const int lane = threadIdx.x % kWave;
+    k.q0 = from[0][lane], k.start = from[1][lane], k.n = from[2][lane], k.kv = from[3][lane];
+    scan = from[4][lane];
   }
-  static __device__ __forceinline__ bool in(int n, int scan, int base, int sum, int at, I8Place& place) {
-    const uint64_t past = __ballot(sum + scan > at);
-    if (!past) return false;
+  // The tile that step `at` (below total) falls in. False where there is none, as only lengths that
+  // contradict themselves could have it; a tile that is found is one of its sequence's.
+  __device__ __forceinline__ bool find(const Int8PrefillArgs& p, int at, I8Place& place) const {
+    const int lane = threadIdx.x % kWave;
+    I8Chunk x = k;
+    int sums = scan, sum = 0, first = p.first;
+    uint64_t past;
+    while ((past = __ballot(sum + sums > at)) == 0) {
+      sum += __builtin_amdgcn_readlane(sums, kWave - 1);
+      first += kWave;
+      if (first >= p.num_seqs) return false;
+      sums = i8_scan(cost(p, first, x));
+    }
     const int i = __ffsll((unsigned long long)past) - 1;
-    place.pair = base + i;
-    place.steps = __builtin_amdgcn_readlane(n, i);
-    place.before = sum + __builtin_amdgcn_readlane(scan, i) - place.steps;
-    return true;
-  }
-  // The pair that step `at` (below total) falls in.
-  __device__ __forceinline__ I8Place find(const Int8PrefillArgs& p, int at) const {
-    const int lane = threadIdx.x % kWave;
-    I8Place place;
-    int sum = 0;
-#pragma unroll
-    for (int i = 0; i < kI8Kept; ++i) {
-      if (in(n[i], scan[i], i * kWave, sum, at, place)) return place;
-      sum += __builtin_amdgcn_readlane(scan[i], kWave - 1);
+    place.k = {__builtin_amdgcn_readlane(x.q0, i), __builtin_amdgcn_readlane(x.start, i),
+               __builtin_amdgcn_readlane(x.n, i), __builtin_amdgcn_readlane(x.kv, i)};
+    place.seq = first + i;
+    if (i > 0) sum += __builtin_amdgcn_readlane(sums, i - 1);
+    // the last tile whose steps start at or before it: 64 candidates at a time
+    const int from = start(place.k);
+    int tile = 0;
+    for (int span = tiles(p, place.k.n); span > 1;) {
+      const int stride = (span + kWave - 1) / kWave, t = lane * stride;
+      const uint64_t behind = __ballot(t < span && sum + i8_cost(p, from, tile + t) <= at);
+      const int last = (63 - __clzll((long long)(behind | 1))) * stride;
+      tile += last;
+      span = min(stride, span - last);
     }
-    for (int base = kI8Kept * kWave;; base += kWave) {
-      const int k = steps(p, base + lane), ks = i8_scan(k);
-      if (in(k, ks, base, sum, at, place)) return place;
-      sum += __builtin_amdgcn_readlane(ks, kWave - 1);
-    }
-  }
-  // Steps of the pairs before `pair`.
-  __device__ __forceinline__ int before(const Int8PrefillArgs& p, int pair) const {
-    const int lane = threadIdx.x % kWave;
-    int sum = 0;
-#pragma unroll
-    for (int i = 0; i < kI8Kept; ++i) {
-      const int last = pair - 1 - i * kWave;               // lane of the last pair before it
-      if (last >= 0) sum += __builtin_amdgcn_readlane(scan[i], min(last, kWave - 1));
-    }
-    for (int base = kI8Kept * kWave; base < pair; base += kWave) {
-      const int scan = i8_scan(steps(p, base + lane));
-      sum += __builtin_amdgcn_readlane(scan, min(pair - 1 - base, kWave - 1));
-    }
-    return sum;
+    place.tile = tile;
+    const int cost = i8_cost(p, from, tile);
+    place.before = sum + cost;
+    place.cost = i8_cost(p, from, tile + 1) - cost;
+    return place.k.n > 0;
   }
 };
 
@@ -641,95 +649,104 @@ prefill_int8_kernel(Int8PrefillArgs p) {
   constexpr int WAVES = i8_prefill_waves(D), ROWS = 32 * WAVES;
   __shared__ __align__(16) I8PrefillLds<D> lds;
   const Int8DecodeArgs& a = p.a;
-  int at, hi;
+  int at, hi, h;
   I8Place place;
   {
     const I8Walk<ROWS> walk(p);
     const int total = walk.total * a.kvh;
-    if (total == 0) return;
     const I8Shares shares(total, p.groups);
-    if ((int)blockIdx.x >= shares.count) return;
-    at = shares.begin(blockIdx.x), hi = shares.begin(blockIdx.x + 1);
-    place = walk.find(p, a.by_kvh(at));
-    if (threadIdx.x < kWave) walk.save(lds.n, lds.scan);
-  }
-  int b = 0, h = 0, tile = 0;
-  for (bool extra = false, more = false; extra || at < hi;) {
-    int s0 = 0, s1, steps;
-    if (!extra) {
-      if (more) place = I8Walk<ROWS>(lds.n, lds.scan).find(p, a.by_kvh(at));
-      if (!more) __syncthreads();                          // (saved)
-      more = true;
-      const unsigned in = at - place.before * a.kvh;
-      h = (int)(in / (unsigned)place.steps);
-      const int c0 = (int)in - h * place.steps, c1 = min(place.steps, c0 + (hi - at));
-      b = p.by_tiles(place.pair), tile = place.pair - b * p.tiles, b += p.first;
-      at += c1 - c0;
-      steps = place.steps - kI8TileCost, s0 = max(0, c0 - kI8TileCost), s1 = c1 - kI8TileCost;
-      if (s1 <= s0) continue;
+    I8Joint joint = {};
+    bool found = false;
+    if (total > 0 && (int)blockIdx.x < shares.count) {
+      at = shares.begin(blockIdx.x), hi = shares.begin(blockIdx.x + 1);
+      found = walk.find(p, a.by_kvh(at), place);
+      h = (int)((unsigned)(at - place.before * a.kvh) / (unsigned)place.cost);
+      found = found && (unsigned)h < (unsigned)a.kvh;
     }
-    const I8Chunk k = i8_chunk(p, b);
-    if (extra) s1 = steps = i8_steps<ROWS>(a, k, tile) - kI8TileCost;
-    i8_piece<D, WAVES>(p, lds, k, b, tile, h, s0, s1, s0 == 0 && s1 == steps, 2 * blockIdx.x + (s0 == 0));
-    // Tiles past the host's bound on the rows follow, whole, the first step of the last tile that it
-    // allows for.
-    extra = (extra || (tile == p.tiles - 1 && s0 == 0)) && i8_steps<ROWS>(a, k, tile + 1) > 0;
-    if (extra) ++tile;
+    if (found) {
+      const int s0 = place.before * a.kvh + h * place.cost + kI8TileCost;
+      const int first = shares.of(s0), last = shares.of(s0 + i8_steps<ROWS>(a, place.k, place.tile) - 1);
+      if (first + 1 == (int)blockIdx.x && last > first && last < shares.count)
+        joint = {first, last, place.k.q0, place.k.n * a.group, place.tile * ROWS, h};
+    }
+    if (threadIdx.x == 0) p.joints[blockIdx.x] = joint;
+    if (!found) return;
+    if (threadIdx.x < kWave) walk.save(lds.walk);
+  }
+  __syncthreads();                                         // (saved)
+  while (true) {
+    const int c0 = at - place.before * a.kvh - h * place.cost, c1 = min(place.cost, c0 + (hi - at));
+    at += c1 - c0;
+    const int steps = i8_steps<ROWS>(a, place.k, place.tile);
+    const int s0 = max(0, c0 - kI8TileCost), s1 = min(c1 - kI8TileCost, steps);
+    if (s1 > s0)
+      i8_piece<D, WAVES>(p, lds, place.k, place.seq, place.tile, h, s0, s1, s0 == 0 && s1 == steps,
+                         2 * blockIdx.x + (s0 == 0));
+    if (at >= hi) return;
+    if (!I8Walk<ROWS>(lds.walk).find(p, a.by_kvh(at), place)) return;
+    h = (int)((unsigned)(at - place.before * a.kvh) / (unsigned)place.cost);
+    if ((unsigned)h >= (unsigned)a.kvh) return;
   }
 }
 
-// Tiles that several workgroups share: D / 4 threads a row, 32 rows a workgroup.
+// Tiles that several workgroups share: kI8MergeRows rows a workgroup, D / 4 threads a row. The
+// workgroups stand for the shares' beginnings: the first one inside a tile has it merged. (At
+// 2048 rows on 4096 cached, 12/2 heads of 128: 9.5 us, 53 MB of partials; 10.5 when each workgroup
+// looked the tile up; 32 rows a workgroup are 1 to 2 us slower.)
 constexpr int kI8MergeRows = 16;
 template <int D, int ROWS>
 __global__ void __launch_bounds__(256) prefill_int8_merge_kernel(Int8PrefillArgs p) {
-  constexpr int PER = 256 / (D / 4), N = 4;                // rows at a time, partials requested at once
+  constexpr int PER = 256 / (D / 4);                       // rows at a time
+  constexpr int R = kI8MergeRows > PER ? kI8MergeRows / PER : 1, N = 4;   // rows of a thread, partials at a time
   const Int8DecodeArgs& a = p.a;
-  const int unit = blockIdx.x / (ROWS / kI8MergeRows);
+  const int g = 1 + (int)(blockIdx.x / (ROWS / kI8MergeRows));
   const int row0 = (int)(blockIdx.x % (ROWS / kI8MergeRows)) * kI8MergeRows;
-  const int pair = a.by_kvh(unit), h = unit - pair * a.kvh;
-  const int seq = p.by_tiles(pair), b = p.first + seq, tile = pair - seq * p.tiles;
-  const I8Chunk k = i8_chunk(p, b);
-  const int rows = k.n * a.group;
-  if (tile * ROWS + row0 >= rows) return;
-  const I8Walk<ROWS> walk(p);
-  const int steps = i8_steps<ROWS>(a, k, tile);
-  const I8Shares shares(walk.total * a.kvh, p.groups);
-  const int g0 = walk.before(p, pair) * a.kvh + h * steps;
-  const int first = shares.of(g0 + kI8TileCost), last = shares.of(g0 + steps - 1);
-  if (first == last) return;                               // one workgroup wrote it
-  const int d = threadIdx.x % (D / 4) * 4;
-  for (int in = row0 + threadIdx.x / (D / 4); in < row0 + kI8MergeRows; in += PER) {
-    const int row = tile * ROWS + in;
-    if (row >= rows) return;
-    float top = -INFINITY, sum = 0.f;
-    float4_t o = {0.f, 0.f, 0.f, 0.f};
-    for (int i0 = first; i0 <= last; i0 += N) {
-      float2_t ml[N];
-      float4_t x[N];
+  const I8Joint j = p.joints[g];
+  if (j.first == j.last || j.row0 + row0 >= j.rows) return;
+  const int in = row0 + threadIdx.x / (D / 4), d = threadIdx.x % (D / 4) * 4;
+  if (PER > kI8MergeRows && in >= row0 + kI8MergeRows) return;
+  float top[R], sum[R];
+  float4_t o[R];
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int64_t at = (int64_t)(2 * min(i0 + i, last) + (i0 + i == first)) * ROWS + in;
-        ml[i] = ld<float2_t>(a.part_ml + 2 * at);
-        x[i] = ld<float4_t>(a.part_o + at * D + d);
-      }
-      float now = top;
+  for (int r = 0; r < R; ++r) top[r] = -INFINITY, sum[r] = 0.f, o[r] = {0.f, 0.f, 0.f, 0.f};
+  for (int i0 = j.first; i0 <= j.last; i0 += N) {
+    float2_t ml[N][R];
+    float4_t x[N][R];
 #pragma unroll
-      for (int i = 0; i < N; ++i) now = i0 + i <= last ? vmax(now, ml[i][0]) : now;
-      const float f = top == -INFINITY ? 0.f : fast_exp2(top - now);
-      sum *= f;
-      o *= f;
-      top = now;
+    for (int i = 0; i < N; ++i) {                          // (rows past the last one hold anything)
+      if (i0 + i > j.last) continue;
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        if (i0 + i > last || ml[i][0] == -INFINITY) continue;
-        const float g = fast_exp2(ml[i][0] - top);
-        sum = fmaf(g, ml[i][1], sum);
-        o += x[i] * g;
+      for (int r = 0; r < R; ++r) {
+        const int64_t at = (int64_t)(2 * (i0 + i) + (i0 + i == j.first)) * ROWS + in + r * PER;
+        ml[i][r] = ld<float2_t>(a.part_ml + 2 * at);
+        x[i][r] = ld<float4_t>(a.part_o + at * D + d);
       }
     }
-    const float f = sum == 0.f ? 0.f : 1.f / sum;
-    const int token = a.by_group(row), head = h * a.group + row - token * a.group;
-    st<half4_t>(a.out + (int64_t)(k.q0 + token) * a.out_st + (int64_t)head * D + d, to_half4(o * f));
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float now = top[r];
+#pragma unroll
+      for (int i = 0; i < N; ++i) now = i0 + i <= j.last ? vmax(now, ml[i][r][0]) : now;
+      const float f = top[r] == -INFINITY ? 0.f : fast_exp2(top[r] - now);
+      sum[r] *= f;
+      o[r] *= f;
+      top[r] = now;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        if (i0 + i > j.last || ml[i][r][0] == -INFINITY) continue;
+        const float e = fast_exp2(ml[i][r][0] - now);
+        sum[r] = fmaf(e, ml[i][r][1], sum[r]);
+        o[r] += x[i][r] * e;
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int row = j.row0 + in + r * PER;
+    if (row >= j.rows) return;
+    const float f = sum[r] == 0.f ? 0.f : 1.f / sum[r];
+    const int token = a.by_group(row), head = j.h * a.group + row - token * a.group;
+    st<half4_t>(a.out + (int64_t)(j.q0 + token) * a.out_st + (int64_t)head * D + d, to_half4(o[r] * f));
   }
 }
 
