@@ -740,6 +740,11 @@ def _int8_args(what: str, k_cache, v_cache, k_scale, v_scale, meta, device) -> t
     return NB, KVH, D, bt, sl, qsl, bt.stride(0) if bt.shape[0] > 1 else bt.shape[1]
 
 
+def _elsewhere(t: torch.Tensor) -> bool:
+    """Whether t lives on another GPU than the current one, where a null stream's launches go."""
+    return t.device.index != torch._C._cuda_getDevice()
+
+
 def kv_write_int8(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                   k_scale: torch.Tensor, v_scale: torch.Tensor, meta) -> None:
     """The step's new rows k, v [T, KVH, D] (strided views of qkv allowed) into an 8-bit paged
@@ -753,6 +758,9 @@ def kv_write_int8(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cac
     if T == 0:
         return
     _check_gpu(k, v)
+    if _elsewhere(k):
+        with torch.cuda.device(k.device):
+            return kv_write_int8(k, v, k_cache, v_cache, k_scale, v_scale, meta)
     NB, ckvh, cd, bt, sl, qsl, bt_st = _int8_args("kv_write_int8", k_cache, v_cache, k_scale, v_scale,
                                                   meta, k.device)
     _require(v.shape == k.shape and v.device == k.device and ckvh == KVH and cd == D,
@@ -775,6 +783,10 @@ def rope_kv_write_int8(qkv: torch.Tensor, positions: torch.Tensor, cos: torch.Te
     returned as [T, H, D]; qkv [T, (H + 2 KVH) D] is left as it is. Rotations are computed wider
     than fp16 and rounded once: q to fp16, k straight to its code."""
     _check_gpu(qkv, positions, cos, sin)
+    if _elsewhere(qkv):
+        with torch.cuda.device(qkv.device):
+            return rope_kv_write_int8(qkv, positions, cos, sin, H, KVH, D, k_cache, v_cache, k_scale,
+                                      v_scale, meta)
     T = qkv.shape[0]
     _require(qkv.dim() == 2 and qkv.stride(1) == 1 and qkv.dtype == torch.float16 and
              qkv.shape[1] >= (H + 2 * KVH) * D,
@@ -809,10 +821,13 @@ def paged_attention_int8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     the bottom-right causal mask. A row that sees a block whose scale is not finite is NaN; a row
     that sees no token is zeros."""
     T, H, D = q.shape
-    out = torch.empty(T, H * D, dtype=q.dtype, device=q.device)
     if T == 0:
-        return out
+        return torch.empty(0, H * D, dtype=q.dtype, device=q.device)
     _check_gpu(q)
+    if _elsewhere(q):
+        with torch.cuda.device(q.device):
+            return paged_attention_int8(q, k_cache, v_cache, k_scale, v_scale, meta, scale)
+    out = torch.empty(T, H * D, dtype=q.dtype, device=q.device)
     NB, KVH, cd, bt, sl, qsl, bt_st = _int8_args("paged_attention_int8", k_cache, v_cache, k_scale,
                                                  v_scale, meta, q.device)
     _require(cd == D and q.stride(2) == 1 and q.dtype == torch.float16,
