@@ -90,15 +90,15 @@ __device__ __forceinline__ I8Seq i8_seq(const Int8DecodeArgs& a, int b) {
 }
 
 // Splits of a sequence's blocks: longer ones where several tiles of rows share them, so that its
-// partials stay those of one tile. (chunk_parts holds them within the host's bounds; past those the
-// splits are fewer, one where its rows pass row_slots.)
+// partials stay those of one tile. (chunk_parts holds them, and row_slots the rows, within the host's
+// bounds; past those there is one split.)
 __device__ __forceinline__ int i8_splits(const Int8DecodeArgs& a, const I8Seq& s, bool decode) {
   const int rows = s.n * a.group, nb = (s.kv + kBlockSize - 1) / kBlockSize;
   if (decode) return i8_splits(nb, a.max_splits);
   if (rows > a.row_slots) return 1;
   const int tiles = s.n == 1 ? 1 : (rows + 15) / 16;
   const int n = i8_splits(nb, min(a.max_splits, kI8MaxSplits / tiles), kI8SplitBlocks * tiles);
-  return max(1, min(n, (int)((unsigned)a.chunk_parts / (unsigned)max(rows, 1))));
+  return n * rows > a.chunk_parts ? 1 : n;
 }
 
 // The first partial of a row.
