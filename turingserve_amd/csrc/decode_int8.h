@@ -220,10 +220,10 @@ __device__ __forceinline__ half8_t i8_vt(const uint32_t (&v)[2][4][I8Pair<D>::VW
 
 template <int D, int t = 0>
 __device__ __forceinline__ void i8_pv(float4_t (&o)[D / 16], const uint32_t (&v)[2][4][I8Pair<D>::VWORDS],
-                                      half8_t p, float alpha) {
+                                      half8_t p) {
   if constexpr (t < D / 16) {
-    o[t] = mfma16x16x32(i8_vt<D, t>(v), p, o[t] * alpha);
-    i8_pv<D, t + 1>(o, v, p, alpha);
+    o[t] = mfma16x16x32(i8_vt<D, t>(v), p, o[t]);
+    i8_pv<D, t + 1>(o, v, p);
   }
 }
 
@@ -255,12 +255,13 @@ __device__ __forceinline__ void i8_step(I8State<D>& st, const I8Pair<D>& x, cons
                                   vmax(vmax(sb[0], sb[1]), vmax(sb[2], sb[3]))));
   // !(<=): a NaN score (a block whose scale is NaN) moves the reference to NaN, where it stays
   const bool move = !(top <= st.m + kI8Rescale);
-  float alpha = 1.f;
   if (__ballot(move)) {
     const float to = vmax(st.m, top);
-    alpha = move ? fast_exp2(st.m - to) : 1.f;             // m = -inf: 0
+    const float alpha = move ? fast_exp2(st.m - to) : 1.f; // m = -inf: 0
     st.l *= alpha;
     st.m = move ? to : st.m;
+#pragma unroll
+    for (int t = 0; t < D / 16; ++t) st.o[t] *= alpha;
   }
   const float neg = st.m == -INFINITY ? 0.f : -st.m;
   float pa[4], pb[4];
@@ -271,7 +272,7 @@ __device__ __forceinline__ void i8_step(I8State<D>& st, const I8Pair<D>& x, cons
 #pragma unroll
   for (int r = 0; r < 4; ++r) p[r] = (half_t)(pa[r] * fva), p[4 + r] = (half_t)(pb[r] * fvb);
   // Codes left past the end are finite, and p is 0 there.
-  i8_pv<D>(st.o, x.v, p, alpha);
+  i8_pv<D>(st.o, x.v, p);
 }
 
 // One split [b0, b1) of a sequence's blocks by one wavefront (of kI8Waves). Blocks are taken 64
