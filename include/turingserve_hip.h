@@ -27,6 +27,8 @@
  *   ts_rope                <- ops/triton_rope.py:27-31      (twin ops/reference.py:31-42)
  *   ts_rope_kv_write       <- rope then kv_write of one layer, fused (model/qwen2.py:26-28, :89)
  *   ts_silu_mul            <- ops/triton_silu_mul.py:21-28  (twin ops/reference.py:26-28)
+ *   ts_kv_write_int8, ts_rope_kv_write_int8, ts_paged_attention_int8  the write and the attention of
+ *                             a K/V cache held in 8 bits (no counterpart in the reference)
  *                             (twin ops/reference.py:45-47 + quant/int8.py:15-16)
  *
  * Conventions shared by every entry point
@@ -41,6 +43,7 @@
  *  - Paged KV cache of one layer: k_cache / v_cache are [num_blocks, num_kv_heads, 16, head_dim]
  *    contiguous (the per-layer views kv_cache[l, 0] / kv_cache[l, 1] of the reference's
  *    [L, 2, num_blocks, KVH, 16, D] tensor, engine/builder.py:76-80). Block 0 is the null block.
+ *    The 8-bit cache has the same blocks, int8, and fp32 scales beside them (ts_kv_write_int8).
  *  - Memory safety instead of undefined behaviour: slot ids outside [0, num_blocks*16) are
  *    skipped like -1, block ids outside [0, num_blocks) read block 0, and a sequence whose
  *    seq_len exceeds 16 * max_blocks_per_seq attends only to the blocks its table holds.
@@ -554,7 +557,8 @@ int ts_rope_kv_write_int8(const void* qkv, int64_t qkv_stride, const int64_t* po
  * V scale is not finite is NaN. A decode row's result does not depend on the rest of the batch
  * given max_seq_len. The host bounds shape the launch only: bounds below the batch's real values
  * are slower, not wrong. head_dim 16, 32, 64, 128 or 256, any number of query heads per KV head; q
- * rows 16-byte aligned, scale > 0. Workspace: the queried size, 256-byte aligned (may be 0).
+ * rows 16-byte aligned, scale > 0. Tables of at most 2^26 blocks a sequence; query_start_loc ascends.
+ * Workspace: the queried size, 256-byte aligned (may be 0). Rows of no sequence are not written.
  */
 size_t ts_paged_attention_int8_workspace_bytes(int32_t num_seqs, int32_t num_decode,
                                                int32_t max_query_len, int32_t max_seq_len,

@@ -6,9 +6,17 @@
 // The rows of a sequence for one KV head, row = token * group + head, stand in tiles of 16 (the rows
 // of an MFMA tile); row i's token sees the first seq_len - n + token + 1 tokens. One workgroup of
 // four wavefronts takes one split of the sequence's blocks for one tile: every code is read once for
-// a whole group of heads. The four wavefronts take pairs of blocks in turn with a running maximum and sum each,
-// meet once at the end in LDS, and either write the row or leave a partial (m, l, O) for the merge
-// launch.
+// a whole group of heads. The four wavefronts take pairs of blocks in turn with a running maximum and
+// sum each, meet once at the end in LDS, and either write the row or leave a partial (m, l, O) for the
+// merge launch.
+//
+// 64 sequences of 128 to 4096 tokens, 12/2 heads of 128: 13.6 us and 4.0 for the merge, 38 MB of codes
+// and scales (7.7 us at a copy's 5.0 TB/s); one sequence of 6000: 7.0 and 3.7. What bounds it is the chain
+// of a workgroup (lengths, table, scales and codes, LDS, partial) and then that of the merge: taking out
+// a tenth of the loop's arithmetic (O scaled in every step) gained 1 %. Two tiles a workgroup (32 rows of
+// a chunk, 253 registers, two workgroups a CU) took 29.0 us instead of 24.7 at 16 sequences of 5 rows,
+// 28/4 heads on 300 to 3000 cached, and 16.5 instead of 13.9 at one of 8 rows on 1024, and were ahead
+// only past some 1500 tiles (16 chunks of 128 rows on 512: 29.2 and 35.8).
 #pragma once
 
 #include "int8_kv.h"
@@ -17,7 +25,11 @@ namespace ts {
 
 constexpr int kI8Waves = 4;
 constexpr int kI8Threads = kI8Waves * kWave;
-constexpr int kI8SplitBlocks = 16;     // blocks of a split, as long as kI8MaxSplits suffice
+// Blocks of a split, as long as kI8MaxSplits suffice. 8, 16 and 32 blocks: 18.2, 17.8 and 18.3 us at the
+// 64 sequences above, 18.9, 18.8 and 20.6 at four of 8000 to 32768 tokens, 11.0, 11.1 and 12.5 at one.
+constexpr int kI8SplitBlocks = 16;
+// A lane of the merge each. 32 and 64: 15.6 and 14.2 us at one sequence of 32768, 41.4 and 27.5 at one of
+// 131072, 20.4 and 23.0 at four of 32768.
 constexpr int kI8MaxSplits = 64;
 constexpr float kI8Rescale = 8.f;      // a row's reference moves when a score passes it by 2^8
 
