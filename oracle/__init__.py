@@ -10,6 +10,8 @@ Contents (numpy; every function cites the reference file:line it restates):
   merge of ``ops/triton_decode_attention.py:144-163`` and a pure-Python brute force.
 * ``oracle.quant``  -- per-row int8 quantisation ``quant/int8.py:8-16`` and the W8A16 product
   ``ops/triton_w8a16.py:11-35`` / the twin ``ops/reference.py:45-47``.
+* ``oracle.int8_cache`` -- the 8-bit paged cache's write, and attention over it in 64 bits with a
+  bound on each output's error (no counterpart in the reference).
 
 How each function is pinned (the reference stores no golden vectors for this path): see the
 tests in ``tests/test_oracle.py`` -- fp64 brute-force loops, closed forms (identity weights,
