@@ -152,6 +152,9 @@ def test_empty_calls_and_workspace_sizes():
     long = size(4, 4, 1, 32768, 0, 12, 2, 128, 256)
     assert long >= 4 * 12 * 64 * (128 + 2) * 4
     assert size(8, 8, 1, 32768, 0, 12, 2, 128, 256) > long
+    # the host's bounds may be anything
+    huge = 2 ** 31 - 1
+    assert size(64, 0, huge, huge, huge, 64, 8, 128, 256) == size(64, 0, 4096, 65536, 65536, 64, 8, 128, 256)
     # chunks of several tiles of 16 rows leave no more partials than one tile, but for a split a tile
     tile = 16 * 64 * (128 + 2) * 4 * 4
     assert tile <= size(4, 0, 16, 32768, 32768, 8, 8, 128, 256) / 8 < 1.01 * tile

@@ -210,8 +210,9 @@ def test_write_past_two_to_the_31_bytes():
     want = oracle_write(c)
     assert_cache((kc[lo:], vc[lo:], ks[lo:], vs[lo:]), want)
     assert not kc[:lo].any() and not vc[:lo].any() and not ks[:lo].any()
-    out = H.paged_attention_int8(q, kc, vc, ks, vs, meta, c.scale)
-    assert_rows(out, c, cache=want)
+    for bound in (33, 30000):                        # tiles of 16 rows, the prompt kernel
+        m = dataclasses.replace(meta, max_prefill_seq_len=bound)
+        assert_rows(H.paged_attention_int8(q, kc, vc, ks, vs, m, c.scale), c, f"{bound}", cache=want)
 
 
 # ------------------------------------------------------------------------------------- decode
@@ -279,6 +280,29 @@ def test_scales_of_very_different_size():
     c.scales[1, c.tables[1, ::3]] = 0
     _, q, _, _, cache, meta = c.on(DEV)
     assert_rows(H.paged_attention_int8(q, *cache, meta, c.scale), c)
+
+
+@pytest.mark.parametrize("bound", [101, 30000])
+def test_scales_too_small_for_fp16(bound):
+    """V scales down to fp32's subnormal numbers: such blocks are zeros, beside others and alone."""
+    c = Case((4, 2, 64), [(99, 1), (30, 1), (40, 60)], num_decode=2, seed=34)
+    c.scales[1, c.tables[0, ::2]] = 1e-40
+    c.scales[1, c.tables[1]] = 1e-42
+    c.scales[1, c.tables[2, 1:3]] = 1e-36
+    c.scales[0, c.tables[2, 3]] = 1e-41
+    _, q, _, _, cache, meta = c.on(DEV)
+    out = H.paged_attention_int8(q, *cache, dataclasses.replace(meta, max_prefill_seq_len=bound), c.scale)
+    assert_rows(out, c, f"{bound}")
+    assert not out[1].any()
+
+
+def test_more_heads_than_a_chunk_may_have_rows():
+    """160 query heads on one KV head: ten tiles a token."""
+    c = Case((160, 1, 16), [(900, 1), (4, 1), (300, 3), (70, 1)], num_decode=2, seed=35)
+    _, q, _, _, cache, meta = c.on(DEV)
+    for bound in (303, 30000):
+        m = dataclasses.replace(meta, max_prefill_seq_len=bound)
+        assert_rows(H.paged_attention_int8(q, *cache, m, c.scale), c, f"{bound}")
 
 
 # ------------------------------------------------------------------------------------- prefill
@@ -497,6 +521,44 @@ def test_decode_graph_replayed_over_growing_sequences():
         ref, bound = O.paged_attention(c.split()[0][rows], codes, scales, c.tables, now, [0, 1, 2, 3],
                                        c.scale)
         assert (np.abs(out.double().cpu().numpy() - ref) <= bound).all(), str(now)
+
+
+def test_chunk_graphs_of_one_pool():
+    """Two captured mixed steps (one for each of the attention's kernels) whose workspaces share a
+    memory pool, replayed in turn with other inputs each time and eager calls in between."""
+    c = Case((14, 2, 64), [(900, 1), (300, 40), (0, 500), (17, 1)], num_decode=1, seed=36)
+    _, q, k, v, cache, meta = c.on(DEV)
+    start = tuple(t.clone() for t in cache)
+    qq, kk, vv = q.clone(), k.clone(), v.clone()
+    metas = [dataclasses.replace(meta, max_prefill_seq_len=b) for b in (500, 30000)]
+
+    def step(m):
+        H.kv_write_int8(kk, vv, *cache, m)
+        return H.paged_attention_int8(qq, *cache, m, c.scale)
+
+    for m in metas:
+        step(m)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for m in metas:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], pool=graphs[0].pool() if len(graphs) > 1 else None):
+            outs.append(step(m))
+    for turn in range(3):
+        for g, out, m in zip(graphs, outs, metas):
+            qq.copy_(q.roll(turn, 0)), kk.copy_(k.roll(turn, 0)), vv.copy_(v.roll(-turn, 0))
+            for t, s in zip(cache, start):
+                t.copy_(s)
+            g.replay()
+            got, codes = out.clone(), tuple(t.clone() for t in cache)
+            for t, s in zip(cache, start):
+                t.copy_(s)
+            assert torch.equal(step(m), got), turn
+            assert all(torch.equal(a, b) for a, b in zip(codes, cache)), turn
+        _, kn, vn = c.split()
+        want = oracle_write(c, np.roll(kn, turn, 0), np.roll(vn, -turn, 0))
+        assert_cache(cache, want)
+        assert_rows(got, c, f"{turn}", cache=want, q=np.roll(c.split()[0], turn, 0))
 
 
 def test_two_streams_at_once():

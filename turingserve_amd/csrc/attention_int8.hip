@@ -41,7 +41,8 @@ static Int8Plan int8_plan(int num_seqs, int num_decode, int max_query_len, int m
   const int64_t chunk_rows = (int64_t)(max_query_len > 0 ? max_query_len : 1) * G;
   const int64_t P = num_seqs - num_decode;
   const int seq = max_prefill_seq_len > 0 ? max_prefill_seq_len : max_seq_len > 0 ? max_seq_len : 1;
-  const int64_t work = P * KVH * ((chunk_rows + 15) / 16) * ((seq + 31) / 32);
+  // (sizes that no batch has may come as bounds: products of four in floating point)
+  const double work = (double)P * KVH * ((chunk_rows + 15) / 16) * ((seq + 31) / 32);
   const bool all = P == 0 || chunk_rows <= kI8ShortRows || (seq <= kI8SmallSeq && work <= kI8SmallWork);
   pl.small = all ? num_seqs : num_decode;
   pl.row_slots = (int)(chunk_rows < kI8ShortRows ? chunk_rows : kI8ShortRows);
@@ -58,10 +59,10 @@ static Int8Plan int8_plan(int num_seqs, int num_decode, int max_query_len, int m
   }
   if (!all) {
     const int tile_rows = 32 * i8_prefill_waves(D);
-    const int64_t tiles = P * KVH * ((chunk_rows + tile_rows - 1) / tile_rows);
-    const int64_t cost = tiles * ((seq - 1) / kI8Keys + 1 + kI8TileCost);
-    const int64_t most = (int64_t)i8_prefill_groups(D) * cus;
-    pl.groups = (int)(cost / kI8MinShare < most ? (cost < kI8MinShare ? 1 : cost / kI8MinShare) : most);
+    const double tiles = (double)P * KVH * ((chunk_rows + tile_rows - 1) / tile_rows);
+    const double shares = tiles * ((seq - 1) / kI8Keys + 1 + kI8TileCost) / kI8MinShare;
+    const int most = i8_prefill_groups(D) * cus;
+    pl.groups = shares < most ? (shares < 1 ? 1 : (int)shares) : most;
     const size_t r = (size_t)2 * pl.groups * tile_rows;
     pl.pre_o = take(at, r * D * sizeof(float));
     pl.pre_ml = take(at, r * 2 * sizeof(float));

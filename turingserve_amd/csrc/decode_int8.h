@@ -128,9 +128,11 @@ __device__ __forceinline__ int i8_kv_len(int len, int max_blocks) {
 }
 
 // A block with a scale that is not finite makes the scores of its visible tokens NaN, and its V
-// scale 0: tokens which a row does not see stay out of it (0 * NaN would not).
+// scale 0: tokens which a row does not see stay out of it (0 * NaN would not). A V scale below 1e-30,
+// whose reciprocal need not be finite, counts as 0: fp16 has no values that small.
 __device__ __forceinline__ void i8_poison(float& ks, float& vs) {
   if (!(fabsf(ks) < INFINITY && fabsf(vs) < INFINITY)) ks = __builtin_nanf(""), vs = 0.f;
+  if (vs < 1e-30f) vs = 0.f;
 }
 
 template <int D>
