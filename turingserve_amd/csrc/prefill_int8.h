@@ -267,9 +267,24 @@ struct I8Stage {
     for (int i = 0; i < N; ++i)
       if (ALL || unit(i) < UNITS) {
         k[i] = ld<uint4_t>(a.kc + base(a, id[i], h) + 16 * (unit(i) % D));
-        const half_t o = id[i] < 0 ? (half_t)__builtin_nanf("") : (half_t)1152.f;
-        off[i] = {o, o};
       }
+    finite(id);
+  }
+  // Ids of a step's blocks from the table itself, and, once the scales are known, their finite ones.
+  static __device__ __forceinline__ void ids(const Int8DecodeArgs& a, const int32_t* table, int last, int (&id)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      int at = min(unit(i), UNITS - 1) / D;
+      if (UNIFORM) at = __builtin_amdgcn_readfirstlane(at);
+      id[i] = clamp_block(table_entry(table + min(at, last)), a.num_blocks);
+    }
+  }
+  __device__ __forceinline__ void finite(const int (&id)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const half_t o = id[i] < 0 ? (half_t)__builtin_nanf("") : (half_t)1152.f;
+      off[i] = {o, o};
+    }
   }
   // Row r of the 4 tokens (one at a time, so that they stand between other work).
   __device__ __forceinline__ void request_v(const Int8DecodeArgs& a, const int (&id)[N], int h, int r) {
@@ -389,6 +404,35 @@ struct I8Exp {
 // The workgroup meets behind the first phase, with no LDS read under way: what the step before staged
 // (K in its third phase, V in its fourth) is read behind that, and this step stages over what was
 // read before it. Returns each row's largest next score.
+// Before the first step: its scores, and the staging that a step does.
+template <int D, typename Mask, typename Work>
+__device__ __forceinline__ float i8_first(I8Rows<D>& w, const half_t* kn, float16_t (&sc)[2], const float* fknp,
+                                          Mask mask, Work work) {
+  typedef I8Rows<D> R;
+  work(0);
+#pragma unroll
+  for (int v = 3; v < 7; ++v) work(v);
+  float16_t zero;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) zero[i] = 0.f;
+#pragma unroll
+  for (int j = 0; j < 2 * R::NQ; ++j)
+    sc[j / R::NQ] = mfma_i8(w.operand(nullptr, kn, nullptr, R::NP + j), w.q[j % R::NQ], j % R::NQ == 0 ? zero : sc[j / R::NQ]);
+  const float4_t fkn = ld<float4_t>(fknp);
+  mask(sc);
+  float top[4];
+#pragma unroll
+  for (int b = 0; b < 4; ++b)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float x = sc[b / 2][8 * (b % 2) + e];
+      top[b] = e == 0 ? x : vmax(top[b], x);
+    }
+  work(1);
+  work(2);
+  return vmax(vmax(top[0] * fkn[0], top[1] * fkn[1]), vmax(top[2] * fkn[2], top[3] * fkn[3]));
+}
+
 template <int D, typename Mask, typename Work>
 __device__ __forceinline__ float i8_step64(I8Rows<D>& w, const half_t* vp, const half_t* kn, const half_t* vc,
                                            float16_t (&sc)[2], half8_t (&pr)[4], const float* fkp,
@@ -513,21 +557,34 @@ __device__ __forceinline__ void i8_piece(const Int8PrefillArgs& p, I8PrefillLds<
     const int blocks = min(nb - w0 * kI8StepBlocks, n * kI8StepBlocks), last = blocks - 1;
     __syncthreads();                                       // the last window's and piece's reads
     constexpr int PER = (kI8Window + THREADS - 1) / THREADS;
+    const int32_t* table = a.block_tables + b * a.bt_stride + w0 * kI8StepBlocks;
+    S stage;
+    int id0[S::N], id1[S::N], id2[S::N];                   // of the next step, the second, the third
+    S::ids(a, table, last, id0);
     int blk[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int at = threadIdx.x + i * THREADS;
-      blk[i] = at < blocks ? clamp_block(a.block_tables[b * a.bt_stride + w0 * kI8StepBlocks + at], a.num_blocks) : 0;
+      blk[i] = at < blocks ? clamp_block(table[at], a.num_blocks) : 0;
+    }
+    float scales[PER][2];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const bool real = (int)threadIdx.x + i * THREADS < blocks;
+      scales[i][0] = real ? a.ks[(int64_t)blk[i] * a.kvh + h] : 0.f;
+      scales[i][1] = real ? a.vs[(int64_t)blk[i] * a.kvh + h] : 0.f;
+    }
+    stage.request_k(a, id0, h);
+    if (w0 == s0) {                                        // q behind what the first scores wait for
+      const half_t* qrow = a.q + (int64_t)(k.q0 + token) * a.q_st + (int64_t)head * a.q_sh;
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) w.q[i] = ld<half8_t>(qrow + 16 * i + 8 * hh);
     }
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int at = threadIdx.x + i * THREADS;
-      float ks = 0.f, vs = 0.f;
-      if (at < blocks) {
-        ks = a.ks[(int64_t)blk[i] * a.kvh + h];
-        vs = a.vs[(int64_t)blk[i] * a.kvh + h];
-        i8_poison(ks, vs);
-      }
+      float ks = scales[i][0], vs = scales[i][1];
+      i8_poison(ks, vs);
       // A K factor of 0 or NaN would leave hidden tokens (-inf) NaN: scores of a factor as small as
       // the least one are 0, and the codes of blocks without finite scales are staged as NaN.
       const float f = ks * a.sl2;
@@ -538,16 +595,9 @@ __device__ __forceinline__ void i8_piece(const Int8PrefillArgs& p, I8PrefillLds<
       }
     }
     __syncthreads();
-    S stage;
-    int id0[S::N], id1[S::N], id2[S::N];                   // of the next step, the second, the third
     S::ids(lds, 0, last, id0);
     S::ids(lds, kI8StepBlocks, last, id1);
-    stage.request_k(a, id0, h);
-    if (w0 == s0) {                                        // q behind what the first scores wait for
-      const half_t* qrow = a.q + (int64_t)(k.q0 + token) * a.q_st + (int64_t)head * a.q_sh;
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i) w.q[i] = ld<half8_t>(qrow + 16 * i + 8 * hh);
-    }
+    stage.finite(id0);
     float top = 0.f;
 #pragma unroll
     for (int i = 0; i < kI8Window; i += kWave) top = fmaxf(top, lds.vs[i + lane]);
@@ -565,22 +615,20 @@ __device__ __forceinline__ void i8_piece(const Int8PrefillArgs& p, I8PrefillLds<
       lds.back[i] = fast_exp2(-f);
     }
     stage.place_k(lds.k[0]);
-    for (int i = threadIdx.x; i < 2 * I8Tile<D>::HALVES / 8; i += THREADS)
-      st<half8_t>(lds.v[0] + 8 * i, half8_t{0, 0, 0, 0, 0, 0, 0, 0});
+    for (int i = threadIdx.x; i < I8Tile<D>::HALVES / 8; i += THREADS)
+      st<half8_t>(lds.v[1] + 8 * i, half8_t{0, 0, 0, 0, 0, 0, 0, 0});
     __syncthreads();
 
     // Step i reads K of step i + 1 in k[(i + 1) % 2], V of steps i - 1 and i in v[(i - 1) % 2] and
-    // v[i % 2], and stages K of step i + 2 and V of step i + 1. The first of them, step -1, has hidden
-    // scores only (and V codes of 0): it is there for the scores of step 0. The loop has no branch
-    // but the mask's and the reference's: past the window's end the last blocks are staged again,
-    // and the scores of the step behind it are not used.
+    // v[i % 2], and stages K of step i + 2 and V of step i + 1. Before the first of them the scores of
+    // step 0 are formed (i8_first; P' of a step before it is 0, on V codes of 0). The loop has no
+    // branch but the mask's and the reference's: past the window's end the last blocks are staged
+    // again, and the scores of the step behind it are not used.
     float16_t sc[2];
     half8_t pr[4];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) sc[0][i] = sc[1][i] = -INFINITY;
-#pragma unroll
     for (int e = 0; e < 8; ++e) pr[2][e] = pr[3][e] = (half_t)0.f;
-    auto step = [&](auto parity, int i) {
+    auto step = [&](auto parity, auto first, int i) {
       constexpr int P = decltype(parity)::value;           // i % 2
       auto work = [&](int part) {
         if (part == 0) {
@@ -602,16 +650,19 @@ __device__ __forceinline__ void i8_piece(const Int8PrefillArgs& p, I8PrefillLds<
               x[kt][e] = key0 + 32 * kt + 8 * (e / 4) + e % 4 < vis ? x[kt][e] : -INFINITY;
         }
       };
-      const int wb = max(i, 0) * kI8StepBlocks;
-      const float best = i8_step64<D>(w, lds.v[1 - P], lds.k[1 - P], lds.v[P], sc, pr, lds.fk + wb, lds.vs + wb,
-                                      lds.back + wb, lds.fk + (i + 1) * kI8StepBlocks, mask, work);
+      const int wb = i * kI8StepBlocks;
+      const float best = decltype(first)::value
+                             ? i8_first<D>(w, lds.k[0], sc, lds.fk, mask, work)
+                             : i8_step64<D>(w, lds.v[1 - P], lds.k[1 - P], lds.v[P], sc, pr, lds.fk + wb, lds.vs + wb,
+                                            lds.back + wb, lds.fk + wb + kI8StepBlocks, mask, work);
       i8_reference<D>(w, i + 1 < n ? best : w.m);          // (its own reference moves none, also a NaN)
 #pragma unroll
       for (int e = 0; e < S::N; ++e) id0[e] = id1[e], id1[e] = id2[e];
     };
-    for (int i = -1; i < n; i += 2) {
-      step(I8Const<1>(), i);
-      if (i + 1 < n) step(I8Const<0>(), i + 1);
+    step(I8Const<1>(), I8Const<1>(), -1);
+    for (int i = 0; i < n; i += 2) {
+      step(I8Const<0>(), I8Const<0>(), i);
+      if (i + 1 < n) step(I8Const<1>(), I8Const<0>(), i + 1);
     }
     const half_t* vl = lds.v[(n - 1) & 1];                 // the last step's second half
 #pragma unroll
