@@ -25,7 +25,7 @@
 // of a sequence's first t tiles have a closed form, so a batch of one long and many short prompts
 // costs what its rows cost.
 //
-// 2048 rows on 4096 cached, 12/2 heads of 128: 85 to 88 us and 9.5 for the merge, 64.4 GFLOP: 680
+// 2048 rows on 4096 cached, 12/2 heads of 128: 84 to 87 us and 9.5 for the merge, 64.4 GFLOP: 690
 // TFLOP/s where a large matrix product reaches 1210. A step of 64 tokens takes eight wavefronts some 3700
 // cycles, of which the MFMAs are 2050; exponentials, operand reads, staging and requests are worth 10 to
 // 14 % each when taken out, so it is the issue of all of them together that bounds it. 64 rows a
@@ -41,8 +41,8 @@ typedef float float16_t __attribute__((ext_vector_type(16)));
 constexpr int kI8Keys = 64;              // tokens of a step
 constexpr int kI8StepBlocks = kI8Keys / kBlockSize;
 constexpr int kI8Window = 256;           // blocks whose ids and scales are held in LDS at a time
-constexpr int kI8MinShare = 6;           // steps (and tiles' costs) that a workgroup is worth: 4, 6, 8 and 16 are
-                                         // 31.4, 31.7, 31.8 and 33 us at five chunks of 90 to 1100 rows
+constexpr int kI8MinShare = 6;           // steps (and tiles' costs) that a workgroup is worth: 31.0, 30.6 and 31.1
+                                         // us with 4, 6 and 8 at five chunks of 90 to 1100 rows
 constexpr float kI8LeastRatio = -30.f;   // log2 of the least V scale ratio
 constexpr float kI8LeastFactor = 1e-30f;
 
@@ -133,8 +133,9 @@ __device__ __forceinline__ int i8_steps(const Int8DecodeArgs& a, const I8Chunk& 
 // C(t + 1) - C(t) > kI8TileCost + 1 + (start + (t + 1) ROWS / group) / 64, and tile t sees at most
 // start + ((t + 1) ROWS - 1) / group + 1 tokens, whose steps are fewer than the sum's last two terms.
 // Steps of a share that fall on a tile's start or behind its last one are nobody's. (At
-// 2048 rows on 4096 cached, 12/2 heads of 128, and five chunks of 90 to 1100, 14/2 heads of 64: 96.0 and
-// 32.1 us with kI8TileCost 3, 94.4 and 31.8 with 5, 94.8 and 31.7 with 7.)
+// 2048 rows on 4096 cached, 12/2 heads of 128, and five chunks of 90 to 1100, 14/2 heads of 64: 93.5 and
+// 30.3 us with kI8TileCost 3, 93.0 and 30.6 with 5, 94.3 and 31.0 with 7; 100.4 and 36.1 with 1, when those
+// with 5 were 97.8 and 36.3.)
 constexpr int kI8TileCost = 5;
 // ROWS / (2 group) of a step's 64 tokens in units of 2^-12, rounded up.
 constexpr int i8_rate(int rows, int group) { return (32 * rows + group - 1) / group; }
@@ -722,9 +723,12 @@ prefill_int8_kernel(Int8PrefillArgs p) {
     }
     if (found) {
       const int s0 = place.before * a.kvh + h * place.cost + kI8TileCost;
-      const int first = shares.of(s0), last = shares.of(s0 + i8_steps<ROWS>(a, place.k, place.tile) - 1);
-      if (first + 1 == (int)blockIdx.x && last > first && last < shares.count)
-        joint = {first, last, place.k.q0, place.k.n * a.group, place.tile * ROWS, h};
+      const int g = blockIdx.x;
+      if (g > 0 && shares.begin(g - 1) <= s0 && s0 < at) {
+        const int last = shares.of(s0 + i8_steps<ROWS>(a, place.k, place.tile) - 1);
+        if (last >= g && last < shares.count)
+          joint = {g - 1, last, place.k.q0, place.k.n * a.group, place.tile * ROWS, h};
+      }
     }
     if (threadIdx.x == 0) p.joints[blockIdx.x] = joint;
     if (!found) return;
