@@ -9,7 +9,7 @@
 // that whatever attends to the block comes out NaN and nothing finite is made up.
 //
 // One workgroup owns one (block, KV head, K or V): it holds the whole block in registers (sixteen
-// lanes a row; a single new row, as a decode step appends, over D / 2 threads), so the maximum, the
+// lanes a row; a single new row spread over D / 2 threads gained nothing), so the maximum, the
 // scale and every row's rewrite need no other workgroup and the result does not depend on the order
 // of anything. A sequence's blocks are found from the step's metadata (query_start_loc, seq_lens,
 // block tables), not from slots: the rows of a block then lie together and its owner knows them without
@@ -19,8 +19,8 @@
 // positions, codes and scale, then angles), so each link asks for everything it can before it waits:
 // 64 appended rows with RoPE, 12/2 heads of 128, 3.5 us (7.7 with a wavefront a block, four rows at a
 // time and a division a code). Larger ones are bound by the rows in flight: a chunk of 2048 rows on 4096
-// cached 6.5 us, 17 MB or 2.6 TB/s; 8192 rows of 32/8 heads 51 us, 185 MB or 3.6 TB/s, of a copy's 5.0.
-// (Rows asked for ahead of the block id cost registers: 54 us there, and nothing gained at the small.)
+// cached 6.5 us, 17 MB or 2.6 TB/s; 8192 rows of 32/8 heads 48 us, 185 MB or 3.8 TB/s, of a copy's 5.0.
+// (Rows asked for ahead of the block id cost registers: 6 % there, and nothing gained at the small.)
 #include <float.h>
 
 #include "int8_kv.h"
@@ -85,7 +85,7 @@ __device__ __forceinline__ float grown(float was, float top) {
 
 // rint(x / scale) for |x| <= 127 scale, by a reciprocal where that decides it: x * rcp is within
 // 127 * 2^-22 of the quotient, so it rounds alike unless it lies that close to a half. `near` is set
-// where the division has to be made.
+// where the division has to be made. (Divisions alone: 24.9 us against 23.3 at 8192 rows, 8 heads of 128.)
 __device__ __forceinline__ float code_of(float x, float rcp, bool& near) {
   const float y = x * rcp, c = rintf(y);
   near = near || fabsf(fabsf(y - c) - 0.5f) < 1.f / 16384.f;
@@ -129,56 +129,36 @@ __device__ __forceinline__ void write_block(const Int8WriteArgs& a, int j, int64
   RowCodes<D> kept;
   if (old) kept.load(block, r, s);
 
-  const bool single = hi - lo == 1;
+  const bool fresh = lane && r >= lo && r < hi;
   RowCodes<D> code;
-  float x1 = 0.f, y1 = 0.f;                                // a single row: one pair a thread
   typename R::Floats x, y;
-  bool fresh;
   float top = 0.f;
-  if (single) {
-    fresh = tid < D / 2;
-    if (fresh) {
-      const int64_t t = row0 + 16 * j + lo;
-      x1 = (float)rows[t * st_t + tid], y1 = (float)rows[t * st_t + tid + D / 2];
-      if (TURN) {
-        const int64_t pos = rope_row(a.positions[t], a.max_pos) * (D / 2);
-        rotate_k(x1, y1, a.cos_t[pos + tid], a.sin_t[pos + tid]);
+  if (fresh) {
+    const int64_t t = row0 + 16 * j + r;
+    const typename R::Halves u = ld<typename R::Halves>(rows + t * st_t + s * R::VEC);
+    const typename R::Halves v = ld<typename R::Halves>(rows + t * st_t + s * R::VEC + D / 2);
+#pragma unroll
+    for (int e = 0; e < R::VEC; ++e) x[e] = (float)u[e], y[e] = (float)v[e];
+    if (TURN) {
+      const int64_t pos = rope_row(a.positions[t], a.max_pos) * (D / 2) + s * R::VEC;
+      const typename R::Floats c = ld<typename R::Floats>(a.cos_t + pos);
+      const typename R::Floats n = ld<typename R::Floats>(a.sin_t + pos);
+#pragma unroll
+      for (int e = 0; e < R::VEC; ++e) {
+        float f = x[e], g = y[e];
+        rotate_k(f, g, c[e], n[e]);
+        x[e] = f, y[e] = g;
       }
-      top = larger(x1, y1);
     }
-  } else {
-    fresh = lane && r >= lo && r < hi;
-    if (fresh) {
-      const int64_t t = row0 + 16 * j + r;
-      const typename R::Halves u = ld<typename R::Halves>(rows + t * st_t + s * R::VEC);
-      const typename R::Halves v = ld<typename R::Halves>(rows + t * st_t + s * R::VEC + D / 2);
 #pragma unroll
-      for (int e = 0; e < R::VEC; ++e) x[e] = (float)u[e], y[e] = (float)v[e];
-      if (TURN) {
-        const int64_t pos = rope_row(a.positions[t], a.max_pos) * (D / 2) + s * R::VEC;
-        const typename R::Floats c = ld<typename R::Floats>(a.cos_t + pos);
-        const typename R::Floats n = ld<typename R::Floats>(a.sin_t + pos);
-#pragma unroll
-        for (int e = 0; e < R::VEC; ++e) {
-          float f = x[e], g = y[e];
-          rotate_k(f, g, c[e], n[e]);
-          x[e] = f, y[e] = g;
-        }
-      }
-#pragma unroll
-      for (int e = 0; e < R::VEC; ++e) top = larger(top, larger(x[e], y[e]));
-    }
+    for (int e = 0; e < R::VEC; ++e) top = larger(top, larger(x[e], y[e]));
   }
   top = largest(top);
   if (tid % kWave == 0) s_top[tid / kWave] = top;
   __syncthreads();
   const float now = grown(was, larger(larger(s_top[0], s_top[1]), larger(s_top[2], s_top[3])));
 
-  if (fresh && single) {
-    int8_t* dst = block + lo * D + tid;
-    dst[0] = now > 0.f ? (int8_t)(int)exact_code(x1, now) : (int8_t)0;
-    dst[D / 2] = now > 0.f ? (int8_t)(int)exact_code(y1, now) : (int8_t)0;
-  } else if (fresh) {
+  if (fresh) {
     const float rcp = now >= FLT_MIN ? 1.f / now : 0.f;    // (scales below the normal numbers divide)
     bool near = !(now >= FLT_MIN);
 #pragma unroll
