@@ -114,5 +114,5 @@ def paged_attention(q, codes, scales, tables, seq_lens, starts, scale: float):
         top = np.abs(v).max() if held else 0.0
         lim = ((2.0 ** -11 + 2 * e + held * 2.0 ** -23) * w + held * 2.0 ** -25 * top
                + 2.0 ** -11 * np.abs(o) + 2.0 ** -25)
-        out[lo:hi], bound[lo:hi] = o.reshape(hi - lo, -1), lim.reshape(hi - lo, -1)
+        out[lo:hi], bound[lo:hi] = o.reshape(-1, H * D), lim.reshape(-1, H * D)
     return out, bound

@@ -68,6 +68,18 @@ def test_twins_match_the_oracle(heads):
     assert (np.abs(out.double().numpy() - ref) <= bound).all()
 
 
+def test_twins_of_sequences_without_rows():
+    c = Case((4, 2, 16), [(20, 1), (40, 0), (0, 0), (5, 20)], num_decode=1, seed=5)
+    _, q, k, v, cache, meta = c.on("cpu")
+    R.kv_write_int8(k, v, *cache, meta)
+    want = c.codes.copy(), c.scales.copy()
+    for j, x in enumerate(c.split()[1:]):
+        O.write(x, want[0][j], want[1][j], c.tables, c.lens, c.starts)
+    assert np.array_equal(torch.stack(cache[:2]).numpy(), want[0])
+    assert np.array_equal(torch.stack(cache[2:]).numpy(), want[1])
+    assert R.paged_attention_int8(q, *cache, meta, c.scale).shape == (c.T, c.H * c.D)
+
+
 def test_rope_twin_matches_the_oracle():
     c = Case((6, 2, 32), [(4, 1), (0, 21), (7, 30)], num_decode=1, seed=3)
     qkv, _, _, _, cache, meta = c.on("cpu")

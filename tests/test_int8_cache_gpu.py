@@ -422,6 +422,28 @@ def test_mixed_batch(heads):
         assert not out[1].any() and not out[int(c.starts[5])].any()
 
 
+def test_sequences_without_rows():
+    """Sequences of no new rows between the others, and a step of rows that belong to none."""
+    c = Case((14, 2, 64), [(100, 1), (40, 0), (0, 0), (5, 20), (300, 0), (70, 60)], num_decode=1, seed=37)
+    qkv, q, k, v, cache, meta = c.on(DEV)
+    H.kv_write_int8(k, v, *cache, meta)
+    want = oracle_write(c)
+    assert_cache(cache, want)
+    for bound in (300, 30000):
+        m = dataclasses.replace(meta, max_prefill_seq_len=bound)
+        assert_rows(H.paged_attention_int8(q, *cache, m, c.scale), c, f"{bound}", cache=want)
+    none = dataclasses.replace(meta, seq_lens=meta.seq_lens[:0], block_tables=meta.block_tables[:0],
+                               query_start_loc=meta.query_start_loc[:1], num_decode=0)
+    cos, sin = rope_tables(c.D, 1e6, 512, DEV)
+    pos = torch.from_numpy(c.pos).to(DEV)
+    H.kv_write_int8(k, v, *cache, none)
+    rotated = H.rope_kv_write_int8(qkv, pos, cos, sin, c.H, c.KVH, c.D, *cache, none)
+    assert_cache(cache, want)
+    assert torch.equal(rotated, H.rope_kv_write_int8(qkv, pos, cos, sin, c.H, c.KVH, c.D,
+                                                     *(t.clone() for t in cache), meta))
+    assert H.paged_attention_int8(q, *cache, none, c.scale).shape == (c.T, c.H * c.D)
+
+
 def test_table_shorter_than_the_sequence():
     c = Case((14, 2, 64), [(299, 1), (50, 200)], num_decode=1, seed=20)
     c.tables = np.ascontiguousarray(c.tables[:, :8])          # 128 tokens of 300 and 250

@@ -303,10 +303,11 @@ static int write_int8(Int8WriteArgs a, bool rope, int D, int max_query_len, cons
              TS_ERR_INVALID_ARG, "%s: num_tokens=%lld num_seqs=%d num_decode=%d", what,
              (long long)a.num_tokens, a.num_seqs, a.num_decode);
   if (a.num_tokens == 0) return TS_OK;
-  TS_REQUIRE(a.k && a.v && a.kc && a.vc && a.ks && a.vs && a.block_tables && a.seq_lens && a.qsl,
+  TS_REQUIRE(a.k && a.v && a.kc && a.vc && a.ks && a.vs &&
+                 (a.num_seqs == 0 || (a.block_tables && a.seq_lens && a.qsl)),
              TS_ERR_INVALID_ARG, "%s: null pointer argument", what);
-  TS_REQUIRE(a.kvh > 0 && a.num_blocks > 0 && a.max_blocks > 0 && a.bt_stride >= a.max_blocks &&
-                 max_query_len >= 0,
+  TS_REQUIRE(a.kvh > 0 && a.num_blocks > 0 && (a.num_seqs == 0 || a.max_blocks > 0) &&
+                 a.bt_stride >= a.max_blocks && max_query_len >= 0,
              TS_ERR_INVALID_ARG, "%s: num_kv_heads=%d num_blocks=%lld max_blocks_per_seq=%d "
              "bt_stride=%lld max_query_len=%d", what, a.kvh, (long long)a.num_blocks, a.max_blocks,
              (long long)a.bt_stride, max_query_len);

@@ -125,6 +125,8 @@ def kv_write_int8(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cac
     qsl, tables = meta.query_start_loc.tolist(), meta.block_tables.tolist()
     for b, length in enumerate(meta.seq_lens.tolist()):
         start = length - (qsl[b + 1] - qsl[b])
+        if start == length:
+            continue
         for j in range(max(start, 0) // 16, -(-length // 16)):
             if j >= len(tables[b]) or not 0 <= tables[b][j] < k_cache.shape[0]:
                 continue
