@@ -144,6 +144,8 @@ odd = ctypes.c_void_p(258)
     (_attend, dict(D=80), N.TS_ERR_UNSUPPORTED, "head_dim 80"),
     (_attend, dict(h=3, kvh=2), N.TS_ERR_INVALID_ARG, "heads"),
     (_attend, dict(nb=0), N.TS_ERR_INVALID_ARG, "num_blocks"),
+    (_attend, dict(seqs=(1 << 20) + 1, ws=P, wsb=1 << 62), N.TS_ERR_UNSUPPORTED, "sequences"),
+    (_attend, dict(T=1 << 30, seqs=4, ws=P, wsb=1 << 62), N.TS_ERR_UNSUPPORTED, "tokens"),
     (_attend, dict(mb=(1 << 26) + 1, bts=1 << 27), N.TS_ERR_INVALID_ARG, "max_blocks"),
     (_attend, dict(qst=130), N.TS_ERR_INVALID_ARG, "misaligned"),
     (_attend, dict(ost=64), N.TS_ERR_INVALID_ARG, "misaligned"),

@@ -151,6 +151,9 @@ extern "C" int ts_paged_attention_int8(const void* q, int64_t q_stride_t, int64_
              TS_ERR_INVALID_ARG, "paged_attention_int8: misaligned q / out / caches");
   TS_REQUIRE(scale > 0.f && scale < INFINITY, TS_ERR_INVALID_ARG,
              "paged_attention_int8: scale must be positive and finite");
+  // The kernels count rows in 31 bits, and splits, of which a sequence has 64 for each tile of rows.
+  TS_REQUIRE(num_seqs <= 1 << 20 && num_tokens < (1ll << 30) / (num_heads / num_kv_heads), TS_ERR_UNSUPPORTED,
+             "paged_attention_int8: %lld tokens of %d sequences", (long long)num_tokens, num_seqs);
   int cus = 0;
   int status = device_cu_count(stream, &cus);
   if (status != TS_OK) return status;
@@ -171,13 +174,13 @@ extern "C" int ts_paged_attention_int8(const void* q, int64_t q_stride_t, int64_
   a.by_kvh = I8Div::by(num_kv_heads), a.by_group = I8Div::by(num_heads / num_kv_heads);
   a.group = num_heads / num_kv_heads, a.qsl = query_start_loc, a.num_tokens = num_tokens;
   a.sl2 = scale * 1.44269504088896340736f;
-  // The kernels count rows in 31 bits, and steps: those of at most `tiles` tiles, each of which sees
-  // what its table holds before the chunk and the chunk (the last term: the rounded rate).
+  // ... and steps: those of at most `tiles` tiles, each of which sees what its table holds before the
+  // chunk and the chunk (the last term: the rounded rate).
   const int tile_rows = 32 * i8_prefill_waves(head_dim);
   const int64_t one = num_tokens * a.group / tile_rows + 1, tiles = one + num_seqs - pl.small;
   const int64_t steps = kI8TileCost + 4 + (max_blocks_per_seq + (num_tokens + 2 * tile_rows) / kBlockSize) /
                         kI8StepBlocks + one / 4096;
-  TS_REQUIRE(num_tokens * a.group < (1ll << 30) && merge_rows(pl, num_decode, num_heads, num_kv_heads) < (1ll << 30) &&
+  TS_REQUIRE(merge_rows(pl, num_decode, num_heads, num_kv_heads) < (1ll << 30) &&
                  (pl.small == num_seqs || tiles * steps * num_kv_heads < (1ll << 31)),
              TS_ERR_UNSUPPORTED, "paged_attention_int8: %lld tokens of %d sequences over tables of %d blocks",
              (long long)num_tokens, num_seqs, max_blocks_per_seq);
