@@ -477,7 +477,8 @@ __global__ void __launch_bounds__(kI8Threads, i8_decode_groups(D)) decode_int8_k
     const int vis = min(kv, max(0, x.seq.start + token + 1));
     const int least = min(kv, max(0, x.seq.start + a.by_group(row0) + 1));
     I8Query<D> q;
-    i8_load_q<D>(a.q + (int64_t)(x.seq.q0 + token) * a.q_st + (int64_t)(h * a.group + row - token * a.group) * a.q_sh,
+    i8_load_q<D>(a.q + (int64_t)(x.seq.q0 + token) * a.q_st +
+                     (int64_t)(h * a.group + row - token * a.group) * a.q_sh,
                  g, c < rows, q);
     I8State<D> st;
     st.m = -INFINITY, st.l = 0.f;

@@ -41,8 +41,9 @@ typedef float float16_t __attribute__((ext_vector_type(16)));
 constexpr int kI8Keys = 64;              // tokens of a step
 constexpr int kI8StepBlocks = kI8Keys / kBlockSize;
 constexpr int kI8Window = 256;           // blocks whose ids and scales are held in LDS at a time
-constexpr int kI8MinShare = 6;           // steps (and tiles' costs) that a workgroup is worth: 31.0, 30.6 and 31.1
-                                         // us with 4, 6 and 8 at five chunks of 90 to 1100 rows
+// Steps (and tiles' costs) that a workgroup is worth: 31.0, 30.6 and 31.1 us with 4, 6 and 8 at five
+// chunks of 90 to 1100 rows, 14/2 heads of 64.
+constexpr int kI8MinShare = 6;
 constexpr float kI8LeastRatio = -30.f;   // log2 of the least V scale ratio
 constexpr float kI8LeastFactor = 1e-30f;
 
@@ -141,7 +142,8 @@ constexpr int kI8TileCost = 5;
 constexpr int i8_rate(int rows, int group) { return (32 * rows + group - 1) / group; }
 
 __device__ __forceinline__ int i8_cost(const Int8PrefillArgs& p, int start, int t) {
-  return t * (kI8TileCost + 2) + (int)(((int64_t)t * ((int64_t)start << 6) + (int64_t)t * (t + 1) * p.rate) >> 12);
+  const int64_t sees = (int64_t)t * ((int64_t)start << 6) + (int64_t)t * (t + 1) * p.rate;
+  return t * (kI8TileCost + 2) + (int)(sees >> 12);
 }
 
 // Where the batch's steps lie: tiles in order, each with all its KV heads.
@@ -272,7 +274,8 @@ struct I8Stage {
     finite(id);
   }
   // Ids of a step's blocks from the table itself, and, once the scales are known, their finite ones.
-  static __device__ __forceinline__ void ids(const Int8DecodeArgs& a, const int32_t* table, int last, int (&id)[N]) {
+  static __device__ __forceinline__ void ids(const Int8DecodeArgs& a, const int32_t* table, int last,
+                                             int (&id)[N]) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       int at = min(unit(i), UNITS - 1) / D;
@@ -418,7 +421,8 @@ __device__ __forceinline__ float i8_first(I8Rows<D>& w, const half_t* kn, float1
   for (int i = 0; i < 16; ++i) zero[i] = 0.f;
 #pragma unroll
   for (int j = 0; j < 2 * R::NQ; ++j)
-    sc[j / R::NQ] = mfma_i8(w.operand(nullptr, kn, nullptr, R::NP + j), w.q[j % R::NQ], j % R::NQ == 0 ? zero : sc[j / R::NQ]);
+    sc[j / R::NQ] = mfma_i8(w.operand(nullptr, kn, nullptr, R::NP + j), w.q[j % R::NQ],
+                            j % R::NQ == 0 ? zero : sc[j / R::NQ]);
   const float4_t fkn = ld<float4_t>(fknp);
   mask(sc);
   float top[4];
@@ -654,8 +658,8 @@ __device__ __forceinline__ void i8_piece(const Int8PrefillArgs& p, I8PrefillLds<
       const int wb = i * kI8StepBlocks;
       const float best = decltype(first)::value
                              ? i8_first<D>(w, lds.k[0], sc, lds.fk, mask, work)
-                             : i8_step64<D>(w, lds.v[1 - P], lds.k[1 - P], lds.v[P], sc, pr, lds.fk + wb, lds.vs + wb,
-                                            lds.back + wb, lds.fk + wb + kI8StepBlocks, mask, work);
+                             : i8_step64<D>(w, lds.v[1 - P], lds.k[1 - P], lds.v[P], sc, pr,
+                                            lds.fk + wb, lds.vs + wb, lds.back + wb, lds.fk + wb + kI8StepBlocks, mask, work);
       i8_reference<D>(w, i + 1 < n ? best : w.m);          // (its own reference moves none, also a NaN)
 #pragma unroll
       for (int e = 0; e < S::N; ++e) id0[e] = id1[e], id1[e] = id2[e];
@@ -668,7 +672,8 @@ __device__ __forceinline__ void i8_piece(const Int8PrefillArgs& p, I8PrefillLds<
     const half_t* vl = lds.v[(n - 1) & 1];                 // the last step's second half
 #pragma unroll
     for (int j = 0; j < R::NP; ++j)
-      w.o[j % DT] = mfma_i8(ld<half8_t>(vl + w.vat[2 + j / DT] + j % DT * 32 * kI8Keys), pr[2 + j / DT], w.o[j % DT]);
+      w.o[j % DT] = mfma_i8(ld<half8_t>(vl + w.vat[2 + j / DT] + j % DT * 32 * kI8Keys), pr[2 + j / DT],
+                            w.o[j % DT]);
   }
 
   // lanes c and c + 32 hold the two halves of row c's sum
