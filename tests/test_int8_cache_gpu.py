@@ -492,6 +492,40 @@ def test_blocks_without_a_finite_scale(heads, side, bad, bound):
     assert (np.abs(out.double().cpu().numpy() - ref) <= bound)[ok].all()
 
 
+@pytest.mark.parametrize("heads", HEADS)
+@pytest.mark.parametrize("bound", [90, 30000])      # tiles of 16 rows, the prompt kernel
+def test_hidden_blocks_have_no_say(heads, bound):
+    """Rows that see only blocks with small V scales, ahead of blocks whose V scales are 2^20 and 2^25
+    times theirs: as exact as if those blocks were not there, and the same bits whatever stands in
+    them."""
+    c = Case(heads, [(0, 90), (0, 90)], seed=38)
+    c.scales[1, c.tables] = 2.0 ** 8
+    c.scales[1, c.tables[0, 0]] = 2.0 ** -12
+    c.scales[1, c.tables[1, 0]] = 2.0 ** -17
+    _, q, _, _, cache, meta = c.on(DEV)
+    meta = dataclasses.replace(meta, max_prefill_seq_len=bound)
+    out = H.paged_attention_int8(q, *cache, meta, c.scale)
+    for b, lo in enumerate(c.starts[:2].tolist()):
+        alone = np.arange(lo, lo + 16)
+        ref, lim = O.paged_attention(c.split()[0][alone], c.codes, c.scales, c.tables[b:b + 1], [16], [0, 16],
+                                     c.scale)
+        err = np.abs(out[lo:lo + 16].double().cpu().numpy() - ref)
+        assert (err <= lim).all(), f"sequence {b}: {(err / lim).max():.3g} of the bound"
+    assert_rows(out, c)
+    # tokens 23 and later of both
+    other = [t.clone() for t in cache]
+    for b in range(2):
+        for t in other[:2]:
+            t[c.tables[b, 1], :, 7:] = t[c.tables[b, 1], :, 7:].flip(0, 1, 2)
+            t[c.tables[b, 2:]] = t[c.tables[b, 2:]].flip(0, 1, 2, 3)
+        for t in other[2:]:
+            t[c.tables[b, 2:]] = torch.exp2(torch.randint(-30, 9, t[c.tables[b, 2:]].shape, device=DEV).float())
+    again = H.paged_attention_int8(q, *other, meta, c.scale)
+    for lo in c.starts[:2].tolist():
+        assert torch.equal(out[lo:lo + 23], again[lo:lo + 23])
+        assert not torch.equal(out[lo + 23:lo + 90], again[lo + 23:lo + 90])
+
+
 def test_attention_refuses():
     c = Case((4, 2, 64), [(7, 1), (9, 20)], num_decode=1, seed=23)
     _, q, _, _, cache, meta = c.on(DEV)

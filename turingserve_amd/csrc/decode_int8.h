@@ -3,6 +3,15 @@
 //
 //   s_j = scale * ks[blk(j)] * (q . code_k[j]),  out = sum_j softmax(s)_j * vs[blk(j)] * code_v[j]
 //
+// A block's V scale goes into the exponent: with t_j = s_j + log2 vs[blk(j)] (s in base 2),
+//   P'_j = 2^(t_j - m) is rounded to fp16 and multiplied by the codes of V, l = sum_j P'_j / vs[blk(j)],
+//   out = sum_j P'_j code_v[j] / l,
+// m being the row's own running maximum of t over the tokens that it sees. So the largest P' of a row is
+// at least 1 whatever its other blocks hold, and tokens that it does not see have no say in its rounding
+// (P against the largest V scale of a split's blocks rounded a row's weights away where hidden blocks
+// had a V scale 2^20 above those that it saw). A V scale below 2^-40 counts as 2^-40, which moves a
+// result by 127 * 2^-40 at most: 2^-8 of fp16's smallest half step.
+//
 // The rows of a sequence for one KV head, row = token * group + head, stand in tiles of 16 (the rows
 // of an MFMA tile); row i's token sees the first seq_len - n + token + 1 tokens. One workgroup of
 // four wavefronts takes one split of the sequence's blocks for one tile: every code is read once for
@@ -127,12 +136,18 @@ __device__ __forceinline__ int i8_kv_len(int len, int max_blocks) {
   return len < 0 ? 0 : (len > most ? (int)most : len);
 }
 
+// A block's V scale in the exponent, and what a weight with it is multiplied by in the row's sum: its
+// exact inverse but for rounding, so that the sum does not feel the logarithm's.
+constexpr float kI8LeastScale = 0x1p-40f;
+__device__ __forceinline__ void i8_value_factors(float vs, float& lv, float& back) {
+  lv = __builtin_amdgcn_logf(fmaxf(vs, kI8LeastScale));
+  back = fast_exp2(-lv);
+}
+
 // A block with a scale that is not finite makes the scores of its visible tokens NaN, and its V
-// scale 0: tokens which a row does not see stay out of it (0 * NaN would not). A V scale below 1e-30,
-// whose reciprocal need not be finite, counts as 0: fp16 has no values that small.
+// scale 0: tokens which a row does not see stay out of it (0 * NaN would not).
 __device__ __forceinline__ void i8_poison(float& ks, float& vs) {
   if (!(fabsf(ks) < INFINITY && fabsf(vs) < INFINITY)) ks = __builtin_nanf(""), vs = 0.f;
-  if (vs < 1e-30f) vs = 0.f;
 }
 
 template <int D>
@@ -241,23 +256,31 @@ __device__ __forceinline__ void i8_pv(float4_t (&o)[D / 16], const uint32_t (&v)
   }
 }
 
-// The state of one wavefront's 16 rows: O^T in units of kColumnUnit times the V scale `vref`.
+// The state of one wavefront's 16 rows: reference, sum, and O^T in units of kColumnUnit.
 template <int D>
 struct I8State {
   float m, l;
   float4_t o[D / 16];
 };
 
-// One pair of blocks (tokens ta .. and tb .. of the sequence): fk / fv the blocks' K factor (scale *
-// log2 e * ks) and V factor (vs / vref). A row sees the tokens below `vis`, all rows of the tile those
-// below `least`.
+// What a block multiplies its scores by (scale * log2 e * ks), adds to them, and multiplies its weights
+// by in a row's sum (i8_value_factors).
+struct I8Factors {
+  float fk, lv, back;
+};
+
+// One pair of blocks (tokens ta .. and tb .. of the sequence). A row sees the tokens below `vis`, all
+// rows of the tile those below `least`.
 template <int D>
-__device__ __forceinline__ void i8_step(I8State<D>& st, const I8Pair<D>& x, const I8Query<D>& q, float fka,
-                                        float fkb, float fva, float fvb, int ta, int tb, int vis, int least,
-                                        int g) {
+__device__ __forceinline__ void i8_step(I8State<D>& st, const I8Pair<D>& x, const I8Query<D>& q,
+                                        const I8Factors& fa, const I8Factors& fb, int ta, int tb, int vis,
+                                        int least, int g) {
   float4_t sa = i8_scores<D>(x.k[0], q), sb = i8_scores<D>(x.k[1], q);
-  sa *= fka;
-  sb *= fkb;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    sa[r] = fmaf(sa[r], fa.fk, fa.lv);
+    sb[r] = fmaf(sb[r], fb.fk, fb.lv);
+  }
   if (tb + kBlockSize > least || ta + kBlockSize > least) {
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -281,22 +304,20 @@ __device__ __forceinline__ void i8_step(I8State<D>& st, const I8Pair<D>& x, cons
   float pa[4], pb[4];
 #pragma unroll
   for (int r = 0; r < 4; ++r) pa[r] = fast_exp2(sa[r] + neg), pb[r] = fast_exp2(sb[r] + neg);
-  st.l += ((pa[0] + pa[1]) + (pa[2] + pa[3])) + ((pb[0] + pb[1]) + (pb[2] + pb[3]));
+  st.l = fmaf((pa[0] + pa[1]) + (pa[2] + pa[3]), fa.back, st.l);
+  st.l = fmaf((pb[0] + pb[1]) + (pb[2] + pb[3]), fb.back, st.l);
   half8_t p;
 #pragma unroll
-  for (int r = 0; r < 4; ++r) p[r] = (half_t)(pa[r] * fva), p[4 + r] = (half_t)(pb[r] * fvb);
+  for (int r = 0; r < 4; ++r) p[r] = (half_t)pa[r], p[4 + r] = (half_t)pb[r];
   // Codes left past the end are finite, and p is 0 there.
   i8_pv<D>(st.o, x.v, p);
 }
 
 // One split [b0, b1) of a sequence's blocks by one wavefront (of kI8Waves). Blocks are taken 64
-// at a time: lane i holds block i's id and scales, and the V scale that P is measured against is
-// the largest so far (rounding P * vs / vref to fp16 then loses only what is far below the
-// block with the largest V).
+// at a time: lane i holds block i's id and factors.
 template <int D>
-__device__ __forceinline__ void i8_split(const Int8DecodeArgs& a, I8State<D>& st, float& vref,
-                                         const I8Query<D>& q, int b, int h, int b0, int b1, int len,
-                                         int vis, int least, int wave) {
+__device__ __forceinline__ void i8_split(const Int8DecodeArgs& a, I8State<D>& st, const I8Query<D>& q, int b,
+                                         int h, int b0, int b1, int len, int vis, int least, int wave) {
   const int lane = threadIdx.x % kWave, c = lane % 16, g = lane / 16;
   const int32_t* table = a.block_tables + b * a.bt_stride;
   const int64_t block_bytes = (int64_t)kBlockSize * D;
@@ -324,6 +345,7 @@ __device__ __forceinline__ void i8_split(const Int8DecodeArgs& a, I8State<D>& st
       i8_load_v<D>(a.vc + ua, c, g, x.v[0]);
       i8_load_v<D>(a.vc + ub, c, g, x.v[1]);
     };
+    float lv, back;
     auto step = [&](I8Pair<D>& x, int i) {
       const int j = min(i + 1, n - 1);
 #pragma unroll
@@ -335,24 +357,16 @@ __device__ __forceinline__ void i8_split(const Int8DecodeArgs& a, I8State<D>& st
       // with an odd count the last pair's second block is its first, wholly past the end
       const int ta = (lo + i) * kBlockSize;
       const int tb = i + 1 < n ? ta + kBlockSize : len;
-      i8_step<D>(st, x, q, lane_f(ks, i), lane_f(ks, j), lane_f(vs, i), lane_f(vs, j), ta, tb,
-                 vis, least, g);
+      i8_step<D>(st, x, q, {lane_f(ks, i), lane_f(lv, i), lane_f(back, i)},
+                 {lane_f(ks, j), lane_f(lv, j), lane_f(back, j)}, ta, tb, vis, least, g);
     };
     constexpr int STEP = 2 * kI8Waves;
     I8Pair<D> x, y;
     int i = 2 * wave;
     if (i < n) load(x, i);
     if (i + STEP < n) load(y, i + STEP);
-    const float top = i8_most(fmaxf(vs, 0.f));
-    if (top > vref) {
-      const float f = vref / top;
-      vref = top;
-#pragma unroll
-      for (int t = 0; t < D / 16; ++t) st.o[t] *= f;
-    }
-    const float inv = vref > 0.f ? 1.f / vref : 0.f;
+    i8_value_factors(vs, lv, back);
     ks *= a.sl2;
-    vs *= inv;
 
     if (i >= n) continue;
     while (true) {
@@ -377,7 +391,7 @@ struct I8DecodeLds {
 
 // The four wavefronts' states meet in LDS; the row (or its partial) is written.
 template <int D>
-__device__ __forceinline__ void i8_finish(const Int8DecodeArgs& a, I8State<D>& st, float vref, int b, int h,
+__device__ __forceinline__ void i8_finish(const Int8DecodeArgs& a, I8State<D>& st, int b, int h,
                                           int q0, int row0, int rows, int split, int splits, int wave,
                                           float* s_o, float* s_ml) {
   constexpr int VW = D / 16;
@@ -409,13 +423,14 @@ __device__ __forceinline__ void i8_finish(const Int8DecodeArgs& a, I8State<D>& s
       sum += f * s_ml[2 * (w * 16 + row) + 1];
       o += ld<float4_t>(s_o + (w * 16 + row) * I8DecodeLds<D>::ROW + d) * f;
     }
+    o *= kColumnUnit;
     if (splits == 1) {
-      const float f = sum == 0.f ? 0.f : kColumnUnit * vref / sum;   // no visible key: zeros
+      const float f = sum == 0.f ? 0.f : 1.f / sum;        // no visible key: zeros
       const int token = a.by_group(row0 + row), head = h * a.group + row0 + row - token * a.group;
       ts::st<half4_t>(a.out + (int64_t)(q0 + token) * a.out_st + (int64_t)head * D + d, to_half4(o * f));
     } else {
       const int64_t at = i8_partial(a, b, h, row0 + row, splits) + split;
-      ts::st<float4_t>(a.part_o + at * D + d, o * (kColumnUnit * vref));
+      ts::st<float4_t>(a.part_o + at * D + d, o);
       if (d == 0) {
         a.part_ml[2 * at] = top;
         a.part_ml[2 * at + 1] = sum;
@@ -484,12 +499,11 @@ __global__ void __launch_bounds__(kI8Threads, i8_decode_groups(D)) decode_int8_k
     st.m = -INFINITY, st.l = 0.f;
 #pragma unroll
     for (int t = 0; t < D / 16; ++t) st.o[t] = {0.f, 0.f, 0.f, 0.f};
-    float vref = 0.f;
     const int nb = (kv + kBlockSize - 1) / kBlockSize;
     const int b0 = (int)((unsigned)(nb * x.split) / (unsigned)x.splits);
     const int b1 = (int)((unsigned)(nb * (x.split + 1)) / (unsigned)x.splits);
-    i8_split<D>(a, st, vref, q, x.b, h, b0, b1, kv, vis, least, wave);
-    i8_finish<D>(a, st, vref, x.b, h, x.seq.q0, row0, rows, x.split, x.splits, wave, lds.o, lds.ml);
+    i8_split<D>(a, st, q, x.b, h, b0, b1, kv, vis, least, wave);
+    i8_finish<D>(a, st, x.b, h, x.seq.q0, row0, rows, x.split, x.splits, wave, lds.o, lds.ml);
   }
 }
 

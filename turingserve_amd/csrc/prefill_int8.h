@@ -8,10 +8,10 @@
 // LDS (exact; the scales stay out of the tiles), and each wavefront computes, on
 // v_mfma_f32_32x32x16_f16,
 //   S^T[64 tokens][32 rows] = K . Q^T,   online softmax in fp32,   O^T += V^T . P^T.
-// A block's K scale multiplies its scores in fp32. Its V scale, measured against the largest one
-// so far (vref), goes into the exponent: P' = 2^(s - m + log2(vs / vref)) is what is rounded to
-// fp16 and multiplied by the codes of V, and a row's sum adds each block's P' times vref / vs. A
-// ratio below 2^-30 counts as 2^-30: at most 127 * 2^-30 of vref.
+// A block's K scale multiplies its scores in fp32. Its V scale goes into the exponent, and the row's
+// reference is the largest of both together among the tokens that it sees (decode_int8.h):
+// P' = 2^(s + log2 vs - m) is what is rounded to fp16 and multiplied by the codes of V, and a row's sum
+// adds each block's P' divided by vs.
 //
 // Lane l is split into c = l % 32 and h = l / 32: a result lane holds S^T[8 (i / 4) + 4 h + i % 4][c],
 // i = 0..15, so a lane's scores all belong to row c, and its P values for a block's 16 tokens (i % 8
@@ -44,7 +44,6 @@ constexpr int kI8Window = 256;           // blocks whose ids and scales are held
 // Steps (and tiles' costs) that a workgroup is worth: 31.0, 30.6 and 31.1 us with 4, 6 and 8 at five
 // chunks of 90 to 1100 rows, 14/2 heads of 64.
 constexpr int kI8MinShare = 6;
-constexpr float kI8LeastRatio = -30.f;   // log2 of the least V scale ratio
 constexpr float kI8LeastFactor = 1e-30f;
 
 template <int N>
@@ -94,8 +93,8 @@ struct I8PrefillLds {
   __align__(16) half_t k[2][I8Tile<D>::HALVES], v[2][I8Tile<D>::HALVES];
   int walk[5][kWave];                                      // I8Walk
   int blk[kI8Window];                                      // the sign bit: a scale is not finite
-  __align__(16) float fk[kI8Window + 4], vs[kI8Window];        // scale * log2 e * ks; log2(vs / vref)
-  __align__(16) float back[kI8Window];                     // vref / vs
+  __align__(16) float fk[kI8Window + 4], lv[kI8Window + 4];    // scale * log2 e * ks; log2 vs
+  __align__(16) float back[kI8Window];                     // 1 / vs
 };
 
 // Rows of one sequence's chunk. (The entry point refuses batches whose rows times heads or steps
@@ -396,6 +395,12 @@ struct I8Exp {
   }
 };
 
+// A row's largest s + log2 vs from its largest score in each of four blocks.
+__device__ __forceinline__ float i8_best(const float (&top)[4], const float4_t& fk, const float4_t& lv) {
+  return vmax(vmax(fmaf(top[0], fk[0], lv[0]), fmaf(top[1], fk[1], lv[1])),
+              vmax(fmaf(top[2], fk[2], lv[2]), fmaf(top[3], fk[3], lv[3])));
+}
+
 // One step of a wavefront. Its scores stand in sc (tokens 0-31, 32-63), P' of the last step's
 // second half in pr[2], pr[3]; the next step's scores replace them. Four phases, each a run of MFMAs
 // beside a share of the vector work:
@@ -411,7 +416,7 @@ struct I8Exp {
 // Before the first step: its scores, and the staging that a step does.
 template <int D, typename Mask, typename Work>
 __device__ __forceinline__ float i8_first(I8Rows<D>& w, const half_t* kn, float16_t (&sc)[2], const float* fknp,
-                                          Mask mask, Work work) {
+                                          const float* lvnp, Mask mask, Work work) {
   typedef I8Rows<D> R;
   work(0);
 #pragma unroll
@@ -423,7 +428,7 @@ __device__ __forceinline__ float i8_first(I8Rows<D>& w, const half_t* kn, float1
   for (int j = 0; j < 2 * R::NQ; ++j)
     sc[j / R::NQ] = mfma_i8(w.operand(nullptr, kn, nullptr, R::NP + j), w.q[j % R::NQ],
                             j % R::NQ == 0 ? zero : sc[j / R::NQ]);
-  const float4_t fkn = ld<float4_t>(fknp);
+  const float4_t fkn = ld<float4_t>(fknp), lvn = ld<float4_t>(lvnp);
   mask(sc);
   float top[4];
 #pragma unroll
@@ -435,18 +440,18 @@ __device__ __forceinline__ float i8_first(I8Rows<D>& w, const half_t* kn, float1
     }
   work(1);
   work(2);
-  return vmax(vmax(top[0] * fkn[0], top[1] * fkn[1]), vmax(top[2] * fkn[2], top[3] * fkn[3]));
+  return i8_best(top, fkn, lvn);
 }
 
 template <int D, typename Mask, typename Work>
 __device__ __forceinline__ float i8_step64(I8Rows<D>& w, const half_t* vp, const half_t* kn, const half_t* vc,
                                            float16_t (&sc)[2], half8_t (&pr)[4], const float* fkp,
-                                           const float* fvp, const float* backp, const float* fknp, Mask mask,
-                                           Work work) {
+                                           const float* lvp, const float* backp, const float* fknp,
+                                           const float* lvnp, Mask mask, Work work) {
   typedef I8Rows<D> R;
   constexpr int NQ = R::NQ, NP = R::NP, AHEAD = R::AHEAD;
   half8_t op[AHEAD];
-  const float4_t fk = ld<float4_t>(fkp), fv = ld<float4_t>(fvp);
+  const float4_t fk = ld<float4_t>(fkp), lv = ld<float4_t>(lvp);
 #pragma unroll
   for (int j = 0; j < AHEAD && j < NP; ++j) op[j] = w.operand(vp, kn, vc, j);
   const float4_t back = ld<float4_t>(backp);
@@ -457,7 +462,7 @@ __device__ __forceinline__ float i8_step64(I8Rows<D>& w, const half_t* vp, const
     return x;
   };
   const float neg = w.m == -INFINITY ? 0.f : -w.m;
-  const float off[4] = {neg + fv[0], neg + fv[1], neg + fv[2], neg + fv[3]};
+  const float off[4] = {neg + lv[0], neg + lv[1], neg + lv[2], neg + lv[3]};
   // exponentials: NP + NQ shares beside the first two phases' MFMAs where both have as many
   constexpr int N = 2 * (NP < NQ ? NP : NQ);
   I8Exp ex;
@@ -493,7 +498,7 @@ __device__ __forceinline__ float i8_step64(I8Rows<D>& w, const half_t* vp, const
     if (j == NQ / 4) work(1);                              // K of a later step to LDS
     __builtin_amdgcn_sched_barrier(0);
   }
-  const float4_t fkn = ld<float4_t>(fknp);
+  const float4_t fkn = ld<float4_t>(fknp), lvn = ld<float4_t>(lvnp);
   mask(sc);
   float top[4];
 #pragma unroll
@@ -508,10 +513,10 @@ __device__ __forceinline__ float i8_step64(I8Rows<D>& w, const half_t* vp, const
     if (j == NP / 2) work(2);                              // V
     __builtin_amdgcn_sched_barrier(0);
   }
-  return vmax(vmax(top[0] * fkn[0], top[1] * fkn[1]), vmax(top[2] * fkn[2], top[3] * fkn[3]));
+  return i8_best(top, fkn, lvn);
 }
 
-// A row's largest score moves its reference; O follows in the next step, behind what was computed
+// A row's largest s + log2 vs moves its reference; O follows in the next step, behind what was computed
 // against the old one.
 template <int D>
 __device__ __forceinline__ void i8_reference(I8Rows<D>& w, float best) {
@@ -553,7 +558,6 @@ __device__ __forceinline__ void i8_piece(const Int8PrefillArgs& p, I8PrefillLds<
 #pragma unroll
     for (int i = 0; i < 16; ++i) w.o[t][i] = 0.f;
   w.m = -INFINITY, w.l = 0.f, w.alpha = 1.f, w.moved = false;
-  float vref = 0.f;
 
   s1 = min(s1, (nb + kI8StepBlocks - 1) / kI8StepBlocks);  // (nothing visible: no step)
   for (int w0 = s0; w0 < s1; w0 += kI8Window / kI8StepBlocks) {
@@ -596,29 +600,13 @@ __device__ __forceinline__ void i8_piece(const Int8PrefillArgs& p, I8PrefillLds<
       if (at < kI8Window) {
         lds.blk[at] = f == f ? blk[i] : blk[i] | (int)0x80000000;
         lds.fk[at] = f > kI8LeastFactor ? f : kI8LeastFactor;
-        lds.vs[at] = vs;
+        i8_value_factors(vs, lds.lv[at], lds.back[at]);
       }
     }
     __syncthreads();
     S::ids(lds, 0, last, id0);
     S::ids(lds, kI8StepBlocks, last, id1);
     stage.finite(id0);
-    float top = 0.f;
-#pragma unroll
-    for (int i = 0; i < kI8Window; i += kWave) top = fmaxf(top, lds.vs[i + lane]);
-    top = i8_most(top);
-    if (top > vref) {
-      const float f = vref / top;
-      vref = top;
-#pragma unroll
-      for (int t = 0; t < DT; ++t) w.o[t] *= f;
-    }
-    __syncthreads();                                       // every wavefront has the maximum
-    for (int i = threadIdx.x; i < kI8Window; i += THREADS) {
-      const float f = vref > 0.f ? fmaxf(__builtin_amdgcn_logf(lds.vs[i] / vref), kI8LeastRatio) : 0.f;
-      lds.vs[i] = f;
-      lds.back[i] = fast_exp2(-f);
-    }
     stage.place_k(lds.k[0]);
     for (int i = threadIdx.x; i < I8Tile<D>::HALVES / 8; i += THREADS)
       st<half8_t>(lds.v[1] + 8 * i, half8_t{0, 0, 0, 0, 0, 0, 0, 0});
@@ -657,9 +645,10 @@ __device__ __forceinline__ void i8_piece(const Int8PrefillArgs& p, I8PrefillLds<
       };
       const int wb = i * kI8StepBlocks;
       const float best = decltype(first)::value
-                             ? i8_first<D>(w, lds.k[0], sc, lds.fk, mask, work)
+                             ? i8_first<D>(w, lds.k[0], sc, lds.fk, lds.lv, mask, work)
                              : i8_step64<D>(w, lds.v[1 - P], lds.k[1 - P], lds.v[P], sc, pr,
-                                            lds.fk + wb, lds.vs + wb, lds.back + wb, lds.fk + wb + kI8StepBlocks, mask, work);
+                                            lds.fk + wb, lds.lv + wb, lds.back + wb,
+                                            lds.fk + wb + kI8StepBlocks, lds.lv + wb + kI8StepBlocks, mask, work);
       i8_reference<D>(w, i + 1 < n ? best : w.m);          // (its own reference moves none, also a NaN)
 #pragma unroll
       for (int e = 0; e < S::N; ++e) id0[e] = id1[e], id1[e] = id2[e];
@@ -682,8 +671,7 @@ __device__ __forceinline__ void i8_piece(const Int8PrefillArgs& p, I8PrefillLds<
   if (wrow + c >= rows) return;
   const int64_t at = (int64_t)slot * ROWS + 32 * wave + c;
   if (!whole && hh == 0) st<float2_t>(a.part_ml + 2 * at, float2_t{w.m, l});
-  vref *= kColumnUnit;
-  const float f = !whole ? vref : l == 0.f ? 0.f : vref / l;   // nothing visible: zeros
+  const float f = !whole ? 1.f : l == 0.f ? 0.f : 1.f / l;     // nothing visible: zeros
   half_t* dst = a.out + (int64_t)(k.q0 + token) * a.out_st + (int64_t)head * D;
 #pragma unroll
   for (int t = 0; t < DT; ++t)
@@ -691,7 +679,7 @@ __device__ __forceinline__ void i8_piece(const Int8PrefillArgs& p, I8PrefillLds<
     for (int i = 0; i < 16; i += 4) {
       const int d = 32 * t + 8 * (i / 4) + 4 * hh;
       if (D < 32 && d >= D) break;
-      const float4_t x = float4_t{w.o[t][i], w.o[t][i + 1], w.o[t][i + 2], w.o[t][i + 3]} * f;
+      const float4_t x = float4_t{w.o[t][i], w.o[t][i + 1], w.o[t][i + 2], w.o[t][i + 3]} * kColumnUnit * f;
       if (whole)
         st<half4_t>(dst + d, to_half4(x));
       else
