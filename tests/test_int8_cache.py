@@ -52,6 +52,38 @@ def test_write_in_pieces_holds_every_row_within_its_steps():
     assert err.max() <= 0.5 * scales[0] * grew * (1 + 1e-5)
 
 
+def _of_different_size():
+    c = Case((12, 2, 128), [(99, 1), (1999, 1), (15, 1), (0, 90)], num_decode=3, seed=16)
+    c.scales[1] = np.exp2(np.random.default_rng(0).integers(-40, 10, c.scales[1].shape)).astype(np.float32)
+    c.scales[1, c.tables[2, 0]] = 2.0 ** -20
+    c.scales[1, c.tables[1, ::3]] = 0
+    return c
+
+
+def _small_ahead_of_large():
+    c = Case((14, 2, 64), [(0, 90), (0, 90)], seed=38)
+    c.scales[1, c.tables] = 2.0 ** 8
+    c.scales[1, c.tables[0, 0]] = 2.0 ** -12
+    c.scales[1, c.tables[1, 0]] = 2.0 ** -17
+    return c
+
+
+@pytest.mark.parametrize("make", [
+    _of_different_size, _small_ahead_of_large,
+    lambda: Case((4, 2, 16), [(0, 1), (0, 40), (16, 530)], num_decode=1, seed=17),
+    lambda: Case((12, 2, 128), [(0, 1), (32, 1), (4095, 1)], num_decode=3, seed=11),
+    lambda: Case((14, 2, 64), [(69999, 1)], num_decode=1, seed=12),
+    lambda: Case((12, 2, 128), [(0, 1), (39, 1), (1999, 1)], num_decode=3, seed=15, k_size=1e5),
+    lambda: Case((12, 2, 128), [(0, 1), (39, 1), (1999, 1)], num_decode=3, seed=15, k_size=0.0)])
+def test_attention_bound_catches_a_lost_result(make):
+    """The oracle's bound is a small part of every (row, head)'s values: less than 1/32 of their rms (or
+    of fp16's smallest normal number), so that a result of zeros, or of other tokens, does not pass."""
+    c = make()
+    ref, bound = O.paged_attention(c.split()[0], c.codes, c.scales, c.tables, c.lens, c.starts, c.scale)
+    rms = lambda x: np.sqrt((x.reshape(c.T, c.H, c.D) ** 2).mean(-1))
+    assert (rms(bound) < np.maximum(rms(ref), 2.0 ** -14) / 32).all()
+
+
 @pytest.mark.parametrize("heads", HEADS)
 def test_twins_match_the_oracle(heads):
     c = Case(heads, [(4, 1), (15, 1), (0, 1), (0, 21), (7, 30)], num_decode=3, seed=2)
