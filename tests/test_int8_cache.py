@@ -5,6 +5,7 @@ from __future__ import annotations
 
 import ctypes
 import dataclasses
+import subprocess
 
 import numpy as np
 import pytest
@@ -16,6 +17,7 @@ from turingserve_amd import _native as N
 from turingserve_amd import get_ops
 from turingserve_amd import hip_ops as H
 from turingserve_amd import reference_ops as R
+from turingserve_amd.csrc import build as B
 from turingserve_amd.quant import Int8KVCache
 from turingserve_amd.qwen2 import rope_tables
 
@@ -187,6 +189,35 @@ odd = ctypes.c_void_p(258)
 ])
 def test_refusals(call, kw, status, text):
     assert call(**kw) == status and text in N.last_error()
+
+
+def test_split_edges_up_to_the_longest_table(tmp_path):
+    """The kernel's own rule, compiled for the host: the splits of up to 2^26 blocks (the longest table
+    that the entry point takes) follow one another, cover every block and differ by one at most."""
+    src = tmp_path / "edges.hip"
+    src.write_text("""#include <cstdio>
+#include "decode_int8.h"
+int main() {
+  const int sizes[] = {1, 15, 63, 64, 65, 1023, 1025, 4375, (1 << 25) - 1, 1 << 25, (1 << 25) + 1,
+                       (1 << 26) - 63, (1 << 26) - 1, 1 << 26};
+  for (int nb : sizes)
+    for (int splits = 1; splits <= ts::kI8MaxSplits; ++splits) {
+      std::printf("%d %d", nb, splits);
+      for (int i = 0; i <= splits; ++i) std::printf(" %d", ts::i8_split_begin(nb, i, splits));
+      std::printf("\\n");
+    }
+}
+""")
+    exe = tmp_path / "edges"
+    subprocess.run([B.hipcc(), *B.COMMON_FLAGS, "--offload-host-only", f"-I{B.HERE}", str(src), "-o", str(exe)],
+                   check=True, capture_output=True)
+    lines = subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.splitlines()
+    assert len(lines) == 14 * 64
+    for line in lines:
+        nb, splits, *edges = map(int, line.split())
+        sizes = np.diff(edges)
+        assert edges[0] == 0 and edges[-1] == nb and len(sizes) == splits
+        assert sizes.min() >= 0 and sizes.max() - sizes.min() <= 1
 
 
 def test_empty_calls_and_workspace_sizes():

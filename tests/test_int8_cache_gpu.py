@@ -241,6 +241,26 @@ def test_decode_of_a_long_sequence(heads):
     assert_rows(H.paged_attention_int8(q, *cache, short, c.scale), c, f"long, unsplit {heads}")
 
 
+@pytest.mark.parametrize("rows,bound", [(1, 1), (2, 2), (2, 200)])   # a decode row, a short chunk, the prompt kernel
+def test_the_longest_table(rows, bound):
+    """2^26 blocks, the longest table that is taken (its entries repeat): K of zeros, V of 64 in all blocks
+    but the last 64th, -64 there. Every sum of these is exact, and their mean is 62 (for the row before the
+    last one, too, once it is rounded)."""
+    nb = 1 << 26
+    codes = torch.zeros(2, 3, 1, 16, 16, dtype=torch.int8, device=DEV)
+    codes[1, 1], codes[1, 2] = 64, -64
+    scales = torch.ones(2, 3, 1, device=DEV)
+    table = torch.ones(1, nb, dtype=torch.int32, device=DEV)
+    table[0, nb - nb // 64:] = 2
+    c = Case((1, 1, 16), [(0, rows)])
+    _, q, _, _, _, _ = c.on(DEV)
+    meta = c.meta(DEV, seq_lens=torch.tensor([16 * nb], dtype=torch.int32, device=DEV), block_tables=table,
+                  num_decode=int(rows == 1), max_query_len=bound, max_seq_len=16 * nb,
+                  max_prefill_seq_len=16 * nb)
+    out = H.paged_attention_int8(q, codes[0], codes[1], scales[0], scales[1], meta, c.scale)
+    assert out.eq(62).all(), out
+
+
 def test_decode_rows_do_not_depend_on_the_batch():
     c = Case((12, 2, 128), [(n - 1, 1) for n in DECODE_LENS * 5], num_decode=5 * len(DECODE_LENS), seed=13)
     _, q, _, _, cache, meta = c.on(DEV)

@@ -50,6 +50,13 @@ __host__ __device__ inline int i8_splits(int nb, int most, int each = kI8SplitBl
   return n < 1 ? 1 : (n > most ? most : n);
 }
 
+// The first block of split `split` of nb blocks (of split `splits`: nb): the first nb % splits of them
+// are one block longer. No product leaves 32 bits: split * (nb / splits) <= nb.
+__host__ __device__ inline int i8_split_begin(int nb, int split, int splits) {
+  const int each = (int)((unsigned)nb / (unsigned)splits), more = nb - each * splits;
+  return split * each + (split < more ? split : more);
+}
+
 // Division of 0 <= x < 2^31 by a number that the host knows: x * mul >> 32 >> shift, with mul =
 // ceil(2^(31 + l) / d) and shift = l - 1 for 2^(l - 1) < d <= 2^l, which is exact there.
 struct I8Div {
@@ -500,8 +507,7 @@ __global__ void __launch_bounds__(kI8Threads, i8_decode_groups(D)) decode_int8_k
 #pragma unroll
     for (int t = 0; t < D / 16; ++t) st.o[t] = {0.f, 0.f, 0.f, 0.f};
     const int nb = (kv + kBlockSize - 1) / kBlockSize;
-    const int b0 = (int)((unsigned)(nb * x.split) / (unsigned)x.splits);
-    const int b1 = (int)((unsigned)(nb * (x.split + 1)) / (unsigned)x.splits);
+    const int b0 = i8_split_begin(nb, x.split, x.splits), b1 = i8_split_begin(nb, x.split + 1, x.splits);
     i8_split<D>(a, st, q, x.b, h, b0, b1, kv, vis, least, wave);
     i8_finish<D>(a, st, x.b, h, x.seq.q0, row0, rows, x.split, x.splits, wave, lds.o, lds.ml);
   }
