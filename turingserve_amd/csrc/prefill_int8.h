@@ -401,19 +401,9 @@ __device__ __forceinline__ float i8_best(const float (&top)[4], const float4_t& 
               vmax(fmaf(top[2], fk[2], lv[2]), fmaf(top[3], fk[3], lv[3])));
 }
 
-// One step of a wavefront. Its scores stand in sc (tokens 0-31, 32-63), P' of the last step's
-// second half in pr[2], pr[3]; the next step's scores replace them. Four phases, each a run of MFMAs
-// beside a share of the vector work:
-//   P'(sc[0])  beside  O += V P' of the last step's second half
-//   P'(sc[1])  beside  sc[0] = K . Q^T of the next step
-//   staging    beside  sc[1] = K . Q^T of the next step
-//   maxima of the next scores, more staging  beside  O += V P' of this step's first half
-// so that no second set of scores is needed (two wavefronts share a SIMD's registers). The order is
-// pinned, MFMA by MFMA: left to itself the compiler sets MFMAs and exponentials one after the other.
-// The workgroup meets behind the first phase, with no LDS read under way: what the step before staged
-// (K in its third phase, V in its fourth) is read behind that, and this step stages over what was
-// read before it. Returns each row's largest next score.
-// Before the first step: its scores, and the staging that a step does.
+// Before the first step of a window: its scores, and the staging that a step does, without a barrier of
+// its own: K of that step (and the V codes of 0 before it) stand behind the one that ends the window's
+// set-up, and what is staged here, over neither, is read behind the first step's.
 template <int D, typename Mask, typename Work>
 __device__ __forceinline__ float i8_first(I8Rows<D>& w, const half_t* kn, float16_t (&sc)[2], const float* fknp,
                                           const float* lvnp, Mask mask, Work work) {
@@ -443,6 +433,18 @@ __device__ __forceinline__ float i8_first(I8Rows<D>& w, const half_t* kn, float1
   return i8_best(top, fkn, lvn);
 }
 
+// One step of a wavefront. Its scores stand in sc (tokens 0-31, 32-63), P' of the last step's
+// second half in pr[2], pr[3]; the next step's scores replace them. Four phases, each a run of MFMAs
+// beside a share of the vector work:
+//   P'(sc[0])  beside  O += V P' of the last step's second half
+//   P'(sc[1])  beside  sc[0] = K . Q^T of the next step
+//   staging    beside  sc[1] = K . Q^T of the next step
+//   maxima of the next scores, more staging  beside  O += V P' of this step's first half
+// so that no second set of scores is needed (two wavefronts share a SIMD's registers). The order is
+// pinned, MFMA by MFMA: left to itself the compiler sets MFMAs and exponentials one after the other.
+// The workgroup meets behind the first phase, with no LDS read under way: what the step before staged
+// (K in its third phase, V in its fourth) is read behind that, and this step stages over what was
+// read before it. Returns each row's largest next score.
 template <int D, typename Mask, typename Work>
 __device__ __forceinline__ float i8_step64(I8Rows<D>& w, const half_t* vp, const half_t* kn, const half_t* vc,
                                            float16_t (&sc)[2], half8_t (&pr)[4], const float* fkp,
