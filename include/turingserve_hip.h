@@ -518,8 +518,13 @@ int ts_silu_mul(const void* gu, int64_t gu_stride, void* out, int64_t out_stride
  *   scale' = max(scale if the block holds earlier rows of the sequence, max|new rows| / 127)
  *   code'  = rint(code * (scale / scale')) of the earlier rows when scale' > scale
  *   code   = rint(row / scale') of the new rows                       (fp32, ties to even)
- * A block whose row 0 is written starts anew; rows past the sequence's end keep their codes. New
- * rows that are not finite make scale' NaN (and their codes 0). Blocks are owned by one workgroup
+ * A block whose row 0 is written starts anew; rows past the sequence's end keep their codes. A scale
+ * never shrinks while a block is filled: where a sequence is shortened inside a block (rejected draft
+ * rows), the block keeps the scale that the rows taken back brought, NaN if they were not finite, and
+ * the rows before them the codes that it left. To undo that, save the codes and scales of the block that
+ * the draft begins in, put them back and write the accepted rows again (blocks that begin within the
+ * draft start anew by themselves).
+ * New rows that are not finite make scale' NaN (and their codes 0). Blocks are owned by one workgroup
  * each, so no two sequences of a call may write into the same block (their rows would race; no
  * access leaves the cache). Block ids outside [0, num_blocks) and blocks past max_blocks_per_seq
  * are skipped. max_query_len shapes the launch only: a bound below the real one is slower, not

@@ -60,3 +60,43 @@ class Case:
                  num_decode=self.num_decode, max_query_len=int(n.max()), max_seq_len=int(self.lens.max()),
                  max_prefill_seq_len=int(self.lens[self.num_decode:].max(initial=0)))
         return AttentionMetadata(**{**f, **changes})
+
+
+def roll_back(ops, device):
+    """Five drafted rows in a block that holds ten, of which two are accepted, then a row behind those,
+    in both namespaces' write: the rejected rows' scale stays in the block, NaN if one of them was not
+    finite; a caller who puts the block's codes and scales back and writes the accepted rows again has
+    what was never drafted."""
+    c = Case((4, 2, 32), [(10, 5)], seed=39)
+    blk = int(c.tables[0, 0])
+    for big in (40.0, np.inf):
+        c.qkv[4, c.H * c.D] = big                        # K of head 0, the last rejected row
+        _, _, k, v, cache, _ = c.on(device)
+
+        def write(rows, length, cache=cache):
+            at = torch.tensor(rows, device=device)
+            ops.kv_write_int8(k[at], v[at], *cache, c.meta(
+                device, seq_lens=torch.tensor([length], dtype=torch.int32, device=device),
+                query_start_loc=torch.tensor([0, len(rows)], dtype=torch.int32, device=device)))
+
+        was = [t[blk].clone() for t in cache]
+        never = tuple(t.clone() for t in cache)
+        write([0, 1], 12, never)
+        write([2], 13, never)
+
+        write([0, 1, 2, 3, 4], 15)
+        drafted = [t[blk].clone() for t in cache]
+        write([2], 13)
+        k_scale = float(cache[2][blk, 0])
+        if np.isfinite(big):
+            assert k_scale == float(drafted[2][0]) == float(np.float32(big) / np.float32(127)) > float(never[2][blk, 0])
+        else:
+            assert np.isnan(k_scale) and np.isfinite(float(never[2][blk, 0]))
+        assert torch.equal(cache[0][blk, 1, :13], drafted[0][1, :13])        # (rows that were there)
+
+        for t, x in zip(cache, was):
+            t[blk] = x
+        write([0, 1], 12)
+        write([2], 13)
+        assert all(torch.equal(a[blk][:, :13] if a.dim() == 4 else a[blk], b[blk][:, :13] if b.dim() == 4 else b[blk])
+                   for a, b in zip(cache, never))

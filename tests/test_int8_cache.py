@@ -12,7 +12,7 @@ import pytest
 import torch
 
 from oracle import int8_cache as O
-from tests.int8_cases import HEADS, Case
+from tests.int8_cases import HEADS, Case, roll_back
 from turingserve_amd import _native as N
 from turingserve_amd import get_ops
 from turingserve_amd import hip_ops as H
@@ -127,6 +127,10 @@ def test_rope_twin_matches_the_oracle():
     assert np.array_equal(torch.stack(cache[:2]).numpy(), want_c)
     assert np.array_equal(torch.stack(cache[2:]).numpy(), want_s)
     assert np.array_equal(q.numpy(), O.rotate(qn, cn, sn).astype(np.float32).astype(np.float16))
+
+
+def test_rows_that_are_taken_back_keep_their_say():
+    roll_back(R, "cpu")
 
 
 def _write(**kw):

@@ -753,7 +753,8 @@ def kv_write_int8(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cac
     are requantised when it grows, and a block whose row 0 is written starts anew. The rows of
     sequence b (query_start_loc[b] .. [b + 1]) are its last ones (positions up to seq_lens[b] - 1)
     and lie where its block table says; slot_mapping is not read. Rows that are not finite make
-    their block's scale NaN. No two sequences of a step may write into one block."""
+    their block's scale NaN. Scales do not shrink while a block is filled, also where a sequence is
+    shortened inside it: the rows taken back keep their say until row 0 is written again. No two sequences of a step may write into one block."""
     T, KVH, D = k.shape
     if T == 0:
         return
