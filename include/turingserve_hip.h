@@ -565,7 +565,10 @@ int ts_rope_kv_write_int8(const void* qkv, int64_t qkv_stride, const int64_t* po
  * V scale is not finite is NaN. A decode row's result does not depend on the rest of the batch
  * given max_seq_len. The host bounds shape the launch only: bounds below the batch's real values
  * are slower, not wrong. head_dim 16, 32, 64, 128 or 256, any number of query heads per KV head; q
- * rows 16-byte aligned, scale > 0. At most 2^20 sequences, tables of at most 2^26 blocks; query_start_loc ascends.
+ * rows 16-byte aligned, scale > 0. At most 2^20 sequences, tables of at most 2^26 blocks;
+ * query_start_loc ascends. Rows, and splits and steps over all KV heads, are counted in 31 bits:
+ * TS_ERR_UNSUPPORTED where the bounds allow more (2^20 sequences of 64 splits at 32 KV heads; a chunk of
+ * 2^20 tokens, of 2^20 cached, at 8 KV heads of 8 query heads).
  * Workspace: the queried size, 256-byte aligned (may be 0). Rows of no sequence are not written.
  */
 size_t ts_paged_attention_int8_workspace_bytes(int32_t num_seqs, int32_t num_decode,

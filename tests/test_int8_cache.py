@@ -195,6 +195,16 @@ def test_refusals(call, kw, status, text):
     assert call(**kw) == status and text in N.last_error()
 
 
+@pytest.mark.parametrize("kw", [
+    dict(seqs=1 << 20, dec=1 << 20, T=1 << 20, h=32, kvh=32, D=16, qst=512, qsh=16, ost=512, ms=1 << 14),   # splits
+    dict(seqs=1, T=1 << 20, mq=1 << 20, ms=1 << 21, mp=1 << 21, mb=1 << 17, bts=1 << 17, h=64, kvh=8, qst=4096,
+         ost=4096),                                                                                        # steps
+])
+def test_more_work_than_is_counted_is_refused_before_the_device_is_asked(kw):
+    """(It used to end where the count did, with the rest of the rows never written.)"""
+    assert _attend(**kw, ws=P, wsb=1 << 62) == N.TS_ERR_UNSUPPORTED and "tables of" in N.last_error()
+
+
 def test_split_edges_up_to_the_longest_table(tmp_path):
     """The kernel's own rule, compiled for the host: the splits of up to 2^26 blocks (the longest table
     that the entry point takes) follow one another, cover every block and differ by one at most."""

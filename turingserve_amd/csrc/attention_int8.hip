@@ -72,6 +72,13 @@ static Int8Plan int8_plan(int num_seqs, int num_decode, int max_query_len, int m
   return pl;
 }
 
+// Workgroups' worth of work in the decode kernel at most, for one KV head: splits of tiles of 16 rows.
+static int64_t decode_items(const Int8Plan& pl, int num_decode, int64_t num_tokens, int G) {
+  const int64_t chunks = pl.small - num_decode;
+  return (int64_t)num_decode * pl.max_splits * ((G + 15) / 16) +
+         (chunks > 0 ? chunks * (pl.max_splits + 1) + num_tokens * G / 16 : 0);
+}
+
 // Rows that the decode kernel's merge goes over.
 static int64_t merge_rows(const Int8Plan& pl, int num_decode, int H, int KVH) {
   return (int64_t)num_decode * H + (int64_t)(pl.small - num_decode) * KVH * pl.row_slots;
@@ -154,11 +161,25 @@ extern "C" int ts_paged_attention_int8(const void* q, int64_t q_stride_t, int64_
   // The kernels count rows in 31 bits, and splits, of which a sequence has 64 for each tile of rows.
   TS_REQUIRE(num_seqs <= 1 << 20 && num_tokens < (1ll << 30) / (num_heads / num_kv_heads), TS_ERR_UNSUPPORTED,
              "paged_attention_int8: %lld tokens of %d sequences", (long long)num_tokens, num_seqs);
+  const int group = num_heads / num_kv_heads;
+  Int8Plan pl = int8_plan(num_seqs, num_decode, max_query_len, max_seq_len, max_prefill_seq_len, num_heads,
+                          num_kv_heads, head_dim, 256);
+  // ... and steps: those of at most `tiles` tiles, each of which sees what its table holds before the
+  // chunk and the chunk (the last term: the rounded rate). (None of this hangs on the number of CUs.)
+  const int tile_rows = 32 * i8_prefill_waves(head_dim);
+  const int64_t one = num_tokens * group / tile_rows + 1, tiles = one + num_seqs - pl.small;
+  const int64_t steps = kI8TileCost + 4 + (max_blocks_per_seq + (num_tokens + 2 * tile_rows) / kBlockSize) /
+                        kI8StepBlocks + one / 4096;
+  TS_REQUIRE(merge_rows(pl, num_decode, num_heads, num_kv_heads) < (1ll << 30) &&
+                 decode_items(pl, num_decode, num_tokens, group) * num_kv_heads < (1ll << 31) &&
+                 (pl.small == num_seqs || tiles * steps * num_kv_heads < (1ll << 31)),
+             TS_ERR_UNSUPPORTED, "paged_attention_int8: %lld tokens of %d sequences over tables of %d blocks",
+             (long long)num_tokens, num_seqs, max_blocks_per_seq);
   int cus = 0;
   int status = device_cu_count(stream, &cus);
   if (status != TS_OK) return status;
-  const Int8Plan pl = int8_plan(num_seqs, num_decode, max_query_len, max_seq_len, max_prefill_seq_len,
-                                num_heads, num_kv_heads, head_dim, cus);
+  pl = int8_plan(num_seqs, num_decode, max_query_len, max_seq_len, max_prefill_seq_len, num_heads,
+                 num_kv_heads, head_dim, cus);
   TS_REQUIRE(pl.bytes == 0 || (workspace && workspace_bytes >= pl.bytes && aligned(workspace, 256)),
              TS_ERR_WORKSPACE, "paged_attention_int8: workspace of %zu bytes, %zu needed", workspace_bytes,
              pl.bytes);
@@ -171,19 +192,9 @@ extern "C" int ts_paged_attention_int8(const void* q, int64_t q_stride_t, int64_
   a.ks = k_scale, a.vs = v_scale, a.num_blocks = num_blocks;
   a.block_tables = block_tables, a.bt_stride = bt_stride, a.max_blocks = max_blocks_per_seq;
   a.seq_lens = seq_lens, a.heads = num_heads, a.kvh = num_kv_heads;
-  a.by_kvh = I8Div::by(num_kv_heads), a.by_group = I8Div::by(num_heads / num_kv_heads);
-  a.group = num_heads / num_kv_heads, a.qsl = query_start_loc, a.num_tokens = num_tokens;
+  a.by_kvh = I8Div::by(num_kv_heads), a.by_group = I8Div::by(group);
+  a.group = group, a.qsl = query_start_loc, a.num_tokens = num_tokens;
   a.sl2 = scale * 1.44269504088896340736f;
-  // ... and steps: those of at most `tiles` tiles, each of which sees what its table holds before the
-  // chunk and the chunk (the last term: the rounded rate).
-  const int tile_rows = 32 * i8_prefill_waves(head_dim);
-  const int64_t one = num_tokens * a.group / tile_rows + 1, tiles = one + num_seqs - pl.small;
-  const int64_t steps = kI8TileCost + 4 + (max_blocks_per_seq + (num_tokens + 2 * tile_rows) / kBlockSize) /
-                        kI8StepBlocks + one / 4096;
-  TS_REQUIRE(merge_rows(pl, num_decode, num_heads, num_kv_heads) < (1ll << 30) &&
-                 (pl.small == num_seqs || tiles * steps * num_kv_heads < (1ll << 31)),
-             TS_ERR_UNSUPPORTED, "paged_attention_int8: %lld tokens of %d sequences over tables of %d blocks",
-             (long long)num_tokens, num_seqs, max_blocks_per_seq);
   if (pl.small > 0) {
     a.num_seqs = pl.small, a.num_decode = num_decode;
     a.row_slots = pl.row_slots, a.max_splits = pl.max_splits, a.chunk_parts = pl.chunk_parts;

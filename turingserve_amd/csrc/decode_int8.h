@@ -474,7 +474,7 @@ __device__ __forceinline__ bool i8_find(const Int8DecodeArgs& a, int item, I8Ite
       const unsigned in = item - (base + of(sum) - of(n)), t = of(tiles);
       x.split = (int)(t == 1 ? in : in / t), x.tile = (int)(in - x.split * t);
       x.seq = {of(s.q0), of(s.n), of(s.kv), of(s.start)};
-      return x.split < x.splits;                           // (only lengths past 31 bits could have it)
+      return x.split < x.splits;                           // (only offsets that do not ascend could have it)
     }
     base += __builtin_amdgcn_readlane(sum, kWave - 1);
   }
@@ -490,7 +490,7 @@ __global__ void __launch_bounds__(kI8Threads, i8_decode_groups(D)) decode_int8_k
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int lane = threadIdx.x % kWave, c = lane % 16, g = lane / 16;
   for (int64_t u = blockIdx.x;; u += gridDim.x) {
-    if (u > INT32_MAX) return;
+    if (u > INT32_MAX) return;                             // (the entry point refuses more)
     const int item = a.by_kvh((int)u), h = (int)u - item * a.kvh;
     I8Item x;
     if (!i8_find(a, item, x)) return;
