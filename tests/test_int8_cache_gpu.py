@@ -155,6 +155,33 @@ def test_write_host_bounds_and_layouts():
         H.kv_write_int8(odd, v, *cache, meta)
 
 
+def test_strides_of_axes_of_one_element_do_not_matter():
+    """One row, or one KV head, cut out of rows of an odd width."""
+    c = Case((1, 1, 64), [(4, 1)], num_decode=1, seed=40)
+    qkv, q, k, v, cache, meta = c.on(DEV)
+    H.kv_write_int8(k, v, *cache, meta)
+    want = H.paged_attention_int8(q, *cache, meta, c.scale)
+    cos, sin = rope_tables(64, 1e6, 8, DEV)
+    pos = torch.from_numpy(c.pos).to(DEV)
+    _, _, _, _, turned, _ = c.on(DEV)
+    rotated = H.rope_kv_write_int8(qkv, pos, cos, sin, 1, 1, 64, *turned, meta)
+
+    def odd(x):                                      # x [1, ...] at the start of a row of 4097 elements
+        wide = torch.zeros(2, 4097, dtype=x.dtype, device=DEV)
+        wide[0, :x.numel()] = x.flatten()
+        return wide[:1, :x.numel()].as_strided(x.shape, (4097,) * (x.dim() - 1) + (1,))
+
+    _, _, _, _, mine, _ = c.on(DEV)
+    H.kv_write_int8(odd(k), odd(v), *mine, meta)
+    assert_cache(mine, oracle_write(c))
+    assert torch.equal(H.paged_attention_int8(odd(q), *mine, meta, c.scale), want)
+    _, _, _, _, mine, _ = c.on(DEV)
+    wide = torch.zeros(1, 193, dtype=torch.float16, device=DEV)
+    wide[:, :192] = qkv
+    assert torch.equal(H.rope_kv_write_int8(wide, pos, cos, sin, 1, 1, 64, *mine, meta), rotated)
+    assert all(torch.equal(a, b) for a, b in zip(mine, turned))
+
+
 def test_rope_write_clamps_positions_and_takes_one_row():
     c = Case((2, 1, 16), [(4, 1)], num_decode=1, seed=8)
     qkv, _, _, _, cache, meta = c.on(DEV)

@@ -745,6 +745,13 @@ def _elsewhere(t: torch.Tensor) -> bool:
     return t.device.index != torch._C._cuda_getDevice()
 
 
+def _row_strides(x: torch.Tensor) -> tuple[int, int]:
+    """Strides of x [T, heads, D] over tokens and heads; those of an axis of one element, which name no
+    address and may be anything, as they are in contiguous rows."""
+    T, heads, D = x.shape
+    return x.stride(0) if T > 1 else heads * D, x.stride(1) if heads > 1 else D
+
+
 def kv_write_int8(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                   k_scale: torch.Tensor, v_scale: torch.Tensor, meta) -> None:
     """The step's new rows k, v [T, KVH, D] (strided views of qkv allowed) into an 8-bit paged
@@ -769,7 +776,7 @@ def kv_write_int8(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cac
     _require(k.dtype == torch.float16 and v.dtype == torch.float16 and k.stride(2) == 1 and
              v.stride(2) == 1, "kv_write_int8: k, v must be fp16 with unit stride over D")
     N.check(N.lib().ts_kv_write_int8(
-        _ptr(k), _ptr(v), k.stride(0), k.stride(1), v.stride(0), v.stride(1), _ptr(k_cache),
+        _ptr(k), _ptr(v), *_row_strides(k), *_row_strides(v), _ptr(k_cache),
         _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), NB, _ptr(bt), bt_st, bt.shape[1], _ptr(sl),
         _ptr(qsl), sl.shape[0], meta.num_decode, int(meta.max_query_len), T, KVH, D, _stream(k)),
         "kv_write_int8")
@@ -807,7 +814,7 @@ def rope_kv_write_int8(qkv: torch.Tensor, positions: torch.Tensor, cos: torch.Te
     pos = positions if (positions.dtype == torch.int64 and positions.is_contiguous()) \
         else positions.to(torch.int64).contiguous()
     N.check(N.lib().ts_rope_kv_write_int8(
-        _ptr(qkv), qkv.stride(0) if T > 1 else qkv.shape[1], _ptr(pos), _ptr(cos), _ptr(sin),
+        _ptr(qkv), qkv.stride(0) if T > 1 else (H + 2 * KVH) * D, _ptr(pos), _ptr(cos), _ptr(sin),
         cos.shape[0], _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), NB,
         _ptr(bt), bt_st, bt.shape[1], _ptr(sl), _ptr(qsl), sl.shape[0], meta.num_decode,
         int(meta.max_query_len), T, H, KVH, D, _stream(qkv)), "rope_kv_write_int8")
@@ -839,8 +846,7 @@ def paged_attention_int8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
                                                                N.cu_count(q.device.index or 0))
     ws = _workspace(ws_bytes, q.device)
     N.check(N.lib().ts_paged_attention_int8(
-        _ptr(q), q.stride(0) if T > 1 else H * D, q.stride(1) if H > 1 else D, _ptr(out), H * D, T,
-        _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), NB, _ptr(bt), bt_st, bt.shape[1],
+        _ptr(q), *_row_strides(q), _ptr(out), H * D, T, _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), NB, _ptr(bt), bt_st, bt.shape[1],
         _ptr(sl), _ptr(qsl), B, S, *bounds, H, KVH, D, float(scale), _ptr(ws), ws_bytes, _stream(q)),
         "paged_attention_int8")
     return out
