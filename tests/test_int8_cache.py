@@ -102,6 +102,32 @@ def test_twins_match_the_oracle(heads):
     assert (np.abs(out.double().numpy() - ref) <= bound).all()
 
 
+@pytest.mark.parametrize("what", ["short table", "fewer positions", "foreign blocks", "nan", "inf"])
+def test_attention_twin_keeps_the_contract(what):
+    """Tables that do not hold the sequence, rows before its first token, ids outside the cache, blocks
+    without a finite scale: as the kernels, by the oracle."""
+    c = Case((4, 2, 16), [(20, 1), (5, 60), (0, 0), (0, 3)], num_decode=1, seed=41)
+    hit = np.zeros((c.T, c.H), bool)
+    if what == "short table":
+        c.tables = np.ascontiguousarray(c.tables[:, :2])
+    elif what == "fewer positions":
+        c.lens[1] = 20
+    elif what == "foreign blocks":
+        c.tables[0, 1], c.tables[1, 1] = c.NB, -1
+    else:
+        c.scales[0 if what == "inf" else 1, c.tables[1, 2], 1] = float(what)
+        hit[1 + 27:61, 2:] = True                        # positions 32 and later of the second sequence
+    _, q, _, _, cache, meta = c.on("cpu")
+    out = R.paged_attention_int8(q, *cache, meta, c.scale).double().numpy()
+    c.tables[(c.tables < 0) | (c.tables >= c.NB)] = 0
+    clean = np.where(np.isfinite(c.scales), c.scales, 0)
+    ref, bound = O.paged_attention(c.split()[0], c.codes, clean, c.tables, c.lens, c.starts, c.scale)
+    rows = np.repeat(hit, c.D, axis=1)
+    assert np.isnan(out[rows]).all() and (np.abs(out - ref) <= bound)[~rows].all()
+    if what == "fewer positions":
+        assert not out[1:41].any() and out[41:61].any()
+
+
 def test_twins_of_sequences_without_rows():
     c = Case((4, 2, 16), [(20, 1), (40, 0), (0, 0), (5, 20)], num_decode=1, seed=5)
     _, q, k, v, cache, meta = c.on("cpu")

@@ -170,18 +170,30 @@ def rope_kv_write_int8(qkv: torch.Tensor, positions: torch.Tensor, cos: torch.Te
 def paged_attention_int8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                          k_scale: torch.Tensor, v_scale: torch.Tensor, meta,
                          scale: float) -> torch.Tensor:
-    """Twin: the sequences' blocks as fp32 values, then attention_with_mask; rows of sequences with
-    seq_len 0 stay 0."""
+    """Twin: the sequences' blocks as fp32 values, then causal attention over the tokens that the table
+    holds (block ids outside the cache read block 0). Rows that see no token are zeros, rows that see a
+    block whose K or V scale is not finite NaN."""
     T, H, D = q.shape
-    KVH = k_cache.shape[1]
+    NB, KVH = k_scale.shape
     out = torch.zeros(T, H * D, dtype=q.dtype, device=q.device)
     qsl = meta.query_start_loc.tolist()
     for b, seq_len in enumerate(meta.seq_lens.tolist()):
         qs, qe = qsl[b], qsl[b + 1]
-        if seq_len == 0 or qe == qs:
+        held = min(seq_len, 16 * meta.block_tables.shape[1])
+        if held <= 0 or qe <= qs:
             continue
-        blocks = meta.block_tables[b, :-(-seq_len // 16)].long()
-        kk, vv = ((c[blocks].float() * s[blocks][:, :, None, None]).permute(0, 2, 1, 3)
-                  .reshape(-1, KVH, D)[:seq_len] for c, s in ((k_cache, k_scale), (v_cache, v_scale)))
-        out[qs:qe] = attention_with_mask(q[qs:qe], kk, vv, scale)
+        blocks = meta.block_tables[b, :-(-held // 16)].long()
+        blocks = torch.where((blocks >= 0) & (blocks < NB), blocks, 0)
+        bad = ~(torch.isfinite(k_scale[blocks]) & torch.isfinite(v_scale[blocks]))
+        kk, vv = ((c[blocks].float() * s[blocks].masked_fill(bad, 0.0)[:, :, None, None])
+                  .permute(1, 0, 2, 3).reshape(KVH, -1, D)[:, :held].repeat_interleave(H // KVH, 0)
+                  for c, s in ((k_cache, k_scale), (v_cache, v_scale)))
+        bad = bad.repeat_interleave(16, 0)[:held].T.repeat_interleave(H // KVH, 0)      # [H, held]
+        last = torch.arange(seq_len - (qe - qs), seq_len, device=q.device)               # a row's own position
+        seen = torch.arange(held, device=q.device) <= last[:, None]                      # [rows, held]
+        scores = torch.matmul(q[qs:qe].float().permute(1, 0, 2), kk.transpose(1, 2).contiguous()) * scale
+        p = torch.softmax(scores.masked_fill(~seen, float("-inf")), dim=-1).masked_fill(~seen, 0.0)
+        o = torch.matmul(p, vv).permute(1, 0, 2)
+        o = o.masked_fill((seen[:, None] & bad).any(-1)[:, :, None], float("nan"))
+        out[qs:qe] = o.reshape(qe - qs, H * D).to(q.dtype)
     return out
