@@ -302,6 +302,51 @@ def test_python_wrappers_refuse():
         H._int8_args("x", *cache, meta, torch.device("cuda", 0))
 
 
+def test_tensors_of_another_gpu_than_the_current_one(monkeypatch):
+    """The ops launch on the device of their rows: the calls are made over with it as the current one
+    (tensors are stood in for; the caches' check, which these do not pass, comes after)."""
+    current, entered = [1], []
+
+    class On:
+        def __init__(self, device):
+            self.device = device
+
+        def __enter__(self):
+            entered.append(self.device)
+            self.was, current[0] = current[0], self.device.index
+
+        def __exit__(self, *_):
+            current[0] = self.was
+
+    class Rows:
+        is_cuda, device, dtype = True, torch.device("cuda", 0), torch.float16
+
+        def __init__(self, *shape):
+            self.shape = shape
+
+        def dim(self):
+            return len(self.shape)
+
+        def stride(self, _):
+            return 1
+
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: current[0], raising=False)
+    monkeypatch.setattr(torch.cuda, "device", On)
+    monkeypatch.setattr(torch, "empty", lambda *shape, **_: Rows(*shape))
+    flat, rows = Rows(2, 48), Rows(2, 1, 16)
+    for call in (lambda c: H.kv_write_int8(rows, rows, c, c, c, c, None),
+                 lambda c: H.rope_kv_write_int8(flat, flat, flat, flat, 1, 1, 16, c, c, c, c, None),
+                 lambda c: H.paged_attention_int8(rows, c, c, c, c, None, 1.0)):
+        with pytest.raises(ValueError, match="caches must be"):
+            call(rows)
+        assert entered.pop() == torch.device("cuda", 0) and not entered and current == [1]
+        current[0] = 0
+        with pytest.raises(ValueError, match="caches must be"):
+            call(rows)
+        assert not entered
+        current[0] = 1
+
+
 def test_cache_container_and_namespaces():
     kv = Int8KVCache.new(3, 5, 2, 32, "cpu")
     kc, vc, ks, vs = kv.layer(1)
