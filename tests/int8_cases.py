@@ -5,6 +5,7 @@ from __future__ import annotations
 import numpy as np
 import torch
 
+from oracle import int8_cache as O
 from turingserve_amd.metadata import AttentionMetadata
 
 BLOCK = 16
@@ -100,3 +101,32 @@ def roll_back(ops, device):
         write([2], 13)
         assert all(torch.equal(a[blk][:, :13] if a.dim() == 4 else a[blk], b[blk][:, :13] if b.dim() == 4 else b[blk])
                    for a, b in zip(cache, never))
+
+
+def near_the_rows(ops, device, heads):
+    """Prompts written in one piece, then attention: as near to attention over the rows themselves as half
+    a code allows. A K value is off by half its block's scale (and 2^-16 of it: the scale's and the quotient's
+    rounding), a score by at most d = scale * sum |q| * that, a weight by a factor within e^(+-2 d), a V value by
+    half its scale; the kernels' own error over the codes comes on top."""
+    c = Case(heads, [(0, 70), (0, 33)], seed=42)
+    _, q, k, v, cache, meta = c.on(device)
+    ops.kv_write_int8(k, v, *cache, meta)
+    out = ops.paged_attention_int8(q, *cache, meta, c.scale).double().cpu().numpy()
+    codes, scales = (torch.stack(t).cpu().numpy() for t in (cache[:2], cache[2:]))
+    _, lim = O.paged_attention(c.split()[0], codes, scales, c.tables, c.lens, c.starts, c.scale)
+    qn, kn, vn = (x.astype(np.float64) for x in c.split())
+    half = 0.5 + 2.0 ** -16
+    g = c.H // c.KVH
+    for b, (_, n) in enumerate(c.items):
+        lo = int(c.starts[b])
+        step = np.repeat(scales[:, c.tables[b, :-(-n // BLOCK)]].astype(np.float64), BLOCK, 1)[:, :n] * half
+        for h in range(c.H):
+            for i in range(n):
+                x, kk, vv = qn[lo + i, h], kn[lo:lo + i + 1, h // g], vn[lo:lo + i + 1, h // g]
+                s = kk @ x * c.scale
+                w = np.exp(s - s.max())
+                w /= w.sum()
+                d = c.scale * np.abs(x).sum() * step[0, :i + 1, h // g].max()
+                off = np.expm1(2 * d) * (w @ np.abs(vv)) + step[1, :i + 1, h // g].max()
+                at = slice(h * c.D, (h + 1) * c.D)
+                assert (np.abs(out[lo + i, at] - w @ vv) <= off + lim[lo + i, at]).all()

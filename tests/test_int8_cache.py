@@ -12,7 +12,7 @@ import pytest
 import torch
 
 from oracle import int8_cache as O
-from tests.int8_cases import HEADS, Case, roll_back
+from tests.int8_cases import HEADS, Case, near_the_rows, roll_back
 from turingserve_amd import _native as N
 from turingserve_amd import get_ops
 from turingserve_amd import hip_ops as H
@@ -153,6 +153,11 @@ def test_rope_twin_matches_the_oracle():
     assert np.array_equal(torch.stack(cache[:2]).numpy(), want_c)
     assert np.array_equal(torch.stack(cache[2:]).numpy(), want_s)
     assert np.array_equal(q.numpy(), O.rotate(qn, cn, sn).astype(np.float32).astype(np.float16))
+
+
+@pytest.mark.parametrize("heads", HEADS)
+def test_attention_over_the_cache_is_near_that_over_the_rows(heads):
+    near_the_rows(R, "cpu", heads)
 
 
 def test_rows_that_are_taken_back_keep_their_say():

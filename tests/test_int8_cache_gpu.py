@@ -10,7 +10,7 @@ import pytest
 import torch
 
 from oracle import int8_cache as O
-from tests.int8_cases import HEADS, Case, roll_back
+from tests.int8_cases import HEADS, Case, near_the_rows, roll_back
 from turingserve_amd import get_ops
 from turingserve_amd import hip_ops as H
 from turingserve_amd.qwen2 import rope_tables
@@ -191,6 +191,11 @@ def test_rope_write_clamps_positions_and_takes_one_row():
     _, _, _, _, last, _ = c.on(DEV)
     b = H.rope_kv_write_int8(qkv, torch.tensor([7], device=DEV), cos, sin, 2, 1, 16, *last, meta)
     assert torch.equal(a, b) and all(torch.equal(x, y) for x, y in zip(cache, last))
+
+
+@pytest.mark.parametrize("heads", HEADS)
+def test_attention_over_the_cache_is_near_that_over_the_rows(heads):
+    near_the_rows(H, DEV, heads)
 
 
 def test_rows_that_are_taken_back_keep_their_say():
