@@ -228,6 +228,7 @@ def test_refusals(call, kw, status, text):
 
 @pytest.mark.parametrize("kw", [
     dict(seqs=1 << 20, dec=1 << 20, T=1 << 20, h=32, kvh=32, D=16, qst=512, qsh=16, ost=512, ms=1 << 14),   # splits
+    dict(seqs=1 << 20, T=1 << 20, h=512, kvh=4, D=16, qst=8192, qsh=16, ost=8192, ms=1 << 14, mp=1 << 14),  # of chunks
     dict(seqs=1, T=1 << 20, mq=1 << 20, ms=1 << 21, mp=1 << 21, mb=1 << 17, bts=1 << 17, h=64, kvh=8, qst=4096,
          ost=4096),                                                                                        # steps
 ])

@@ -72,11 +72,12 @@ static Int8Plan int8_plan(int num_seqs, int num_decode, int max_query_len, int m
   return pl;
 }
 
-// Workgroups' worth of work in the decode kernel at most, for one KV head: splits of tiles of 16 rows.
+// Work items of the decode kernel at most (splits of tiles of 16 rows), for one KV head. A chunk of one
+// row has max_splits for each of its tiles, a longer one 64 over all of them, or one a tile.
 static int64_t decode_items(const Int8Plan& pl, int num_decode, int64_t num_tokens, int G) {
-  const int64_t chunks = pl.small - num_decode;
-  return (int64_t)num_decode * pl.max_splits * ((G + 15) / 16) +
-         (chunks > 0 ? chunks * (pl.max_splits + 1) + num_tokens * G / 16 : 0);
+  const int64_t row = (int64_t)pl.max_splits * ((G + 15) / 16), chunks = pl.small - num_decode;
+  const int64_t split = pl.max_splits > 1 ? (row > kI8MaxSplits ? row : kI8MaxSplits) : 0;
+  return num_decode * row + (chunks > 0 ? chunks * (split + 1) + num_tokens * G / 16 : 0);
 }
 
 // Rows that the decode kernel's merge goes over.
