@@ -14,6 +14,7 @@
  *   ts_paged_attention     <- ops/triton_ops.py:60-71        (twin ops/reference.py:94-111)
  *                             (+ ts_paged_attention_workspace_bytes)
  *   ts_w8a16_gemm          <- ops/triton_w8a16.py:38-51 and ops/triton_ops.py:74-91
+ *                             (twin ops/reference.py:45-47 + quant/int8.py:15-16)
  *   ts_w8a16_gemm_v        <- the same with the tuned per-bucket config (autopilot/tuner.py)
  *   ts_w8a16_glu           <- model/qwen2.py:35-36, silu_mul(linear(x, gate_up)) fused
  *                             (ops/triton_ops.py:74-91 + ops/triton_silu_mul.py:21-28)
@@ -29,7 +30,6 @@
  *   ts_silu_mul            <- ops/triton_silu_mul.py:21-28  (twin ops/reference.py:26-28)
  *   ts_kv_write_int8, ts_rope_kv_write_int8, ts_paged_attention_int8  the write and the attention of
  *                             a K/V cache held in 8 bits (no counterpart in the reference)
- *                             (twin ops/reference.py:45-47 + quant/int8.py:15-16)
  *
  * Conventions shared by every entry point
  *  - Plain pointers to device memory; the caller owns every buffer. The library never

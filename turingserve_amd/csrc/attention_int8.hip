@@ -11,6 +11,12 @@ namespace ts {
 //   otherwise sequences up to kI8SmallSeq tokens, each tile's in one piece, of kI8SmallWork (tile, pair
 //   of blocks) steps at most: 4 chunks of 128 on 2048 34.6 / 40.8, 16 of 128 on 512 35.4 / 41.5; above
 //   them 16 of 64 on 2048 51.7 / 44.6, 4 of 512 on 1024 53.3 / 44.1, one of 64 on 4096 35.7 / 33.7.
+// The same lines at other heads (of twelve shapes each, one is off by more than a tenth, the last here):
+//   14/2 heads of 64: 16 chunks of 8 on 4096 23.4 / 24.0, 16 of 16 27.7 / 25.9, one of 16 on 8192 19.0 /
+//   19.1, 4 of 128 on 2048 23.1 / 26.1; above them 16 of 32 on 4096 41.8 / 31.4, one of 64 25.5 / 18.2,
+//   4 of 512 on 1024 43.3 / 36.5; 8/8 heads of 64: 16 of 16 on 4096 27.1 / 41.4; above them 4 of 512 on
+//   1024 33.5 / 28.5; 16/4 heads of 32: 16 of 8 on 4096 19.0 / 24.4, 16 of 32 (128 rows) 33.7 / 26.9.
+// The choice is one for the batch, by its largest chunk.
 constexpr int kI8ShortRows = 128;
 constexpr int kI8SmallSeq = 2048;
 constexpr int64_t kI8SmallWork = 32768;

@@ -19,8 +19,8 @@
 // sum each, meet once at the end in LDS, and either write the row or leave a partial (m, l, O) for the
 // merge launch.
 //
-// 64 sequences of 128 to 4096 tokens, 12/2 heads of 128: 13.6 us and 4.0 for the merge, 38 MB of codes
-// and scales (7.7 us at a copy's 5.0 TB/s); one sequence of 6000: 7.0 and 3.7. What bounds it is the chain
+// 64 sequences of 128 to 4096 tokens, 12/2 heads of 128: 12.7 us and 4.7 for the merge, 38 MB of codes
+// and scales (7.7 us at a copy's 5.0 TB/s); one sequence of 6000: 7.1 to 7.9 and 3.8. What bounds it is the chain
 // of a workgroup (lengths, table, scales and codes, LDS, partial) and then that of the merge: taking out
 // a tenth of the loop's arithmetic (O scaled in every step) gained 1 %. Two tiles a workgroup (32 rows of
 // a chunk, 253 registers, two workgroups a CU) took 29.0 us instead of 24.7 at 16 sequences of 5 rows,

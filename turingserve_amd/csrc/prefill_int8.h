@@ -30,6 +30,7 @@
 // cycles, of which the MFMAs are 2050; exponentials, operand reads, staging and requests are worth 10 to
 // 14 % each when taken out, so it is the issue of all of them together that bounds it. 64 rows a
 // wavefront (four of them) read half the operands and took 115 us: the registers moved through AGPRs.
+// (Three registers are spilled at head_dim 128: stored once a workgroup, read once a tile's piece.)
 #pragma once
 
 #include "decode_int8.h"
