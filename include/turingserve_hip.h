@@ -561,7 +561,7 @@ int ts_rope_kv_write_int8(const void* qkv, int64_t qkv_stride, const int64_t* po
  * product each weight times its block's V scale is rounded to fp16, measured against (at most) the
  * largest such product among the tokens that the row sees: off by 2^-11 of itself, or 2^-25 of that
  * largest one where it is below 2^-14 of it. V scales below 2^-40 count as 2^-40 (results move by
- * 127 * 2^-40 at most). Rows that see no token are zeros; a row that sees a block whose K or
+ * 127 * 2^-40 at most), those above 2^100 as 2^100. Rows that see no token are zeros; a row that sees a block whose K or
  * V scale is not finite is NaN. A decode row's result does not depend on the rest of the batch
  * given max_seq_len. The host bounds shape the launch only: bounds below the batch's real values
  * are slower, not wrong. head_dim 16, 32, 64, 128 or 256, any number of query heads per KV head; q

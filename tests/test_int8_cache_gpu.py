@@ -352,6 +352,25 @@ def test_scales_too_small_for_fp16(bound):
     assert not out[1].any()
 
 
+@pytest.mark.parametrize("heads", [(4, 2, 64), (12, 2, 128)])
+@pytest.mark.parametrize("bound", [101, 30000])
+@pytest.mark.parametrize("big", [1e37, 3e38])
+def test_scales_too_large_for_fp16(heads, bound, big):
+    """V scales that are finite in fp32 only: codes of 0 stay 0, others are infinite, and blocks that a row
+    does not see leave it as it is."""
+    c = Case(heads, [(99, 1), (20, 1), (0, 60)], num_decode=2, seed=43)
+    c.scales[1, c.tables[0]] = big                   # zeros only
+    c.codes[1, c.tables[0]] = 0
+    c.scales[1, c.tables[1, :2]] = big               # one sign a column
+    c.codes[1, c.tables[1, :2]] = np.where(np.arange(c.D) % 2, 1, -1)
+    c.scales[1, c.tables[2, 3]] = big                # tokens 48 .. 59
+    _, q, _, _, cache, meta = c.on(DEV)
+    out = H.paged_attention_int8(q, *cache, dataclasses.replace(meta, max_prefill_seq_len=bound), c.scale)
+    assert not out[0].any()
+    assert out[1].isinf().all() and (out[1].view(c.H, c.D) > 0).eq(torch.arange(c.D, device=DEV) % 2 == 1).all()
+    assert_rows(out, c, rows=slice(2, 50))
+
+
 def test_more_heads_than_a_chunk_may_have_rows():
     """160 query heads on one KV head: ten tiles a token."""
     c = Case((160, 1, 16), [(900, 1), (4, 1), (300, 3), (70, 1)], num_decode=2, seed=35)

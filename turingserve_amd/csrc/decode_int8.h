@@ -144,10 +144,11 @@ __device__ __forceinline__ int i8_kv_len(int len, int max_blocks) {
 }
 
 // A block's V scale in the exponent, and what a weight with it is multiplied by in the row's sum: its
-// exact inverse but for rounding, so that the sum does not feel the logarithm's.
-constexpr float kI8LeastScale = 0x1p-40f;
+// exact inverse but for rounding, so that the sum does not feel the logarithm's. (Scales above 2^100,
+// whose inverse need not be a normal number, count as 2^100: any code of theirs is infinite in fp16.)
+constexpr float kI8LeastScale = 0x1p-40f, kI8MostScale = 0x1p100f;
 __device__ __forceinline__ void i8_value_factors(float vs, float& lv, float& back) {
-  lv = __builtin_amdgcn_logf(fmaxf(vs, kI8LeastScale));
+  lv = __builtin_amdgcn_logf(__builtin_amdgcn_fmed3f(vs, kI8LeastScale, kI8MostScale));
   back = fast_exp2(-lv);
 }
 
