@@ -237,15 +237,11 @@ def prepare(case, seed):
 
     ops = state["ops"] = get_ops("hip")
     cache = state["cache"] = Int4KVCache.new(layers, b["blocks"], kvh, d, "cuda")
-    # what the cache was written with: block after block, as one prompt's rows
-    n, i32 = b["blocks"] * BLOCK, dict(dtype=torch.int32, device="cuda")
-    whole = AttentionMetadata(
-        query_start_loc=torch.tensor([0, n], **i32), seq_lens=torch.tensor([n], **i32),
-        block_tables=torch.arange(b["blocks"], **i32)[None], num_decode=0, max_query_len=n,
-        slot_mapping=torch.arange(n, device="cuda"), max_seq_len=n, max_prefill_seq_len=n)
+    # what the cache was written with: slot after slot
+    n = b["blocks"] * BLOCK
     for i in range(layers):
         k, v = (old[i, j].transpose(1, 2).reshape(n, kvh, d) for j in range(2))
-        ops.kv_write_int4(k, v, *cache.layer(i), whole)
+        ops.kv_write_int4(k, v, *cache.layer(i), torch.arange(n, device="cuda"))
     state["meta"] = AttentionMetadata(
         query_start_loc=b["query_start_loc"], seq_lens=b["seq_lens"], block_tables=b["tables"],
         slot_mapping=_slots(b), num_decode=b["num_decode"], max_query_len=b["max_query_len"],
@@ -300,9 +296,10 @@ def _run_own(s):
     for i in range(case["layers"]):
         if case["rope"]:
             out.append(ops.rope_kv_write_int4(s["qkv"][i], s["batch"]["positions"], s["cos"],
-                                              s["sin"], h, kvh, d, *cache.layer(i), meta))
+                                              s["sin"], h, kvh, d, *cache.layer(i),
+                                              meta.slot_mapping))
         else:
-            ops.kv_write_int4(s["k"][i], s["v"][i], *cache.layer(i), meta)
+            ops.kv_write_int4(s["k"][i], s["v"][i], *cache.layer(i), meta.slot_mapping)
     return dict(q=out, cache=ops.kv_read_int4(cache.data, s["batch"]["used"]))
 
 
