@@ -30,6 +30,8 @@
  *   ts_silu_mul            <- ops/triton_silu_mul.py:21-28  (twin ops/reference.py:26-28)
  *   ts_kv_write_int8, ts_rope_kv_write_int8, ts_paged_attention_int8  the write and the attention of
  *                             a K/V cache held in 8 bits (no counterpart in the reference)
+ *   ts_kv_write_int4, ts_rope_kv_write_int4, ts_kv_read_int4, ts_paged_attention_int4  the same of one
+ *                             held in 4 bits, and its blocks as fp16 (no counterpart either)
  *
  * Conventions shared by every entry point
  *  - Plain pointers to device memory; the caller owns every buffer. The library never
@@ -43,7 +45,8 @@
  *  - Paged KV cache of one layer: k_cache / v_cache are [num_blocks, num_kv_heads, 16, head_dim]
  *    contiguous (the per-layer views kv_cache[l, 0] / kv_cache[l, 1] of the reference's
  *    [L, 2, num_blocks, KVH, 16, D] tensor, engine/builder.py:76-80). Block 0 is the null block.
- *    The 8-bit cache has the same blocks, int8, and fp32 scales beside them (ts_kv_write_int8).
+ *    The 8-bit cache has the same blocks, int8, and fp32 scales beside them (ts_kv_write_int8); the
+ *    4-bit one has units of bytes in their place (ts_kv_write_int4).
  *  - Memory safety instead of undefined behaviour: slot ids outside [0, num_blocks*16) are
  *    skipped like -1, block ids outside [0, num_blocks) read block 0, and a sequence whose
  *    seq_len exceeds 16 * max_blocks_per_seq attends only to the blocks its table holds.
@@ -582,6 +585,79 @@ int ts_paged_attention_int8(const void* q, int64_t q_stride_t, int64_t q_stride_
                             const void* v_cache, const float* k_scale, const float* v_scale,
                             int64_t num_blocks, const int32_t* block_tables, int64_t bt_stride,
                             int32_t max_blocks_per_seq, const int32_t* seq_lens,
+                            const int32_t* query_start_loc, int32_t num_seqs, int32_t num_decode,
+                            int32_t max_query_len, int32_t max_seq_len, int32_t max_prefill_seq_len,
+                            int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, float scale,
+                            void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * The 4-bit paged cache of one layer: k_cache / v_cache uint8 [num_blocks, num_kv_heads, B] contiguous,
+ * B = 8 D + 64 G bytes for the 16 rows of a block of one KV head, G = D / 32 groups of 32 channels (one of
+ * 16 at head_dim D = 16). The first 8 D bytes are codes: 8 channels are a 32-bit word whose nibbles hold,
+ * low ones first, the channels 0 2 4 6 1 3 5 7; K's words are [16 rows][D / 8], V's [D / 8][16 rows]. Then,
+ * for each row and group, two fp16 numbers: K's [16 rows][G][step, low], V's [G][4][step, low][4 rows].
+ * A code stands for fp16(low + code * step), rounded once. 1.25 D bytes a row and KV head for K and V
+ * (1.5 D at 16) where fp16 takes 4 D. The reference has no such cache; the step's metadata is the same.
+ *
+ * ts_kv_write_int4: for every token t with 0 <= s = slot_mapping[t] < 16 num_blocks, rows k[t] and v[t] go
+ * to row s % 16 of block s / 16; other slots are skipped. Per KV head and group, in fp32 rounded to
+ * nearest:
+ *   low  = fp16(least value)
+ *   step = (largest value - low) / 15, 0 where that is negative, rounded towards zero to fp16
+ *   code = rint((value - low) / step) within 0 .. 15, 0 where step is 0
+ * so that a value is off by about half a step, and by a step and a few units in the last place of its
+ * group's numbers at most at the group's upper end. A token whose K or V row of a head is not finite in
+ * fp16 (|value| > 65504) is NaN in that head: codes and steps 0, lows NaN, K and V. What stood in a slot
+ * has no say, and no other row is touched. No two tokens of a call may have the same slot (each would leave
+ * parts of its row; no access leaves the cache). k / v rows fp16, 16-byte aligned; head_dim 16, 32, 64,
+ * 128 or 256; tokens times heads below 2^30.
+ *
+ * ts_rope_kv_write_int4: the same for the k and v heads of qkv [T, (H + 2 KVH) D], k rotated first
+ * (rotate-half RoPE by the fp32 tables, computed in 64 bits and rounded to fp32), with the rotated q
+ * rows, rounded once, in q_out [T, H, D] (contiguous); qkv is not written. Rows 16-byte aligned.
+ * positions[t] outside [0, max_position) use the table's nearest row.
+ *
+ * ts_kv_read_int4: what the blocks blocks[0 .. n - 1] of a cache [num_layers, 2 (K, V), num_blocks,
+ * num_kv_heads, B] stand for, as the fp16 cache [num_layers, 2, n, num_kv_heads, 16, head_dim] in `out`, all
+ * 16 rows of each. Ids outside [0, num_blocks) read block 0. Every entry of the result is a
+ * number that attention over the 4-bit cache uses.
+ */
+int ts_kv_write_int4(const void* k, const void* v, int64_t k_stride_t, int64_t k_stride_h,
+                     int64_t v_stride_t, int64_t v_stride_h, void* k_cache, void* v_cache,
+                     int64_t num_blocks, const int64_t* slot_mapping, int64_t num_tokens,
+                     int32_t num_kv_heads, int32_t head_dim, void* stream);
+
+int ts_rope_kv_write_int4(const void* qkv, int64_t qkv_stride, const int64_t* positions,
+                          const float* cos_table, const float* sin_table, int64_t max_position,
+                          void* q_out, void* k_cache, void* v_cache, int64_t num_blocks,
+                          const int64_t* slot_mapping, int64_t num_tokens, int32_t num_heads,
+                          int32_t num_kv_heads, int32_t head_dim, void* stream);
+
+int ts_kv_read_int4(const void* cache, int32_t num_layers, int64_t num_blocks, int32_t num_kv_heads,
+                    int32_t head_dim, const int32_t* blocks, int32_t n, void* out, void* stream);
+
+/*
+ * Attention over a 4-bit paged cache: the contract of ts_paged_attention (decode rows
+ * [0, num_decode), one query row each; then the query_start_loc rows of the other sequences under
+ * the bottom-right causal mask) with K and V the fp16 numbers that the codes stand for. Products in fp16
+ * with fp32 sums; scores, softmax statistics and outputs' sums are fp32. Before the P.V product a weight is
+ * rounded to fp16, measured against (at most) the row's largest one: off by 2^-11 of itself, or 2^-25 of
+ * that largest one where it is below 2^-14 of it. Rows that see no token are zeros; a row that sees a
+ * token of NaN is NaN; tokens that it does not see have no say. A decode row's result does not depend
+ * on the rest of the batch given max_seq_len. The host bounds shape the launch only: bounds below the
+ * batch's real values are slower, not wrong. head_dims, heads, alignment, limits and the workspace as for
+ * ts_paged_attention_int8. Rows of no sequence are not written.
+ */
+size_t ts_paged_attention_int4_workspace_bytes(int32_t num_seqs, int32_t num_decode,
+                                               int32_t max_query_len, int32_t max_seq_len,
+                                               int32_t max_prefill_seq_len, int32_t num_heads,
+                                               int32_t num_kv_heads, int32_t head_dim,
+                                               int32_t cu_count);
+
+int ts_paged_attention_int4(const void* q, int64_t q_stride_t, int64_t q_stride_h, void* out,
+                            int64_t out_stride_t, int64_t num_tokens, const void* k_cache,
+                            const void* v_cache, int64_t num_blocks, const int32_t* block_tables,
+                            int64_t bt_stride, int32_t max_blocks_per_seq, const int32_t* seq_lens,
                             const int32_t* query_start_loc, int32_t num_seqs, int32_t num_decode,
                             int32_t max_query_len, int32_t max_seq_len, int32_t max_prefill_seq_len,
                             int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, float scale,

@@ -24,7 +24,8 @@ LIB_PATH = os.path.join(LIB_DIR, "libturingserve_hip.so")
 PROBES_PATH = os.path.join(LIB_DIR, "libturingserve_probes.so")
 BUILD_DIR = os.path.join(HERE, "_build")
 SOURCES = ["capi.hip", "kv_write.hip", "decode.hip", "prefill.hip", "ragged.hip", "w8a16.hip",
-           "small_ops.hip", "metadata.hip", "kv_write_int8.hip", "attention_int8.hip"]
+           "small_ops.hip", "metadata.hip", "kv_write_int8.hip", "attention_int8.hip",
+           "kv_write_int4.hip", "attention_int4.hip"]
 PROBE_SOURCES = ["probes.hip"]
 ARCH = "gfx950"
 
@@ -43,6 +44,7 @@ SOURCE_FLAGS = {
     "prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "ragged.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "attention_int8.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "attention_int4.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 
 

@@ -397,8 +397,8 @@ struct I8DecodeLds {
   float ml[2 * kI8Waves * 16];
 };
 
-// The four wavefronts' states meet in LDS; the row (or its partial) is written.
-template <int D>
+// The four wavefronts' states (O in units of 1 / UNIT) meet in LDS; the row (or its partial) is written.
+template <int D, int UNIT>
 __device__ __forceinline__ void i8_finish(const Int8DecodeArgs& a, I8State<D>& st, int b, int h,
                                           int q0, int row0, int rows, int split, int splits, int wave,
                                           float* s_o, float* s_ml) {
@@ -431,7 +431,7 @@ __device__ __forceinline__ void i8_finish(const Int8DecodeArgs& a, I8State<D>& s
       sum += f * s_ml[2 * (w * 16 + row) + 1];
       o += ld<float4_t>(s_o + (w * 16 + row) * I8DecodeLds<D>::ROW + d) * f;
     }
-    o *= kColumnUnit;
+    o *= (float)UNIT;
     if (splits == 1) {
       const float f = sum == 0.f ? 0.f : 1.f / sum;        // no visible key: zeros
       const int token = a.by_group(row0 + row), head = h * a.group + row0 + row - token * a.group;
@@ -510,7 +510,7 @@ __global__ void __launch_bounds__(kI8Threads, i8_decode_groups(D)) decode_int8_k
     const int nb = (kv + kBlockSize - 1) / kBlockSize;
     const int b0 = i8_split_begin(nb, x.split, x.splits), b1 = i8_split_begin(nb, x.split + 1, x.splits);
     i8_split<D>(a, st, q, x.b, h, b0, b1, kv, vis, least, wave);
-    i8_finish<D>(a, st, x.b, h, x.seq.q0, row0, rows, x.split, x.splits, wave, lds.o, lds.ml);
+    i8_finish<D, (int)kColumnUnit>(a, st, x.b, h, x.seq.q0, row0, rows, x.split, x.splits, wave, lds.o, lds.ml);
   }
 }
 

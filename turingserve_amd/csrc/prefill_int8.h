@@ -697,11 +697,10 @@ __device__ __forceinline__ void i8_piece(const Int8PrefillArgs& p, I8PrefillLds<
 constexpr int i8_prefill_waves(int D) { return D == 128 ? 8 : 4; }
 constexpr int i8_prefill_groups(int D) { return D > 128 ? 1 : 8 / i8_prefill_waves(D); }
 
-template <int D>
-__global__ void __launch_bounds__(i8_prefill_waves(D) * kWave, D > 128 ? 1 : 2)
-prefill_int8_kernel(Int8PrefillArgs p) {
-  constexpr int WAVES = i8_prefill_waves(D), ROWS = 32 * WAVES;
-  __shared__ __align__(16) I8PrefillLds<D> lds;
+// A workgroup's share of the batch's steps, tile by tile: piece(place, KV head, its steps [s0, s1), whether
+// these are all of the tile's, the partial's place). Every thread of the workgroup calls it.
+template <int ROWS, typename Piece>
+__device__ __forceinline__ void i8_share(const Int8PrefillArgs& p, int (*saved)[kWave], Piece piece) {
   const Int8DecodeArgs& a = p.a;
   int at, hi, h;
   I8Place place;
@@ -728,7 +727,7 @@ prefill_int8_kernel(Int8PrefillArgs p) {
     }
     if (threadIdx.x == 0) p.joints[blockIdx.x] = joint;
     if (!found) return;
-    if (threadIdx.x < kWave) walk.save(lds.walk);
+    if (threadIdx.x < kWave) walk.save(saved);
   }
   __syncthreads();                                         // (saved)
   while (true) {
@@ -736,14 +735,22 @@ prefill_int8_kernel(Int8PrefillArgs p) {
     at += c1 - c0;
     const int steps = i8_steps<ROWS>(a, place.k, place.tile);
     const int s0 = max(0, c0 - kI8TileCost), s1 = min(c1 - kI8TileCost, steps);
-    if (s1 > s0)
-      i8_piece<D, WAVES>(p, lds, place.k, place.seq, place.tile, h, s0, s1, s0 == 0 && s1 == steps,
-                         2 * blockIdx.x + (s0 == 0));
+    if (s1 > s0) piece(place, h, s0, s1, s0 == 0 && s1 == steps, 2 * (int)blockIdx.x + (s0 == 0));
     if (at >= hi) return;
-    if (!I8Walk<ROWS>(lds.walk).find(p, a.by_kvh(at), place)) return;
+    if (!I8Walk<ROWS>(saved).find(p, a.by_kvh(at), place)) return;
     h = (int)((unsigned)(at - place.before * a.kvh) / (unsigned)place.cost);
     if ((unsigned)h >= (unsigned)a.kvh) return;
   }
+}
+
+template <int D>
+__global__ void __launch_bounds__(i8_prefill_waves(D) * kWave, D > 128 ? 1 : 2)
+prefill_int8_kernel(Int8PrefillArgs p) {
+  constexpr int WAVES = i8_prefill_waves(D), ROWS = 32 * WAVES;
+  __shared__ __align__(16) I8PrefillLds<D> lds;
+  i8_share<ROWS>(p, lds.walk, [&](const I8Place& place, int h, int s0, int s1, bool whole, int slot) {
+    i8_piece<D, WAVES>(p, lds, place.k, place.seq, place.tile, h, s0, s1, whole, slot);
+  });
 }
 
 // Tiles that several workgroups share: kI8MergeRows rows a workgroup, D / 4 threads a row. The

@@ -5,7 +5,8 @@ that never hands out the null block 0 (kv/block_allocator.py:16-62), continuous 
 decodes scheduled first and prompts prefilled in chunks under a token budget
 (scheduler/scheduler.py:65-130), an input builder per step (host or device) and graph replay of
 pure-decode steps (runner/model_runner.py:20-28). Sampling is greedy argmax. kv_cache_dtype
-"int8" keeps K and V as 8-bit codes with a scale for each block and KV head.
+"int8" keeps K and V as 8-bit codes with a scale for each block and KV head, "int4" as 4-bit codes with
+two numbers for each token, KV head and group of 32 channels.
 """
 
 from __future__ import annotations

@@ -19,14 +19,15 @@ import torch.nn.functional as F
 
 from turingserve_amd import _native as N
 from turingserve_amd import tuner
-from turingserve_amd.quant import LinearWeight
+from turingserve_amd.quant import LinearWeight, int4_head_dim
 
 __all__ = ["kv_write", "paged_attention", "linear", "lm_head_int8", "logits_int8", "w8a16_linear",
            "decode_attention_v1", "decode_attention_v2", "decode_attention_v3",
            "prefill_attention", "rmsnorm", "rmsnorm_residual", "rope_", "silu_mul", "w8a16_glu",
            "gate_up_silu", "rope_kv_write_", "decode_kv_write_attention",
            "decode_rope_kv_write_attention", "kv_write_int8", "rope_kv_write_int8",
-           "paged_attention_int8"]
+           "paged_attention_int8", "kv_write_int4", "rope_kv_write_int4", "kv_read_int4",
+           "paged_attention_int4", "decode_split_map_int4"]
 
 DEFAULT_PARTITION = 0            # v3 split size when the caller names none: 0 = own-length
 
@@ -728,6 +729,12 @@ def _int8_args(what: str, k_cache, v_cache, k_scale, v_scale, meta, device) -> t
     for s in (k_scale, v_scale):
         _require(s.dtype == torch.float32 and s.shape == (NB, KVH) and s.is_contiguous(),
                  "{}: scales must be contiguous fp32 [num_blocks, KVH]", what)
+    return NB, KVH, D, *_step_args(what, meta, device, k_cache, v_cache, k_scale, v_scale)
+
+
+def _step_args(what: str, meta, device, *caches) -> tuple:
+    """Checks of the step's metadata and the tensors' devices; (block tables, seq_lens, query_start_loc,
+    table stride)."""
     bt = meta.block_tables
     if bt.dtype != torch.int32 or bt.stride(1) != 1:
         bt = bt.to(torch.int32).contiguous()
@@ -735,9 +742,9 @@ def _int8_args(what: str, k_cache, v_cache, k_scale, v_scale, meta, device) -> t
     B = sl.shape[0]
     _require(bt.shape[0] >= B and qsl.shape[0] >= B + 1 and 0 <= meta.num_decode <= B,
              "{}: metadata of {} sequences", what, B)
-    for t in (k_cache, v_cache, k_scale, v_scale, bt, sl, qsl):
+    for t in (*caches, bt, sl, qsl):
         _require(t.device == device, "{}: every tensor must live on the same GPU", what)
-    return NB, KVH, D, bt, sl, qsl, bt.stride(0) if bt.shape[0] > 1 else bt.shape[1]
+    return bt, sl, qsl, bt.stride(0) if bt.shape[0] > 1 else bt.shape[1]
 
 
 def _elsewhere(t: torch.Tensor) -> bool:
@@ -849,4 +856,151 @@ def paged_attention_int8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
         _ptr(q), *_row_strides(q), _ptr(out), H * D, T, _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), NB, _ptr(bt), bt_st, bt.shape[1],
         _ptr(sl), _ptr(qsl), B, S, *bounds, H, KVH, D, float(scale), _ptr(ws), ws_bytes, _stream(q)),
         "paged_attention_int8")
+    return out
+
+
+# ------------------------------------------------------------------------------------------
+# The 4-bit paged cache: codes with a step and a low for each row and group of 32 channels
+# ------------------------------------------------------------------------------------------
+def _int4_cache(what: str, k_cache: torch.Tensor, v_cache: torch.Tensor) -> tuple[int, int, int]:
+    """Checks of one layer's caches; (NB, KVH, D)."""
+    shape = k_cache.shape
+    D = int4_head_dim(shape[2]) if len(shape) == 3 else None
+    if D is None or shape != v_cache.shape:
+        raise ValueError(f"{what}: caches must be [num_blocks, KVH, unit bytes], got {tuple(shape)}")
+    _require(k_cache.dtype == torch.uint8 and v_cache.dtype == torch.uint8 and
+             k_cache.is_contiguous() and v_cache.is_contiguous(),
+             "{}: caches must be contiguous uint8", what)
+    return shape[0], shape[1], D
+
+
+def _slots(what: str, slot_mapping: torch.Tensor, T: int, device) -> torch.Tensor:
+    _require(slot_mapping.shape[0] >= T, "{}: slot_mapping shorter than the rows", what)
+    _require(slot_mapping.device == device, "{}: every tensor must live on the same GPU", what)
+    return slot_mapping if (slot_mapping.dtype == torch.int64 and slot_mapping.is_contiguous()) \
+        else slot_mapping.to(torch.int64).contiguous()
+
+
+def kv_write_int4(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                  slot_mapping: torch.Tensor) -> None:
+    """kv_write into a 4-bit paged cache: rows k, v [T, KVH, D] (strided views of qkv allowed) into the
+    slots of slot_mapping, caches [NB, KVH, unit bytes] uint8 (quant.Int4KVCache). For each row, KV head
+    and group of 32 channels (16 at head_dim 16): low its least value in fp16, step (largest - low) / 15
+    rounded towards zero to fp16, codes rint((value - low) / step), each standing for fp16(low + code *
+    step). A row depends on nothing but itself; what stood in its slot is gone. A token whose K or V row
+    of a head is not finite in fp16 becomes NaN in that head. Slots outside the cache are skipped (-1:
+    padding); no two rows may have the same slot."""
+    T, KVH, D = k.shape
+    if T == 0:
+        return
+    _check_gpu(k, v)
+    if _elsewhere(k):
+        with torch.cuda.device(k.device):
+            return kv_write_int4(k, v, k_cache, v_cache, slot_mapping)
+    NB, ckvh, cd = _int4_cache("kv_write_int4", k_cache, v_cache)
+    _require(v.shape == k.shape and ckvh == KVH and cd == D, "kv_write_int4: shape mismatch")
+    _require(k.dtype == torch.float16 and v.dtype == torch.float16 and k.stride(2) == 1 and
+             v.stride(2) == 1, "kv_write_int4: k, v must be fp16 with unit stride over D")
+    _require(v.device == k_cache.device == v_cache.device == k.device,
+             "kv_write_int4: every tensor must live on the same GPU")
+    slots = _slots("kv_write_int4", slot_mapping, T, k.device)
+    N.check(N.lib().ts_kv_write_int4(
+        _ptr(k), _ptr(v), *_row_strides(k), *_row_strides(v), _ptr(k_cache), _ptr(v_cache), NB,
+        _ptr(slots), T, KVH, D, _stream(k)), "kv_write_int4")
+
+
+def rope_kv_write_int4(qkv: torch.Tensor, positions: torch.Tensor, cos: torch.Tensor,
+                       sin: torch.Tensor, H: int, KVH: int, D: int, k_cache: torch.Tensor,
+                       v_cache: torch.Tensor, slot_mapping: torch.Tensor) -> torch.Tensor:
+    """kv_write_int4 of qkv's k and v heads with k rotated on the way (rotate-half RoPE by the fp32
+    tables cos / sin [max_len, D / 2]), in one launch with the rotation of q, which is returned as
+    [T, H, D]; qkv [T, (H + 2 KVH) D] is left as it is. Rotations are computed wider than fp16 and
+    rounded once: q to fp16, k straight to its code."""
+    _check_gpu(qkv, positions, cos, sin)
+    if _elsewhere(qkv):
+        with torch.cuda.device(qkv.device):
+            return rope_kv_write_int4(qkv, positions, cos, sin, H, KVH, D, k_cache, v_cache, slot_mapping)
+    T = qkv.shape[0]
+    _require(qkv.dim() == 2 and qkv.stride(1) == 1 and qkv.dtype == torch.float16 and
+             qkv.shape[1] >= (H + 2 * KVH) * D,
+             "rope_kv_write_int4: qkv must be fp16 [T, (H + 2 KVH) D]")
+    q = torch.empty(T, H, D, dtype=qkv.dtype, device=qkv.device)
+    if T == 0:
+        return q
+    NB, ckvh, cd = _int4_cache("rope_kv_write_int4", k_cache, v_cache)
+    _require(ckvh == KVH and cd == D, "rope_kv_write_int4: cache shape mismatch")
+    _require(cos.dtype == torch.float32 and sin.dtype == torch.float32 and cos.is_contiguous()
+             and sin.is_contiguous() and cos.shape == sin.shape and cos.dim() == 2 and
+             cos.shape[1] == D // 2,
+             "rope_kv_write_int4: tables must be contiguous fp32 [max_len, D / 2]")
+    _require(positions.shape[0] >= T and positions.device == qkv.device == cos.device == sin.device
+             == k_cache.device == v_cache.device,
+             "rope_kv_write_int4: positions shorter than qkv, or tensors of several devices")
+    pos = positions if (positions.dtype == torch.int64 and positions.is_contiguous()) \
+        else positions.to(torch.int64).contiguous()
+    slots = _slots("rope_kv_write_int4", slot_mapping, T, qkv.device)
+    N.check(N.lib().ts_rope_kv_write_int4(
+        _ptr(qkv), qkv.stride(0) if T > 1 else (H + 2 * KVH) * D, _ptr(pos), _ptr(cos), _ptr(sin),
+        cos.shape[0], _ptr(q), _ptr(k_cache), _ptr(v_cache), NB, _ptr(slots), T, H, KVH, D,
+        _stream(qkv)), "rope_kv_write_int4")
+    return q
+
+
+def kv_read_int4(cache: torch.Tensor, blocks: torch.Tensor) -> torch.Tensor:
+    """What blocks [n] of a 4-bit cache [L, 2, NB, KVH, unit bytes] (Int4KVCache.data, or some of its
+    layers) stand for, as the fp16 cache [L, 2, n, KVH, 16, D] whose block i is blocks[i]: attention over
+    it with tables renumbered so is attention over the 4-bit cache. Ids outside the cache read
+    block 0."""
+    _check_gpu(cache, blocks)
+    if _elsewhere(cache):
+        with torch.cuda.device(cache.device):
+            return kv_read_int4(cache, blocks)
+    D = int4_head_dim(cache.shape[4]) if cache.dim() == 5 and cache.shape[1] == 2 else None
+    _require(D is not None and cache.dtype == torch.uint8 and cache.is_contiguous(),
+             "kv_read_int4: cache must be contiguous uint8 [L, 2, num_blocks, KVH, unit bytes], got {}",
+             tuple(cache.shape))
+    _require(blocks.dim() == 1 and blocks.device == cache.device,
+             "kv_read_int4: blocks must be [n] on the cache's GPU")
+    L, _, NB, KVH, _ = cache.shape
+    if blocks.dtype != torch.int32:                        # (ids past 31 bits must not wrap into the cache)
+        blocks = blocks.clamp(-1, min(NB, 2 ** 31 - 1)).to(torch.int32)
+    ids, n = blocks.contiguous(), blocks.shape[0]
+    out = torch.empty(L, 2, n, KVH, 16, D, dtype=torch.float16, device=cache.device)
+    N.check(N.lib().ts_kv_read_int4(_ptr(cache), L, NB, KVH, D, _ptr(ids), n, _ptr(out),
+                                    _stream(cache)), "kv_read_int4")
+    return out
+
+
+def decode_split_map_int4(meta, H: int, KVH: int, D: int, num_blocks: int, device):
+    """The step's split map for paged_attention_int4: None, which makes every call look its splits up."""
+    return None
+
+
+def paged_attention_int4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, meta,
+                         scale: float, split_map=None) -> torch.Tensor:
+    """paged_attention over a 4-bit cache (see kv_write_int4): q [T, H, D] -> [T, H*D], one row for each
+    of the first num_decode sequences, the rows of query_start_loc for the others under the
+    bottom-right causal mask. A row that sees a token of NaN is NaN; a row that sees no token is
+    zeros."""
+    T, H, D = q.shape
+    if T == 0:
+        return torch.empty(0, H * D, dtype=q.dtype, device=q.device)
+    _check_gpu(q)
+    if _elsewhere(q):
+        with torch.cuda.device(q.device):
+            return paged_attention_int4(q, k_cache, v_cache, meta, scale, split_map)
+    out = torch.empty(T, H * D, dtype=q.dtype, device=q.device)
+    NB, KVH, cd = _int4_cache("paged_attention_int4", k_cache, v_cache)
+    bt, sl, qsl, bt_st = _step_args("paged_attention_int4", meta, q.device, k_cache, v_cache)
+    _require(cd == D and q.stride(2) == 1 and q.dtype == torch.float16,
+             "paged_attention_int4: q must be fp16 [T, H, D] with unit stride over D")
+    B, S = sl.shape[0], meta.num_decode
+    bounds = (int(meta.max_query_len), int(meta.max_seq_len), _prefill_seq_bound(meta))
+    ws_bytes = N.lib().ts_paged_attention_int4_workspace_bytes(B, S, *bounds, H, KVH, D,
+                                                               N.cu_count(q.device.index or 0))
+    ws = _workspace(ws_bytes, q.device)
+    N.check(N.lib().ts_paged_attention_int4(
+        _ptr(q), *_row_strides(q), _ptr(out), H * D, T, _ptr(k_cache), _ptr(v_cache), NB, _ptr(bt),
+        bt_st, bt.shape[1], _ptr(sl), _ptr(qsl), B, S, *bounds, H, KVH, D, float(scale), _ptr(ws),
+        ws_bytes, _stream(q)), "paged_attention_int4")
     return out

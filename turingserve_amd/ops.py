@@ -19,7 +19,10 @@ def _reference() -> SimpleNamespace:
         silu_mul=r.silu_mul, rope_=r.rope_, linear=r.linear, kv_write=r.kv_write,
         paged_attention=r.paged_attention, dense_causal_attention=r.dense_causal_attention,
         attention_with_mask=r.attention_with_mask, kv_write_int8=r.kv_write_int8,
-        rope_kv_write_int8=r.rope_kv_write_int8, paged_attention_int8=r.paged_attention_int8)
+        rope_kv_write_int8=r.rope_kv_write_int8, paged_attention_int8=r.paged_attention_int8,
+        kv_write_int4=r.kv_write_int4, rope_kv_write_int4=r.rope_kv_write_int4,
+        kv_read_int4=r.kv_read_int4, paged_attention_int4=r.paged_attention_int4,
+        decode_split_map_int4=r.decode_split_map_int4)
 
 
 def _hip() -> SimpleNamespace:
@@ -47,6 +50,11 @@ def _hip() -> SimpleNamespace:
     ns.kv_write_int8 = h.kv_write_int8
     ns.rope_kv_write_int8 = h.rope_kv_write_int8
     ns.paged_attention_int8 = h.paged_attention_int8
+    ns.kv_write_int4 = h.kv_write_int4
+    ns.rope_kv_write_int4 = h.rope_kv_write_int4
+    ns.kv_read_int4 = h.kv_read_int4
+    ns.paged_attention_int4 = h.paged_attention_int4
+    ns.decode_split_map_int4 = h.decode_split_map_int4
     return ns
 
 

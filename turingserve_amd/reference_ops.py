@@ -11,7 +11,8 @@ from __future__ import annotations
 import torch
 import torch.nn.functional as F
 
-from turingserve_amd.quant import LinearWeight, dequantize
+from turingserve_amd.quant import (INT4_NIBBLES, LinearWeight, dequantize, int4_quantise,
+                                   int4_views)
 
 
 def rmsnorm(x: torch.Tensor, w: torch.Tensor, eps: float) -> torch.Tensor:
@@ -195,5 +196,94 @@ def paged_attention_int8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
         p = torch.softmax(scores.masked_fill(~seen, float("-inf")), dim=-1).masked_fill(~seen, 0.0)
         o = torch.matmul(p, vv).permute(1, 0, 2)
         o = o.masked_fill((seen[:, None] & bad).any(-1)[:, :, None], float("nan"))
+        out[qs:qe] = o.reshape(qe - qs, H * D).to(q.dtype)
+    return out
+
+
+def kv_write_int4(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                  slot_mapping: torch.Tensor) -> None:
+    """Twin of the quantising write into a 4-bit paged cache ([NB, KVH, unit bytes] uint8). k, v
+    [T, KVH, D] in any floating type; slots outside the cache are skipped."""
+    slots = slot_mapping[:k.shape[0]]
+    keep = (slots >= 0) & (slots < 16 * k_cache.shape[0])
+    slots = slots[keep]
+    k, v = k[keep].float(), v[keep].float()
+    bad = ~((k.abs() <= 65504).all(-1) & (v.abs() <= 65504).all(-1))[..., None]       # [T, KVH, 1]
+    for x, cache, values in ((k, k_cache, False), (v, v_cache, True)):
+        codes, steps, lows = int4_quantise(x.masked_fill(bad, 0.0))
+        codes = codes.flatten(-2).unflatten(-1, (-1, 8))[..., INT4_NIBBLES]
+        to_codes, to_steps, to_lows = int4_views(cache, values)
+        to_codes[slots // 16, :, slots % 16] = codes[..., 0::2] | codes[..., 1::2] << 4
+        lows = lows.masked_fill(bad, torch.nan)
+        if not values:
+            to_steps[slots // 16, :, slots % 16] = steps
+            to_lows[slots // 16, :, slots % 16] = lows
+        else:
+            to_steps[slots // 16, :, slots % 16 // 4, slots % 4] = steps
+            to_lows[slots // 16, :, slots % 16 // 4, slots % 4] = lows
+
+
+def rope_kv_write_int4(qkv: torch.Tensor, positions: torch.Tensor, cos: torch.Tensor,
+                       sin: torch.Tensor, H: int, KVH: int, D: int, k_cache: torch.Tensor,
+                       v_cache: torch.Tensor, slot_mapping: torch.Tensor) -> torch.Tensor:
+    """Twin: rotate-half RoPE of q (returned, [T, H, D], rounded once) and k (rounded to fp32), then
+    kv_write_int4 of the rotated k and of v."""
+    T, half = qkv.shape[0], D // 2
+    pos = positions[:T].clamp(0, cos.shape[0] - 1)
+    c, s = cos[pos].double()[:, None], sin[pos].double()[:, None]
+    x = qkv[:, :(H + 2 * KVH) * D].view(T, H + 2 * KVH, D)
+    x1, x2 = x[:, :H + KVH, :half].double(), x[:, :H + KVH, half:].double()
+    qk = torch.cat([x1 * c - x2 * s, x2 * c + x1 * s], dim=-1).float()
+    kv_write_int4(qk[:, H:], x[:, H + KVH:], k_cache, v_cache, slot_mapping)
+    return qk[:, :H].to(qkv.dtype)
+
+
+def kv_read_int4(cache: torch.Tensor, blocks: torch.Tensor) -> torch.Tensor:
+    """Twin: the values of `blocks` [n] (ids outside the cache read block 0) of a 4-bit cache
+    [L, 2, NB, KVH, unit bytes], as an fp16 cache [L, 2, n, KVH, 16, D] holds them."""
+    ids = torch.where((blocks >= 0) & (blocks < cache.shape[2]), blocks, 0).long()
+    return torch.stack([_int4_values(cache[:, j, ids], bool(j)) for j in range(2)], dim=1)
+
+
+def _int4_values(cache: torch.Tensor, values: bool) -> torch.Tensor:
+    """What units [..., unit bytes] stand for, [..., 16, D] fp16."""
+    codes, steps, lows = int4_views(cache.contiguous(), values)
+    if values:
+        steps, lows = steps.flatten(-3, -2), lows.flatten(-3, -2)                     # [..., 16, G]
+    nibbles = torch.stack([codes & 15, codes >> 4], dim=-1).flatten(-2)               # [..., 16, D / 8, 8]
+    order = torch.tensor(INT4_NIBBLES, device=cache.device).argsort()
+    x = nibbles[..., order].flatten(-2).unflatten(-1, (steps.shape[-1], -1)).double()
+    return (x * steps.double()[..., None] + lows.double()[..., None]).flatten(-2).half()
+
+
+def decode_split_map_int4(meta, H: int, KVH: int, D: int, num_blocks: int, device):
+    """Twin: attention here needs no map."""
+    return None
+
+
+def paged_attention_int4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, meta,
+                         scale: float, split_map=None) -> torch.Tensor:
+    """Twin: the sequences' blocks as fp16 values, then causal attention over the tokens that the table
+    holds (block ids outside the cache read block 0). Rows that see no token are zeros, rows that see a
+    token whose K is NaN are NaN."""
+    T, H, D = q.shape
+    NB, KVH = k_cache.shape[:2]
+    out = torch.zeros(T, H * D, dtype=q.dtype, device=q.device)
+    qsl = meta.query_start_loc.tolist()
+    for b, seq_len in enumerate(meta.seq_lens.tolist()):
+        qs, qe = qsl[b], qsl[b + 1]
+        held = min(seq_len, 16 * meta.block_tables.shape[1])
+        if held <= 0 or qe <= qs:
+            continue
+        blocks = meta.block_tables[b, :-(-held // 16)].long()
+        blocks = torch.where((blocks >= 0) & (blocks < NB), blocks, 0)
+        kk, vv = (_int4_values(c[blocks], values).float().permute(1, 0, 2, 3).reshape(KVH, -1, D)[:, :held]
+                  .repeat_interleave(H // KVH, 0) for c, values in ((k_cache, False), (v_cache, True)))
+        last = torch.arange(seq_len - (qe - qs), seq_len, device=q.device)            # a row's own position
+        seen = torch.arange(held, device=q.device) <= last[:, None]                   # [rows, held]
+        scores = torch.matmul(q[qs:qe].float().permute(1, 0, 2), kk.transpose(1, 2).contiguous()) * scale
+        p = torch.softmax(scores.masked_fill(~seen, float("-inf")), dim=-1)
+        p = p.masked_fill(~seen.any(-1)[:, None], 0.0)
+        o = torch.matmul(p, vv.nan_to_num(0.0)).permute(1, 0, 2)
         out[qs:qe] = o.reshape(qe - qs, H * D).to(q.dtype)
     return out
