@@ -5,7 +5,7 @@ namespace ts {
 
 struct Int8Kernels {
   template <int D>
-  static void decode(const Int8DecodeArgs& a, int64_t rows, int cus, hipStream_t s) {
+  static void decode(const Int8DecodeArgs& a, int64_t rows, int cus, void*, hipStream_t s) {
     // Every split of the batch, at most as many workgroups as the CUs hold; the rest go round.
     const int64_t most = a.num_seqs > a.num_decode ? INT32_MAX : (int64_t)a.num_decode * a.max_splits;
     const int64_t units = most * a.kvh * ((a.group + 15) / 16);
@@ -54,5 +54,5 @@ extern "C" int ts_paged_attention_int8(const void* q, int64_t q_stride_t, int64_
       {q, q_stride_t, q_stride_h, out, out_stride_t, num_tokens, k_cache, v_cache, k_scale, v_scale, num_blocks,
        block_tables, bt_stride, max_blocks_per_seq, seq_lens, query_start_loc, num_seqs, num_decode, max_query_len,
        max_seq_len, max_prefill_seq_len, num_heads, num_kv_heads, head_dim, scale, workspace, workspace_bytes,
-       stream});
+       stream, nullptr});
 }

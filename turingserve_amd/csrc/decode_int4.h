@@ -183,17 +183,19 @@ __device__ __forceinline__ void i4_step(I8State<D>& st, const I4Block<D> (&x)[2]
 }
 
 // One split [b0, b1) of a sequence's blocks by one wavefront (of kI8Waves). Blocks are taken 64 at a
-// time: lane i holds block i's id.
-template <int D>
+// time: lane i holds block i's id; with `known` the first kI8SplitBlocks come from there.
+template <int D, bool KNOWN>
 __device__ __forceinline__ void i4_split(const Int8DecodeArgs& a, I8State<D>& st, const I8Query<D>& q, int b,
-                                         int h, int b0, int b1, int len, int vis, int least, int wave) {
+                                         int h, int b0, int b1, int len, int vis, int least, int wave,
+                                         const int* known) {
   const int lane = threadIdx.x % kWave, c = lane % 16, g = lane / 16;
   const int32_t* table = a.block_tables + b * a.bt_stride;
   const uint8_t *kc = reinterpret_cast<const uint8_t*>(a.kc), *vc = reinterpret_cast<const uint8_t*>(a.vc);
-  for (int lo = b0; lo < b1; lo += kWave) {
-    const int n = min(b1 - lo, kWave);
+  for (int lo = b0, n; lo < b1; lo += n) {
+    const bool first = KNOWN && lo == b0;
+    n = min(b1 - lo, first ? kI8SplitBlocks : kWave);
     int blk = 0;
-    if (lane < n) blk = clamp_block(table[lo + lane], a.num_blocks);
+    if (lane < n) blk = clamp_block(first ? known[lane] : table[lo + lane], a.num_blocks);
     auto load = [&](I4Block<D> (&x)[2], int i) {           // blocks i, i + 1 of the 64
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
@@ -214,16 +216,11 @@ __device__ __forceinline__ void i4_split(const Int8DecodeArgs& a, I8State<D>& st
     int i = 2 * wave;
     if (i < n) load(x, i);
     if (i + STEP < n) load(y, i + STEP);
-    if (i >= n) continue;
-    while (true) {
+#pragma unroll 1
+    for (; i < n; i += STEP) {
       step(x, i);
-      if (i + 2 * STEP < n) load(x, i + 2 * STEP);
-      i += STEP;
-      if (i >= n) break;
-      step(y, i);
+      x[0] = y[0], x[1] = y[1];
       if (i + 2 * STEP < n) load(y, i + 2 * STEP);
-      i += STEP;
-      if (i >= n) break;
     }
   }
 }
@@ -252,8 +249,196 @@ __global__ void __launch_bounds__(kI8Threads, i8_decode_groups(D)) decode_int4_k
     for (int t = 0; t < D / 16; ++t) st.o[t] = {0.f, 0.f, 0.f, 0.f};
     const int nb = (kv + kBlockSize - 1) / kBlockSize;
     const int b0 = i8_split_begin(nb, x.split, x.splits), b1 = i8_split_begin(nb, x.split + 1, x.splits);
-    i4_split<D>(a, st, q, x.b, h, b0, b1, kv, vis, least, wave);
+    i4_split<D, false>(a, st, q, x.b, h, b0, b1, kv, vis, least, wave, nullptr);
     i8_finish<D, 1>(a, st, x.b, h, x.seq.q0, row0, rows, x.split, x.splits, wave, lds.o, lds.ml);
+  }
+}
+
+// Four dims of a row from its n partials: load(k, m, l, o) gives partial k's. Unnormalised, with the row's
+// sum in `sum`. Both forms of the merge come here, so that a row has the same bits from either. Little code
+// in a loop: what a launch of a few microseconds runs once, it waits for from the instruction cache.
+template <typename Load>
+__device__ __forceinline__ float4_t i4_merge(int n, Load load, float& sum) {
+  constexpr int N = 8;                                     // requested at a time
+  float m = -INFINITY;
+  float4_t o = {0.f, 0.f, 0.f, 0.f};
+  sum = 0.f;
+#pragma unroll 1
+  for (int k0 = 0; k0 < n; k0 += N) {
+    float mk[N], lk[N], to = m;
+    float4_t x[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) load(min(k0 + i, n - 1), mk[i], lk[i], x[i]);
+#pragma unroll
+    for (int i = 0; i < N; ++i) to = vmax(to, mk[i]);
+    const float neg = to == -INFINITY ? 0.f : -to, alpha = fast_exp2(m + neg);
+    m = to;
+    sum *= alpha;
+    o *= alpha;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float w = k0 + i < n ? fast_exp2(mk[i] + neg) : 0.f;
+      sum = fmaf(w, lk[i], sum);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = fmaf(w, x[i][e], o[e]);
+    }
+  }
+  return o;
+}
+
+// Rows of sequences with more than one split, as a launch of its own: four dims of a row a thread.
+template <int D>
+__global__ void __launch_bounds__(kI8Threads) decode_int4_merge_kernel(Int8DecodeArgs a) {
+  constexpr int PER_ROW = D / 4;
+  const int id = blockIdx.x * (kI8Threads / PER_ROW) + threadIdx.x / PER_ROW, d = threadIdx.x % PER_ROW * 4;
+  const int behind = id - a.num_decode * a.heads;          // of the sequences past num_decode
+  const int unit = behind < 0 ? a.by_group(id) : a.by_slots(behind);
+  const int r = behind < 0 ? id - unit * a.group : behind - unit * a.row_slots;
+  const int seq0 = a.by_kvh(unit), h = unit - seq0 * a.kvh, b = behind < 0 ? seq0 : a.num_decode + seq0;
+  if (b >= a.num_seqs) return;
+  const I8Seq seq = i8_seq(a, b);
+  const int splits = i8_splits(a, seq, behind < 0);
+  if (splits == 1 || r >= seq.n * a.group) return;
+  const int64_t row = i8_partial(a, b, h, r, splits);
+  float sum;
+  const float4_t o = i4_merge(splits, [&](int k, float& m, float& l, float4_t& x) {
+    const float2_t ml = ld<float2_t>(a.part_ml + 2 * (row + k));
+    m = ml[0], l = ml[1], x = ld<float4_t>(a.part_o + (row + k) * D + d);
+  }, sum);
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;          // (nothing visible)
+  const int token = a.by_group(r), head = h * a.group + r - token * a.group;
+  st<half4_t>(a.out + (int64_t)(seq.q0 + token) * a.out_st + (int64_t)head * D + d, to_half4(o * inv));
+}
+
+// A pure-decode step's split map: what decode_int4_kernel looks up, worked out once for all layers of
+// the step, and the counters that let a launch merge its own splits. int32: a header that names the
+// plan, an entry for each split that the host's bounds allow (numbered densely, the real ones first) and a
+// counter for each (sequence, KV head, tile of 16 heads), 0 between launches.
+struct I4Map {
+  static constexpr int kMagic = 0x344d5354, kHeader = 32, kEntry = 32, kIds = 8, kMaxSeqs = 4096;
+  // of an entry: sequence (-1: behind the last split), split, splits, tokens, first and last block of
+  // the split, id of the sequence's last block; from kIds on those of the split's first 16 blocks
+  int* at;
+  __host__ __device__ static int64_t entries(int num_seqs, int max_splits) { return (int64_t)num_seqs * max_splits; }
+  __host__ __device__ static int64_t ints(int num_seqs, int max_splits, int kvh, int group) {
+    return kHeader + entries(num_seqs, max_splits) * kEntry + (int64_t)num_seqs * kvh * ((group + 15) / 16);
+  }
+  __device__ __forceinline__ bool names(const Int8DecodeArgs& a) const {
+    return table_entry(at) == kMagic && table_entry(at + 1) == a.num_seqs && table_entry(at + 2) == a.max_splits &&
+           table_entry(at + 3) == a.kvh && table_entry(at + 4) == a.group && table_entry(at + 5) == a.max_blocks;
+  }
+  __device__ __forceinline__ const int* entry(int slot) const { return at + kHeader + (int64_t)slot * kEntry; }
+  __device__ __forceinline__ int* counter(const Int8DecodeArgs& a, int b, int h, int tile) const {
+    return at + kHeader + entries(a.num_seqs, a.max_splits) * kEntry +
+           ((int64_t)b * a.kvh + h) * ((a.group + 15) / 16) + tile;
+  }
+};
+static_assert(I4Map::kEntry >= I4Map::kIds + kI8SplitBlocks, "a split's blocks fit its entry");
+
+// A wavefront an entry.
+static __global__ void __launch_bounds__(kI8Threads) decode_int4_map_kernel(Int8DecodeArgs a, I4Map map) {
+  const int lane = threadIdx.x % kWave;
+  const int64_t id = (int64_t)blockIdx.x * kI8Threads + threadIdx.x;
+  const int64_t counters = (int64_t)a.num_seqs * a.kvh * ((a.group + 15) / 16);
+  for (int64_t i = id; i < counters; i += (int64_t)gridDim.x * kI8Threads) *(map.counter(a, 0, 0, 0) + i) = 0;
+  if (id < I4Map::kHeader) {
+    const int name[6] = {I4Map::kMagic, a.num_seqs, a.max_splits, a.kvh, a.group, a.max_blocks};
+    int v = 0;
+#pragma unroll
+    for (int i = 0; i < 6; ++i) v = id == i ? name[i] : v;
+    map.at[id] = v;
+  }
+  const int64_t slot = id / kWave;
+  if (slot >= I4Map::entries(a.num_seqs, a.max_splits)) return;
+  // one tile of heads: item = split (a.group = 1 for the lookup, every sequence one row)
+  Int8DecodeArgs one = a;
+  one.group = 1;
+  I8Item x;
+  int v = lane == 0 ? -1 : 0;
+  if (i8_find(one, (int)slot, x)) {
+    const int32_t* table = a.block_tables + x.b * a.bt_stride;
+    const int nb = (x.seq.kv + kBlockSize - 1) / kBlockSize;
+    const int b0 = i8_split_begin(nb, x.split, x.splits), b1 = i8_split_begin(nb, x.split + 1, x.splits);
+    const int name[6] = {x.b, x.split, x.splits, x.seq.kv, b0, b1};
+    if (lane >= I4Map::kIds && lane < I4Map::kIds + kI8SplitBlocks && b0 + lane - I4Map::kIds < b1)
+      v = clamp_block(table[b0 + lane - I4Map::kIds], a.num_blocks);
+    if (lane == 6 && nb > 0) v = clamp_block(table[nb - 1], a.num_blocks);
+#pragma unroll
+    for (int i = 0; i < 6; ++i) v = lane == i ? name[i] : v;
+  }
+  if (lane < I4Map::kEntry) const_cast<int*>(map.entry((int)slot))[lane] = v;
+}
+
+// decode_int4_kernel for a step with a map: decode rows only. A workgroup has its split and block ids one
+// load after it starts, and the last split of a row tile to finish merges all of them, so that no
+// launch follows.
+template <int D>
+__global__ void __launch_bounds__(kI8Threads, i8_decode_groups(D))
+decode_int4_mapped_kernel(Int8DecodeArgs a, I4Map map, I8Div by_units) {
+  __shared__ __align__(16) I8DecodeLds<D> lds;
+  __shared__ int s_last;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int lane = threadIdx.x % kWave, c = lane % 16, g = lane / 16;
+  const int tiles = (a.group + 15) / 16, units = a.kvh * tiles;
+  if (!map.names(a)) {                                     // built for another plan: every row is NaN
+    const half_t nan = (half_t)__builtin_nanf("");
+    for (int64_t row = blockIdx.x; row < a.num_seqs; row += gridDim.x)
+      for (int i = threadIdx.x; i < a.heads * D; i += kI8Threads) a.out[row * a.out_st + i] = nan;
+    return;
+  }
+  const int64_t slots = I4Map::entries(a.num_seqs, a.max_splits);
+  for (int64_t u = blockIdx.x; u < slots * units; u += gridDim.x) {
+    const int slot = by_units((int)u), unit = (int)u - slot * units;
+    const int h = tiles == 1 ? unit : unit / tiles, tile = tiles == 1 ? 0 : unit - h * tiles;
+    const int* e = map.entry(slot);
+    const int b = table_entry(e), split = table_entry(e + 1), splits = table_entry(e + 2);
+    const int kv = table_entry(e + 3), b0 = table_entry(e + 4), b1 = table_entry(e + 5), last = table_entry(e + 6);
+    if (b < 0) return;
+    const int row0 = 16 * tile, rows = min(a.group - row0, 16);
+    I8Query<D> q;
+    i4_load_q<D>(a.q + (int64_t)b * a.q_st + (int64_t)(h * a.group + row0 + min(c, rows - 1)) * a.q_sh, g, c < rows, q);
+    // a map of an earlier step: the sequence's length or its last block have moved
+    const int len = i8_kv_len(a.seq_lens[b], a.max_blocks);
+    const int end = kv > 0 ? clamp_block(a.block_tables[b * a.bt_stride + (kv - 1) / kBlockSize], a.num_blocks) : last;
+    I8State<D> st;
+    st.m = -INFINITY, st.l = 0.f;
+#pragma unroll
+    for (int t = 0; t < D / 16; ++t) st.o[t] = {0.f, 0.f, 0.f, 0.f};
+    i4_split<D, true>(a, st, q, b, h, b0, b1, kv, kv, kv, wave, e + I4Map::kIds);
+    if (len != kv || end != last) st.m = __builtin_nanf("");
+    if (splits == 1) {
+      i8_finish<D, 1>(a, st, b, h, b, row0, rows, 0, 1, wave, lds.o, lds.ml);
+      continue;
+    }
+    // device-coherent partials: another workgroup, of any XCD, may merge them
+    const int64_t base = ((int64_t)(b * a.kvh + h) * a.group + row0) * a.max_splits;
+    const auto r_o = coherent_rsrc(a.part_o + base * D), r_ml = coherent_rsrc(a.part_ml + base * 2);
+    i8_meet<D, 1>(st, rows, wave, lds.o, lds.ml, [&](int row, int d, float4_t o, float top, float sum) {
+      const int at = row * a.max_splits + split;
+      coherent_store4(r_o, (at * D + d) * 4, o);
+      if (d == 0) coherent_store(r_ml, at * 8, top), coherent_store(r_ml, at * 8 + 4, sum);
+    });
+    __builtin_amdgcn_s_waitcnt(kWaitVmcntZero);            // they have arrived before the workgroup counts
+    __syncthreads();
+    int* counter = map.counter(a, b, h, tile);
+    if (threadIdx.x == 0)
+      s_last = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == splits - 1;
+    __syncthreads();
+    if (!s_last) continue;
+    int id = threadIdx.x;                                  // (so that nothing of this is worked out ahead, and held)
+    asm volatile("" : "+v"(id));
+#pragma unroll 1
+    for (; id < rows * (D / 4); id += kI8Threads) {
+      const int row = id / (D / 4), d = id % (D / 4) * 4;
+      float sum;
+      const float4_t o = i4_merge(splits, [&](int k, float& m, float& l, float4_t& x) {
+        const int at = row * a.max_splits + k;
+        m = coherent_load(r_ml, at * 8), l = coherent_load(r_ml, at * 8 + 4), x = coherent_load4(r_o, (at * D + d) * 4);
+      }, sum);
+      const float f = sum == 0.f ? 0.f : 1.f / sum;
+      ts::st<half4_t>(a.out + (int64_t)b * a.out_st + (int64_t)(h * a.group + row0 + row) * D + d, to_half4(o * f));
+    }
+    if (threadIdx.x == 0) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
 }
 

@@ -397,11 +397,11 @@ struct I8DecodeLds {
   float ml[2 * kI8Waves * 16];
 };
 
-// The four wavefronts' states (O in units of 1 / UNIT) meet in LDS; the row (or its partial) is written.
-template <int D, int UNIT>
-__device__ __forceinline__ void i8_finish(const Int8DecodeArgs& a, I8State<D>& st, int b, int h,
-                                          int q0, int row0, int rows, int split, int splits, int wave,
-                                          float* s_o, float* s_ml) {
+// The four wavefronts' states (O in units of 1 / UNIT) meet in LDS: emit(row, d, o, reference, sum) for 4 dims
+// of each row, unnormalised.
+template <int D, int UNIT, typename Emit>
+__device__ __forceinline__ void i8_meet(const I8State<D>& st, int rows, int wave, float* s_o, float* s_ml,
+                                        Emit emit) {
   constexpr int VW = D / 16;
   const int lane = threadIdx.x % kWave, c = lane % 16, g = lane / 16;
   const float l = rows_sum(st.l);
@@ -432,6 +432,16 @@ __device__ __forceinline__ void i8_finish(const Int8DecodeArgs& a, I8State<D>& s
       o += ld<float4_t>(s_o + (w * 16 + row) * I8DecodeLds<D>::ROW + d) * f;
     }
     o *= (float)UNIT;
+    emit(row, d, o, top, sum);
+  }
+}
+
+// The row (or its partial) is written.
+template <int D, int UNIT>
+__device__ __forceinline__ void i8_finish(const Int8DecodeArgs& a, I8State<D>& st, int b, int h,
+                                          int q0, int row0, int rows, int split, int splits, int wave,
+                                          float* s_o, float* s_ml) {
+  i8_meet<D, UNIT>(st, rows, wave, s_o, s_ml, [&](int row, int d, float4_t o, float top, float sum) {
     if (splits == 1) {
       const float f = sum == 0.f ? 0.f : 1.f / sum;        // no visible key: zeros
       const int token = a.by_group(row0 + row), head = h * a.group + row0 + row - token * a.group;
@@ -444,7 +454,7 @@ __device__ __forceinline__ void i8_finish(const Int8DecodeArgs& a, I8State<D>& s
         a.part_ml[2 * at + 1] = sum;
       }
     }
-  }
+  });
 }
 
 // Item `item` of the batch's (split, row tile) pairs, numbered densely over the sequences. Every

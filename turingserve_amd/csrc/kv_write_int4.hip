@@ -6,8 +6,9 @@
 // more than the largest value (the nearest one could leave the fp16 range at 65504); that costs at most
 // 15 units in the step's last place, 0.015 of a step, where a code is off by half of one.
 //
-// A thread holds the octets o and o + D / 16 of a row of K and of V, D / 16 threads a row: the rotation's
-// pairs in one thread, the groups' extremes over 4 neighbouring lanes at most.
+// A thread holds an octet of a row of K or of V, those of a (token, KV head) side by side in a wavefront: a
+// group's extremes come over 4 neighbouring lanes, a rotation's partner from a second load, and whether
+// the row is finite from a ballot. q (RoPE form) is rotated by the rest of the grid, two octets a thread.
 #include "int4_kv.h"
 #include "decode_int8.h"
 #include "rope.h"
@@ -22,8 +23,8 @@ struct Int4WriteArgs {
   uint8_t *kc, *vc;
   int64_t num_blocks;
   const int64_t* slots;
-  int num_tokens, kvh, units;             // units a token: q heads in the RoPE form, then KV heads
-  I8Div by_units;
+  int num_tokens, kvh;
+  I8Div by_kvh;
   // RoPE form
   const half_t* q;
   int64_t q_st;
@@ -31,180 +32,177 @@ struct Int4WriteArgs {
   const int64_t* positions;
   const float *cos_t, *sin_t;
   int64_t max_pos;
-  int heads;
+  int heads, kv_groups;                   // workgroups before the first of q
+  I8Div by_heads;
 };
 
-// Smallest and largest of a group: over the lane's octets that belong to it, then over its lanes.
-struct I4Span {
-  float lo, hi;
-  __device__ __forceinline__ void add(float x) { lo = fminf(lo, x), hi = fmaxf(hi, x); }
-  template <int MASK>
-  __device__ __forceinline__ void meet() {
-    lo = fminf(lo, shfl_xor(lo, MASK)), hi = fmaxf(hi, shfl_xor(hi, MASK));
+struct I4Rotation {
+  float4_t c[2], n[2];                    // cosines and sines of 8 pairs
+  __device__ __forceinline__ void load(const Int4WriteArgs& a, int t, int half_dim, int at) {
+    const int64_t pos = rope_row(a.positions[t], a.max_pos) * half_dim + at;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      c[i] = ld<float4_t>(a.cos_t + pos + 4 * i), n[i] = ld<float4_t>(a.sin_t + pos + 4 * i);
   }
 };
 
-struct I4Numbers {
-  half_t step, low;
-};
-__device__ __forceinline__ I4Numbers i4_numbers(const I4Span& s) {
-  I4Numbers n;
-  n.low = (half_t)(s.lo + 0.f);                            // (-0 as 0)
-  const float span = fmaxf(s.hi - (float)n.low, 0.f) / 15.f;
-  half_t step = (half_t)span;
-  if ((float)step > span) step = __builtin_bit_cast(half_t, (uint16_t)(__builtin_bit_cast(uint16_t, step) - 1));
-  n.step = step;
-  return n;
+// Over the lanes of a group (LANES of a quad), on the VALU.
+template <int CTRL>
+__device__ __forceinline__ float i4_quad(float x) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true));
 }
-__device__ __forceinline__ uint32_t i4_word(const float (&x)[8], I4Numbers n) {
-  const float low = (float)n.low, step = (float)n.step;
+
+// rint((x - low) / step) within 0 .. 15 of 8 channels, as an octet's word. By the reciprocal where that
+// decides it: the quotient is below 31 (a subnormal step may be little more than half the span's fifteenth), the
+// product with v_rcp_f32's result (one unit in the last place) within 31 * 1.5 * 2^-23 < 2^-17 of it, so it
+// rounds alike unless it lies that close to a half; then the division is made.
+__device__ __forceinline__ uint32_t i4_word(const float (&x)[8], float low, float step) {
+  const float rcp = __builtin_amdgcn_rcpf(step);           // (steps are 2^-24 at least, or 0)
   uint32_t w = 0;
-  if (step > 0.f) {
+  float worst = 0.f;
 #pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float y = (x[e] - low) * rcp, c = rintf(y);
+    worst = fmaxf(worst, fabsf(y - c));
+    w |= (uint32_t)(int)__builtin_amdgcn_fmed3f(c, 0.f, 15.f) << 4 * (e / 2 + 4 * (e % 2));
+  }
+  if (worst > 0.5f - 1.f / 65536.f) {
+    w = 0;
+#pragma unroll 1
     for (int e = 0; e < 8; ++e) {
-      const float c = fminf(fmaxf(rintf((x[e] - low) / step), 0.f), 15.f);
+      float v = x[0];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) v = i == e ? x[i] : v;
+      const float c = fminf(fmaxf(rintf((v - low) / step), 0.f), 15.f);
       w |= (uint32_t)(int)c << 4 * (e / 2 + 4 * (e % 2));
     }
   }
-  return w;
+  return step > 0.f ? w : 0;
 }
 
-__device__ __forceinline__ void i4_load8(const half_t* p, float (&x)[8]) {
-  const half8_t h = ld<half8_t>(p);
-#pragma unroll
-  for (int e = 0; e < 8; ++e) x[e] = (float)h[e];
-}
-
-// The two octets of a row of K (or V), `at` lanes from the row's first one, as codes and numbers.
-template <int D, bool VALUES>
-__device__ __forceinline__ void i4_store_row(uint8_t* unit, int row, int at, const float (&x)[8],
-                                             const float (&y)[8], bool bad) {
+template <int D, bool ROPE>
+__device__ __forceinline__ void i4_write_kv(const Int4WriteArgs& a) {
   typedef I4Unit<D> U;
-  constexpr int HALF = D / 16;                             // octets of half a row, lanes of a row
-  I4Span s = {INFINITY, -INFINITY}, t = {INFINITY, -INFINITY};
+  constexpr int OCTETS = D / 8, LANES = U::GROUP / 8, PER = 2 * OCTETS;   // lanes of a group, of a (token, head)
+  const int item = (int)(blockIdx.x * (kI4Threads / PER) + threadIdx.x / PER), in = threadIdx.x % PER;
+  const int t = a.by_kvh(item), h = item - t * a.kvh, side = in / OCTETS, octet = in % OCTETS;
+  if (t >= a.num_tokens) return;                           // (all lanes of an item)
+  const int64_t slot = a.slots[t];
+  const half_t* row = side == 0 ? a.k + t * a.k_st + h * a.k_sh : a.v + t * a.v_st + h * a.v_sh;
+  const half8_t own = ld<half8_t>(row + 8 * octet);
+  float x[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) s.add(x[e]), (D >= 64 ? t : s).add(y[e]);
-  constexpr int LANES = HALF < 4 ? HALF : 4;               // of a group
-  if constexpr (LANES > 1) s.template meet<1>(), t.template meet<1>();
-  if constexpr (LANES > 2) s.template meet<2>(), t.template meet<2>();
-  I4Numbers n = i4_numbers(s), m = D >= 64 ? i4_numbers(t) : n;
-  uint32_t a = i4_word(x, n), b = i4_word(y, m);
-  if (bad) {
-    a = b = 0;
-    n = m = {(half_t)0.f, (half_t)__builtin_nanf("")};
-  }
-  *reinterpret_cast<uint32_t*>(unit + (VALUES ? U::v_word(row, at) : U::k_word(row, at))) = a;
-  *reinterpret_cast<uint32_t*>(unit + (VALUES ? U::v_word(row, at + HALF) : U::k_word(row, at + HALF))) = b;
-  if (at % LANES) return;
+  for (int e = 0; e < 8; ++e) x[e] = (float)own[e];
+  if (ROPE && side == 0) {
+    // in 64 bits, where the products are exact, rounded once to 32: a quotient's last bits decide a code
+    const half8_t other = ld<half8_t>(row + 8 * (octet ^ (OCTETS / 2)));
+    I4Rotation r;
+    r.load(a, t, D / 2, 8 * (octet % (OCTETS / 2)));
+    const double sign = octet < OCTETS / 2 ? -1.0 : 1.0;
 #pragma unroll
-  for (int i = 0; i < (D >= 64 ? 2 : 1); ++i) {
-    const int group = at / LANES + i * (U::GROUPS / 2);
-    const I4Numbers z = i == 0 ? n : m;
-    if constexpr (VALUES) {
-      *reinterpret_cast<half_t*>(unit + U::v_numbers(row, group)) = z.step;
-      *reinterpret_cast<half_t*>(unit + U::v_numbers(row, group) + 8) = z.low;
-    } else {
-      st<half2_t>(unit + U::k_numbers(row, group), half2_t{z.step, z.low});
-    }
+    for (int e = 0; e < 8; ++e)
+      x[e] = (float)fma((double)(float)other[e] * sign, (double)r.n[e / 4][e % 4],
+                        (double)x[e] * (double)r.c[e / 4][e % 4]);
   }
-}
-
-__device__ __forceinline__ bool i4_not_fp16(const float (&x)[8]) {
+  float lo = x[0], hi = x[0];
   bool bad = false;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) bad = bad || !(fabsf(x[e]) <= 65504.f);
-  return bad;
+  for (int e = 0; e < 8; ++e) {
+    lo = fminf(lo, x[e]), hi = fmaxf(hi, x[e]);
+    bad = bad || !(fabsf(x[e]) <= 65504.f);
+  }
+  if constexpr (LANES > 1) lo = fminf(lo, i4_quad<0xb1>(lo)), hi = fmaxf(hi, i4_quad<0xb1>(hi));   // 1 0 3 2
+  if constexpr (LANES > 2) lo = fminf(lo, i4_quad<0x4e>(lo)), hi = fmaxf(hi, i4_quad<0x4e>(hi));   // 2 3 0 1
+  const uint64_t lost = __ballot(bad), mine = PER == kWave ? ~0ull : ((1ull << PER % kWave) - 1)
+                                                                       << (threadIdx.x % kWave / PER * PER);
+  half_t low = (half_t)(lo + 0.f);                         // (-0 as 0)
+  const float span = fmaxf(hi - (float)low, 0.f) / 15.f;
+  half_t step = (half_t)span;
+  if ((float)step > span) step = __builtin_bit_cast(half_t, (uint16_t)(__builtin_bit_cast(uint16_t, step) - 1));
+  uint32_t w = i4_word(x, (float)low, (float)step);
+  if (lost & mine) w = 0, step = (half_t)0.f, low = (half_t)__builtin_nanf("");
+  if (slot < 0 || slot >= a.num_blocks * kBlockSize) return;
+  const int64_t unit = ((slot / kBlockSize) * a.kvh + h) * U::BYTES;
+  const int at = (int)(slot % kBlockSize), group = octet / LANES;
+  if (side == 0) {
+    st<uint32_t>(a.kc + unit + U::k_word(at, octet), w);
+    if (octet % LANES == 0) st<half2_t>(a.kc + unit + U::k_numbers(at, group), half2_t{step, low});
+  } else {
+    st<uint32_t>(a.vc + unit + U::v_word(at, octet), w);
+    if (octet % LANES == 0) {
+      st<half_t>(a.vc + unit + U::v_numbers(at, group), step);
+      st<half_t>(a.vc + unit + U::v_numbers(at, group) + 8, low);
+    }
+  }
 }
 
 template <int D, bool ROPE>
 __global__ void __launch_bounds__(kI4Threads) kv_write_int4_kernel(Int4WriteArgs a) {
-  constexpr int HALF = D / 16;
-  const int64_t id = (int64_t)blockIdx.x * kI4Threads + threadIdx.x;
-  const int item = (int)(id / HALF), at = (int)(id % HALF);
-  const int t = a.by_units(item), u = item - t * a.units;
-  if (t >= a.num_tokens) return;                           // (whole rows: HALF divides the workgroup)
-  float c[8], n[8];
+  if (!ROPE || (int)blockIdx.x < a.kv_groups) return i4_write_kv<D, ROPE>(a);
   if constexpr (ROPE) {
-    const int64_t pos = rope_row(a.positions[t], a.max_pos) * (D / 2) + 8 * at;
-    const float4_t c0 = ld<float4_t>(a.cos_t + pos), c1 = ld<float4_t>(a.cos_t + pos + 4);
-    const float4_t n0 = ld<float4_t>(a.sin_t + pos), n1 = ld<float4_t>(a.sin_t + pos + 4);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) c[e] = c0[e], c[4 + e] = c1[e], n[e] = n0[e], n[4 + e] = n1[e];
-  }
-  if (ROPE && u < a.heads) {
-    const half_t* src = a.q + t * a.q_st + (int64_t)u * D + 8 * at;
-    half_t* dst = a.q_out + ((int64_t)t * a.heads + u) * D + 8 * at;
-    float x[8], y[8];
-    i4_load8(src, x), i4_load8(src + D / 2, y);
-    half8_t p, r;
+    constexpr int PER = D / 16;
+    const int item = (int)((blockIdx.x - a.kv_groups) * (kI4Threads / PER) + threadIdx.x / PER);
+    const int t = a.by_heads(item), h = item - t * a.heads, at = 8 * (threadIdx.x % PER);
+    if (t >= a.num_tokens) return;
+    const half_t* src = a.q + t * a.q_st + (int64_t)h * D + at;
+    half_t* dst = a.q_out + ((int64_t)t * a.heads + h) * D + at;
+    const half8_t x = ld<half8_t>(src), y = ld<half8_t>(src + D / 2);
+    I4Rotation r;
+    r.load(a, t, D / 2, at);
+    half8_t p, s;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {                          // in fp32, rounded once
-      p[e] = (half_t)fmaf(-y[e], n[e], x[e] * c[e]);
-      r[e] = (half_t)fmaf(x[e], n[e], y[e] * c[e]);
+      const float f = (float)x[e], g = (float)y[e], c = r.c[e / 4][e % 4], n = r.n[e / 4][e % 4];
+      p[e] = (half_t)fmaf(-g, n, f * c);
+      s[e] = (half_t)fmaf(f, n, g * c);
     }
     st(dst, p);
-    st(dst + D / 2, r);
-    return;
+    st(dst + D / 2, s);
   }
-  const int h = ROPE ? u - a.heads : u;
-  const int64_t slot = a.slots[t];
-  const half_t* k = a.k + t * a.k_st + h * a.k_sh + 8 * at;
-  const half_t* v = a.v + t * a.v_st + h * a.v_sh + 8 * at;
-  float x[8], y[8], z[8], w[8];
-  i4_load8(k, x), i4_load8(k + D / 2, y);
-  i4_load8(v, z), i4_load8(v + D / 2, w);
-  if (ROPE) {
-    // in 64 bits, where the products are exact, rounded once to 32: a quotient's last bits decide a code
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const double f = x[e], g = y[e], cc = c[e], nn = n[e];
-      x[e] = (float)fma(-g, nn, f * cc);
-      y[e] = (float)fma(f, nn, g * cc);
-    }
-  }
-  int bad = i4_not_fp16(x) || i4_not_fp16(y) || i4_not_fp16(z) || i4_not_fp16(w);
-#pragma unroll
-  for (int m = 1; m < HALF; m <<= 1) bad |= __shfl_xor(bad, m, kWave);
-  const bool inside = slot >= 0 && slot < a.num_blocks * kBlockSize;
-  if (!inside) return;                                     // (all lanes of a row)
-  const int64_t unit = ((slot / kBlockSize) * a.kvh + h) * I4Unit<D>::BYTES;
-  const int row = (int)(slot % kBlockSize);
-  i4_store_row<D, false>(a.kc + unit, row, at, x, y, bad);
-  i4_store_row<D, true>(a.vc + unit, row, at, z, w, bad);
 }
 
 struct Int4ReadArgs {
   const uint8_t* cache;
   const int32_t* blocks;
   half_t* out;
-  int64_t num_blocks, layer_blocks;       // (layer, K or V) pairs times blocks asked for
-  int n, kvh;
+  int64_t num_blocks;
+  int n, kvh, units;                      // blocks asked for; units of the result
+  I8Div by_n, by_kvh;
 };
 
-// One thread an octet: 16 bytes of fp16 from one word and its numbers.
+// Sixteen bytes of a V unit are an octet of four rows, so a thread takes an octet of four rows: of K a word a
+// row (consecutive lanes have consecutive words, and the rows of a request follow one another), of V all of
+// them at once. D / 2 threads a unit; every store is 16 bytes, of whole rows.
 template <int D>
 __global__ void __launch_bounds__(kI4Threads) kv_read_int4_kernel(Int4ReadArgs a) {
   typedef I4Unit<D> U;
-  constexpr int PER = kBlockSize * D / 8;                  // octets of a unit
-  const int64_t id = (int64_t)blockIdx.x * kI4Threads + threadIdx.x;
-  const int64_t unit = id / PER;                           // of the output: ((layer, side), block, head)
-  const int in = (int)(id % PER), row = in / (D / 8), octet = in % (D / 8);
-  const int64_t lb = unit / a.kvh;
-  const int h = (int)(unit - lb * a.kvh);
-  if (lb >= a.layer_blocks) return;
-  const int64_t side = lb / a.n;
+  constexpr int PER = D / 2, OCTETS = D / 8;
+  const int unit = (int)(blockIdx.x * (kI4Threads / PER) + threadIdx.x / PER), in = threadIdx.x % PER;
+  if (unit >= a.units) return;
+  const int lb = a.by_kvh(unit), h = unit - lb * a.kvh;    // (layer, K or V) and block; head
+  const int side = a.by_n(lb);
   const int blk = clamp_block(a.blocks[lb - side * a.n], a.num_blocks);
-  const uint8_t* src = a.cache + ((side * a.num_blocks + blk) * a.kvh + h) * U::BYTES;
-  const int group = octet * 8 / U::GROUP;
-  uint32_t w, n;
-  if (side % 2 == 0) {
-    w = ld<uint32_t>(src + U::k_word(row, octet));
-    n = ld<uint32_t>(src + U::k_numbers(row, group));
+  const uint8_t* src = a.cache + (((int64_t)side * a.num_blocks + blk) * a.kvh + h) * U::BYTES;
+  half_t* dst = a.out + (int64_t)unit * (kBlockSize * D);
+  const int quad = in / OCTETS, octet = in % OCTETS, group = 8 * octet / U::GROUP;
+  uint32_t w[4], n[4];
+  const bool is_v = side & 1;
+  if (!is_v) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      w[r] = ld<uint32_t>(src + U::k_word(4 * r + quad, octet));
+      n[r] = ld<uint32_t>(src + U::k_numbers(4 * r + quad, group));
+    }
   } else {
-    w = ld<uint32_t>(src + U::v_word(row, octet));
-    n = ld<uint16_t>(src + U::v_numbers(row, group)) | (uint32_t)ld<uint16_t>(src + U::v_numbers(row, group) + 8) << 16;
+    const uint4_t v = ld<uint4_t>(src + U::v_word(4 * quad, octet)), m = ld<uint4_t>(src + U::v_numbers(4 * quad, group));
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      w[r] = v[r];
+      n[r] = __builtin_amdgcn_perm(m[2 + r / 2], m[r / 2], r % 2 ? 0x07060302u : 0x05040100u);   // step, low
+    }
   }
-  st<half8_t>(a.out + id * 8, i4_octet(w, n));
+#pragma unroll
+  for (int r = 0; r < 4; ++r) st<half8_t>(dst + (is_v ? 4 * quad + r : 4 * r + quad) * D + 8 * octet, i4_octet(w[r], n[r]));
 }
 
 static bool int4_head_dim(int D) { return D == 16 || D == 32 || D == 64 || D == 128 || D == 256; }
@@ -231,8 +229,13 @@ static int write_int4(Int4WriteArgs a, bool rope, int64_t num_tokens, int D, con
   const int64_t units = (rope ? (int64_t)a.heads : 0) + a.kvh;
   TS_REQUIRE(units < (1ll << 30) && num_tokens < (1ll << 30) / units, TS_ERR_UNSUPPORTED,
              "%s: %lld tokens of %lld heads", what, (long long)num_tokens, (long long)units);
-  a.num_tokens = (int)num_tokens, a.units = (int)units, a.by_units = I8Div::by((int)units);
-  const int64_t grid = (num_tokens * units * (D / 16) + kI4Threads - 1) / kI4Threads;
+  a.num_tokens = (int)num_tokens, a.by_kvh = I8Div::by(a.kvh);
+  a.kv_groups = (int)((num_tokens * a.kvh * (D / 4) + kI4Threads - 1) / kI4Threads);
+  int64_t grid = a.kv_groups;
+  if (rope) {
+    a.by_heads = I8Div::by(a.heads);
+    grid += (num_tokens * a.heads * (D / 16) + kI4Threads - 1) / kI4Threads;
+  }
   TS_REQUIRE(grid < (1ll << 31), TS_ERR_UNSUPPORTED, "%s: %lld workgroups", what, (long long)grid);
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   switch (D) {
@@ -301,12 +304,11 @@ extern "C" int ts_kv_read_int4(const void* cache, int32_t num_layers, int64_t nu
   TS_REQUIRE(int4_head_dim(head_dim), TS_ERR_UNSUPPORTED, "kv_read_int4: head_dim %d (16, 32, 64, 128, 256)", head_dim);
   TS_REQUIRE(aligned(cache, 16) && aligned(out, 16), TS_ERR_INVALID_ARG,
              "kv_read_int4: cache and out must be 16-byte aligned");
-  Int4ReadArgs a = {static_cast<const uint8_t*>(cache), blocks, static_cast<half_t*>(out), num_blocks,
-                    2 * (int64_t)num_layers * n, n, num_kv_heads};
-  const double octets = 4.0 * num_layers * n * num_kv_heads * head_dim;
-  TS_REQUIRE(octets < (double)(1ll << 31) * kI4Threads, TS_ERR_UNSUPPORTED, "kv_read_int4: %d blocks of %d layers", n,
-             num_layers);
-  const unsigned grid = (unsigned)(((int64_t)octets + kI4Threads - 1) / kI4Threads);
+  const double units = 2.0 * num_layers * n * num_kv_heads;
+  TS_REQUIRE(units < (double)(1ll << 30), TS_ERR_UNSUPPORTED, "kv_read_int4: %d blocks of %d layers", n, num_layers);
+  Int4ReadArgs a = {static_cast<const uint8_t*>(cache), blocks, static_cast<half_t*>(out), num_blocks, n,
+                    num_kv_heads, (int)units, I8Div::by(n), I8Div::by(num_kv_heads)};
+  const unsigned grid = (unsigned)(((int64_t)a.units * (head_dim / 2) + kI4Threads - 1) / kI4Threads);
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   switch (head_dim) {
     case 16: kv_read_int4_kernel<16><<<grid, kI4Threads, 0, s>>>(a); break;

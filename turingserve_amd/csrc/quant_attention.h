@@ -1,6 +1,6 @@
 // What the attentions over the quantised paged caches share on the host: how a batch is split between
 // the decode kernel and the prompt kernel, the workspace, the checks and the launches. The formats'
-// kernels come in as a class `Kernels` with decode<D>(args, rows, cus, stream) and
+// kernels come in as a class `Kernels` with decode<D>(args, rows, cus, split map, stream) and
 // prefill<D>(args, stream).
 #pragma once
 
@@ -116,6 +116,7 @@ struct QuantCall {
   void* workspace;
   size_t workspace_bytes;
   void* stream;
+  void* split_map;                       // (the 4-bit cache's, checked by its entry point)
 };
 
 static size_t quant_workspace_bytes(int num_seqs, int num_decode, int max_query_len, int max_seq_len,
@@ -194,11 +195,11 @@ static int quant_attention(const char* what, const QuantCall& c) {
     a.part_ml = reinterpret_cast<float*>(ws + pl.dec_ml);
     const int64_t rows = merge_rows(pl, c.num_decode, c.heads, c.kvh);
     switch (c.head_dim) {
-      case 16: Kernels::template decode<16>(a, rows, cus, s); break;
-      case 32: Kernels::template decode<32>(a, rows, cus, s); break;
-      case 64: Kernels::template decode<64>(a, rows, cus, s); break;
-      case 128: Kernels::template decode<128>(a, rows, cus, s); break;
-      default: Kernels::template decode<256>(a, rows, cus, s); break;
+      case 16: Kernels::template decode<16>(a, rows, cus, c.split_map, s); break;
+      case 32: Kernels::template decode<32>(a, rows, cus, c.split_map, s); break;
+      case 64: Kernels::template decode<64>(a, rows, cus, c.split_map, s); break;
+      case 128: Kernels::template decode<128>(a, rows, cus, c.split_map, s); break;
+      default: Kernels::template decode<256>(a, rows, cus, c.split_map, s); break;
     }
     status = check_launch(what);
     if (status != TS_OK) return status;

@@ -79,7 +79,10 @@ def int4_unit_bytes(head_dim: int) -> int:
 
 def int4_head_dim(unit_bytes: int) -> int | None:
     """The head_dim of a 4-bit cache by its units' bytes (None: of no such cache)."""
-    return next((d for d in (16, 32, 64, 128, 256) if int4_unit_bytes(d) == unit_bytes), None)
+    return _INT4_DIMS.get(unit_bytes)
+
+
+_INT4_DIMS = {int4_unit_bytes(d): d for d in (16, 32, 64, 128, 256)}
 
 
 def int4_quantise(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
