@@ -30,9 +30,8 @@
  *   ts_silu_mul            <- ops/triton_silu_mul.py:21-28  (twin ops/reference.py:26-28)
  *   ts_kv_write_int8, ts_rope_kv_write_int8, ts_paged_attention_int8  the write and the attention of
  *                             a K/V cache held in 8 bits (no counterpart in the reference)
- *   ts_kv_write_int4, ts_rope_kv_write_int4, ts_kv_read_int4, ts_decode_split_map_int4,
- *   ts_paged_attention_int4   the same of one held in 4 bits, and its blocks as fp16 (no counterpart
- *                             either)
+ *   ts_kv_write_int4, ts_rope_kv_write_int4, ts_kv_read_int4, ts_paged_attention_int4  the same of one
+ *                             held in 4 bits, and its blocks as fp16 (no counterpart either)
  *
  * Conventions shared by every entry point
  *  - Plain pointers to device memory; the caller owns every buffer. The library never
@@ -648,27 +647,7 @@ int ts_kv_read_int4(const void* cache, int32_t num_layers, int64_t num_blocks, i
  * on the rest of the batch given max_seq_len. The host bounds shape the launch only: bounds below the
  * batch's real values are slower, not wrong. head_dims, heads, alignment, limits and the workspace as for
  * ts_paged_attention_int8. Rows of no sequence are not written.
- *
- * split_map / split_map_bytes: NULL / 0, or, for a step of decode rows alone, a map that
- * ts_decode_split_map_int4 built from the same seq_lens, block tables, num_seqs, heads, head_dim,
- * max_seq_len and max_blocks_per_seq: the launch then reads its splits and block ids from it and merges
- * its own splits (no launch follows); the results are the same bits. A map built for other sizes poisons
- * the rows (NaN), one of an earlier step those whose length or last block have moved; one smaller than
- * the plan needs is an error. Calls that share a map must not overlap in time (its counters are
- * shared; one stream orders them).
- *
- * ts_decode_split_map_int4: such a map, once a step (one launch), after seq_lens and the tables are final.
- * ts_decode_split_map_int4_bytes(): its size, 0 where nothing is split or for more than 4096 sequences (no
- * map is built then, and the calls take NULL). 128-byte aligned; it needs no initialisation.
  */
-size_t ts_decode_split_map_int4_bytes(int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads,
-                                      int32_t head_dim, int32_t max_seq_len);
-
-int ts_decode_split_map_int4(const int32_t* block_tables, int64_t bt_stride, int32_t max_blocks_per_seq,
-                             int64_t num_blocks, const int32_t* seq_lens, int32_t num_seqs,
-                             int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
-                             int32_t max_seq_len, void* split_map, size_t split_map_bytes, void* stream);
-
 size_t ts_paged_attention_int4_workspace_bytes(int32_t num_seqs, int32_t num_decode,
                                                int32_t max_query_len, int32_t max_seq_len,
                                                int32_t max_prefill_seq_len, int32_t num_heads,
@@ -682,8 +661,7 @@ int ts_paged_attention_int4(const void* q, int64_t q_stride_t, int64_t q_stride_
                             const int32_t* query_start_loc, int32_t num_seqs, int32_t num_decode,
                             int32_t max_query_len, int32_t max_seq_len, int32_t max_prefill_seq_len,
                             int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, float scale,
-                            void* workspace, size_t workspace_bytes, void* stream, void* split_map,
-                            size_t split_map_bytes);
+                            void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

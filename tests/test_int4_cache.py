@@ -179,30 +179,12 @@ def _read(**kw):
 
 def _attend(**kw):
     a = dict(q=P, qst=128, qsh=64, out=P, ost=128, T=1, kc=P, vc=P, nb=4, bt=P, bts=4, mb=4, sl=P, qsl=P,
-             seqs=1, dec=0, mq=1, ms=64, mp=64, h=2, kvh=1, D=64, scale=0.125, ws=None, wsb=0,
-             stream=None, map=None, mapb=0)
+             seqs=1, dec=0, mq=1, ms=64, mp=64, h=2, kvh=1, D=64, scale=0.125, ws=None, wsb=0)
     a.update(kw)
-    return N.lib().ts_paged_attention_int4(*a.values())
-
-
-def _map(**kw):
-    a = dict(bt=P, bts=64, mb=64, nb=4, sl=P, seqs=1, h=2, kvh=1, D=64, ms=1024, map=None, mapb=0)
-    a.update(kw)
-    return N.lib().ts_decode_split_map_int4(*a.values(), None)
+    return N.lib().ts_paged_attention_int4(*a.values(), None)
 
 
 @pytest.mark.parametrize("call,kw,status,text", [
-    (_map, dict(seqs=-1), N.TS_ERR_UNSUPPORTED, "sequences"),
-    (_map, dict(seqs=4097), N.TS_ERR_UNSUPPORTED, "4096"),
-    (_map, dict(h=3, kvh=2), N.TS_ERR_INVALID_ARG, "heads"),
-    (_map, dict(D=80), N.TS_ERR_UNSUPPORTED, "head_dim 80"),
-    (_map, dict(sl=None), N.TS_ERR_INVALID_ARG, "null"),
-    (_map, dict(bts=63), N.TS_ERR_INVALID_ARG, "bt_stride"),
-    (_map, dict(), N.TS_ERR_WORKSPACE, "map of 0 bytes"),
-    (_map, dict(map=odd, mapb=1 << 20), N.TS_ERR_WORKSPACE, "aligned"),
-    (_attend, dict(map=P, mapb=1 << 20), N.TS_ERR_INVALID_ARG, "decode rows alone"),
-    (_attend, dict(map=P, mapb=100, dec=1, ms=1024), N.TS_ERR_INVALID_ARG, "split map of 100 bytes"),
-    (_attend, dict(map=odd, mapb=1 << 20, dec=1, ms=1024), N.TS_ERR_INVALID_ARG, "aligned"),
     (_write, dict(T=-1), N.TS_ERR_INVALID_ARG, "num_tokens"),
     (_write, dict(k=None), N.TS_ERR_INVALID_ARG, "null"),
     (_write, dict(slots=None), N.TS_ERR_INVALID_ARG, "null"),
@@ -255,11 +237,6 @@ def test_empty_calls_and_workspace_sizes():
     assert size(64, 64, 1, 256, 0, 12, 2, 128, 256) == 0                 # one split a row
     long = size(4, 4, 1, 32768, 0, 12, 2, 128, 256)
     assert long >= 4 * 12 * 64 * (128 + 2) * 4
-    assert _map(seqs=0) == N.TS_OK and _map(ms=256) == N.TS_OK           # nothing to map
-    size4 = N.lib().ts_decode_split_map_int4_bytes
-    assert size4(1, 2, 1, 64, 256) == 0 and size4(4097, 2, 1, 64, 4096) == 0 and size4(4, 3, 2, 64, 4096) == 0
-    assert size4(64, 12, 2, 128, 4096) == 4 * (32 + 64 * 16 * 32 + 64 * 2)
-    assert size4(64, 40, 2, 128, 1 << 30) == 4 * (32 + 64 * 64 * 32 + 64 * 4)
     # the host's bounds may be anything
     huge = 2 ** 31 - 1
     assert size(64, 0, huge, huge, huge, 64, 8, 128, 256) == size(64, 0, 4096, 65536, 65536, 64, 8, 128, 256)
@@ -350,8 +327,7 @@ def test_cache_container_and_namespaces():
     with pytest.raises(ValueError, match="head_dim 48"):
         Int4KVCache.new(1, 1, 1, 48, "cpu")
     ref, hip = get_ops("reference"), get_ops("hip")
-    for op in ("kv_write_int4", "rope_kv_write_int4", "kv_read_int4", "paged_attention_int4",
-               "decode_split_map_int4"):
+    for op in ("kv_write_int4", "rope_kv_write_int4", "kv_read_int4", "paged_attention_int4"):
         assert getattr(ref, op) is getattr(R, op) and getattr(hip, op) is getattr(H, op)
 
 

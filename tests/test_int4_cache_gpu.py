@@ -34,8 +34,8 @@ def assert_cache(cache, want, what=""):
     assert np.array_equal(got, want), f"{what}: {int((got != want).sum())} bytes differ"
 
 
-def attend(q, cache, meta, scale, **kw):
-    return H.paged_attention_int4(q, cache[0, 0], cache[0, 1], meta, scale, **kw)
+def attend(q, cache, meta, scale):
+    return H.paged_attention_int4(q, cache[0, 0], cache[0, 1], meta, scale)
 
 
 def assert_rows(out, c, what="", rows=slice(None), **kw):
@@ -412,70 +412,9 @@ def test_one_long_prompt_among_many_short_ones(heads):
         assert_rows(attend(q, cache, m, c.scale), c, f"{bounds}", cache=want)
 
 
-def split_map(c, meta):
-    return H.decode_split_map_int4(meta, c.H, c.KVH, c.D, c.NB, DEV)
-
-
-@pytest.mark.parametrize("heads", HEADS + [(300, 1, 16)])
-def test_a_split_map_changes_no_bit(heads):
-    """With the step's map, shared by several calls, and without one; host bounds of all sizes."""
-    c = Case(heads, [(max(n - 1, 0), 1) for n in DECODE_LENS + [0, 20000]], num_decode=18, seed=60)
-    c.lens[16] = 0
-    _, q, _, _, cache, meta = c.on(DEV)
-    assert_rows(attend(q, cache, meta, c.scale), c, f"{heads}")
-    for bound in (20000, 300, 32768, 140000):
-        m = dataclasses.replace(meta, max_seq_len=bound)
-        want = attend(q, cache, m, c.scale)
-        shared = split_map(c, m)
-        for _ in range(3):
-            assert torch.equal(attend(q, cache, m, c.scale, split_map=shared), want), bound
-    assert split_map(c, dataclasses.replace(meta, max_seq_len=256)) is None          # one split a row
-    assert split_map(c, dataclasses.replace(meta, num_decode=17)) is None            # a chunk beside them
-
-
-def test_a_split_map_of_many_sequences():
-    """More entries than one lookup holds, most of them behind the batch's last split."""
-    lens = [(37 * i) % 900 for i in range(400)]
-    c = Case((4, 2, 32), [(max(n - 1, 0), 1) for n in lens], num_decode=400, seed=61)
-    c.lens[:] = lens
-    _, q, _, _, cache, meta = c.on(DEV)
-    m = dataclasses.replace(meta, max_seq_len=30000)
-    out = attend(q, cache, m, c.scale, split_map=split_map(c, m))
-    assert_rows(out, c)
-    assert torch.equal(out, attend(q, cache, m, c.scale))
-
-
-def test_split_maps_of_other_steps_poison():
-    """A map of an earlier step: the rows whose length or last block has moved are NaN, the others right; of
-    another plan: all rows. Afterwards a fresh map, and the old one on the old step, are right again."""
-    c = Case((12, 2, 128), [(n - 1, 1) for n in (300, 4000, 40, 1000)], num_decode=4, seed=62)
-    _, q, _, _, cache, meta = c.on(DEV)
-    want = attend(q, cache, meta, c.scale)
-    old = split_map(c, meta)
-    lens, tables = meta.seq_lens.clone(), meta.block_tables.clone()
-    lens[1] -= 1
-    tables[3, 62] = tables[0, 3]                     # the last of 63 blocks
-    tables[0, 3] = tables[0, 4]                      # (another one than the last: not looked at)
-    moved = dataclasses.replace(meta, seq_lens=lens, block_tables=tables, max_seq_len=meta.max_seq_len)
-    got = attend(q, cache, moved, c.scale, split_map=old)
-    assert got[[1, 3]].isnan().all() and torch.equal(got[[0, 2]], want[[0, 2]])
-    assert torch.equal(attend(q, cache, moved, c.scale, split_map=split_map(c, moved)),
-                       attend(q, cache, moved, c.scale))
-    assert torch.equal(attend(q, cache, meta, c.scale, split_map=old), want)
-    far = dataclasses.replace(meta, max_seq_len=20000)
-    for other in (split_map(c, far), H.decode_split_map_int4(meta, 24, 2, 128, c.NB, DEV)):
-        assert attend(q, cache, meta, c.scale, split_map=other).isnan().all()
-        torch.cuda.synchronize()
-    with pytest.raises(ValueError, match="split map of"):
-        attend(q, cache, far, c.scale, split_map=old)
-    with pytest.raises(ValueError, match="decode rows alone"):
-        attend(q, cache, dataclasses.replace(meta, num_decode=3), c.scale, split_map=old)
-
-
 def test_decode_graph_replayed_over_growing_sequences():
-    """A captured step of two layers (writes, the split map, attention) with max_seq_len of the longest
-    that it may meet, replayed while the lengths grow, with eager calls, with and without a map, between the
-    replays."""
+    """A captured step of two layers (writes, attention) with max_seq_len of the longest that it may meet,
+    replayed while the lengths grow, with eager calls between the replays."""
     c = Case((12, 2, 128), [(0, 600), (0, 600), (0, 600)], seed=24)
     _, kn, vn = c.split()
     _, q, k, v, cache, meta = c.on(DEV)
@@ -486,12 +425,11 @@ def test_decode_graph_replayed_over_growing_sequences():
     step = c.meta(DEV, seq_lens=lens, num_decode=3, max_query_len=1, max_seq_len=600, slot_mapping=slots,
                   query_start_loc=torch.arange(4, dtype=torch.int32, device=DEV))
 
-    def once(mapped=True):
-        shared = split_map(c, step) if mapped else None
+    def once():
         outs = []
         for i in range(2):
             H.kv_write_int4(kk, vv, cache[i, 0], cache[i, 1], slots)
-            outs.append(H.paged_attention_int4(qq, cache[i, 0], cache[i, 1], step, c.scale, split_map=shared))
+            outs.append(H.paged_attention_int4(qq, cache[i, 0], cache[i, 1], step, c.scale))
         return torch.stack(outs)
 
     assert not once().any()                           # lengths 0
@@ -507,7 +445,7 @@ def test_decode_graph_replayed_over_growing_sequences():
         lens.copy_(torch.tensor(now)), slots.copy_(torch.from_numpy(mine))
         graph.replay()
         got = out.clone()
-        assert torch.equal(got, once()) and torch.equal(got, once(False)), now
+        assert torch.equal(got, once()), now
         O.write(kn[rows], vn[rows], *want, mine)
         assert_cache(cache[:1], want, str(now))
         ref, bound = O.paged_attention(c.split()[0][rows], *want, c.tables, now, [0, 1, 2, 3], c.scale)
@@ -607,7 +545,7 @@ def test_rows_behind_the_last_sequence_are_not_written():
             q.data_ptr(), q.stride(0), 64, out.data_ptr(), 256, c.T, cache[0, 0].data_ptr(),
             cache[0, 1].data_ptr(), c.NB, meta.block_tables.data_ptr(), c.tables.shape[1], c.tables.shape[1],
             meta.seq_lens.data_ptr(), meta.query_start_loc.data_ptr(), 2, 1, 130, 230, bound, 4, 2, 64, c.scale,
-            ws.data_ptr(), size, torch.cuda.current_stream().cuda_stream, None, 0), "attention")
+            ws.data_ptr(), size, torch.cuda.current_stream().cuda_stream), "attention")
         assert_rows(out, c)
         assert out[-3:].eq(7).all()
 

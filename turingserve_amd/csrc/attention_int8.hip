@@ -4,8 +4,10 @@
 namespace ts {
 
 struct Int8Kernels {
+  static constexpr int kSplitBlocks = kI8SplitBlocks;
+
   template <int D>
-  static void decode(const Int8DecodeArgs& a, int64_t rows, int cus, void*, hipStream_t s) {
+  static void decode(const Int8DecodeArgs& a, int64_t rows, int cus, hipStream_t s) {
     // Every split of the batch, at most as many workgroups as the CUs hold; the rest go round.
     const int64_t most = a.num_seqs > a.num_decode ? INT32_MAX : (int64_t)a.num_decode * a.max_splits;
     const int64_t units = most * a.kvh * ((a.group + 15) / 16);
@@ -33,7 +35,7 @@ extern "C" size_t ts_paged_attention_int8_workspace_bytes(int32_t num_seqs, int3
                                                           int32_t max_prefill_seq_len,
                                                           int32_t num_heads, int32_t num_kv_heads,
                                                           int32_t head_dim, int32_t cu_count) {
-  return quant_workspace_bytes(num_seqs, num_decode, max_query_len, max_seq_len, max_prefill_seq_len, num_heads,
+  return quant_workspace_bytes<Int8Kernels>(num_seqs, num_decode, max_query_len, max_seq_len, max_prefill_seq_len, num_heads,
                                num_kv_heads, head_dim, cu_count);
 }
 
@@ -54,5 +56,5 @@ extern "C" int ts_paged_attention_int8(const void* q, int64_t q_stride_t, int64_
       {q, q_stride_t, q_stride_h, out, out_stride_t, num_tokens, k_cache, v_cache, k_scale, v_scale, num_blocks,
        block_tables, bt_stride, max_blocks_per_seq, seq_lens, query_start_loc, num_seqs, num_decode, max_query_len,
        max_seq_len, max_prefill_seq_len, num_heads, num_kv_heads, head_dim, scale, workspace, workspace_bytes,
-       stream, nullptr});
+       stream});
 }

@@ -16,6 +16,9 @@
 
 namespace ts {
 
+constexpr int kI4Waves = 4, kI4Threads = kI4Waves * kWave;
+constexpr int kI4SplitBlocks = 16;       // blocks of a split, as long as kI8MaxSplits suffice
+
 // One block's words of a lane (c, g): K of token c, channels (D / 4) g .. of D >= 64 (8 g .. of 32, 4 g ..
 // of 16); V of tokens 4 g + r, channels VW c .. VW c + VW - 1.
 template <int D>
@@ -84,88 +87,74 @@ __device__ __forceinline__ void i4_load_q(const half_t* row, int g, bool real, I
 }
 
 template <int D>
-__device__ __forceinline__ float4_t i4_scores(const I4Block<D>& x, const I8Query<D>& q, int g) {
+__device__ __forceinline__ float4_t i4_scores(const I4Bits& k, const I4Block<D>& x, const I8Query<D>& q, int g) {
   float4_t s = {0.f, 0.f, 0.f, 0.f};
   if constexpr (D >= 32) {
 #pragma unroll
-    for (int i = 0; i < I4Block<D>::KW; ++i) s = mfma16x16x32(i4_octet(x.k[i], x.kn[i / 4]), q.x[i], s);
+    for (int i = 0; i < I4Block<D>::KW; ++i) s = mfma16x16x32(i4_octet(k, x.k[i], x.kn[i / 4]), q.x[i], s);
   } else {
-    const half8_t k = i4_octet(x.k[0] >> (8 * (g & 1)), x.kn[0]);    // (half an octet)
-    s = mfma16x16x16(lo4(k), lo4(q.x[0]), s);
+    s = mfma16x16x16(lo4(i4_octet(k, x.k[0] >> (8 * (g & 1)), x.kn[0])), lo4(q.x[0]), s);   // (half an octet)
   }
   return s;
 }
 
-// V's words of a block ready for the columns: two tokens to a word, even and odd channels apart.
-template <int D>
-struct I4Columns {
-  static constexpr int VO = I4Block<D>::VO;
-  uint32_t w[VO][2][2], w8[VO][2][2];                      // [octet][tokens 0 1, 2 3][even, odd]
-  half2_t step[2], low[2];
-  __device__ __forceinline__ I4Columns(const I4Block<D>& x, int c) {
+// Output tiles 2 P + ODD of an octet, P from 0 on: w the four pairs of tokens (blocks a and b), one channel a
+// nibble.
+template <int D, int ODD, int P>
+__device__ __forceinline__ void i4_tiles(const I4Bits& k, float4_t* o, const uint32_t (&w)[4], const half2_t (&step)[4],
+                                         const half2_t (&low)[4], half8_t p) {
+  if constexpr (2 * P + ODD < D / 16 && P < 4) {
+    half2_t v[4];
 #pragma unroll
-    for (int i = 0; i < VO; ++i) {
-      uint32_t v[4];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        v[r] = x.v[i][r];
-        // the lane's channels first: 4 (c % 2) .., 2 (c % 4) .., c % 8 of the octet
-        if constexpr (D == 64) v[r] >>= 8 * (c & 1);
-        if constexpr (D == 32) v[r] >>= 4 * (c & 3);
-        if constexpr (D == 16) v[r] >>= 4 * (c / 2 & 3) + 16 * (c & 1);
-      }
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        w[i][j][0] = i4_even(v[2 * j], v[2 * j + 1]);
-        w[i][j][1] = i4_odd(v[2 * j], v[2 * j + 1]);
-#pragma unroll
-        for (int o = 0; o < 2; ++o) w8[i][j][o] = w[i][j][o] >> 8;
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < 2; ++j) step[j] = i4_half2(x.vn[j]), low[j] = i4_finite(x.vn[2 + j]);
-  }
-  // Tokens 2 j, 2 j + 1 of the lane's channel t.
-  template <int t>
-  __device__ __forceinline__ half2_t at(int j) const {
-    return i4_values<t % 8 / 2>(w[t / 8][j][t % 2], w8[t / 8][j][t % 2], step[j], low[j]);
-  }
-};
-
-// O^T += V^T . P^T over the pair, output tile t taking channels VW i + t.
-template <int D, int t = 0>
-__device__ __forceinline__ void i4_pv(float4_t (&o)[D / 16], const I4Columns<D>& va, const I4Columns<D>& vb,
-                                      half8_t p) {
-  if constexpr (t < D / 16) {
-    const half2_t a = va.template at<t>(0), b = va.template at<t>(1);
-    const half2_t c = vb.template at<t>(0), d = vb.template at<t>(1);
-    o[t] = mfma16x16x32(half8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]}, p, o[t]);
-    i4_pv<D, t + 1>(o, va, vb, p);
+    for (int i = 0; i < 4; ++i) v[i] = i4_values<P>(k, w[i], w[i] >> 8, step[i], low[i]);
+    const half8_t x = {v[0][0], v[0][1], v[1][0], v[1][1], v[2][0], v[2][1], v[3][0], v[3][1]};
+    o[2 * P + ODD] = mfma16x16x32(x, p, o[2 * P + ODD]);
+    i4_tiles<D, ODD, P + 1>(k, o, w, step, low, p);
   }
 }
 
-// One pair of blocks (tokens ta .. and tb .. of the sequence). A row sees the tokens below `vis`, all
-// rows of the tile those below `least`. sl2: scale * log2(e) > 0.
+// O^T += V^T . P^T over the pair, output tile t taking channels VW i + t: the even channels of an octet, then
+// the odd ones, two tokens to a register.
 template <int D>
-__device__ __forceinline__ void i4_step(I8State<D>& st, const I4Block<D> (&x)[2], const I8Query<D>& q, float sl2,
-                                        int ta, int tb, int vis, int least, int c, int g) {
-  float4_t sa = i4_scores<D>(x[0], q, g), sb = i4_scores<D>(x[1], q, g);
-  if (tb + kBlockSize > least || ta + kBlockSize > least) {
+__device__ __forceinline__ void i4_pv(const I4Bits& k, float4_t (&o)[D / 16], const I4Block<D> (&x)[2], int c,
+                                      half8_t p) {
+  half2_t step[4], low[4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      sa[r] = ta + 4 * g + r < vis ? sa[r] : -INFINITY;
-      sb[r] = tb + 4 * g + r < vis ? sb[r] : -INFINITY;
+  for (int i = 0; i < 4; ++i) step[i] = i4_half2(x[i / 2].vn[i % 2]), low[i] = i4_finite(x[i / 2].vn[2 + i % 2]);
+#pragma unroll
+  for (int j = 0; j < I4Block<D>::VO; ++j) {
+    uint32_t w[4];
+    auto word = [&](int i) {
+      uint32_t v = x[i / 4].v[j][i % 4];
+      // the lane's channels first: 4 (c % 2) .., 2 (c % 4) .., c % 8 of the octet
+      if constexpr (D == 64) v >>= 8 * (c & 1);
+      if constexpr (D == 32) v >>= 4 * (c & 3);
+      if constexpr (D == 16) v >>= 4 * (c / 2 & 3) + 16 * (c & 1);
+      return v;
+    };
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = i4_even(word(2 * i), word(2 * i + 1));
+    i4_tiles<D, 0, 0>(k, o + 8 * j, w, step, low, p);
+    if constexpr (D >= 32) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = i4_odd(word(2 * i), word(2 * i + 1));
+      i4_tiles<D, 1, 0>(k, o + 8 * j, w, step, low, p);
     }
   }
+}
+
+// The softmax of the scores over a pair of blocks: its reference and sum moved on, O with them; P.
+template <int D>
+__device__ __forceinline__ half8_t i4_softmax(I8State<D>& st, const float4_t& sa, const float4_t& sb, float sl2) {
   const float top = rows_max(vmax(vmax(vmax(sa[0], sa[1]), vmax(sa[2], sa[3])),
                                   vmax(vmax(sb[0], sb[1]), vmax(sb[2], sb[3])))) * sl2;
   // !(<=): a NaN score (a token of NaN) moves the reference to NaN, where it stays
-  const bool move = !(top <= st.m + kI8Rescale);
-  if (__ballot(move)) {
-    const float to = vmax(st.m, top);
-    const float alpha = move ? fast_exp2(st.m - to) : 1.f; // m = -inf: 0
+  const float was = st.m;
+  const bool move = !(top <= was + kI8Rescale);
+  st.m = move ? vmax(was, top) : was;
+  if (__ballot(move && was != -INFINITY)) {                // (before a row's first token all is 0)
+    const float alpha = move ? fast_exp2(was - st.m) : 1.f;
     st.l *= alpha;
-    st.m = move ? to : st.m;
 #pragma unroll
     for (int t = 0; t < D / 16; ++t) st.o[t] *= alpha;
   }
@@ -177,64 +166,156 @@ __device__ __forceinline__ void i4_step(I8State<D>& st, const I4Block<D> (&x)[2]
   half8_t p;
 #pragma unroll
   for (int r = 0; r < 4; ++r) p[r] = (half_t)pa[r], p[4 + r] = (half_t)pb[r];
-  // What stands past the end is finite (i4_finite), and p is 0 there.
-  const I4Columns<D> va(x[0], c), vb(x[1], c);
-  i4_pv<D>(st.o, va, vb, p);
+  return p;
 }
 
-// One split [b0, b1) of a sequence's blocks by one wavefront (of kI8Waves). Blocks are taken 64 at a
-// time: lane i holds block i's id; with `known` the first kI8SplitBlocks come from there.
-template <int D, bool KNOWN>
-__device__ __forceinline__ void i4_split(const Int8DecodeArgs& a, I8State<D>& st, const I8Query<D>& q, int b,
-                                         int h, int b0, int b1, int len, int vis, int least, int wave,
-                                         const int* known) {
+// One pair of blocks (tokens ta .. and tb .. of the sequence). A row sees the tokens below `vis`, all
+// rows of the tile those below `least`. sl2: scale * log2(e) > 0. next_k() requests the next pair's K as
+// soon as this one's is used up, next_v() its V.
+template <int D, typename NextK, typename NextV>
+__device__ __forceinline__ void i4_step(const I4Bits& k, I8State<D>& st, const I4Block<D> (&x)[2],
+                                        const I8Query<D>& q, float sl2, int ta, int tb, int vis, int least, int c,
+                                        int g, NextK next_k, NextV next_v) {
+  float4_t sa = i4_scores<D>(k, x[0], q, g), sb = i4_scores<D>(k, x[1], q, g);
+  next_k();
+  if (tb + kBlockSize > least || ta + kBlockSize > least) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      sa[r] = ta + 4 * g + r < vis ? sa[r] : -INFINITY;
+      sb[r] = tb + 4 * g + r < vis ? sb[r] : -INFINITY;
+    }
+  }
+  const half8_t p = i4_softmax<D>(st, sa, sb, sl2);
+  // What stands past the end is finite (i4_finite), and p is 0 there.
+  i4_pv<D>(k, st.o, x, c, p);
+  next_v();
+}
+
+// One split [b0, b1) of a sequence's blocks by one wavefront (of kI4Waves). Blocks are taken 64 at a
+// time: lane i holds block i's id.
+template <int D>
+__device__ __forceinline__ void i4_split(const Int8DecodeArgs& a, I8State<D>& st, const I8Query<D>& q, int b, int h,
+                                         int b0, int b1, int len, int vis, int least, int wave) {
   const int lane = threadIdx.x % kWave, c = lane % 16, g = lane / 16;
   const int32_t* table = a.block_tables + b * a.bt_stride;
   const uint8_t *kc = reinterpret_cast<const uint8_t*>(a.kc), *vc = reinterpret_cast<const uint8_t*>(a.vc);
-  for (int lo = b0, n; lo < b1; lo += n) {
-    const bool first = KNOWN && lo == b0;
-    n = min(b1 - lo, first ? kI8SplitBlocks : kWave);
+  for (int lo = b0; lo < b1; lo += kWave) {
+    const int n = min(b1 - lo, kWave);
     int blk = 0;
-    if (lane < n) blk = clamp_block(first ? known[lane] : table[lo + lane], a.num_blocks);
-    auto load = [&](I4Block<D> (&x)[2], int i) {           // blocks i, i + 1 of the 64
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int id = __builtin_amdgcn_readlane(blk, min(i + u, n - 1));
-        const int64_t unit = ((int64_t)id * a.kvh + h) * I4Unit<D>::BYTES;
-        i4_load_k<D>(kc + unit, c, g, x[u]);
-        i4_load_v<D>(vc + unit, c, g, x[u]);
-      }
+    if (lane < n) blk = clamp_block(table[lo + lane], a.num_blocks);
+    auto unit = [&](int i) {                               // of block i of the 64, or of the last one
+      return ((int64_t)__builtin_amdgcn_readlane(blk, min(i, n - 1)) * a.kvh + h) * I4Unit<D>::BYTES;
     };
-    auto step = [&](I4Block<D> (&x)[2], int i) {
+    constexpr int STEP = 2 * kI4Waves;
+    const I4Bits k;
+    I4Block<D> x[2];
+    int i = 2 * wave;
+    if (i >= n) continue;
+    int64_t at[2] = {unit(i), unit(i + 1)};
+#pragma unroll
+    for (int u = 0; u < 2; ++u) i4_load_k<D>(kc + at[u], c, g, x[u]);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) i4_load_v<D>(vc + at[u], c, g, x[u]);
+#pragma unroll 1
+    for (; i < n; i += STEP) {
       // with an odd count the last pair's second block is its first, wholly past the end
       const int ta = (lo + i) * kBlockSize;
       const int tb = i + 1 < n ? ta + kBlockSize : len;
-      i4_step<D>(st, x, q, a.sl2, ta, tb, vis, least, c, g);
-    };
-    constexpr int STEP = 2 * kI8Waves;
-    I4Block<D> x[2], y[2];
-    int i = 2 * wave;
-    if (i < n) load(x, i);
-    if (i + STEP < n) load(y, i + STEP);
-#pragma unroll 1
-    for (; i < n; i += STEP) {
-      step(x, i);
-      x[0] = y[0], x[1] = y[1];
-      if (i + 2 * STEP < n) load(y, i + 2 * STEP);
+      const bool more = i + STEP < n;
+      if (more) at[0] = unit(i + STEP), at[1] = unit(i + STEP + 1);
+      i4_step<D>(k, st, x, q, a.sl2, ta, tb, vis, least, c, g, [&] {
+        if (!more) return;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) i4_load_k<D>(kc + at[u], c, g, x[u]);
+      }, [&] {
+        if (!more) return;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) i4_load_v<D>(vc + at[u], c, g, x[u]);
+      });
     }
   }
 }
 
 template <int D>
-__global__ void __launch_bounds__(kI8Threads, i8_decode_groups(D)) decode_int4_kernel(Int8DecodeArgs a) {
-  __shared__ __align__(16) I8DecodeLds<D> lds;
+struct I4DecodeLds {
+  static constexpr int ROW = D + 4;      // floats of a row: rows start on different banks
+  float o[kI4Waves * 16 * ROW];
+  __align__(16) float m[16][kI4Waves], l[16][kI4Waves];
+};
+
+__device__ __forceinline__ float i4_largest(const float (&m)[kI4Waves]) {
+  float top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < kI4Waves; i += 4) {
+    const float4_t x = ld<float4_t>(m + i);
+    top = vmax(top, vmax(vmax(x[0], x[1]), vmax(x[2], x[3])));
+  }
+  return top;
+}
+
+// The wavefronts' states meet in LDS, each brought to the rows' common reference first: emit(row, d, o,
+// reference, sum) for 4 dims of each row, unnormalised.
+template <int D, typename Emit>
+__device__ __forceinline__ void i4_meet(const I8State<D>& st, int rows, int wave, I4DecodeLds<D>& lds, Emit emit) {
+  constexpr int VW = D / 16, ROW = I4DecodeLds<D>::ROW;
+  int id = threadIdx.x;                                    // (so that no place is worked out ahead, and held)
+  asm volatile("" : "+v"(id));
+  const int lane = id % kWave, c = lane % 16, g = lane / 16;
+  const float l = rows_sum(st.l);
+  __syncthreads();                                         // the last item's reads of LDS
+  if (g == 0) lds.m[c][wave] = st.m;
+  __syncthreads();
+  if (c < rows) {
+    const float top = i4_largest(lds.m[c]), f = st.m == -INFINITY ? 0.f : fast_exp2(st.m - top);
+    float* dst = lds.o + (wave * 16 + c) * ROW;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int t = 0; t < VW; ++t) dst[VW * (4 * g + r) + t] = st.o[t][r] * f;
+    if (g == 0) lds.l[c][wave] = l * f;
+  }
+  __syncthreads();
+  for (int u = id; u < rows * (D / 4); u += kI4Threads) {
+    const int row = u / (D / 4), d = u % (D / 4) * 4;
+    float4_t o = ld<float4_t>(lds.o + row * ROW + d), s = ld<float4_t>(&lds.l[row][0]);
+#pragma unroll
+    for (int w = 1; w < kI4Waves; ++w) o += ld<float4_t>(lds.o + (w * 16 + row) * ROW + d);
+#pragma unroll
+    for (int i = 4; i < kI4Waves; i += 4) s += ld<float4_t>(&lds.l[row][i]);
+    emit(row, d, o, i4_largest(lds.m[row]), (s[0] + s[1]) + (s[2] + s[3]));
+  }
+}
+
+// The row (or its partial) is written.
+template <int D>
+__device__ __forceinline__ void i4_finish(const Int8DecodeArgs& a, const I8State<D>& st, int b, int h, int q0,
+                                          int row0, int rows, int split, int splits, int wave, I4DecodeLds<D>& lds) {
+  i4_meet<D>(st, rows, wave, lds, [&](int row, int d, float4_t o, float top, float sum) {
+    if (splits == 1) {
+      const float f = sum == 0.f ? 0.f : 1.f / sum;        // no visible key: zeros
+      const int token = a.by_group(row0 + row), head = h * a.group + row0 + row - token * a.group;
+      ts::st<half4_t>(a.out + (int64_t)(q0 + token) * a.out_st + (int64_t)head * D + d, to_half4(o * f));
+    } else {
+      const int64_t at = i8_partial(a, b, h, row0 + row, splits) + split;
+      ts::st<float4_t>(a.part_o + at * D + d, o);
+      if (d == 0) ts::st<float2_t>(a.part_ml + 2 * at, float2_t{top, sum});
+    }
+  });
+}
+
+// Workgroups that a CU holds at once, by registers.
+constexpr int i4_decode_groups(int D) { return D > 128 ? 2 : 4; }
+
+template <int D>
+__global__ void __launch_bounds__(kI4Threads, i4_decode_groups(D)) decode_int4_kernel(Int8DecodeArgs a) {
+  __shared__ __align__(16) I4DecodeLds<D> lds;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int lane = threadIdx.x % kWave, c = lane % 16, g = lane / 16;
   for (int64_t u = blockIdx.x;; u += gridDim.x) {
     if (u > INT32_MAX) return;                             // (the entry point refuses more)
     const int item = a.by_kvh((int)u), h = (int)u - item * a.kvh;
     I8Item x;
-    if (!i8_find(a, item, x)) return;
+    if (!i8_find<kI4SplitBlocks>(a, item, x)) return;
     const int row0 = 16 * x.tile, rows = min(x.seq.n * a.group - row0, 16), kv = x.seq.kv;
     const int row = row0 + min(c, rows - 1), token = a.by_group(row);
     const int vis = min(kv, max(0, x.seq.start + token + 1));
@@ -249,196 +330,8 @@ __global__ void __launch_bounds__(kI8Threads, i8_decode_groups(D)) decode_int4_k
     for (int t = 0; t < D / 16; ++t) st.o[t] = {0.f, 0.f, 0.f, 0.f};
     const int nb = (kv + kBlockSize - 1) / kBlockSize;
     const int b0 = i8_split_begin(nb, x.split, x.splits), b1 = i8_split_begin(nb, x.split + 1, x.splits);
-    i4_split<D, false>(a, st, q, x.b, h, b0, b1, kv, vis, least, wave, nullptr);
-    i8_finish<D, 1>(a, st, x.b, h, x.seq.q0, row0, rows, x.split, x.splits, wave, lds.o, lds.ml);
-  }
-}
-
-// Four dims of a row from its n partials: load(k, m, l, o) gives partial k's. Unnormalised, with the row's
-// sum in `sum`. Both forms of the merge come here, so that a row has the same bits from either. Little code
-// in a loop: what a launch of a few microseconds runs once, it waits for from the instruction cache.
-template <typename Load>
-__device__ __forceinline__ float4_t i4_merge(int n, Load load, float& sum) {
-  constexpr int N = 8;                                     // requested at a time
-  float m = -INFINITY;
-  float4_t o = {0.f, 0.f, 0.f, 0.f};
-  sum = 0.f;
-#pragma unroll 1
-  for (int k0 = 0; k0 < n; k0 += N) {
-    float mk[N], lk[N], to = m;
-    float4_t x[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) load(min(k0 + i, n - 1), mk[i], lk[i], x[i]);
-#pragma unroll
-    for (int i = 0; i < N; ++i) to = vmax(to, mk[i]);
-    const float neg = to == -INFINITY ? 0.f : -to, alpha = fast_exp2(m + neg);
-    m = to;
-    sum *= alpha;
-    o *= alpha;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float w = k0 + i < n ? fast_exp2(mk[i] + neg) : 0.f;
-      sum = fmaf(w, lk[i], sum);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] = fmaf(w, x[i][e], o[e]);
-    }
-  }
-  return o;
-}
-
-// Rows of sequences with more than one split, as a launch of its own: four dims of a row a thread.
-template <int D>
-__global__ void __launch_bounds__(kI8Threads) decode_int4_merge_kernel(Int8DecodeArgs a) {
-  constexpr int PER_ROW = D / 4;
-  const int id = blockIdx.x * (kI8Threads / PER_ROW) + threadIdx.x / PER_ROW, d = threadIdx.x % PER_ROW * 4;
-  const int behind = id - a.num_decode * a.heads;          // of the sequences past num_decode
-  const int unit = behind < 0 ? a.by_group(id) : a.by_slots(behind);
-  const int r = behind < 0 ? id - unit * a.group : behind - unit * a.row_slots;
-  const int seq0 = a.by_kvh(unit), h = unit - seq0 * a.kvh, b = behind < 0 ? seq0 : a.num_decode + seq0;
-  if (b >= a.num_seqs) return;
-  const I8Seq seq = i8_seq(a, b);
-  const int splits = i8_splits(a, seq, behind < 0);
-  if (splits == 1 || r >= seq.n * a.group) return;
-  const int64_t row = i8_partial(a, b, h, r, splits);
-  float sum;
-  const float4_t o = i4_merge(splits, [&](int k, float& m, float& l, float4_t& x) {
-    const float2_t ml = ld<float2_t>(a.part_ml + 2 * (row + k));
-    m = ml[0], l = ml[1], x = ld<float4_t>(a.part_o + (row + k) * D + d);
-  }, sum);
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;          // (nothing visible)
-  const int token = a.by_group(r), head = h * a.group + r - token * a.group;
-  st<half4_t>(a.out + (int64_t)(seq.q0 + token) * a.out_st + (int64_t)head * D + d, to_half4(o * inv));
-}
-
-// A pure-decode step's split map: what decode_int4_kernel looks up, worked out once for all layers of
-// the step, and the counters that let a launch merge its own splits. int32: a header that names the
-// plan, an entry for each split that the host's bounds allow (numbered densely, the real ones first) and a
-// counter for each (sequence, KV head, tile of 16 heads), 0 between launches.
-struct I4Map {
-  static constexpr int kMagic = 0x344d5354, kHeader = 32, kEntry = 32, kIds = 8, kMaxSeqs = 4096;
-  // of an entry: sequence (-1: behind the last split), split, splits, tokens, first and last block of
-  // the split, id of the sequence's last block; from kIds on those of the split's first 16 blocks
-  int* at;
-  __host__ __device__ static int64_t entries(int num_seqs, int max_splits) { return (int64_t)num_seqs * max_splits; }
-  __host__ __device__ static int64_t ints(int num_seqs, int max_splits, int kvh, int group) {
-    return kHeader + entries(num_seqs, max_splits) * kEntry + (int64_t)num_seqs * kvh * ((group + 15) / 16);
-  }
-  __device__ __forceinline__ bool names(const Int8DecodeArgs& a) const {
-    return table_entry(at) == kMagic && table_entry(at + 1) == a.num_seqs && table_entry(at + 2) == a.max_splits &&
-           table_entry(at + 3) == a.kvh && table_entry(at + 4) == a.group && table_entry(at + 5) == a.max_blocks;
-  }
-  __device__ __forceinline__ const int* entry(int slot) const { return at + kHeader + (int64_t)slot * kEntry; }
-  __device__ __forceinline__ int* counter(const Int8DecodeArgs& a, int b, int h, int tile) const {
-    return at + kHeader + entries(a.num_seqs, a.max_splits) * kEntry +
-           ((int64_t)b * a.kvh + h) * ((a.group + 15) / 16) + tile;
-  }
-};
-static_assert(I4Map::kEntry >= I4Map::kIds + kI8SplitBlocks, "a split's blocks fit its entry");
-
-// A wavefront an entry.
-static __global__ void __launch_bounds__(kI8Threads) decode_int4_map_kernel(Int8DecodeArgs a, I4Map map) {
-  const int lane = threadIdx.x % kWave;
-  const int64_t id = (int64_t)blockIdx.x * kI8Threads + threadIdx.x;
-  const int64_t counters = (int64_t)a.num_seqs * a.kvh * ((a.group + 15) / 16);
-  for (int64_t i = id; i < counters; i += (int64_t)gridDim.x * kI8Threads) *(map.counter(a, 0, 0, 0) + i) = 0;
-  if (id < I4Map::kHeader) {
-    const int name[6] = {I4Map::kMagic, a.num_seqs, a.max_splits, a.kvh, a.group, a.max_blocks};
-    int v = 0;
-#pragma unroll
-    for (int i = 0; i < 6; ++i) v = id == i ? name[i] : v;
-    map.at[id] = v;
-  }
-  const int64_t slot = id / kWave;
-  if (slot >= I4Map::entries(a.num_seqs, a.max_splits)) return;
-  // one tile of heads: item = split (a.group = 1 for the lookup, every sequence one row)
-  Int8DecodeArgs one = a;
-  one.group = 1;
-  I8Item x;
-  int v = lane == 0 ? -1 : 0;
-  if (i8_find(one, (int)slot, x)) {
-    const int32_t* table = a.block_tables + x.b * a.bt_stride;
-    const int nb = (x.seq.kv + kBlockSize - 1) / kBlockSize;
-    const int b0 = i8_split_begin(nb, x.split, x.splits), b1 = i8_split_begin(nb, x.split + 1, x.splits);
-    const int name[6] = {x.b, x.split, x.splits, x.seq.kv, b0, b1};
-    if (lane >= I4Map::kIds && lane < I4Map::kIds + kI8SplitBlocks && b0 + lane - I4Map::kIds < b1)
-      v = clamp_block(table[b0 + lane - I4Map::kIds], a.num_blocks);
-    if (lane == 6 && nb > 0) v = clamp_block(table[nb - 1], a.num_blocks);
-#pragma unroll
-    for (int i = 0; i < 6; ++i) v = lane == i ? name[i] : v;
-  }
-  if (lane < I4Map::kEntry) const_cast<int*>(map.entry((int)slot))[lane] = v;
-}
-
-// decode_int4_kernel for a step with a map: decode rows only. A workgroup has its split and block ids one
-// load after it starts, and the last split of a row tile to finish merges all of them, so that no
-// launch follows.
-template <int D>
-__global__ void __launch_bounds__(kI8Threads, i8_decode_groups(D))
-decode_int4_mapped_kernel(Int8DecodeArgs a, I4Map map, I8Div by_units) {
-  __shared__ __align__(16) I8DecodeLds<D> lds;
-  __shared__ int s_last;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int lane = threadIdx.x % kWave, c = lane % 16, g = lane / 16;
-  const int tiles = (a.group + 15) / 16, units = a.kvh * tiles;
-  if (!map.names(a)) {                                     // built for another plan: every row is NaN
-    const half_t nan = (half_t)__builtin_nanf("");
-    for (int64_t row = blockIdx.x; row < a.num_seqs; row += gridDim.x)
-      for (int i = threadIdx.x; i < a.heads * D; i += kI8Threads) a.out[row * a.out_st + i] = nan;
-    return;
-  }
-  const int64_t slots = I4Map::entries(a.num_seqs, a.max_splits);
-  for (int64_t u = blockIdx.x; u < slots * units; u += gridDim.x) {
-    const int slot = by_units((int)u), unit = (int)u - slot * units;
-    const int h = tiles == 1 ? unit : unit / tiles, tile = tiles == 1 ? 0 : unit - h * tiles;
-    const int* e = map.entry(slot);
-    const int b = table_entry(e), split = table_entry(e + 1), splits = table_entry(e + 2);
-    const int kv = table_entry(e + 3), b0 = table_entry(e + 4), b1 = table_entry(e + 5), last = table_entry(e + 6);
-    if (b < 0) return;
-    const int row0 = 16 * tile, rows = min(a.group - row0, 16);
-    I8Query<D> q;
-    i4_load_q<D>(a.q + (int64_t)b * a.q_st + (int64_t)(h * a.group + row0 + min(c, rows - 1)) * a.q_sh, g, c < rows, q);
-    // a map of an earlier step: the sequence's length or its last block have moved
-    const int len = i8_kv_len(a.seq_lens[b], a.max_blocks);
-    const int end = kv > 0 ? clamp_block(a.block_tables[b * a.bt_stride + (kv - 1) / kBlockSize], a.num_blocks) : last;
-    I8State<D> st;
-    st.m = -INFINITY, st.l = 0.f;
-#pragma unroll
-    for (int t = 0; t < D / 16; ++t) st.o[t] = {0.f, 0.f, 0.f, 0.f};
-    i4_split<D, true>(a, st, q, b, h, b0, b1, kv, kv, kv, wave, e + I4Map::kIds);
-    if (len != kv || end != last) st.m = __builtin_nanf("");
-    if (splits == 1) {
-      i8_finish<D, 1>(a, st, b, h, b, row0, rows, 0, 1, wave, lds.o, lds.ml);
-      continue;
-    }
-    // device-coherent partials: another workgroup, of any XCD, may merge them
-    const int64_t base = ((int64_t)(b * a.kvh + h) * a.group + row0) * a.max_splits;
-    const auto r_o = coherent_rsrc(a.part_o + base * D), r_ml = coherent_rsrc(a.part_ml + base * 2);
-    i8_meet<D, 1>(st, rows, wave, lds.o, lds.ml, [&](int row, int d, float4_t o, float top, float sum) {
-      const int at = row * a.max_splits + split;
-      coherent_store4(r_o, (at * D + d) * 4, o);
-      if (d == 0) coherent_store(r_ml, at * 8, top), coherent_store(r_ml, at * 8 + 4, sum);
-    });
-    __builtin_amdgcn_s_waitcnt(kWaitVmcntZero);            // they have arrived before the workgroup counts
-    __syncthreads();
-    int* counter = map.counter(a, b, h, tile);
-    if (threadIdx.x == 0)
-      s_last = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == splits - 1;
-    __syncthreads();
-    if (!s_last) continue;
-    int id = threadIdx.x;                                  // (so that nothing of this is worked out ahead, and held)
-    asm volatile("" : "+v"(id));
-#pragma unroll 1
-    for (; id < rows * (D / 4); id += kI8Threads) {
-      const int row = id / (D / 4), d = id % (D / 4) * 4;
-      float sum;
-      const float4_t o = i4_merge(splits, [&](int k, float& m, float& l, float4_t& x) {
-        const int at = row * a.max_splits + k;
-        m = coherent_load(r_ml, at * 8), l = coherent_load(r_ml, at * 8 + 4), x = coherent_load4(r_o, (at * D + d) * 4);
-      }, sum);
-      const float f = sum == 0.f ? 0.f : 1.f / sum;
-      ts::st<half4_t>(a.out + (int64_t)b * a.out_st + (int64_t)(h * a.group + row0 + row) * D + d, to_half4(o * f));
-    }
-    if (threadIdx.x == 0) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    i4_split<D>(a, st, q, x.b, h, b0, b1, kv, vis, least, wave);
+    i4_finish<D>(a, st, x.b, h, x.seq.q0, row0, rows, x.split, x.splits, wave, lds);
   }
 }
 

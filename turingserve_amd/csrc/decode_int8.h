@@ -120,9 +120,10 @@ __device__ __forceinline__ I8Seq i8_seq(const Int8DecodeArgs& a, int b) {
 // Splits of a sequence's blocks: longer ones where several tiles of rows share them, so that its
 // partials stay those of one tile. (chunk_parts holds them, and row_slots the rows, within the host's
 // bounds; past those there is one split.)
+template <int EACH = kI8SplitBlocks>
 __device__ __forceinline__ int i8_splits(const Int8DecodeArgs& a, const I8Seq& s, bool decode) {
   const int rows = s.n * a.group, nb = (s.kv + kBlockSize - 1) / kBlockSize;
-  if (decode) return i8_splits(nb, a.max_splits);
+  if (decode) return i8_splits(nb, a.max_splits, EACH);
   if (rows > a.row_slots) return 1;
   const int tiles = s.n == 1 ? 1 : (rows + 15) / 16;
   const int n = i8_splits(nb, min(a.max_splits, kI8MaxSplits / tiles), kI8SplitBlocks * tiles);
@@ -397,11 +398,11 @@ struct I8DecodeLds {
   float ml[2 * kI8Waves * 16];
 };
 
-// The four wavefronts' states (O in units of 1 / UNIT) meet in LDS: emit(row, d, o, reference, sum) for 4 dims
-// of each row, unnormalised.
-template <int D, int UNIT, typename Emit>
-__device__ __forceinline__ void i8_meet(const I8State<D>& st, int rows, int wave, float* s_o, float* s_ml,
-                                        Emit emit) {
+// The four wavefronts' states meet in LDS; the row (or its partial) is written.
+template <int D>
+__device__ __forceinline__ void i8_finish(const Int8DecodeArgs& a, I8State<D>& st, int b, int h,
+                                          int q0, int row0, int rows, int split, int splits, int wave,
+                                          float* s_o, float* s_ml) {
   constexpr int VW = D / 16;
   const int lane = threadIdx.x % kWave, c = lane % 16, g = lane / 16;
   const float l = rows_sum(st.l);
@@ -431,17 +432,7 @@ __device__ __forceinline__ void i8_meet(const I8State<D>& st, int rows, int wave
       sum += f * s_ml[2 * (w * 16 + row) + 1];
       o += ld<float4_t>(s_o + (w * 16 + row) * I8DecodeLds<D>::ROW + d) * f;
     }
-    o *= (float)UNIT;
-    emit(row, d, o, top, sum);
-  }
-}
-
-// The row (or its partial) is written.
-template <int D, int UNIT>
-__device__ __forceinline__ void i8_finish(const Int8DecodeArgs& a, I8State<D>& st, int b, int h,
-                                          int q0, int row0, int rows, int split, int splits, int wave,
-                                          float* s_o, float* s_ml) {
-  i8_meet<D, UNIT>(st, rows, wave, s_o, s_ml, [&](int row, int d, float4_t o, float top, float sum) {
+    o *= kColumnUnit;
     if (splits == 1) {
       const float f = sum == 0.f ? 0.f : 1.f / sum;        // no visible key: zeros
       const int token = a.by_group(row0 + row), head = h * a.group + row0 + row - token * a.group;
@@ -454,7 +445,7 @@ __device__ __forceinline__ void i8_finish(const Int8DecodeArgs& a, I8State<D>& s
         a.part_ml[2 * at + 1] = sum;
       }
     }
-  });
+  }
 }
 
 // Item `item` of the batch's (split, row tile) pairs, numbered densely over the sequences. Every
@@ -464,6 +455,7 @@ struct I8Item {
   I8Seq seq;
 };
 
+template <int EACH = kI8SplitBlocks>
 __device__ __forceinline__ bool i8_find(const Int8DecodeArgs& a, int item, I8Item& x) {
   const int lane = threadIdx.x % kWave;
   int base = 0;
@@ -472,7 +464,7 @@ __device__ __forceinline__ bool i8_find(const Int8DecodeArgs& a, int item, I8Ite
     I8Seq s = {};
     if (s0 + lane < a.num_seqs) {
       s = i8_seq(a, s0 + lane);
-      splits = i8_splits(a, s, s0 + lane < a.num_decode);
+      splits = i8_splits<EACH>(a, s, s0 + lane < a.num_decode);
       tiles = (s.n * a.group + 15) / 16;
     }
     const int n = splits * tiles, sum = i8_scan(n);
@@ -520,7 +512,7 @@ __global__ void __launch_bounds__(kI8Threads, i8_decode_groups(D)) decode_int8_k
     const int nb = (kv + kBlockSize - 1) / kBlockSize;
     const int b0 = i8_split_begin(nb, x.split, x.splits), b1 = i8_split_begin(nb, x.split + 1, x.splits);
     i8_split<D>(a, st, q, x.b, h, b0, b1, kv, vis, least, wave);
-    i8_finish<D, (int)kColumnUnit>(a, st, x.b, h, x.seq.q0, row0, rows, x.split, x.splits, wave, lds.o, lds.ml);
+    i8_finish<D>(a, st, x.b, h, x.seq.q0, row0, rows, x.split, x.splits, wave, lds.o, lds.ml);
   }
 }
 
@@ -528,7 +520,7 @@ __global__ void __launch_bounds__(kI8Threads, i8_decode_groups(D)) decode_int8_k
 // row's first partials and every split's (m, l) are requested before the sequence's length is known
 // (they lie in the workspace whatever it is), the others at once after it. (A workgroup a row, its
 // eight groups meeting in LDS, took twice as long at 2240 rows of a few splits: 10.5 us.)
-template <int D>
+template <int D, int EACH = kI8SplitBlocks>
 __global__ void __launch_bounds__(kI8Threads) decode_int8_merge_kernel(Int8DecodeArgs a) {
   constexpr int PER_ROW = D / 4, GROUPS = kWave / PER_ROW;
   constexpr int N = 64 / GROUPS < 16 ? 64 / GROUPS : 16;   // partials of a lane at a time
@@ -548,7 +540,7 @@ __global__ void __launch_bounds__(kI8Threads) decode_int8_merge_kernel(Int8Decod
   };
   if (behind < 0) request((int64_t)slot * a.max_splits, a.max_splits);
   const I8Seq seq = i8_seq(a, b);
-  const int splits = i8_splits(a, seq, behind < 0);
+  const int splits = i8_splits<EACH>(a, seq, behind < 0);
   if (splits == 1 || r >= seq.n * a.group) return;
   const int64_t row = i8_partial(a, b, h, r, splits);
   const float* part = a.part_o + row * D + d;

@@ -36,31 +36,42 @@ struct I4Unit {
 
 __device__ __forceinline__ half2_t i4_half2(uint32_t w) { return __builtin_bit_cast(half2_t, w); }
 
+// What the widening takes beside a word, held in registers: with the exponent of 1024 in one and the masks in
+// scalar ones a nibble is masked and placed by one instruction (literals would make two of it).
+struct I4Bits {
+  uint32_t one, low, high;
+  __device__ __forceinline__ I4Bits() {
+    asm("v_mov_b32 %0, 0x64006400" : "=v"(one));
+    asm("s_mov_b32 %0, 0x000f000f" : "=s"(low));
+    asm("s_mov_b32 %0, 0x00f000f0" : "=s"(high));
+  }
+};
+
 // Nibble P of each half of w (w8: w >> 8) as packed fp16, exactly: under the exponent of 1024 a nibble in
 // bits 0 .. 3 is 1024 + code, one in bits 4 .. 7 is 1024 + 16 code.
 template <int P>
-__device__ __forceinline__ half2_t i4_codes(uint32_t w, uint32_t w8) {
+__device__ __forceinline__ half2_t i4_codes(const I4Bits& k, uint32_t w, uint32_t w8) {
   const uint32_t x = P < 2 ? w : w8;
   if constexpr (P % 2 == 0) {
     const half2_t off = {(half_t)-1024.f, (half_t)-1024.f};
-    return i4_half2((x & 0x000f000fu) | 0x64006400u) + off;
+    return i4_half2((x & k.low) | k.one) + off;
   } else {
     const half2_t by = {(half_t)0.0625f, (half_t)0.0625f}, off = {(half_t)-64.f, (half_t)-64.f};
-    return __builtin_elementwise_fma(i4_half2((x & 0x00f000f0u) | 0x64006400u), by, off);
+    return __builtin_elementwise_fma(i4_half2((x & k.high) | k.one), by, off);
   }
 }
 template <int P>
-__device__ __forceinline__ half2_t i4_values(uint32_t w, uint32_t w8, half2_t step, half2_t low) {
-  return __builtin_elementwise_fma(i4_codes<P>(w, w8), step, low);
+__device__ __forceinline__ half2_t i4_values(const I4Bits& k, uint32_t w, uint32_t w8, half2_t step, half2_t low) {
+  return __builtin_elementwise_fma(i4_codes<P>(k, w, w8), step, low);
 }
 
 // The octet of a word whose numbers are `n` (step in the low half, low in the high one), in the order of
 // its channels.
-__device__ __forceinline__ half8_t i4_octet(uint32_t w, uint32_t n) {
+__device__ __forceinline__ half8_t i4_octet(const I4Bits& k, uint32_t w, uint32_t n) {
   const half2_t p = i4_half2(n), step = {p[0], p[0]}, low = {p[1], p[1]};
   const uint32_t w8 = w >> 8;
-  const half2_t a = i4_values<0>(w, w8, step, low), b = i4_values<1>(w, w8, step, low);
-  const half2_t c = i4_values<2>(w, w8, step, low), d = i4_values<3>(w, w8, step, low);
+  const half2_t a = i4_values<0>(k, w, w8, step, low), b = i4_values<1>(k, w, w8, step, low);
+  const half2_t c = i4_values<2>(k, w, w8, step, low), d = i4_values<3>(k, w, w8, step, low);
   return {a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
@@ -74,9 +85,11 @@ __device__ __forceinline__ uint32_t i4_odd(uint32_t row0, uint32_t row1) {
 
 // A low of NaN stands for a token whose row was not finite. Its K makes the scores of the rows that see it
 // NaN; its V has to stay out of the rows that do not, where its weight is 0: any number does.
+// (The instruction returns the other operand for a NaN; maxnum would quiet its operand first.)
 __device__ __forceinline__ half2_t i4_finite(uint32_t lows) {
-  const half2_t least = {(half_t)-65504.f, (half_t)-65504.f};
-  return __builtin_elementwise_max(i4_half2(lows), least);
+  uint32_t x;
+  asm("v_pk_max_f16 %0, %1, %2" : "=v"(x) : "v"(lows), "s"(0xfbfffbffu));    // -65504
+  return i4_half2(x);
 }
 
 }  // namespace ts

@@ -15,7 +15,7 @@
 
 namespace ts {
 
-constexpr int kI4Threads = 256;
+constexpr int kI4WriteThreads = 256;
 
 struct Int4WriteArgs {
   const half_t *k, *v;                    // rows of the step (k, v heads)
@@ -84,7 +84,7 @@ template <int D, bool ROPE>
 __device__ __forceinline__ void i4_write_kv(const Int4WriteArgs& a) {
   typedef I4Unit<D> U;
   constexpr int OCTETS = D / 8, LANES = U::GROUP / 8, PER = 2 * OCTETS;   // lanes of a group, of a (token, head)
-  const int item = (int)(blockIdx.x * (kI4Threads / PER) + threadIdx.x / PER), in = threadIdx.x % PER;
+  const int item = (int)(blockIdx.x * (kI4WriteThreads / PER) + threadIdx.x / PER), in = threadIdx.x % PER;
   const int t = a.by_kvh(item), h = item - t * a.kvh, side = in / OCTETS, octet = in % OCTETS;
   if (t >= a.num_tokens) return;                           // (all lanes of an item)
   const int64_t slot = a.slots[t];
@@ -137,11 +137,11 @@ __device__ __forceinline__ void i4_write_kv(const Int4WriteArgs& a) {
 }
 
 template <int D, bool ROPE>
-__global__ void __launch_bounds__(kI4Threads) kv_write_int4_kernel(Int4WriteArgs a) {
+__global__ void __launch_bounds__(kI4WriteThreads) kv_write_int4_kernel(Int4WriteArgs a) {
   if (!ROPE || (int)blockIdx.x < a.kv_groups) return i4_write_kv<D, ROPE>(a);
   if constexpr (ROPE) {
     constexpr int PER = D / 16;
-    const int item = (int)((blockIdx.x - a.kv_groups) * (kI4Threads / PER) + threadIdx.x / PER);
+    const int item = (int)((blockIdx.x - a.kv_groups) * (kI4WriteThreads / PER) + threadIdx.x / PER);
     const int t = a.by_heads(item), h = item - t * a.heads, at = 8 * (threadIdx.x % PER);
     if (t >= a.num_tokens) return;
     const half_t* src = a.q + t * a.q_st + (int64_t)h * D + at;
@@ -174,10 +174,10 @@ struct Int4ReadArgs {
 // row (consecutive lanes have consecutive words, and the rows of a request follow one another), of V all of
 // them at once. D / 2 threads a unit; every store is 16 bytes, of whole rows.
 template <int D>
-__global__ void __launch_bounds__(kI4Threads) kv_read_int4_kernel(Int4ReadArgs a) {
+__global__ void __launch_bounds__(kI4WriteThreads) kv_read_int4_kernel(Int4ReadArgs a) {
   typedef I4Unit<D> U;
   constexpr int PER = D / 2, OCTETS = D / 8;
-  const int unit = (int)(blockIdx.x * (kI4Threads / PER) + threadIdx.x / PER), in = threadIdx.x % PER;
+  const int unit = (int)(blockIdx.x * (kI4WriteThreads / PER) + threadIdx.x / PER), in = threadIdx.x % PER;
   if (unit >= a.units) return;
   const int lb = a.by_kvh(unit), h = unit - lb * a.kvh;    // (layer, K or V) and block; head
   const int side = a.by_n(lb);
@@ -185,6 +185,7 @@ __global__ void __launch_bounds__(kI4Threads) kv_read_int4_kernel(Int4ReadArgs a
   const uint8_t* src = a.cache + (((int64_t)side * a.num_blocks + blk) * a.kvh + h) * U::BYTES;
   half_t* dst = a.out + (int64_t)unit * (kBlockSize * D);
   const int quad = in / OCTETS, octet = in % OCTETS, group = 8 * octet / U::GROUP;
+  const I4Bits k;
   uint32_t w[4], n[4];
   const bool is_v = side & 1;
   if (!is_v) {
@@ -202,7 +203,7 @@ __global__ void __launch_bounds__(kI4Threads) kv_read_int4_kernel(Int4ReadArgs a
     }
   }
 #pragma unroll
-  for (int r = 0; r < 4; ++r) st<half8_t>(dst + (is_v ? 4 * quad + r : 4 * r + quad) * D + 8 * octet, i4_octet(w[r], n[r]));
+  for (int r = 0; r < 4; ++r) st<half8_t>(dst + (is_v ? 4 * quad + r : 4 * r + quad) * D + 8 * octet, i4_octet(k, w[r], n[r]));
 }
 
 static bool int4_head_dim(int D) { return D == 16 || D == 32 || D == 64 || D == 128 || D == 256; }
@@ -210,9 +211,9 @@ static bool int4_head_dim(int D) { return D == 16 || D == 32 || D == 64 || D == 
 template <int D>
 static void launch_write(const Int4WriteArgs& a, bool rope, unsigned grid, hipStream_t s) {
   if (rope)
-    kv_write_int4_kernel<D, true><<<grid, kI4Threads, 0, s>>>(a);
+    kv_write_int4_kernel<D, true><<<grid, kI4WriteThreads, 0, s>>>(a);
   else
-    kv_write_int4_kernel<D, false><<<grid, kI4Threads, 0, s>>>(a);
+    kv_write_int4_kernel<D, false><<<grid, kI4WriteThreads, 0, s>>>(a);
 }
 
 static int write_int4(Int4WriteArgs a, bool rope, int64_t num_tokens, int D, const char* what, void* stream) {
@@ -230,11 +231,11 @@ static int write_int4(Int4WriteArgs a, bool rope, int64_t num_tokens, int D, con
   TS_REQUIRE(units < (1ll << 30) && num_tokens < (1ll << 30) / units, TS_ERR_UNSUPPORTED,
              "%s: %lld tokens of %lld heads", what, (long long)num_tokens, (long long)units);
   a.num_tokens = (int)num_tokens, a.by_kvh = I8Div::by(a.kvh);
-  a.kv_groups = (int)((num_tokens * a.kvh * (D / 4) + kI4Threads - 1) / kI4Threads);
+  a.kv_groups = (int)((num_tokens * a.kvh * (D / 4) + kI4WriteThreads - 1) / kI4WriteThreads);
   int64_t grid = a.kv_groups;
   if (rope) {
     a.by_heads = I8Div::by(a.heads);
-    grid += (num_tokens * a.heads * (D / 16) + kI4Threads - 1) / kI4Threads;
+    grid += (num_tokens * a.heads * (D / 16) + kI4WriteThreads - 1) / kI4WriteThreads;
   }
   TS_REQUIRE(grid < (1ll << 31), TS_ERR_UNSUPPORTED, "%s: %lld workgroups", what, (long long)grid);
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
@@ -308,14 +309,14 @@ extern "C" int ts_kv_read_int4(const void* cache, int32_t num_layers, int64_t nu
   TS_REQUIRE(units < (double)(1ll << 30), TS_ERR_UNSUPPORTED, "kv_read_int4: %d blocks of %d layers", n, num_layers);
   Int4ReadArgs a = {static_cast<const uint8_t*>(cache), blocks, static_cast<half_t*>(out), num_blocks, n,
                     num_kv_heads, (int)units, I8Div::by(n), I8Div::by(num_kv_heads)};
-  const unsigned grid = (unsigned)(((int64_t)a.units * (head_dim / 2) + kI4Threads - 1) / kI4Threads);
+  const unsigned grid = (unsigned)(((int64_t)a.units * (head_dim / 2) + kI4WriteThreads - 1) / kI4WriteThreads);
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   switch (head_dim) {
-    case 16: kv_read_int4_kernel<16><<<grid, kI4Threads, 0, s>>>(a); break;
-    case 32: kv_read_int4_kernel<32><<<grid, kI4Threads, 0, s>>>(a); break;
-    case 64: kv_read_int4_kernel<64><<<grid, kI4Threads, 0, s>>>(a); break;
-    case 128: kv_read_int4_kernel<128><<<grid, kI4Threads, 0, s>>>(a); break;
-    default: kv_read_int4_kernel<256><<<grid, kI4Threads, 0, s>>>(a); break;
+    case 16: kv_read_int4_kernel<16><<<grid, kI4WriteThreads, 0, s>>>(a); break;
+    case 32: kv_read_int4_kernel<32><<<grid, kI4WriteThreads, 0, s>>>(a); break;
+    case 64: kv_read_int4_kernel<64><<<grid, kI4WriteThreads, 0, s>>>(a); break;
+    case 128: kv_read_int4_kernel<128><<<grid, kI4WriteThreads, 0, s>>>(a); break;
+    default: kv_read_int4_kernel<256><<<grid, kI4WriteThreads, 0, s>>>(a); break;
   }
   return check_launch("kv_read_int4");
 }

@@ -28,6 +28,7 @@ struct I4Stage {
   static constexpr int N = (UNITS + THREADS - 1) / THREADS;
   static constexpr bool ALL = UNITS % THREADS == 0;        // every thread has N units
   static constexpr bool UNIFORM = D >= kWave;              // a wavefront's unit lies in one block
+  I4Bits bits;
   uint32_t k[N][2], kn[N];
   uint4_t v[N], vn[N];
 
@@ -79,15 +80,15 @@ struct I4Stage {
     for (int i = 0; i < N; ++i)
       if (ALL || unit(i) < UNITS) {
         const int key = unit(i) / (D / 16), chunk = 2 * (unit(i) % (D / 16));
-        st<half8_t>(tile + I8Tile<D>::k_at(key, chunk), i4_octet(k[i][0], kn[i]));
-        st<half8_t>(tile + I8Tile<D>::k_at(key, chunk + 1), i4_octet(k[i][1], kn[i]));
+        st<half8_t>(tile + I8Tile<D>::k_at(key, chunk), i4_octet(bits, k[i][0], kn[i]));
+        st<half8_t>(tile + I8Tile<D>::k_at(key, chunk + 1), i4_octet(bits, k[i][1], kn[i]));
       }
   }
   template <int P>
-  static __device__ __forceinline__ void place_column(half_t* tile, uint32_t a, uint32_t a8, uint32_t b, uint32_t b8,
+  __device__ __forceinline__ void place_column(half_t* tile, uint32_t a, uint32_t a8, uint32_t b, uint32_t b8,
                                                       uint4_t n, half2_t low0, half2_t low1, int block, int quad,
-                                                      int d0) {
-    const half2_t x = i4_values<P>(a, a8, i4_half2(n[0]), low0), y = i4_values<P>(b, b8, i4_half2(n[1]), low1);
+                                               int d0) const {
+    const half2_t x = i4_values<P>(bits, a, a8, i4_half2(n[0]), low0), y = i4_values<P>(bits, b, b8, i4_half2(n[1]), low1);
     st<half4_t>(tile + I8Tile<D>::v_at(d0 + 2 * P, block, quad & 1) + 4 * (quad >> 1),
                 half4_t{x[0], x[1], y[0], y[1]});
   }

@@ -1,7 +1,8 @@
 // What the attentions over the quantised paged caches share on the host: how a batch is split between
 // the decode kernel and the prompt kernel, the workspace, the checks and the launches. The formats'
-// kernels come in as a class `Kernels` with decode<D>(args, rows, cus, split map, stream) and
-// prefill<D>(args, stream).
+// kernels come in as a class `Kernels` with decode<D>(args, rows, cus, stream) and
+// prefill<D>(args, stream), and
+// kSplitBlocks, the blocks of a split.
 #pragma once
 
 #include "prefill_int8.h"
@@ -43,8 +44,8 @@ static size_t take(size_t& at, size_t bytes) {
   return here;
 }
 
-static QuantPlan quant_plan(int num_seqs, int num_decode, int max_query_len, int max_seq_len,
-                          int max_prefill_seq_len, int H, int KVH, int D, int cus) {
+static QuantPlan quant_plan(int split_blocks, int num_seqs, int num_decode, int max_query_len, int max_seq_len,
+                            int max_prefill_seq_len, int H, int KVH, int D, int cus) {
   QuantPlan pl = {};
   size_t at = 0;
   const int64_t nb = ((int64_t)(max_seq_len > 0 ? max_seq_len : 0) + kBlockSize - 1) / kBlockSize;
@@ -58,7 +59,7 @@ static QuantPlan quant_plan(int num_seqs, int num_decode, int max_query_len, int
   pl.small = all ? num_seqs : num_decode;
   pl.row_slots = (int)(chunk_rows < kI8ShortRows ? chunk_rows : kI8ShortRows);
   if (pl.row_slots < G) pl.row_slots = G;
-  pl.max_splits = i8_splits((int)nb, kI8MaxSplits);
+  pl.max_splits = i8_splits((int)nb, kI8MaxSplits, split_blocks);
   const int row_tiles = (pl.row_slots + 15) / 16;
   pl.chunk_parts = row_tiles == 1 ? pl.row_slots * pl.max_splits : 16 * (pl.max_splits + row_tiles);
   if (pl.chunk_parts < G * pl.max_splits) pl.chunk_parts = G * pl.max_splits;   // (chunks of one row)
@@ -116,16 +117,16 @@ struct QuantCall {
   void* workspace;
   size_t workspace_bytes;
   void* stream;
-  void* split_map;                       // (the 4-bit cache's, checked by its entry point)
 };
 
+template <class Kernels>
 static size_t quant_workspace_bytes(int num_seqs, int num_decode, int max_query_len, int max_seq_len,
                                     int max_prefill_seq_len, int heads, int kvh, int head_dim, int cus) {
   if (num_seqs <= 0 || num_decode < 0 || num_decode > num_seqs || kvh <= 0 || heads < kvh || heads % kvh != 0 ||
       !quant_head_dim(head_dim))
     return 0;
-  return quant_plan(num_seqs, num_decode, max_query_len, max_seq_len, max_prefill_seq_len, heads, kvh, head_dim,
-                    cus > 0 ? cus : 256).bytes;
+  return quant_plan(Kernels::kSplitBlocks, num_seqs, num_decode, max_query_len, max_seq_len, max_prefill_seq_len,
+                    heads, kvh, head_dim, cus > 0 ? cus : 256).bytes;
 }
 
 template <class Kernels, bool SCALES>
@@ -155,8 +156,8 @@ static int quant_attention(const char* what, const QuantCall& c) {
   TS_REQUIRE(c.num_seqs <= 1 << 20 && c.num_tokens < (1ll << 30) / (c.heads / c.kvh), TS_ERR_UNSUPPORTED,
              "%s: %lld tokens of %d sequences", what, (long long)c.num_tokens, c.num_seqs);
   const int group = c.heads / c.kvh;
-  QuantPlan pl = quant_plan(c.num_seqs, c.num_decode, c.max_query_len, c.max_seq_len, c.max_prefill_seq_len,
-                            c.heads, c.kvh, c.head_dim, 256);
+  QuantPlan pl = quant_plan(Kernels::kSplitBlocks, c.num_seqs, c.num_decode, c.max_query_len, c.max_seq_len,
+                            c.max_prefill_seq_len, c.heads, c.kvh, c.head_dim, 256);
   // ... and steps: those of at most `tiles` tiles, each of which sees what its table holds before the
   // chunk and the chunk (the last term: the rounded rate). (None of this hangs on the number of CUs.)
   const int tile_rows = 32 * i8_prefill_waves(c.head_dim);
@@ -171,8 +172,8 @@ static int quant_attention(const char* what, const QuantCall& c) {
   int cus = 0;
   int status = device_cu_count(c.stream, &cus);
   if (status != TS_OK) return status;
-  pl = quant_plan(c.num_seqs, c.num_decode, c.max_query_len, c.max_seq_len, c.max_prefill_seq_len, c.heads, c.kvh,
-                  c.head_dim, cus);
+  pl = quant_plan(Kernels::kSplitBlocks, c.num_seqs, c.num_decode, c.max_query_len, c.max_seq_len,
+                  c.max_prefill_seq_len, c.heads, c.kvh, c.head_dim, cus);
   TS_REQUIRE(pl.bytes == 0 || (c.workspace && c.workspace_bytes >= pl.bytes && aligned(c.workspace, 256)),
              TS_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", what, c.workspace_bytes, pl.bytes);
   char* ws = static_cast<char*>(c.workspace);
@@ -195,11 +196,11 @@ static int quant_attention(const char* what, const QuantCall& c) {
     a.part_ml = reinterpret_cast<float*>(ws + pl.dec_ml);
     const int64_t rows = merge_rows(pl, c.num_decode, c.heads, c.kvh);
     switch (c.head_dim) {
-      case 16: Kernels::template decode<16>(a, rows, cus, c.split_map, s); break;
-      case 32: Kernels::template decode<32>(a, rows, cus, c.split_map, s); break;
-      case 64: Kernels::template decode<64>(a, rows, cus, c.split_map, s); break;
-      case 128: Kernels::template decode<128>(a, rows, cus, c.split_map, s); break;
-      default: Kernels::template decode<256>(a, rows, cus, c.split_map, s); break;
+      case 16: Kernels::template decode<16>(a, rows, cus, s); break;
+      case 32: Kernels::template decode<32>(a, rows, cus, s); break;
+      case 64: Kernels::template decode<64>(a, rows, cus, s); break;
+      case 128: Kernels::template decode<128>(a, rows, cus, s); break;
+      default: Kernels::template decode<256>(a, rows, cus, s); break;
     }
     status = check_launch(what);
     if (status != TS_OK) return status;

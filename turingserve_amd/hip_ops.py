@@ -27,7 +27,7 @@ __all__ = ["kv_write", "paged_attention", "linear", "lm_head_int8", "logits_int8
            "gate_up_silu", "rope_kv_write_", "decode_kv_write_attention",
            "decode_rope_kv_write_attention", "kv_write_int8", "rope_kv_write_int8",
            "paged_attention_int8", "kv_write_int4", "rope_kv_write_int4", "kv_read_int4",
-           "paged_attention_int4", "decode_split_map_int4"]
+           "paged_attention_int4"]
 
 DEFAULT_PARTITION = 0            # v3 split size when the caller names none: 0 = own-length
 
@@ -971,46 +971,19 @@ def kv_read_int4(cache: torch.Tensor, blocks: torch.Tensor) -> torch.Tensor:
     return out
 
 
-def decode_split_map_int4(meta, H: int, KVH: int, D: int, num_blocks: int, device):
-    """The split map of a pure-decode step over a 4-bit cache (ts_decode_split_map_int4): built once,
-    after the step's lengths and tables are final, and passed as split_map= to every layer's
-    paged_attention_int4 of the same step, whose launch then merges its own splits (the same bits). Calls
-    that share a map are ordered on one stream. Returns (int32 device tensor, bytes), or None where there
-    is nothing to map (no splits, chunks in the batch, more than 4096 sequences; the calls then take
-    split_map=None)."""
-    S = meta.num_decode
-    if S == 0 or meta.seq_lens.shape[0] != S:
-        return None
-    nb = N.lib().ts_decode_split_map_int4_bytes(S, H, KVH, D, int(meta.max_seq_len))
-    if nb == 0:
-        return None
-    _check_gpu(meta.seq_lens)
-    if _elsewhere(meta.seq_lens):
-        with torch.cuda.device(meta.seq_lens.device):
-            return decode_split_map_int4(meta, H, KVH, D, num_blocks, device)
-    bt, sl, _, bt_st = _step_args("decode_split_map_int4", meta, torch.device(device, meta.seq_lens.device.index)
-                                  if isinstance(device, str) else device)
-    buf = torch.empty(nb // 4, dtype=torch.int32, device=sl.device)
-    N.check(N.lib().ts_decode_split_map_int4(_ptr(bt), bt_st, bt.shape[1], int(num_blocks), _ptr(sl), S, H,
-                                             KVH, D, int(meta.max_seq_len), _ptr(buf), nb, _stream(buf)),
-            "decode_split_map_int4")
-    return buf, nb
-
-
 def paged_attention_int4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, meta,
-                         scale: float, split_map=None) -> torch.Tensor:
+                         scale: float) -> torch.Tensor:
     """paged_attention over a 4-bit cache (see kv_write_int4): q [T, H, D] -> [T, H*D], one row for each
     of the first num_decode sequences, the rows of query_start_loc for the others under the
     bottom-right causal mask. A row that sees a token of NaN is NaN; a row that sees no token is
-    zeros. split_map: decode_split_map_int4()'s result for this step (same meta) or None; the output is
-    the same either way."""
+    zeros."""
     T, H, D = q.shape
     if T == 0:
         return torch.empty(0, H * D, dtype=q.dtype, device=q.device)
     _check_gpu(q)
     if _elsewhere(q):
         with torch.cuda.device(q.device):
-            return paged_attention_int4(q, k_cache, v_cache, meta, scale, split_map)
+            return paged_attention_int4(q, k_cache, v_cache, meta, scale)
     out = torch.empty(T, H * D, dtype=q.dtype, device=q.device)
     NB, KVH, cd = _int4_cache("paged_attention_int4", k_cache, v_cache)
     bt, sl, qsl, bt_st = _step_args("paged_attention_int4", meta, q.device, k_cache, v_cache)
@@ -1024,5 +997,5 @@ def paged_attention_int4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     N.check(N.lib().ts_paged_attention_int4(
         _ptr(q), *_row_strides(q), _ptr(out), H * D, T, _ptr(k_cache), _ptr(v_cache), NB, _ptr(bt),
         bt_st, bt.shape[1], _ptr(sl), _ptr(qsl), B, S, *bounds, H, KVH, D, float(scale), _ptr(ws),
-        ws_bytes, _stream(q), *_map_args(split_map)), "paged_attention_int4")
+        ws_bytes, _stream(q)), "paged_attention_int4")
     return out

@@ -195,7 +195,7 @@ class Qwen2Model:
             q = ops.rope_kv_write_int4(ops.linear(x, lw.qkv_proj), positions, self.cos, self.sin,
                                        c.num_heads, c.num_kv_heads, c.head_dim, *cache,
                                        meta.slot_mapping)
-            a = ops.paged_attention_int4(q, *cache, meta, self.scale, split_map=split_map)
+            a = ops.paged_attention_int4(q, *cache, meta, self.scale)
             x, residual = self._project_norm(a, lw.o_proj, residual, lw.post_attention_norm)
             return self._mlp_act(x, lw), residual
         k_cache, v_cache = kv_cache[index, 0], kv_cache[index, 1]
@@ -248,14 +248,11 @@ class Qwen2Model:
         the final norm): the same values, without a separate split-K reduction launch."""
         c, layers = self.cfg, self.w.layers
         fused = self.pure_decode(meta, input_ids.shape[0])
-        # one decode split map per step, read by every layer's decode launch
-        build_map, blocks = None, 0
-        if fused and isinstance(kv_cache, Int4KVCache):
-            build_map, blocks = self.ops.decode_split_map_int4, kv_cache.data.shape[2]
-        elif fused and not isinstance(kv_cache, Int8KVCache):
-            build_map, blocks = getattr(self.ops, "decode_split_map", None), kv_cache.shape[2]
-        split_map = (build_map(meta, c.num_heads, c.num_kv_heads, c.head_dim, blocks, kv_cache.device)
-                     if build_map is not None else None)
+        # one decode split map per step, read by every layer's fused decode launch
+        build_map = (getattr(self.ops, "decode_split_map", None)
+                     if fused and not isinstance(kv_cache, (Int8KVCache, Int4KVCache)) else None)
+        split_map = (build_map(meta, c.num_heads, c.num_kv_heads, c.head_dim, kv_cache.shape[2],
+                               kv_cache.device) if build_map is not None else None)
         h = self.w.embed_tokens[input_ids]
         residual = h
         x = self.ops.rmsnorm(h, layers[0].input_norm, c.rms_norm_eps)

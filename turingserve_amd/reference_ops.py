@@ -256,13 +256,8 @@ def _int4_values(cache: torch.Tensor, values: bool) -> torch.Tensor:
     return (x * steps.double()[..., None] + lows.double()[..., None]).flatten(-2).half()
 
 
-def decode_split_map_int4(meta, H: int, KVH: int, D: int, num_blocks: int, device):
-    """Twin: attention here needs no map."""
-    return None
-
-
 def paged_attention_int4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, meta,
-                         scale: float, split_map=None) -> torch.Tensor:
+                         scale: float) -> torch.Tensor:
     """Twin: the sequences' blocks as fp16 values, then causal attention over the tokens that the table
     holds (block ids outside the cache read block 0). Rows that see no token are zeros, rows that see a
     token whose K is NaN are NaN."""
