@@ -261,15 +261,15 @@ def test_python_wrappers_refuse():
         with pytest.raises(ValueError, match="caches must be"):
             H._int4_cache("x", *bad)
     with pytest.raises(ValueError, match="shorter"):
-        H._slots("x", meta.slot_mapping[:3], 6, torch.device("cpu"))
+        H._slots("x", meta.slot_mapping[:3], 6, -1)
     with pytest.raises(ValueError, match="same GPU"):
-        H._slots("x", meta.slot_mapping, 6, torch.device("cuda", 0))
-    for change in (dict(num_decode=3), dict(query_start_loc=meta.query_start_loc[:2]),
+        H._slots("x", meta.slot_mapping, 6, 0)
+    for change in (dict(num_decode=3), dict(num_decode=-1), dict(query_start_loc=meta.query_start_loc[:2]),
                    dict(block_tables=meta.block_tables[:1])):
         with pytest.raises(ValueError, match="metadata"):
-            H._step_args("x", dataclasses.replace(meta, **change), torch.device("cpu"), *layer)
-    with pytest.raises(ValueError, match="same GPU"):
-        H._step_args("x", meta, torch.device("cuda", 0), *layer)
+            H._int4_meta("x", dataclasses.replace(meta, **change))
+    with pytest.raises(ValueError, match="on the GPU"):
+        H._on_gpu("x", *layer)
 
 
 def test_tensors_of_another_gpu_than_the_current_one(monkeypatch):
@@ -283,22 +283,22 @@ def test_tensors_of_another_gpu_than_the_current_one(monkeypatch):
 
         def __enter__(self):
             entered.append(self.device)
-            self.was, current[0] = current[0], self.device.index
+            self.was, current[0] = current[0], self.device
 
         def __exit__(self, *_):
             current[0] = self.was
 
     class Rows:
-        is_cuda, device, dtype = True, torch.device("cuda", 0), torch.float16
+        device, dtype = torch.device("cuda", 0), torch.float16
 
         def __init__(self, *shape):
             self.shape = shape
 
-        def dim(self):
-            return len(self.shape)
+        def get_device(self):
+            return 0
 
-        def stride(self, _):
-            return 1
+        def stride(self):
+            return (1,) * len(self.shape)
 
     monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: current[0], raising=False)
     monkeypatch.setattr(torch.cuda, "device", On)
@@ -310,7 +310,7 @@ def test_tensors_of_another_gpu_than_the_current_one(monkeypatch):
                  lambda c: H.paged_attention_int4(rows, c, c, None, 1.0)):
         with pytest.raises(ValueError, match="cache.* must be"):
             call(rows)
-        assert entered.pop() == torch.device("cuda", 0) and not entered and current == [1]
+        assert entered.pop() == 0 and not entered and current == [1]
         current[0] = 0
         with pytest.raises(ValueError, match="cache.* must be"):
             call(rows)

@@ -647,6 +647,10 @@ def test_attention_refuses():
     odd = torch.empty(q.numel() + 1, dtype=torch.float16, device=DEV)[1:].view(q.shape)
     with pytest.raises(ValueError, match="misaligned"):
         attend(odd, cache, meta, c.scale)
+    for change in (dict(num_decode=3), dict(num_decode=-1), dict(query_start_loc=meta.query_start_loc[:2]),
+                   dict(block_tables=meta.block_tables[:1])):
+        with pytest.raises(ValueError, match="metadata of 2"):
+            attend(q, cache, dataclasses.replace(meta, **change), c.scale)
     assert attend(q[:0], cache, meta, c.scale).shape == (0, 256)
 
 

@@ -729,12 +729,6 @@ def _int8_args(what: str, k_cache, v_cache, k_scale, v_scale, meta, device) -> t
     for s in (k_scale, v_scale):
         _require(s.dtype == torch.float32 and s.shape == (NB, KVH) and s.is_contiguous(),
                  "{}: scales must be contiguous fp32 [num_blocks, KVH]", what)
-    return NB, KVH, D, *_step_args(what, meta, device, k_cache, v_cache, k_scale, v_scale)
-
-
-def _step_args(what: str, meta, device, *caches) -> tuple:
-    """Checks of the step's metadata and the tensors' devices; (block tables, seq_lens, query_start_loc,
-    table stride)."""
     bt = meta.block_tables
     if bt.dtype != torch.int32 or bt.stride(1) != 1:
         bt = bt.to(torch.int32).contiguous()
@@ -742,9 +736,9 @@ def _step_args(what: str, meta, device, *caches) -> tuple:
     B = sl.shape[0]
     _require(bt.shape[0] >= B and qsl.shape[0] >= B + 1 and 0 <= meta.num_decode <= B,
              "{}: metadata of {} sequences", what, B)
-    for t in (*caches, bt, sl, qsl):
+    for t in (k_cache, v_cache, k_scale, v_scale, bt, sl, qsl):
         _require(t.device == device, "{}: every tensor must live on the same GPU", what)
-    return bt, sl, qsl, bt.stride(0) if bt.shape[0] > 1 else bt.shape[1]
+    return NB, KVH, D, bt, sl, qsl, bt.stride(0) if bt.shape[0] > 1 else bt.shape[1]
 
 
 def _elsewhere(t: torch.Tensor) -> bool:
@@ -862,23 +856,48 @@ def paged_attention_int8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
 # ------------------------------------------------------------------------------------------
 # The 4-bit paged cache: codes with a step and a low for each row and group of 32 channels
 # ------------------------------------------------------------------------------------------
+# These wrappers are most of a small eager call's time, so they ask tensors for as little as they can:
+# device numbers (-1: not on a GPU) in place of device objects, strides at once, no calls for checks that hold.
 def _int4_cache(what: str, k_cache: torch.Tensor, v_cache: torch.Tensor) -> tuple[int, int, int]:
     """Checks of one layer's caches; (NB, KVH, D)."""
     shape = k_cache.shape
     D = int4_head_dim(shape[2]) if len(shape) == 3 else None
     if D is None or shape != v_cache.shape:
         raise ValueError(f"{what}: caches must be [num_blocks, KVH, unit bytes], got {tuple(shape)}")
-    _require(k_cache.dtype == torch.uint8 and v_cache.dtype == torch.uint8 and
-             k_cache.is_contiguous() and v_cache.is_contiguous(),
-             "{}: caches must be contiguous uint8", what)
+    if not (k_cache.dtype == v_cache.dtype == torch.uint8 and k_cache.is_contiguous() and v_cache.is_contiguous()):
+        raise ValueError(f"{what}: caches must be contiguous uint8")
     return shape[0], shape[1], D
 
 
-def _slots(what: str, slot_mapping: torch.Tensor, T: int, device) -> torch.Tensor:
-    _require(slot_mapping.shape[0] >= T, "{}: slot_mapping shorter than the rows", what)
-    _require(slot_mapping.device == device, "{}: every tensor must live on the same GPU", what)
+def _slots(what: str, slot_mapping: torch.Tensor, T: int, device: int) -> torch.Tensor:
+    if slot_mapping.shape[0] < T:
+        raise ValueError(f"{what}: slot_mapping shorter than the rows")
+    if slot_mapping.get_device() != device:
+        raise ValueError(f"{what}: every tensor must live on the same GPU")
     return slot_mapping if (slot_mapping.dtype == torch.int64 and slot_mapping.is_contiguous()) \
         else slot_mapping.to(torch.int64).contiguous()
+
+
+def _int4_meta(what: str, meta) -> tuple:
+    """A step's block tables, seq_lens and query_start_loc as the kernels take them, the number of
+    sequences and of those at the front that decode."""
+    bt, sl, qsl, S = meta.block_tables, _i32(meta.seq_lens), _i32(meta.query_start_loc), int(meta.num_decode)
+    if bt.dtype != torch.int32 or bt.stride(1) != 1:
+        bt = bt.to(torch.int32).contiguous()
+    B = sl.shape[0]
+    if bt.shape[0] < B or qsl.shape[0] <= B or not 0 <= S <= B:
+        raise ValueError(f"{what}: metadata of {B} sequences")
+    return bt, sl, qsl, B, S
+
+
+def _on_gpu(what: str, *ts: torch.Tensor) -> int:
+    """The tensors' GPU."""
+    device = ts[0].get_device()
+    for t in ts:
+        if t.get_device() != device or device < 0:
+            raise ValueError(f"{what}: every tensor must live on the same GPU" if device >= 0 else
+                             "hip backend: every tensor must live on the GPU")
+    return device
 
 
 def kv_write_int4(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -893,20 +912,25 @@ def kv_write_int4(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cac
     T, KVH, D = k.shape
     if T == 0:
         return
-    _check_gpu(k, v)
-    if _elsewhere(k):
-        with torch.cuda.device(k.device):
+    device = _on_gpu("kv_write_int4", k, v)
+    if device != torch._C._cuda_getDevice():
+        with torch.cuda.device(device):
             return kv_write_int4(k, v, k_cache, v_cache, slot_mapping)
     NB, ckvh, cd = _int4_cache("kv_write_int4", k_cache, v_cache)
-    _require(v.shape == k.shape and ckvh == KVH and cd == D, "kv_write_int4: shape mismatch")
-    _require(k.dtype == torch.float16 and v.dtype == torch.float16 and k.stride(2) == 1 and
-             v.stride(2) == 1, "kv_write_int4: k, v must be fp16 with unit stride over D")
-    _require(v.device == k_cache.device == v_cache.device == k.device,
-             "kv_write_int4: every tensor must live on the same GPU")
-    slots = _slots("kv_write_int4", slot_mapping, T, k.device)
-    N.check(N.lib().ts_kv_write_int4(
-        _ptr(k), _ptr(v), *_row_strides(k), *_row_strides(v), _ptr(k_cache), _ptr(v_cache), NB,
-        _ptr(slots), T, KVH, D, _stream(k)), "kv_write_int4")
+    _on_gpu("kv_write_int4", k, k_cache, v_cache)
+    ks, vs = k.stride(), v.stride()
+    if v.shape != k.shape or ckvh != KVH or cd != D:
+        raise ValueError("kv_write_int4: shape mismatch")
+    if not (k.dtype == v.dtype == torch.float16 and ks[2] == 1 and vs[2] == 1):
+        raise ValueError("kv_write_int4: k, v must be fp16 with unit stride over D")
+    slots = _slots("kv_write_int4", slot_mapping, T, device)
+    # (strides of an axis of one element name no address, and may be anything)
+    status = N.lib().ts_kv_write_int4(
+        k.data_ptr(), v.data_ptr(), ks[0] if T > 1 else KVH * D, ks[1] if KVH > 1 else D,
+        vs[0] if T > 1 else KVH * D, vs[1] if KVH > 1 else D, k_cache.data_ptr(), v_cache.data_ptr(), NB,
+        slots.data_ptr(), T, KVH, D, torch._C._cuda_getCurrentRawStream(device))
+    if status:
+        N.check(status, "kv_write_int4")
 
 
 def rope_kv_write_int4(qkv: torch.Tensor, positions: torch.Tensor, cos: torch.Tensor,
@@ -916,33 +940,36 @@ def rope_kv_write_int4(qkv: torch.Tensor, positions: torch.Tensor, cos: torch.Te
     tables cos / sin [max_len, D / 2]), in one launch with the rotation of q, which is returned as
     [T, H, D]; qkv [T, (H + 2 KVH) D] is left as it is. Rotations are computed wider than fp16 and
     rounded once: q to fp16, k straight to its code."""
-    _check_gpu(qkv, positions, cos, sin)
-    if _elsewhere(qkv):
-        with torch.cuda.device(qkv.device):
+    device = _on_gpu("rope_kv_write_int4", qkv, positions, cos, sin)
+    if device != torch._C._cuda_getDevice():
+        with torch.cuda.device(device):
             return rope_kv_write_int4(qkv, positions, cos, sin, H, KVH, D, k_cache, v_cache, slot_mapping)
-    T = qkv.shape[0]
-    _require(qkv.dim() == 2 and qkv.stride(1) == 1 and qkv.dtype == torch.float16 and
-             qkv.shape[1] >= (H + 2 * KVH) * D,
-             "rope_kv_write_int4: qkv must be fp16 [T, (H + 2 KVH) D]")
-    q = torch.empty(T, H, D, dtype=qkv.dtype, device=qkv.device)
+    shape, qs = qkv.shape, qkv.stride()
+    if len(shape) != 2 or qs[1] != 1 or qkv.dtype != torch.float16 or shape[1] < (H + 2 * KVH) * D:
+        raise ValueError("rope_kv_write_int4: qkv must be fp16 [T, (H + 2 KVH) D]")
+    T = shape[0]
+    q = torch.empty(T, H, D, dtype=torch.float16, device=qkv.device)
     if T == 0:
         return q
     NB, ckvh, cd = _int4_cache("rope_kv_write_int4", k_cache, v_cache)
-    _require(ckvh == KVH and cd == D, "rope_kv_write_int4: cache shape mismatch")
-    _require(cos.dtype == torch.float32 and sin.dtype == torch.float32 and cos.is_contiguous()
-             and sin.is_contiguous() and cos.shape == sin.shape and cos.dim() == 2 and
-             cos.shape[1] == D // 2,
-             "rope_kv_write_int4: tables must be contiguous fp32 [max_len, D / 2]")
-    _require(positions.shape[0] >= T and positions.device == qkv.device == cos.device == sin.device
-             == k_cache.device == v_cache.device,
-             "rope_kv_write_int4: positions shorter than qkv, or tensors of several devices")
+    _on_gpu("rope_kv_write_int4", qkv, k_cache, v_cache)
+    if ckvh != KVH or cd != D:
+        raise ValueError("rope_kv_write_int4: cache shape mismatch")
+    cshape = cos.shape
+    if not (cos.dtype == sin.dtype == torch.float32 and cos.is_contiguous() and sin.is_contiguous()
+            and cshape == sin.shape and len(cshape) == 2 and cshape[1] == D // 2):
+        raise ValueError("rope_kv_write_int4: tables must be contiguous fp32 [max_len, D / 2]")
+    if positions.shape[0] < T:
+        raise ValueError("rope_kv_write_int4: positions shorter than qkv")
     pos = positions if (positions.dtype == torch.int64 and positions.is_contiguous()) \
         else positions.to(torch.int64).contiguous()
-    slots = _slots("rope_kv_write_int4", slot_mapping, T, qkv.device)
-    N.check(N.lib().ts_rope_kv_write_int4(
-        _ptr(qkv), qkv.stride(0) if T > 1 else (H + 2 * KVH) * D, _ptr(pos), _ptr(cos), _ptr(sin),
-        cos.shape[0], _ptr(q), _ptr(k_cache), _ptr(v_cache), NB, _ptr(slots), T, H, KVH, D,
-        _stream(qkv)), "rope_kv_write_int4")
+    slots = _slots("rope_kv_write_int4", slot_mapping, T, device)
+    status = N.lib().ts_rope_kv_write_int4(
+        qkv.data_ptr(), qs[0] if T > 1 else (H + 2 * KVH) * D, pos.data_ptr(), cos.data_ptr(), sin.data_ptr(),
+        cshape[0], q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), NB, slots.data_ptr(), T, H, KVH, D,
+        torch._C._cuda_getCurrentRawStream(device))
+    if status:
+        N.check(status, "rope_kv_write_int4")
     return q
 
 
@@ -951,23 +978,26 @@ def kv_read_int4(cache: torch.Tensor, blocks: torch.Tensor) -> torch.Tensor:
     layers) stand for, as the fp16 cache [L, 2, n, KVH, 16, D] whose block i is blocks[i]: attention over
     it with tables renumbered so is attention over the 4-bit cache. Ids outside the cache read
     block 0."""
-    _check_gpu(cache, blocks)
-    if _elsewhere(cache):
-        with torch.cuda.device(cache.device):
+    device = _on_gpu("kv_read_int4", cache, blocks)
+    if device != torch._C._cuda_getDevice():
+        with torch.cuda.device(device):
             return kv_read_int4(cache, blocks)
-    D = int4_head_dim(cache.shape[4]) if cache.dim() == 5 and cache.shape[1] == 2 else None
-    _require(D is not None and cache.dtype == torch.uint8 and cache.is_contiguous(),
-             "kv_read_int4: cache must be contiguous uint8 [L, 2, num_blocks, KVH, unit bytes], got {}",
-             tuple(cache.shape))
-    _require(blocks.dim() == 1 and blocks.device == cache.device,
-             "kv_read_int4: blocks must be [n] on the cache's GPU")
-    L, _, NB, KVH, _ = cache.shape
+    shape = cache.shape
+    D = int4_head_dim(shape[4]) if len(shape) == 5 and shape[1] == 2 else None
+    if D is None or cache.dtype != torch.uint8 or not cache.is_contiguous():
+        raise ValueError("kv_read_int4: cache must be contiguous uint8 [L, 2, num_blocks, KVH, unit bytes], "
+                         f"got {tuple(shape)}")
+    if blocks.dim() != 1:
+        raise ValueError("kv_read_int4: blocks must be [n]")
+    L, _, NB, KVH, _ = shape
     if blocks.dtype != torch.int32:                        # (ids past 31 bits must not wrap into the cache)
         blocks = blocks.clamp(-1, min(NB, 2 ** 31 - 1)).to(torch.int32)
     ids, n = blocks.contiguous(), blocks.shape[0]
     out = torch.empty(L, 2, n, KVH, 16, D, dtype=torch.float16, device=cache.device)
-    N.check(N.lib().ts_kv_read_int4(_ptr(cache), L, NB, KVH, D, _ptr(ids), n, _ptr(out),
-                                    _stream(cache)), "kv_read_int4")
+    status = N.lib().ts_kv_read_int4(cache.data_ptr(), L, NB, KVH, D, ids.data_ptr(), n, out.data_ptr(),
+                                     torch._C._cuda_getCurrentRawStream(device))
+    if status:
+        N.check(status, "kv_read_int4")
     return out
 
 
@@ -980,22 +1010,27 @@ def paged_attention_int4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     T, H, D = q.shape
     if T == 0:
         return torch.empty(0, H * D, dtype=q.dtype, device=q.device)
-    _check_gpu(q)
-    if _elsewhere(q):
-        with torch.cuda.device(q.device):
+    device = _on_gpu("paged_attention_int4", q)
+    if device != torch._C._cuda_getDevice():
+        with torch.cuda.device(device):
             return paged_attention_int4(q, k_cache, v_cache, meta, scale)
-    out = torch.empty(T, H * D, dtype=q.dtype, device=q.device)
     NB, KVH, cd = _int4_cache("paged_attention_int4", k_cache, v_cache)
-    bt, sl, qsl, bt_st = _step_args("paged_attention_int4", meta, q.device, k_cache, v_cache)
-    _require(cd == D and q.stride(2) == 1 and q.dtype == torch.float16,
-             "paged_attention_int4: q must be fp16 [T, H, D] with unit stride over D")
-    B, S = sl.shape[0], meta.num_decode
+    qs = q.stride()
+    if cd != D or qs[2] != 1 or q.dtype != torch.float16:
+        raise ValueError("paged_attention_int4: q must be fp16 [T, H, D] with unit stride over D")
+    bt, sl, qsl, B, S = _int4_meta("paged_attention_int4", meta)
+    rows, width = bt.shape
+    _on_gpu("paged_attention_int4", q, k_cache, v_cache, bt, sl, qsl)
+    out = torch.empty(T, H * D, dtype=torch.float16, device=q.device)
+    L = N.lib()
     bounds = (int(meta.max_query_len), int(meta.max_seq_len), _prefill_seq_bound(meta))
-    ws_bytes = N.lib().ts_paged_attention_int4_workspace_bytes(B, S, *bounds, H, KVH, D,
-                                                               N.cu_count(q.device.index or 0))
+    ws_bytes = L.ts_paged_attention_int4_workspace_bytes(B, S, *bounds, H, KVH, D, N.cu_count(device))
     ws = _workspace(ws_bytes, q.device)
-    N.check(N.lib().ts_paged_attention_int4(
-        _ptr(q), *_row_strides(q), _ptr(out), H * D, T, _ptr(k_cache), _ptr(v_cache), NB, _ptr(bt),
-        bt_st, bt.shape[1], _ptr(sl), _ptr(qsl), B, S, *bounds, H, KVH, D, float(scale), _ptr(ws),
-        ws_bytes, _stream(q)), "paged_attention_int4")
+    status = L.ts_paged_attention_int4(
+        q.data_ptr(), qs[0] if T > 1 else H * D, qs[1] if H > 1 else D, out.data_ptr(), H * D, T,
+        k_cache.data_ptr(), v_cache.data_ptr(), NB, bt.data_ptr(), bt.stride(0) if rows > 1 else width, width,
+        sl.data_ptr(), qsl.data_ptr(), B, S, *bounds, H, KVH, D, float(scale), _ptr(ws), ws_bytes,
+        torch._C._cuda_getCurrentRawStream(device))
+    if status:
+        N.check(status, "paged_attention_int4")
     return out

@@ -8,7 +8,7 @@ to fp32 is exact).
 
 from __future__ import annotations
 
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 
 import torch
 
@@ -115,7 +115,7 @@ def int4_views(cache: torch.Tensor, values: bool) -> tuple[torch.Tensor, torch.T
     return codes.unflatten(-1, (D // 8, 16, 4)).transpose(-3, -2), steps, lows
 
 
-@dataclass
+@dataclass(frozen=True)
 class Int4KVCache:
     """The 4-bit paged KV cache of every layer: uint8 [L, 2, num_blocks, KVH, bytes], the bytes of a block
     of one KV head holding its 16 rows' codes and, for each row and group of 32 channels, fp16 step
@@ -123,6 +123,10 @@ class Int4KVCache:
     KVH * 1.25 D bytes (1.5 D at head_dim 16) where fp16 takes KVH * 4 D."""
 
     data: torch.Tensor
+    layers: tuple = field(init=False, repr=False, compare=False)     # (k_cache, v_cache) of each layer
+
+    def __post_init__(self) -> None:
+        object.__setattr__(self, "layers", tuple(tuple(x.unbind()) for x in self.data.unbind()))
 
     @classmethod
     def new(cls, num_layers: int, num_blocks: int, num_kv_heads: int, head_dim: int,
@@ -137,5 +141,5 @@ class Int4KVCache:
         return self.data.device
 
     def layer(self, index: int) -> tuple[torch.Tensor, torch.Tensor]:
-        """(k_cache, v_cache) of one layer, as the ops take them."""
-        return self.data[index, 0], self.data[index, 1]
+        """(k_cache, v_cache) of one layer, views of data, as the ops take them."""
+        return self.layers[index]
