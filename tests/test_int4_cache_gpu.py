@@ -375,6 +375,25 @@ def test_decode_rows_do_not_depend_on_the_batch():
         assert torch.equal(attend(q[i:i + 1], cache, one, c.scale)[0], whole[i])
 
 
+@pytest.mark.parametrize("heads", [(12, 2, 128), (4, 1, 256), (14, 2, 64), (4, 2, 16)])
+def test_one_decode_row_over_tables_of_any_width(heads):
+    """One sequence's splits start up to 15 blocks before a multiple of 16, or anywhere (past 1024 blocks):
+    lengths at those edges, over tables that end with the sequence or before it, among foreign ids."""
+    for n in (0, 1, 16, 17, 256, 257, 271, 273, 289, 545, 1009, 4081, 16384, 16385, 16700):
+        c = Case(heads, [(max(n - 1, 0), 1)], num_decode=1, seed=n)
+        c.lens[:] = n
+        _, q, _, _, cache, meta = c.on(DEV)
+        want = c.cache
+        assert_rows(attend(q, cache, meta, c.scale), c, f"{n} tokens", cache=want)
+        if n > 32:
+            c.tables = np.ascontiguousarray(c.tables[:, :n // 16 - 1])
+            bad = torch.from_numpy(c.tables).to(DEV)
+            bad[0, 1], bad[0, -1] = c.NB + 7, -1
+            c.tables[0, 1] = c.tables[0, -1] = 0
+            m = dataclasses.replace(meta, block_tables=bad)
+            assert_rows(attend(q, cache, m, c.scale), c, f"{n} tokens, fewer blocks", cache=want)
+
+
 def test_decode_of_more_rows_than_a_lookup_holds():
     """300 sequences, some empty: rows without tokens are zeros."""
     lens = [(7 * i) % 40 for i in range(300)]

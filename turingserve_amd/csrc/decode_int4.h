@@ -191,20 +191,28 @@ __device__ __forceinline__ void i4_step(const I4Bits& k, I8State<D>& st, const I
   next_v();
 }
 
+// Entries of a sequence's table from block `from` on, one a lane, loaded ahead of its length.
+struct I4Window {
+  int from, entry;
+};
+
 // One split [b0, b1) of a sequence's blocks by one wavefront (of kI4Waves). Blocks are taken 64 at a
-// time: lane i holds block i's id.
-template <int D>
+// time: lane i holds block i's id (i + from's that of a window that holds the split).
+template <int D, bool DIRECT>
 __device__ __forceinline__ void i4_split(const Int8DecodeArgs& a, I8State<D>& st, const I8Query<D>& q, int b, int h,
-                                         int b0, int b1, int len, int vis, int least, int wave) {
+                                         int b0, int b1, int len, int vis, int least, int wave, I4Window ahead) {
   const int lane = threadIdx.x % kWave, c = lane % 16, g = lane / 16;
   const int32_t* table = a.block_tables + b * a.bt_stride;
   const uint8_t *kc = reinterpret_cast<const uint8_t*>(a.kc), *vc = reinterpret_cast<const uint8_t*>(a.vc);
   for (int lo = b0; lo < b1; lo += kWave) {
     const int n = min(b1 - lo, kWave);
-    int blk = 0;
-    if (lane < n) blk = clamp_block(table[lo + lane], a.num_blocks);
+    int blk = 0, first = 0;
+    if (DIRECT && b0 >= ahead.from && b1 <= ahead.from + kWave)
+      blk = clamp_block(ahead.entry, a.num_blocks), first = b0 - ahead.from;
+    else if (lane < n)
+      blk = clamp_block(table[lo + lane], a.num_blocks);
     auto unit = [&](int i) {                               // of block i of the 64, or of the last one
-      return ((int64_t)__builtin_amdgcn_readlane(blk, min(i, n - 1)) * a.kvh + h) * I4Unit<D>::BYTES;
+      return ((int64_t)__builtin_amdgcn_readlane(blk, first + min(i, n - 1)) * a.kvh + h) * I4Unit<D>::BYTES;
     };
     constexpr int STEP = 2 * kI4Waves;
     const I4Bits k;
@@ -306,7 +314,10 @@ __device__ __forceinline__ void i4_finish(const Int8DecodeArgs& a, const I8State
 // Workgroups that a CU holds at once, by registers.
 constexpr int i4_decode_groups(int D) { return D > 128 ? 2 : 4; }
 
-template <int D>
+// DIRECT: decode rows of one tile alone, a workgroup for each split that the host's bound allows. It knows its
+// split at once, so that the row of q, the length and the part of the table where the split must lie (as long
+// as splits are of kI4SplitBlocks) are requested together.
+template <int D, bool DIRECT>
 __global__ void __launch_bounds__(kI4Threads, i4_decode_groups(D)) decode_int4_kernel(Int8DecodeArgs a) {
   __shared__ __align__(16) I4DecodeLds<D> lds;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -314,24 +325,40 @@ __global__ void __launch_bounds__(kI4Threads, i4_decode_groups(D)) decode_int4_k
   for (int64_t u = blockIdx.x;; u += gridDim.x) {
     if (u > INT32_MAX) return;                             // (the entry point refuses more)
     const int item = a.by_kvh((int)u), h = (int)u - item * a.kvh;
-    I8Item x;
-    if (!i8_find<kI4SplitBlocks>(a, item, x)) return;
-    const int row0 = 16 * x.tile, rows = min(x.seq.n * a.group - row0, 16), kv = x.seq.kv;
+    I8Item x = {};
+    I4Window ahead = {};
+    if constexpr (DIRECT) {
+      x.b = a.by_splits(item), x.split = item - x.b * a.max_splits, x.tile = 0;
+      if (x.b >= a.num_seqs) return;
+      ahead.from = max(x.split - 1, 0) * kI4SplitBlocks;
+      ahead.entry = a.block_tables[x.b * a.bt_stride + min(ahead.from + lane, a.max_blocks - 1)];
+      x.seq.q0 = x.b, x.seq.n = 1;
+    } else {
+      if (!i8_find<kI4SplitBlocks>(a, item, x)) return;
+    }
+    const int row0 = 16 * x.tile, rows = min(x.seq.n * a.group - row0, 16);
     const int row = row0 + min(c, rows - 1), token = a.by_group(row);
-    const int vis = min(kv, max(0, x.seq.start + token + 1));
-    const int least = min(kv, max(0, x.seq.start + a.by_group(row0) + 1));
     I8Query<D> q;
     i4_load_q<D>(a.q + (int64_t)(x.seq.q0 + token) * a.q_st +
                      (int64_t)(h * a.group + row - token * a.group) * a.q_sh,
                  g, c < rows, q);
+    if constexpr (DIRECT) {
+      x.seq = i8_seq(a, x.b);
+      x.splits = i8_splits<kI4SplitBlocks>(a, x.seq, true);
+      if (x.split >= x.splits) return;
+    }
+    const int kv = x.seq.kv;
+    const int vis = min(kv, max(0, x.seq.start + token + 1));
+    const int least = min(kv, max(0, x.seq.start + a.by_group(row0) + 1));
     I8State<D> st;
     st.m = -INFINITY, st.l = 0.f;
 #pragma unroll
     for (int t = 0; t < D / 16; ++t) st.o[t] = {0.f, 0.f, 0.f, 0.f};
     const int nb = (kv + kBlockSize - 1) / kBlockSize;
     const int b0 = i8_split_begin(nb, x.split, x.splits), b1 = i8_split_begin(nb, x.split + 1, x.splits);
-    i4_split<D>(a, st, q, x.b, h, b0, b1, kv, vis, least, wave);
+    i4_split<D, DIRECT>(a, st, q, x.b, h, b0, b1, kv, vis, least, wave, ahead);
     i4_finish<D>(a, st, x.b, h, x.seq.q0, row0, rows, x.split, x.splits, wave, lds);
+    if constexpr (DIRECT) return;
   }
 }
 

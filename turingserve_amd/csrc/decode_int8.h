@@ -88,7 +88,7 @@ struct Int8DecodeArgs {
   int64_t num_tokens;
   int num_seqs, num_decode;                      // sequences; the first num_decode have one row each
   int heads, kvh, group;                         // group = heads / kvh
-  I8Div by_kvh, by_group, by_slots;
+  I8Div by_kvh, by_group, by_slots, by_splits;   // (by max_splits)
   float sl2;                                     // scale * log2(e)
   // Partials, D floats each and (m, l): max_splits for each row of the first num_decode sequences, then
   // chunk_parts for each (sequence, KV head) of the others, whose rows have as many as they have
@@ -524,6 +524,7 @@ template <int D, int EACH = kI8SplitBlocks>
 __global__ void __launch_bounds__(kI8Threads) decode_int8_merge_kernel(Int8DecodeArgs a) {
   constexpr int PER_ROW = D / 4, GROUPS = kWave / PER_ROW;
   constexpr int N = 64 / GROUPS < 16 ? 64 / GROUPS : 16;   // partials of a lane at a time
+  constexpr int FIRST = N < 8 ? N : 8;                     // of them requested before the length is known
   const int lane = threadIdx.x % kWave;
   const int slot = blockIdx.x * kI8Waves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int behind = slot - a.num_decode * a.heads;        // of the sequences past num_decode
@@ -536,7 +537,8 @@ __global__ void __launch_bounds__(kI8Threads) decode_int8_merge_kernel(Int8Decod
   float4_t x[N];
   auto request = [&](int64_t row, int n) {                 // its first partials, all its (m, l)
     ml = ld<float2_t>(a.part_ml + 2 * (row + min(lane, n - 1)));
-    x[0] = ld<float4_t>(a.part_o + (row + min(group, n - 1)) * D + d);
+#pragma unroll
+    for (int i = 0; i < FIRST; ++i) x[i] = ld<float4_t>(a.part_o + (row + min(group + i * GROUPS, n - 1)) * D + d);
   };
   if (behind < 0) request((int64_t)slot * a.max_splits, a.max_splits);
   const I8Seq seq = i8_seq(a, b);
@@ -553,16 +555,12 @@ __global__ void __launch_bounds__(kI8Threads) decode_int8_merge_kernel(Int8Decod
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int k = i0 + group + i * GROUPS;
-      if ((i > 0 || i0 > 0) && k < splits) x[i] = ld<float4_t>(part + (int64_t)k * D);
+      if ((i >= FIRST || i0 > 0) && k < splits) x[i] = ld<float4_t>(part + (int64_t)k * D);
     }
     if (i0 == 0) {
-      float top = m;
-#pragma unroll
-      for (int k = 1; k < kWave; k <<= 1) top = vmax(top, shfl_xor(top, k));
+      const float top = i8_wave_max(m);                    // (by all lanes: not within the choice below)
       f = m == -INFINITY ? 0.f : fast_exp2(m - top);
-      sum = lane < splits ? f * ml[1] : 0.f;
-#pragma unroll
-      for (int k = 1; k < kWave; k <<= 1) sum += shfl_xor(sum, k);
+      sum = i8_wave_sum(lane < splits ? f * ml[1] : 0.f);
     }
 #pragma unroll
     for (int i = 0; i < N; ++i) {

@@ -75,4 +75,24 @@ __device__ __forceinline__ float i8_most(float x) {        // the largest of 64 
   return __int_as_float(__builtin_amdgcn_readlane(v, kWave - 1));
 }
 
+// Max / sum over all 64 lanes, on the VALU: quads by DPP permutation, then halves of 8 and of 16 mirrored
+// (whose lanes agree by then), then the rows. The pairing, and so every rounding, is that of lanes
+// i ^ 1, 2, 4 .. 32, whose shuffles through the LDS unit take over a hundred cycles each. Every lane takes part.
+template <int CTRL>
+__device__ __forceinline__ float i8_lane(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float i8_wave_max(float v) {
+  v = vmax(v, i8_lane<0xb1>(v));                          // quad: 1 0 3 2
+  v = vmax(v, i8_lane<0x4e>(v));                          // quad: 2 3 0 1
+  v = vmax(v, i8_lane<0x141>(v));                         // row_half_mirror
+  return rows_max(vmax(v, i8_lane<0x140>(v)));            // row_mirror
+}
+__device__ __forceinline__ float i8_wave_sum(float v) {
+  v += i8_lane<0xb1>(v);
+  v += i8_lane<0x4e>(v);
+  v += i8_lane<0x141>(v);
+  return rows_sum(v + i8_lane<0x140>(v));
+}
+
 }  // namespace ts

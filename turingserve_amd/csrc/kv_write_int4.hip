@@ -46,12 +46,6 @@ struct I4Rotation {
   }
 };
 
-// Over the lanes of a group (LANES of a quad), on the VALU.
-template <int CTRL>
-__device__ __forceinline__ float i4_quad(float x) {
-  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true));
-}
-
 // rint((x - low) / step) within 0 .. 15 of 8 channels, as an octet's word. By the reciprocal where that
 // decides it: the quotient is below 31 (a subnormal step may be little more than half the span's fifteenth), the
 // product with v_rcp_f32's result (one unit in the last place) within 31 * 1.5 * 2^-23 < 2^-17 of it, so it
@@ -111,8 +105,8 @@ __device__ __forceinline__ void i4_write_kv(const Int4WriteArgs& a) {
     lo = fminf(lo, x[e]), hi = fmaxf(hi, x[e]);
     bad = bad || !(fabsf(x[e]) <= 65504.f);
   }
-  if constexpr (LANES > 1) lo = fminf(lo, i4_quad<0xb1>(lo)), hi = fmaxf(hi, i4_quad<0xb1>(hi));   // 1 0 3 2
-  if constexpr (LANES > 2) lo = fminf(lo, i4_quad<0x4e>(lo)), hi = fmaxf(hi, i4_quad<0x4e>(hi));   // 2 3 0 1
+  if constexpr (LANES > 1) lo = fminf(lo, i8_lane<0xb1>(lo)), hi = fmaxf(hi, i8_lane<0xb1>(hi));   // 1 0 3 2
+  if constexpr (LANES > 2) lo = fminf(lo, i8_lane<0x4e>(lo)), hi = fmaxf(hi, i8_lane<0x4e>(hi));   // 2 3 0 1
   const uint64_t lost = __ballot(bad), mine = PER == kWave ? ~0ull : ((1ull << PER % kWave) - 1)
                                                                        << (threadIdx.x % kWave / PER * PER);
   half_t low = (half_t)(lo + 0.f);                         // (-0 as 0)
