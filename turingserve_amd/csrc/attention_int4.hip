@@ -9,7 +9,7 @@ struct Int4Kernels {
   static constexpr int kSplitBlocks = kI4SplitBlocks;
 
   template <int D>
-  static void decode(const Int8DecodeArgs& a, int64_t rows, int cus, hipStream_t s) {
+  static void decode(const Int8DecodeArgs& a, int cus, hipStream_t s) {
     // Every split of the batch, at most as many workgroups as the CUs hold; the rest go round. Where all that the
     // host's bound allows fit at once, each knows its split without the lengths (us a pass of four layers of 12/2
     // heads of 128, so and by the lookup: one sequence of 6000 tokens 34.6 / 38.4, four of up to 32768 59.2 / 62.0,
@@ -21,16 +21,11 @@ struct Int4Kernels {
       decode_int4_kernel<D, true><<<(unsigned)units, kI4Threads, 0, s>>>(a);
     else
       decode_int4_kernel<D, false><<<(unsigned)(units < cap ? units : cap), kI4Threads, 0, s>>>(a);
-    if (a.max_splits > 1)
-      decode_int8_merge_kernel<D, kI4SplitBlocks><<<(unsigned)((rows + kI8Waves - 1) / kI8Waves), kI8Threads, 0, s>>>(a);
   }
 
   template <int D>
   static void prefill(const Int8PrefillArgs& p, hipStream_t s) {
-    constexpr int WAVES = i8_prefill_waves(D), ROWS = 32 * WAVES;
-    prefill_int4_kernel<D><<<p.groups, WAVES * kWave, 0, s>>>(p);
-    if (p.groups > 1)
-      prefill_int8_merge_kernel<D, ROWS><<<(p.groups - 1) * (ROWS / kI8MergeRows), 256, 0, s>>>(p);
+    prefill_int4_kernel<D><<<p.groups, i8_prefill_waves(D) * kWave, 0, s>>>(p);
   }
 };
 

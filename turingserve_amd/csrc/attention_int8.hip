@@ -7,22 +7,17 @@ struct Int8Kernels {
   static constexpr int kSplitBlocks = kI8SplitBlocks;
 
   template <int D>
-  static void decode(const Int8DecodeArgs& a, int64_t rows, int cus, hipStream_t s) {
+  static void decode(const Int8DecodeArgs& a, int cus, hipStream_t s) {
     // Every split of the batch, at most as many workgroups as the CUs hold; the rest go round.
     const int64_t most = a.num_seqs > a.num_decode ? INT32_MAX : (int64_t)a.num_decode * a.max_splits;
     const int64_t units = most * a.kvh * ((a.group + 15) / 16);
     const int64_t cap = (int64_t)i8_decode_groups(D) * cus;
     decode_int8_kernel<D><<<(unsigned)(units < cap ? units : cap), kI8Threads, 0, s>>>(a);
-    if (a.max_splits > 1)
-      decode_int8_merge_kernel<D><<<(unsigned)((rows + kI8Waves - 1) / kI8Waves), kI8Threads, 0, s>>>(a);
   }
 
   template <int D>
   static void prefill(const Int8PrefillArgs& p, hipStream_t s) {
-    constexpr int WAVES = i8_prefill_waves(D), ROWS = 32 * WAVES;
-    prefill_int8_kernel<D><<<p.groups, WAVES * kWave, 0, s>>>(p);
-    if (p.groups > 1)
-      prefill_int8_merge_kernel<D, ROWS><<<(p.groups - 1) * (ROWS / kI8MergeRows), 256, 0, s>>>(p);
+    prefill_int8_kernel<D><<<p.groups, i8_prefill_waves(D) * kWave, 0, s>>>(p);
   }
 };
 

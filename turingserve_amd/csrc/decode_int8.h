@@ -521,12 +521,11 @@ __global__ void __launch_bounds__(kI8Threads, i8_decode_groups(D)) decode_int8_k
 // (they lie in the workspace whatever it is), the others at once after it. (A workgroup a row, its
 // eight groups meeting in LDS, took twice as long at 2240 rows of a few splits: 10.5 us.)
 template <int D, int EACH = kI8SplitBlocks>
-__global__ void __launch_bounds__(kI8Threads) decode_int8_merge_kernel(Int8DecodeArgs a) {
+__device__ __forceinline__ void i8_merge_row(const Int8DecodeArgs& a, int slot) {
   constexpr int PER_ROW = D / 4, GROUPS = kWave / PER_ROW;
   constexpr int N = 64 / GROUPS < 16 ? 64 / GROUPS : 16;   // partials of a lane at a time
   constexpr int FIRST = N < 8 ? N : 8;                     // of them requested before the length is known
   const int lane = threadIdx.x % kWave;
-  const int slot = blockIdx.x * kI8Waves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int behind = slot - a.num_decode * a.heads;        // of the sequences past num_decode
   const int unit = behind < 0 ? a.by_group(slot) : a.by_slots(behind);
   const int r = behind < 0 ? slot - unit * a.group : behind - unit * a.row_slots;
@@ -577,6 +576,16 @@ __global__ void __launch_bounds__(kI8Threads) decode_int8_merge_kernel(Int8Decod
   const float inv = sum == 0.f ? 0.f : 1.f / sum;          // (nothing visible)
   const int token = a.by_group(r), head = h * a.group + r - token * a.group;
   st<half4_t>(a.out + (int64_t)(seq.q0 + token) * a.out_st + (int64_t)head * D + d, to_half4(o * inv));
+}
+
+// The wavefront's row, of workgroup `group`.
+__device__ __forceinline__ int i8_merge_slot(int group) {
+  return group * kI8Waves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+}
+
+template <int D, int EACH = kI8SplitBlocks>
+__global__ void __launch_bounds__(kI8Threads) decode_int8_merge_kernel(Int8DecodeArgs a) {
+  i8_merge_row<D, EACH>(a, i8_merge_slot(blockIdx.x));
 }
 
 }  // namespace ts

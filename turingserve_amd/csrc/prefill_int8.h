@@ -759,12 +759,12 @@ prefill_int8_kernel(Int8PrefillArgs p) {
 // looked the tile up; 32 rows a workgroup are 1 to 2 us slower.)
 constexpr int kI8MergeRows = 16;
 template <int D, int ROWS>
-__global__ void __launch_bounds__(256) prefill_int8_merge_kernel(Int8PrefillArgs p) {
+__device__ __forceinline__ void i8_merge_tile(const Int8PrefillArgs& p, int group) {
   constexpr int PER = 256 / (D / 4);                       // rows at a time
   constexpr int R = kI8MergeRows > PER ? kI8MergeRows / PER : 1, N = 4;   // rows of a thread, partials at a time
   const Int8DecodeArgs& a = p.a;
-  const int g = 1 + (int)(blockIdx.x / (ROWS / kI8MergeRows));
-  const int row0 = (int)(blockIdx.x % (ROWS / kI8MergeRows)) * kI8MergeRows;
+  const int g = 1 + group / (ROWS / kI8MergeRows);
+  const int row0 = group % (ROWS / kI8MergeRows) * kI8MergeRows;
   const I8Joint j = p.joints[g];
   if (j.first == j.last || j.row0 + row0 >= j.rows) return;
   const int in = row0 + threadIdx.x / (D / 4), d = threadIdx.x % (D / 4) * 4;
@@ -812,6 +812,18 @@ __global__ void __launch_bounds__(256) prefill_int8_merge_kernel(Int8PrefillArgs
     const int token = a.by_group(row), head = j.h * a.group + row - token * a.group;
     st<half4_t>(a.out + (int64_t)(j.q0 + token) * a.out_st + (int64_t)head * D + d, to_half4(o[r] * f));
   }
+}
+
+template <int D, int ROWS>
+__global__ void __launch_bounds__(256) prefill_int8_merge_kernel(Int8PrefillArgs p) {
+  i8_merge_tile<D, ROWS>(p, blockIdx.x);
+}
+
+// Both merges of a batch that needs both, the tiles' first: `tiles` workgroups of them.
+template <int D, int ROWS, int EACH>
+__global__ void __launch_bounds__(256) int8_merge_kernel(Int8DecodeArgs a, Int8PrefillArgs p, int tiles) {
+  if ((int)blockIdx.x < tiles) return i8_merge_tile<D, ROWS>(p, blockIdx.x);
+  i8_merge_row<D, EACH>(a, i8_merge_slot((int)blockIdx.x - tiles));
 }
 
 }  // namespace ts

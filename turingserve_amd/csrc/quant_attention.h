@@ -1,8 +1,8 @@
 // What the attentions over the quantised paged caches share on the host: how a batch is split between
-// the decode kernel and the prompt kernel, the workspace, the checks and the launches. The formats'
-// kernels come in as a class `Kernels` with decode<D>(args, rows, cus, stream) and
-// prefill<D>(args, stream), and
-// kSplitBlocks, the blocks of a split.
+// the decode kernel and the prompt kernel, the workspace, the checks, the launches, and the merge of both
+// kernels' partials in one launch (two launches: 46.5 us a layer where one takes 43.5, 16 decode rows beside
+// 512 prompt rows on 3000 cached, 12/2 heads of 128, 4 bits). The formats' kernels come in as a class `Kernels` with decode<D>(args, cus, stream) and
+// prefill<D>(args, stream), and kSplitBlocks, the blocks of a split.
 #pragma once
 
 #include "prefill_int8.h"
@@ -22,6 +22,12 @@ namespace ts {
 //   19.1, 4 of 128 on 2048 23.1 / 26.1; above them 16 of 32 on 4096 41.8 / 31.4, one of 64 25.5 / 18.2,
 //   4 of 512 on 1024 43.3 / 36.5; 8/8 heads of 64: 16 of 16 on 4096 27.1 / 41.4; above them 4 of 512 on
 //   1024 33.5 / 28.5; 16/4 heads of 32: 16 of 8 on 4096 19.0 / 24.4, 16 of 32 (128 rows) 33.7 / 26.9.
+// And with the 4-bit cache (the last one is its worst miss):
+//   12/2 heads of 128: 16 chunks of 8 on 4096 30.2 / 41.2, 16 of 21 43.3 / 44.2, 16 of 128 on 512 37.3 / 41.0,
+//   one of 1000 29.7 / 34.9; above the lines one of 42 on 4096 39.9 / 32.6, 16 of 32 65.0 / 47.5, 4 of 512 on
+//   1024 65.1 / 51.1; 14/2 heads of 64: 16 of 8 on 4096 25.6 / 27.5, 16 of 128 on 512 29.7 / 32.9, above one of
+//   64 on 4096 30.9 / 21.7; 8/8 heads of 64: 16 of 21 on 4096 36.3 / 45.3; 28/4 heads of 128, above: 16 of 21
+//   84.8 / 62.8; 14/2 heads of 64: one of 1000 26.4 / 23.6.
 // The choice is one for the batch, by its largest chunk.
 constexpr int kI8ShortRows = 128;
 constexpr int kI8SmallSeq = 2048;
@@ -129,6 +135,23 @@ static size_t quant_workspace_bytes(int num_seqs, int num_decode, int max_query_
                     heads, kvh, head_dim, cus > 0 ? cus : 256).bytes;
 }
 
+// The launches of a batch: `rows` rows for the decode kernel's merge (0: it has no sequences), prompts
+// unless p.groups is 0.
+template <class Kernels, int D>
+static void quant_launch(const Int8DecodeArgs& a, int64_t rows, const Int8PrefillArgs& p, int cus, hipStream_t s) {
+  constexpr int ROWS = 32 * i8_prefill_waves(D), EACH = Kernels::kSplitBlocks;
+  const unsigned row_groups = rows > 0 && a.max_splits > 1 ? (unsigned)((rows + kI8Waves - 1) / kI8Waves) : 0;
+  const unsigned tile_groups = p.groups > 1 ? (unsigned)(p.groups - 1) * (ROWS / kI8MergeRows) : 0;
+  if (rows > 0) Kernels::template decode<D>(a, cus, s);
+  if (p.groups > 0) Kernels::template prefill<D>(p, s);
+  if (row_groups > 0 && tile_groups > 0)
+    int8_merge_kernel<D, ROWS, EACH><<<tile_groups + row_groups, 256, 0, s>>>(a, p, (int)tile_groups);
+  else if (row_groups > 0)
+    decode_int8_merge_kernel<D, EACH><<<row_groups, kI8Threads, 0, s>>>(a);
+  else if (tile_groups > 0)
+    prefill_int8_merge_kernel<D, ROWS><<<tile_groups, 256, 0, s>>>(p);
+}
+
 template <class Kernels, bool SCALES>
 static int quant_attention(const char* what, const QuantCall& c) {
   TS_REQUIRE(c.num_seqs >= 0 && c.num_decode >= 0 && c.num_decode <= c.num_seqs && c.num_decode <= c.num_tokens,
@@ -188,41 +211,32 @@ static int quant_attention(const char* what, const QuantCall& c) {
   a.by_kvh = I8Div::by(c.kvh), a.by_group = I8Div::by(group);
   a.group = group, a.qsl = c.query_start_loc, a.num_tokens = c.num_tokens;
   a.sl2 = c.scale * 1.44269504088896340736f;
-  if (pl.small > 0) {
-    a.num_seqs = pl.small, a.num_decode = c.num_decode;
-    a.row_slots = pl.row_slots, a.max_splits = pl.max_splits, a.chunk_parts = pl.chunk_parts;
-    a.by_slots = I8Div::by(pl.row_slots), a.by_splits = I8Div::by(pl.max_splits);
-    a.part_o = reinterpret_cast<float*>(ws + pl.dec_o);
-    a.part_ml = reinterpret_cast<float*>(ws + pl.dec_ml);
-    const int64_t rows = merge_rows(pl, c.num_decode, c.heads, c.kvh);
-    switch (c.head_dim) {
-      case 16: Kernels::template decode<16>(a, rows, cus, s); break;
-      case 32: Kernels::template decode<32>(a, rows, cus, s); break;
-      case 64: Kernels::template decode<64>(a, rows, cus, s); break;
-      case 128: Kernels::template decode<128>(a, rows, cus, s); break;
-      default: Kernels::template decode<256>(a, rows, cus, s); break;
-    }
-    status = check_launch(what);
-    if (status != TS_OK) return status;
-  }
+  Int8PrefillArgs p = {};
   if (c.num_seqs > pl.small) {
-    Int8PrefillArgs p = {};
     p.a = a;
     p.a.part_o = reinterpret_cast<float*>(ws + pl.pre_o);
     p.a.part_ml = reinterpret_cast<float*>(ws + pl.pre_ml);
     p.joints = reinterpret_cast<I8Joint*>(ws + pl.joints);
     p.num_seqs = c.num_seqs, p.first = pl.small, p.groups = pl.groups;
     p.rate = i8_rate(32 * i8_prefill_waves(c.head_dim), a.group);
-    switch (c.head_dim) {
-      case 16: Kernels::template prefill<16>(p, s); break;
-      case 32: Kernels::template prefill<32>(p, s); break;
-      case 64: Kernels::template prefill<64>(p, s); break;
-      case 128: Kernels::template prefill<128>(p, s); break;
-      default: Kernels::template prefill<256>(p, s); break;
-    }
-    status = check_launch(what);
   }
-  return status;
+  int64_t rows = 0;
+  if (pl.small > 0) {
+    a.num_seqs = pl.small, a.num_decode = c.num_decode;
+    a.row_slots = pl.row_slots, a.max_splits = pl.max_splits, a.chunk_parts = pl.chunk_parts;
+    a.by_slots = I8Div::by(pl.row_slots), a.by_splits = I8Div::by(pl.max_splits);
+    a.part_o = reinterpret_cast<float*>(ws + pl.dec_o);
+    a.part_ml = reinterpret_cast<float*>(ws + pl.dec_ml);
+    rows = merge_rows(pl, c.num_decode, c.heads, c.kvh);
+  }
+  switch (c.head_dim) {
+    case 16: quant_launch<Kernels, 16>(a, rows, p, cus, s); break;
+    case 32: quant_launch<Kernels, 32>(a, rows, p, cus, s); break;
+    case 64: quant_launch<Kernels, 64>(a, rows, p, cus, s); break;
+    case 128: quant_launch<Kernels, 128>(a, rows, p, cus, s); break;
+    default: quant_launch<Kernels, 256>(a, rows, p, cus, s); break;
+  }
+  return check_launch(what);
 }
 
 }  // namespace ts
