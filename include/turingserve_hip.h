@@ -597,7 +597,9 @@ int ts_paged_attention_int8(const void* q, int64_t q_stride_t, int64_t q_stride_
  * low ones first, the channels 0 2 4 6 1 3 5 7; K's words are [16 rows][D / 8], V's [D / 8][16 rows]. Then,
  * for each row and group, two fp16 numbers: K's [16 rows][G][step, low], V's [G][4][step, low][4 rows].
  * A code stands for fp16(low + code * step), rounded once. 1.25 D bytes a row and KV head for K and V
- * (1.5 D at 16) where fp16 takes 4 D. The reference has no such cache; the step's metadata is the same.
+ * (1.5 D at 16) where fp16 takes 4 D. All bytes are zeros to begin with: attention multiplies rows that
+ * it does not see by 0, so they have to be numbers. The reference has no such cache; the step's metadata
+ * is the same.
  *
  * ts_kv_write_int4: for every token t with 0 <= s = slot_mapping[t] < 16 num_blocks, rows k[t] and v[t] go
  * to row s % 16 of block s / 16; other slots are skipped. Per KV head and group, in fp32 rounded to

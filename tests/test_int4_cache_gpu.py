@@ -108,6 +108,9 @@ def test_read_matches_the_oracle(heads):
     far = torch.tensor([2 ** 32 + 1, -2 ** 32 + 2, 2 ** 62], device=DEV)
     got = H.kv_read_int4(cache[1:2], far).cpu().numpy()
     assert np.array_equal(got[0, 0], O.values_of(*O.unpack(both[1, 0], heads[2], False))[[0, 0, 0]])
+    for dtype in (torch.uint8, torch.int8, torch.int16):
+        got = H.kv_read_int4(cache[:1], torch.tensor([3, 1, 100], dtype=dtype, device=DEV)).cpu().numpy()
+        assert np.array_equal(got[0, 1], O.values_of(*O.unpack(both[0, 1], heads[2], True))[[3, 1, 0]])
     wide = torch.tensor(ids, dtype=torch.int32, device=DEV).repeat_interleave(2)[::2]
     assert np.array_equal(H.kv_read_int4(cache, wide).cpu().numpy()[2, 1], O.values_of(
         *O.unpack(both[2, 1], heads[2], True))[real])

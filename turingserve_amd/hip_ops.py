@@ -991,7 +991,7 @@ def kv_read_int4(cache: torch.Tensor, blocks: torch.Tensor) -> torch.Tensor:
         raise ValueError("kv_read_int4: blocks must be [n]")
     L, _, NB, KVH, _ = shape
     if blocks.dtype != torch.int32:                        # (ids past 31 bits must not wrap into the cache)
-        blocks = blocks.clamp(-1, min(NB, 2 ** 31 - 1)).to(torch.int32)
+        blocks = blocks.to(torch.int64).clamp(-1, min(NB, 2 ** 31 - 1)).to(torch.int32)
     ids, n = blocks.contiguous(), blocks.shape[0]
     out = torch.empty(L, 2, n, KVH, 16, D, dtype=torch.float16, device=cache.device)
     status = N.lib().ts_kv_read_int4(cache.data_ptr(), L, NB, KVH, D, ids.data_ptr(), n, out.data_ptr(),
