@@ -11,10 +11,10 @@ struct Int4Kernels {
   template <int D>
   static void decode(const Int8DecodeArgs& a, int cus, hipStream_t s) {
     // Every split of the batch, at most as many workgroups as the CUs hold; the rest go round. Where all that the
-    // host's bound allows fit at once, each knows its split without the lengths (us a pass of four layers of 12/2
-    // heads of 128, so and by the lookup: one sequence of 6000 tokens 34.6 / 38.4, four of up to 32768 59.2 / 62.0,
-    // eight of up to 4000 36.4 / 40.6). Beyond that those past a sequence's end hold up the others: 64 sequences of
-    // up to 4096 83.5 / 60.0.
+    // host's bound allows fit at once, each knows its split without the lengths. Us a pass of four layers of 12/2
+    // heads of 128, so and by the lookup: one sequence of 6000 tokens 34.5 / 38.4, four of 8000 to 32768 62.5 /
+    // 64.8, eight of 500 to 4000 36.5 / 40.4, eight of 500 under a bound of 32768 36.2 / 38.1. Beyond that those
+    // past a sequence's end take the others' places: 64 sequences of up to 4096 72 / 60.
     const int64_t most = a.num_seqs > a.num_decode ? INT32_MAX : (int64_t)a.num_decode * a.max_splits;
     const int64_t units = most * a.kvh * ((a.group + 15) / 16), cap = (int64_t)i4_decode_groups(D) * cus;
     if (a.group <= 16 && units <= cap)

@@ -316,7 +316,10 @@ constexpr int i4_decode_groups(int D) { return D > 128 ? 2 : 4; }
 
 // DIRECT: decode rows of one tile alone, a workgroup for each split that the host's bound allows. It knows its
 // split at once, so that the row of q, the length and the part of the table where the split must lie (as long
-// as splits are of kI4SplitBlocks) are requested together.
+// as splits are of kI4SplitBlocks) are requested together. First splits come first: those past a sequence's
+// end, which a graph's bound leaves many of, are dispatched behind the real ones. A split's (sequence, KV
+// head)s are shifted by its number, and by half of them every 256 workgroups, so that no XCD (a workgroup in
+// eight) and no CU has the splits of one sequence alone.
 template <int D, bool DIRECT>
 __global__ void __launch_bounds__(kI4Threads, i4_decode_groups(D)) decode_int4_kernel(Int8DecodeArgs a) {
   __shared__ __align__(16) I4DecodeLds<D> lds;
@@ -324,16 +327,22 @@ __global__ void __launch_bounds__(kI4Threads, i4_decode_groups(D)) decode_int4_k
   const int lane = threadIdx.x % kWave, c = lane % 16, g = lane / 16;
   for (int64_t u = blockIdx.x;; u += gridDim.x) {
     if (u > INT32_MAX) return;                             // (the entry point refuses more)
-    const int item = a.by_kvh((int)u), h = (int)u - item * a.kvh;
+    int h;
     I8Item x = {};
     I4Window ahead = {};
     if constexpr (DIRECT) {
-      x.b = a.by_splits(item), x.split = item - x.b * a.max_splits, x.tile = 0;
-      if (x.b >= a.num_seqs) return;
+      const int units = a.num_seqs * a.kvh;
+      x.split = a.by_units((int)u);
+      const int first = x.split * units;
+      int unit = (int)u - first + x.split + first / 256 * (units / 2);
+      unit -= a.by_units(unit) * units;
+      x.b = a.by_kvh(unit), h = unit - x.b * a.kvh;
       ahead.from = max(x.split - 1, 0) * kI4SplitBlocks;
       ahead.entry = a.block_tables[x.b * a.bt_stride + min(ahead.from + lane, a.max_blocks - 1)];
       x.seq.q0 = x.b, x.seq.n = 1;
     } else {
+      const int item = a.by_kvh((int)u);
+      h = (int)u - item * a.kvh;
       if (!i8_find<kI4SplitBlocks>(a, item, x)) return;
     }
     const int row0 = 16 * x.tile, rows = min(x.seq.n * a.group - row0, 16);

@@ -88,7 +88,7 @@ struct Int8DecodeArgs {
   int64_t num_tokens;
   int num_seqs, num_decode;                      // sequences; the first num_decode have one row each
   int heads, kvh, group;                         // group = heads / kvh
-  I8Div by_kvh, by_group, by_slots, by_splits;   // (by max_splits)
+  I8Div by_kvh, by_group, by_slots, by_units;    // (by num_seqs kvh)
   float sl2;                                     // scale * log2(e)
   // Partials, D floats each and (m, l): max_splits for each row of the first num_decode sequences, then
   // chunk_parts for each (sequence, KV head) of the others, whose rows have as many as they have

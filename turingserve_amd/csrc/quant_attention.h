@@ -224,7 +224,7 @@ static int quant_attention(const char* what, const QuantCall& c) {
   if (pl.small > 0) {
     a.num_seqs = pl.small, a.num_decode = c.num_decode;
     a.row_slots = pl.row_slots, a.max_splits = pl.max_splits, a.chunk_parts = pl.chunk_parts;
-    a.by_slots = I8Div::by(pl.row_slots), a.by_splits = I8Div::by(pl.max_splits);
+    a.by_slots = I8Div::by(pl.row_slots), a.by_units = I8Div::by((int64_t)pl.small * c.kvh < 1 << 30 ? pl.small * c.kvh : 1);
     a.part_o = reinterpret_cast<float*>(ws + pl.dec_o);
     a.part_ml = reinterpret_cast<float*>(ws + pl.dec_ml);
     rows = merge_rows(pl, c.num_decode, c.heads, c.kvh);
