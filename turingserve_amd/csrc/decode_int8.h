@@ -19,8 +19,8 @@
 // sum each, meet once at the end in LDS, and either write the row or leave a partial (m, l, O) for the
 // merge launch.
 //
-// 64 sequences of 128 to 4096 tokens, 12/2 heads of 128: 12.7 us and 4.7 for the merge, 38 MB of codes
-// and scales (7.7 us at a copy's 5.0 TB/s); one sequence of 6000: 7.1 to 7.9 and 3.8. What bounds it is the chain
+// 64 sequences of 128 to 4096 tokens, 12/2 heads of 128: 12.7 us and 4.1 for the merge, 38 MB of codes
+// and scales (7.7 us at a copy's 5.0 TB/s); one sequence of 6000: 7.1 to 8.2 and 3.8. What bounds it is the chain
 // of a workgroup (lengths, table, scales and codes, LDS, partial) and then that of the merge: taking out
 // a tenth of the loop's arithmetic (O scaled in every step) gained 1 %. Two tiles a workgroup (32 rows of
 // a chunk, 253 registers, two workgroups a CU) took 29.0 us instead of 24.7 at 16 sequences of 5 rows,
@@ -519,7 +519,9 @@ __global__ void __launch_bounds__(kI8Threads, i8_decode_groups(D)) decode_int8_k
 // Rows of sequences with more than one split: one wavefront a row, D / 4 lanes a partial. A decode
 // row's first partials and every split's (m, l) are requested before the sequence's length is known
 // (they lie in the workspace whatever it is), the others at once after it. (A workgroup a row, its
-// eight groups meeting in LDS, took twice as long at 2240 rows of a few splits: 10.5 us.)
+// eight groups meeting in LDS, took twice as long at 2240 rows of a few splits: 10.5 us. One partial ahead
+// of the length and reductions by shuffles: 40.0 us a pass of four layers of one sequence of 6000 in 4 bits,
+// 38.4 so; sixteen ahead no less.)
 template <int D, int EACH = kI8SplitBlocks>
 __device__ __forceinline__ void i8_merge_row(const Int8DecodeArgs& a, int slot) {
   constexpr int PER_ROW = D / 4, GROUPS = kWave / PER_ROW;
