@@ -408,6 +408,27 @@ def test_decode_of_more_rows_than_a_lookup_holds():
     assert not out[torch.tensor(lens, device=DEV) == 0].any()
 
 
+@pytest.mark.parametrize("heads,far", [((8, 8, 64), 1400), ((28, 4, 128), 2800), ((4, 1, 256), 5000)])
+def test_more_splits_than_workgroups(heads, far):
+    """60 sequences, some without tokens, whose splits are more than the chip holds at once: decode rows alone,
+    the same bits as one by one, then half of them as short chunks."""
+    lens = [(far // 15 * i + 7 * i) % far for i in range(60)]
+    c = Case(heads, [(max(n - 1, 0), 1) for n in lens], num_decode=60, seed=54)
+    c.lens[:] = lens
+    assert sum(max(1, -(-n // 256)) for n in lens) * c.KVH > (512 if c.D > 128 else 1024)
+    _, q, _, _, cache, meta = c.on(DEV)
+    out = attend(q, cache, meta, c.scale)
+    assert_rows(out, c, "decode rows")
+    for i in (1, 31, 59):
+        one = dataclasses.replace(meta, seq_lens=meta.seq_lens[i:i + 1], num_decode=1,
+                                  block_tables=meta.block_tables[i:i + 1],
+                                  query_start_loc=meta.query_start_loc[:2])
+        assert torch.equal(attend(q[i:i + 1], cache, one, c.scale)[0], out[i])
+    c = Case(heads, [(max(n - 1, 0), 1 + i % 5 * (i > 29)) for i, n in enumerate(lens)], num_decode=30, seed=55)
+    _, q, _, _, cache, meta = c.on(DEV)
+    assert_rows(attend(q, cache, meta, c.scale), c, "beside chunks")
+
+
 @pytest.mark.parametrize("k_size", [0.0, 1e-4, 30.0, 3000.0])
 def test_decode_of_flat_and_steep_scores(k_size):
     c = Case((12, 2, 128), [(n - 1, 1) for n in (1, 40, 700, 2000)], num_decode=4, seed=15, k_size=k_size)

@@ -14,11 +14,16 @@ struct Int4Kernels {
     // host's bound allows fit at once, each knows its split without the lengths. Us a pass of four layers of 12/2
     // heads of 128, so and by the lookup: one sequence of 6000 tokens 34.5 / 38.4, four of 8000 to 32768 62.5 /
     // 64.8, eight of 500 to 4000 36.5 / 40.4, eight of 500 under a bound of 32768 36.2 / 38.1. Beyond that those
-    // past a sequence's end take the others' places: 64 sequences of up to 4096 72 / 60.
+    // past a sequence's end take the others' places: 64 sequences of up to 4096 72 / 60. A second item's place is
+    // kept for up to 64 sequences, a lane each: those 64 58.4 where a new lookup makes them 60.5, 64 of 2000 to 8000
+    // of 8/8 heads of 64 (two layers) 123 / 131, 48 rows beside a chunk of 512 88.5 / 91. For up to 256, in LDS, it
+    // gained 3 % there and lost as much below.
     const int64_t most = a.num_seqs > a.num_decode ? INT32_MAX : (int64_t)a.num_decode * a.max_splits;
     const int64_t units = most * a.kvh * ((a.group + 15) / 16), cap = (int64_t)i4_decode_groups(D) * cus;
     if (a.group <= 16 && units <= cap)
-      decode_int4_kernel<D, true><<<(unsigned)units, kI4Threads, 0, s>>>(a);
+      decode_int4_direct_kernel<D><<<(unsigned)units, kI4Threads, 0, s>>>(a);
+    else if (a.num_seqs <= kWave)
+      decode_int4_kernel<D, true><<<(unsigned)(units < cap ? units : cap), kI4Threads, 0, s>>>(a);
     else
       decode_int4_kernel<D, false><<<(unsigned)(units < cap ? units : cap), kI4Threads, 0, s>>>(a);
   }

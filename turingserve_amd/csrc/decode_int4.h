@@ -202,14 +202,14 @@ __device__ __forceinline__ void i4_step(const I4Bits& k, I8State<D>& st, const I
   next_v();
 }
 
-// Entries of a sequence's table from block `from` on, one a lane, loaded ahead of its length.
+// Entries of a sequence's table from block `from` on, one a lane, asked for ahead of its split (or none).
 struct I4Window {
-  int from, entry;
+  int from = INT32_MAX, entry = 0;
 };
 
 // One split [b0, b1) of a sequence's blocks by one wavefront (of kI4Waves). Blocks are taken 64 at a
 // time: lane i holds block i's id (i + from's that of a window that holds the split).
-template <int D, bool DIRECT>
+template <int D>
 __device__ __forceinline__ void i4_split(const Int8DecodeArgs& a, I8State<D>& st, const I8Query<D>& q, int b, int h,
                                          int b0, int b1, int len, int vis, int least, int wave, I4Window ahead) {
   const int lane = threadIdx.x % kWave, c = lane % 16, g = lane / 16;
@@ -218,7 +218,7 @@ __device__ __forceinline__ void i4_split(const Int8DecodeArgs& a, I8State<D>& st
   for (int lo = b0; lo < b1; lo += kWave) {
     const int n = min(b1 - lo, kWave);
     int blk = 0, first = 0;
-    if (DIRECT && b0 >= ahead.from && b1 <= ahead.from + kWave)
+    if (b0 >= ahead.from && b1 - ahead.from <= kWave)
       blk = clamp_block(ahead.entry, a.num_blocks), first = b0 - ahead.from;
     else if (lane < n)
       blk = clamp_block(table[lo + lane], a.num_blocks);
@@ -325,60 +325,146 @@ __device__ __forceinline__ void i4_finish(const Int8DecodeArgs& a, const I8State
 // Workgroups that a CU holds at once, by registers.
 constexpr int i4_decode_groups(int D) { return D > 128 ? 2 : 4; }
 
-// DIRECT: decode rows of one tile alone, a workgroup for each split that the host's bound allows. It knows its
-// split at once, so that the row of q, the length and the part of the table where the split must lie (as long
-// as splits are of kI4SplitBlocks) are requested together. First splits come first: those past a sequence's
+// i8_find of up to 64 sequences in two parts: what a lane holds of its sequence, which every wavefront leaves in
+// LDS (all of them the same), and an item's place, so that a workgroup's later items need neither the lengths nor
+// the sums again.
+struct I4Found {
+  int kv, start, q0, n, splits, tiles, sum;                // sum: items up to and with this sequence
+};
+__device__ __forceinline__ I4Found i4_found(const Int8DecodeArgs& a) {
+  const int lane = threadIdx.x % kWave;
+  I4Found f = {};
+  if (lane < a.num_seqs) {
+    const I8Seq s = i8_seq(a, lane);
+    f.kv = s.kv, f.start = s.start, f.q0 = s.q0, f.n = s.n;
+    f.splits = i8_splits<kI4SplitBlocks>(a, s, lane < a.num_decode);
+    f.tiles = (s.n * a.group + 15) / 16;
+  }
+  f.sum = i8_scan(f.splits * f.tiles);
+  return f;
+}
+__device__ __forceinline__ bool i4_pick(const I4Found& f, int item, I8Item& x) {
+  const uint64_t past = __ballot(f.sum > item);
+  if (!past) return false;
+  x.b = __ffsll((unsigned long long)past) - 1;
+  auto of = [&](int v) { return __builtin_amdgcn_readlane(v, x.b); };
+  x.splits = of(f.splits);
+  const unsigned t = of(f.tiles), in = item - (of(f.sum) - x.splits * (int)t);
+  x.split = (int)(t == 1 ? in : in / t), x.tile = (int)(in - x.split * t);
+  x.seq = {of(f.q0), of(f.n), of(f.kv), of(f.start)};
+  return x.split < x.splits;                               // (as i8_find)
+}
+
+// The blocks of an item's split.
+__device__ __forceinline__ void i4_blocks(const I8Item& x, int& b0, int& b1) {
+  const int nb = (x.seq.kv + kBlockSize - 1) / kBlockSize;
+  b0 = i8_split_begin(nb, x.split, x.splits), b1 = i8_split_begin(nb, x.split + 1, x.splits);
+}
+
+// The rows of q of an item of KV head h.
+template <int D>
+__device__ __forceinline__ void i4_query(const Int8DecodeArgs& a, const I8Item& x, int h, I8Query<D>& q) {
+  const int c = threadIdx.x % 16, g = threadIdx.x % kWave / 16;
+  const int row0 = 16 * x.tile, rows = min(x.seq.n * a.group - row0, 16);
+  const int row = row0 + min(c, rows - 1), token = a.by_group(row);
+  i4_load_q<D>(a.q + (int64_t)(x.seq.q0 + token) * a.q_st +
+                   (int64_t)(h * a.group + row - token * a.group) * a.q_sh,
+               g, c < rows, q);
+}
+
+template <int D>
+__device__ __forceinline__ void i4_item(const Int8DecodeArgs& a, const I8Item& x, int h, const I8Query<D>& q,
+                                        const I4Window& ahead, I8State<D>& st, int wave) {
+  const int row0 = 16 * x.tile, rows = min(x.seq.n * a.group - row0, 16), kv = x.seq.kv;
+  const int token = a.by_group(row0 + min((int)threadIdx.x % 16, rows - 1));
+  const int vis = min(kv, max(0, x.seq.start + token + 1));
+  const int least = min(kv, max(0, x.seq.start + a.by_group(row0) + 1));
+  st.m = -INFINITY, st.l = 0.f;
+#pragma unroll
+  for (int t = 0; t < D / 16; ++t) st.o[t] = {0.f, 0.f, 0.f, 0.f};
+  int b0, b1;
+  i4_blocks(x, b0, b1);
+  i4_split<D>(a, st, q, x.b, h, b0, b1, kv, vis, least, wave, ahead);
+}
+template <int D>
+__device__ __forceinline__ void i4_finish(const Int8DecodeArgs& a, const I8Item& x, int h, const I8State<D>& st, int wave,
+                                          I4DecodeLds<D>& lds) {
+  const int row0 = 16 * x.tile;
+  i4_finish<D>(a, st, x.b, h, x.seq.q0, row0, min(x.seq.n * a.group - row0, 16), x.split, x.splits, wave, lds);
+}
+
+// Decode rows of one tile alone, a workgroup for each split that the host's bound allows. It knows its split at
+// once, so that the row of q, the length and the part of the table where the split must lie (as long as
+// splits are of kI4SplitBlocks) are requested together. First splits come first: those past a sequence's
 // end, which a graph's bound leaves many of, are dispatched behind the real ones. A split's (sequence, KV
 // head)s are shifted by its number, and by half of them every 256 workgroups, so that no XCD (a workgroup in
 // eight) and no CU has the splits of one sequence alone.
-template <int D, bool DIRECT>
+template <int D>
+__global__ void __launch_bounds__(kI4Threads, i4_decode_groups(D)) decode_int4_direct_kernel(Int8DecodeArgs a) {
+  __shared__ __align__(16) I4DecodeLds<D> lds;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;
+  const int units = a.num_seqs * a.kvh, u = blockIdx.x;
+  I8Item x;
+  x.split = a.by_units(u), x.tile = 0;
+  const int first = x.split * units;
+  int unit = u - first + x.split + first / 256 * (units / 2);
+  unit -= a.by_units(unit) * units;
+  x.b = a.by_kvh(unit);
+  const int h = unit - x.b * a.kvh;
+  I4Window ahead;
+  ahead.from = max(x.split - 1, 0) * kI4SplitBlocks;
+  ahead.entry = a.block_tables[x.b * a.bt_stride + min(ahead.from + lane, a.max_blocks - 1)];
+  x.seq.q0 = x.b, x.seq.n = 1;
+  I8Query<D> q;
+  i4_query<D>(a, x, h, q);
+  x.seq = i8_seq(a, x.b);
+  x.splits = i8_splits<kI4SplitBlocks>(a, x.seq, true);
+  if (x.split >= x.splits) return;
+  I8State<D> st;
+  i4_item<D>(a, x, h, q, ahead, st, wave);
+  i4_finish<D>(a, x, h, st, wave, lds);
+}
+
+// Every item of a batch, as many workgroups as the CUs hold, which go round. FEW: up to 64 sequences, of which
+// the next item's place and the ids of its blocks are at hand when one ends.
+template <int D, bool FEW>
 __global__ void __launch_bounds__(kI4Threads, i4_decode_groups(D)) decode_int4_kernel(Int8DecodeArgs a) {
   __shared__ __align__(16) I4DecodeLds<D> lds;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int lane = threadIdx.x % kWave, c = lane % 16, g = lane / 16;
-  for (int64_t u = blockIdx.x;; u += gridDim.x) {
-    if (u > INT32_MAX) return;                             // (the entry point refuses more)
-    int h;
-    I8Item x = {};
-    I4Window ahead = {};
-    if constexpr (DIRECT) {
-      const int units = a.num_seqs * a.kvh;
-      x.split = a.by_units((int)u);
-      const int first = x.split * units;
-      int unit = (int)u - first + x.split + first / 256 * (units / 2);
-      unit -= a.by_units(unit) * units;
-      x.b = a.by_kvh(unit), h = unit - x.b * a.kvh;
-      ahead.from = max(x.split - 1, 0) * kI4SplitBlocks;
-      ahead.entry = a.block_tables[x.b * a.bt_stride + min(ahead.from + lane, a.max_blocks - 1)];
-      x.seq.q0 = x.b, x.seq.n = 1;
-    } else {
-      const int item = a.by_kvh((int)u);
-      h = (int)u - item * a.kvh;
+  __shared__ int saved[FEW ? 7 : 1][kWave];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;
+  I8Item x;
+  I4Window ahead;
+  if constexpr (FEW) {
+    const I4Found f = i4_found(a);
+    if (!i4_pick(f, a.by_kvh((int)blockIdx.x), x)) return;
+    saved[0][lane] = f.kv, saved[1][lane] = f.start, saved[2][lane] = f.q0, saved[3][lane] = f.n;
+    saved[4][lane] = f.splits, saved[5][lane] = f.tiles, saved[6][lane] = f.sum;
+  }
+  for (int64_t u = blockIdx.x; u <= INT32_MAX; u += gridDim.x) {     // (the entry point refuses more)
+    const int item = a.by_kvh((int)u), h = (int)u - item * a.kvh;
+    if constexpr (!FEW) {
       if (!i8_find<kI4SplitBlocks>(a, item, x)) return;
     }
-    const int row0 = 16 * x.tile, rows = min(x.seq.n * a.group - row0, 16);
-    const int row = row0 + min(c, rows - 1), token = a.by_group(row);
     I8Query<D> q;
-    i4_load_q<D>(a.q + (int64_t)(x.seq.q0 + token) * a.q_st +
-                     (int64_t)(h * a.group + row - token * a.group) * a.q_sh,
-                 g, c < rows, q);
-    if constexpr (DIRECT) {
-      x.seq = i8_seq(a, x.b);
-      x.splits = i8_splits<kI4SplitBlocks>(a, x.seq, true);
-      if (x.split >= x.splits) return;
-    }
-    const int kv = x.seq.kv;
-    const int vis = min(kv, max(0, x.seq.start + token + 1));
-    const int least = min(kv, max(0, x.seq.start + a.by_group(row0) + 1));
+    i4_query<D>(a, x, h, q);
     I8State<D> st;
-    st.m = -INFINITY, st.l = 0.f;
-#pragma unroll
-    for (int t = 0; t < D / 16; ++t) st.o[t] = {0.f, 0.f, 0.f, 0.f};
-    const int nb = (kv + kBlockSize - 1) / kBlockSize;
-    const int b0 = i8_split_begin(nb, x.split, x.splits), b1 = i8_split_begin(nb, x.split + 1, x.splits);
-    i4_split<D, DIRECT>(a, st, q, x.b, h, b0, b1, kv, vis, least, wave, ahead);
-    i4_finish<D>(a, st, x.b, h, x.seq.q0, row0, rows, x.split, x.splits, wave, lds);
-    if constexpr (DIRECT) return;
+    i4_item<D>(a, x, h, q, ahead, st, wave);
+    const I8Item now = x;
+    bool more = true;
+    if constexpr (FEW) {
+      const int64_t next = u + gridDim.x;
+      const I4Found f = {saved[0][lane], saved[1][lane], saved[2][lane], saved[3][lane],
+                         saved[4][lane], saved[5][lane], saved[6][lane]};
+      more = next <= INT32_MAX && i4_pick(f, a.by_kvh((int)next), x);
+      ahead.from = INT32_MAX;
+      if (more) {
+        int b0, b1;
+        i4_blocks(x, b0, b1);
+        if (b1 > b0) ahead.from = b0, ahead.entry = a.block_tables[x.b * a.bt_stride + min(b0 + lane, b1 - 1)];
+      }
+    }
+    i4_finish<D>(a, now, h, st, wave, lds);
+    if (!more) return;
   }
 }
 
