@@ -10,8 +10,8 @@
 // rounded to fp16, m being the row's running reference, which a new score moves only when it passes it
 // by 2^8; sums and accumulators are fp32.
 //
-// 64 sequences of 128 to 4096 tokens, 12/2 heads of 128: 11.0 us and 4.0 for the merge, 24 MB of cache (4.9 us
-// at a copy's 4.85 TB/s); one sequence of 6000: 5.2 (4.3) and 2.8 (2.3). The large ones are bound by the issue
+// 64 sequences of 128 to 4096 tokens, 12/2 heads of 128: 11.0 us (9.5 at least) and 4.0 for the merge, 24 MB of cache
+// (4.9 us at a copy's 4.85 TB/s); one sequence of 6000: 5.1 (4.2) and 2.8 (2.3). The large ones are bound by the issue
 // of vector instructions, some 400 a pair of blocks at head_dim 128, half of them the widening, four
 // wavefronts a SIMD; the small ones by a workgroup's chain: length and table 1.2 us, first codes 0.75, two
 // pairs 1.8, the wavefronts' meeting and the partial 0.9, then the merge's launch. Twice the blocks a split
@@ -208,10 +208,12 @@ struct I4Window {
 };
 
 // One split [b0, b1) of a sequence's blocks by one wavefront (of kI4Waves). Blocks are taken 64 at a
-// time: lane i holds block i's id (i + from's that of a window that holds the split).
+// time: lane i holds block i's id (i + from's that of a window that holds the split). x is the kernel's: as a local
+// here it took four registers more.
 template <int D>
 __device__ __forceinline__ void i4_split(const Int8DecodeArgs& a, I8State<D>& st, const I8Query<D>& q, int b, int h,
-                                         int b0, int b1, int len, int vis, int least, int wave, I4Window ahead) {
+                                         int b0, int b1, int len, int vis, int least, int wave, I4Window ahead,
+                                         I4Block<D> (&x)[2]) {
   const int lane = threadIdx.x % kWave, c = lane % 16, g = lane / 16;
   const int32_t* table = a.block_tables + b * a.bt_stride;
   const uint8_t *kc = reinterpret_cast<const uint8_t*>(a.kc), *vc = reinterpret_cast<const uint8_t*>(a.vc);
@@ -227,7 +229,6 @@ __device__ __forceinline__ void i4_split(const Int8DecodeArgs& a, I8State<D>& st
     };
     constexpr int STEP = 2 * kI4Waves;
     const I4Bits k;
-    I4Block<D> x[2];
     int i = 2 * wave;
     if (i >= n) continue;
     int64_t at[2] = {unit(i), unit(i + 1)};
@@ -374,7 +375,7 @@ __device__ __forceinline__ void i4_query(const Int8DecodeArgs& a, const I8Item& 
 
 template <int D>
 __device__ __forceinline__ void i4_item(const Int8DecodeArgs& a, const I8Item& x, int h, const I8Query<D>& q,
-                                        const I4Window& ahead, I8State<D>& st, int wave) {
+                                        const I4Window& ahead, I8State<D>& st, int wave, I4Block<D> (&blocks)[2]) {
   const int row0 = 16 * x.tile, rows = min(x.seq.n * a.group - row0, 16), kv = x.seq.kv;
   const int token = a.by_group(row0 + min((int)threadIdx.x % 16, rows - 1));
   const int vis = min(kv, max(0, x.seq.start + token + 1));
@@ -384,7 +385,7 @@ __device__ __forceinline__ void i4_item(const Int8DecodeArgs& a, const I8Item& x
   for (int t = 0; t < D / 16; ++t) st.o[t] = {0.f, 0.f, 0.f, 0.f};
   int b0, b1;
   i4_blocks(x, b0, b1);
-  i4_split<D>(a, st, q, x.b, h, b0, b1, kv, vis, least, wave, ahead);
+  i4_split<D>(a, st, q, x.b, h, b0, b1, kv, vis, least, wave, ahead, blocks);
 }
 template <int D>
 __device__ __forceinline__ void i4_finish(const Int8DecodeArgs& a, const I8Item& x, int h, const I8State<D>& st, int wave,
@@ -421,7 +422,8 @@ __global__ void __launch_bounds__(kI4Threads, i4_decode_groups(D)) decode_int4_d
   x.splits = i8_splits<kI4SplitBlocks>(a, x.seq, true);
   if (x.split >= x.splits) return;
   I8State<D> st;
-  i4_item<D>(a, x, h, q, ahead, st, wave);
+  I4Block<D> blocks[2];
+  i4_item<D>(a, x, h, q, ahead, st, wave, blocks);
   i4_finish<D>(a, x, h, st, wave, lds);
 }
 
@@ -448,7 +450,8 @@ __global__ void __launch_bounds__(kI4Threads, i4_decode_groups(D)) decode_int4_k
     I8Query<D> q;
     i4_query<D>(a, x, h, q);
     I8State<D> st;
-    i4_item<D>(a, x, h, q, ahead, st, wave);
+    I4Block<D> blocks[2];
+    i4_item<D>(a, x, h, q, ahead, st, wave, blocks);
     const I8Item now = x;
     bool more = true;
     if constexpr (FEW) {

@@ -5,7 +5,7 @@
 // way to LDS; there are no scales left over, so a score's exponent is one product-sum, P = 2^(s - m), and a
 // row's sum is that of its P.
 //
-// 2048 rows on 4096 cached, 12/2 heads of 128: 88.5 us, 0.73 PFLOP/s (a product of 8192^3 in fp16 reaches 1.09),
+// 2048 rows on 4096 cached, 12/2 heads of 128: 84.3 to 88.5 us, 0.73 to 0.76 PFLOP/s (a product of 8192^3 in fp16 reaches 1.09),
 // and 9.2 for the merge; the 8-bit kernel 84.9 and 9.5. Bound as that one: matrix units, vector units and LDS
 // are each busy about two fifths of the time, in two wavefronts a SIMD. Five ragged prompts of 90 to 1100 rows,
 // 14/2 heads of 64: 25.0 and 4.9 us, a tile's start before some eight steps. Without effect (a pass of two
