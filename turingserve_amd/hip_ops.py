@@ -14,6 +14,8 @@ block_m) are accepted and ignored: the HIP kernels fix their own tile shapes.
 
 from __future__ import annotations
 
+import functools
+
 import torch
 import torch.nn.functional as F
 
@@ -881,13 +883,24 @@ def _slots(what: str, slot_mapping: torch.Tensor, T: int, device: int) -> torch.
 def _int4_meta(what: str, meta) -> tuple:
     """A step's block tables, seq_lens and query_start_loc as the kernels take them, the number of
     sequences and of those at the front that decode."""
-    bt, sl, qsl, S = meta.block_tables, _i32(meta.seq_lens), _i32(meta.query_start_loc), int(meta.num_decode)
-    if bt.dtype != torch.int32 or bt.stride(1) != 1:
-        bt = bt.to(torch.int32).contiguous()
+    int32 = torch.int32
+    bt, sl, qsl, S = meta.block_tables, meta.seq_lens, meta.query_start_loc, int(meta.num_decode)
+    if sl.dtype != int32 or not sl.is_contiguous():
+        sl = _i32(sl)
+    if qsl.dtype != int32 or not qsl.is_contiguous():
+        qsl = _i32(qsl)
+    if bt.dtype != int32 or bt.stride(1) != 1:
+        bt = bt.to(int32).contiguous()
     B = sl.shape[0]
     if bt.shape[0] < B or qsl.shape[0] <= B or not 0 <= S <= B:
         raise ValueError(f"{what}: metadata of {B} sequences")
     return bt, sl, qsl, B, S
+
+
+@functools.lru_cache(maxsize=1024)
+def _int4_workspace_bytes(*sizes: int) -> int:
+    """Of these sizes alone; a step's layers have the same."""
+    return N.lib().ts_paged_attention_int4_workspace_bytes(*sizes)
 
 
 def _on_gpu(what: str, *ts: torch.Tensor) -> int:
@@ -1010,9 +1023,9 @@ def paged_attention_int4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     T, H, D = q.shape
     if T == 0:
         return torch.empty(0, H * D, dtype=q.dtype, device=q.device)
-    device = _on_gpu("paged_attention_int4", q)
-    if device != torch._C._cuda_getDevice():
-        with torch.cuda.device(device):
+    device = q.get_device()
+    if device < 0 or device != torch._C._cuda_getDevice():
+        with torch.cuda.device(_on_gpu("paged_attention_int4", q)):
             return paged_attention_int4(q, k_cache, v_cache, meta, scale)
     NB, KVH, cd = _int4_cache("paged_attention_int4", k_cache, v_cache)
     qs = q.stride()
@@ -1022,15 +1035,14 @@ def paged_attention_int4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     rows, width = bt.shape
     _on_gpu("paged_attention_int4", q, k_cache, v_cache, bt, sl, qsl)
     out = torch.empty(T, H * D, dtype=torch.float16, device=q.device)
-    L = N.lib()
     bounds = (int(meta.max_query_len), int(meta.max_seq_len), _prefill_seq_bound(meta))
-    ws_bytes = L.ts_paged_attention_int4_workspace_bytes(B, S, *bounds, H, KVH, D, N.cu_count(device))
-    ws = _workspace(ws_bytes, q.device)
-    status = L.ts_paged_attention_int4(
+    ws_bytes = _int4_workspace_bytes(B, S, *bounds, H, KVH, D, N.cu_count(device))
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
+    status = N.lib().ts_paged_attention_int4(
         q.data_ptr(), qs[0] if T > 1 else H * D, qs[1] if H > 1 else D, out.data_ptr(), H * D, T,
         k_cache.data_ptr(), v_cache.data_ptr(), NB, bt.data_ptr(), bt.stride(0) if rows > 1 else width, width,
-        sl.data_ptr(), qsl.data_ptr(), B, S, *bounds, H, KVH, D, float(scale), _ptr(ws), ws_bytes,
-        torch._C._cuda_getCurrentRawStream(device))
+        sl.data_ptr(), qsl.data_ptr(), B, S, *bounds, H, KVH, D, float(scale),
+        ws.data_ptr() if ws_bytes else None, ws_bytes, torch._C._cuda_getCurrentRawStream(device))
     if status:
         N.check(status, "paged_attention_int4")
     return out
