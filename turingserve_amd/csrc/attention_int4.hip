@@ -43,8 +43,8 @@ extern "C" size_t ts_paged_attention_int4_workspace_bytes(int32_t num_seqs, int3
                                                           int32_t max_prefill_seq_len,
                                                           int32_t num_heads, int32_t num_kv_heads,
                                                           int32_t head_dim, int32_t cu_count) {
-  return quant_workspace_bytes<Int4Kernels>(num_seqs, num_decode, max_query_len, max_seq_len, max_prefill_seq_len, num_heads,
-                               num_kv_heads, head_dim, cu_count);
+  return quant_workspace_bytes<Int4Kernels>(num_seqs, num_decode, max_query_len, max_seq_len, max_prefill_seq_len,
+                                            num_heads, num_kv_heads, head_dim, cu_count);
 }
 
 extern "C" int ts_paged_attention_int4(const void* q, int64_t q_stride_t, int64_t q_stride_h, void* out,

@@ -388,8 +388,8 @@ __device__ __forceinline__ void i4_item(const Int8DecodeArgs& a, const I8Item& x
   i4_split<D>(a, st, q, x.b, h, b0, b1, kv, vis, least, wave, ahead, blocks);
 }
 template <int D>
-__device__ __forceinline__ void i4_finish(const Int8DecodeArgs& a, const I8Item& x, int h, const I8State<D>& st, int wave,
-                                          I4DecodeLds<D>& lds) {
+__device__ __forceinline__ void i4_finish(const Int8DecodeArgs& a, const I8Item& x, int h, const I8State<D>& st,
+                                          int wave, I4DecodeLds<D>& lds) {
   const int row0 = 16 * x.tile;
   i4_finish<D>(a, st, x.b, h, x.seq.q0, row0, min(x.seq.n * a.group - row0, 16), x.split, x.splits, wave, lds);
 }

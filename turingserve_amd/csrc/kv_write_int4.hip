@@ -197,7 +197,8 @@ __global__ void __launch_bounds__(kI4WriteThreads) kv_read_int4_kernel(Int4ReadA
       n[r] = ld<uint32_t>(src + U::k_numbers(4 * r + quad, group));
     }
   } else {
-    const uint4_t v = ld<uint4_t>(src + U::v_word(4 * quad, octet)), m = ld<uint4_t>(src + U::v_numbers(4 * quad, group));
+    const uint4_t v = ld<uint4_t>(src + U::v_word(4 * quad, octet));
+    const uint4_t m = ld<uint4_t>(src + U::v_numbers(4 * quad, group));
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       w[r] = v[r];
@@ -205,7 +206,8 @@ __global__ void __launch_bounds__(kI4WriteThreads) kv_read_int4_kernel(Int4ReadA
     }
   }
 #pragma unroll
-  for (int r = 0; r < 4; ++r) st<half8_t>(dst + (is_v ? 4 * quad + r : 4 * r + quad) * D + 8 * octet, i4_octet(k, w[r], n[r]));
+  for (int r = 0; r < 4; ++r)
+    st<half8_t>(dst + (is_v ? 4 * quad + r : 4 * r + quad) * D + 8 * octet, i4_octet(k, w[r], n[r]));
 }
 
 static bool int4_head_dim(int D) { return D == 16 || D == 32 || D == 64 || D == 128 || D == 256; }

@@ -5,8 +5,8 @@
 // way to LDS; there are no scales left over, so a score's exponent is one product-sum, P = 2^(s - m), and a
 // row's sum is that of its P.
 //
-// 2048 rows on 4096 cached, 12/2 heads of 128: 84.3 to 88.5 us, 0.73 to 0.76 PFLOP/s (a product of 8192^3 in fp16 reaches 1.09),
-// and 9.2 for the merge; the 8-bit kernel 84.9 and 9.5. Bound as that one: matrix units, vector units and LDS
+// 2048 rows on 4096 cached, 12/2 heads of 128: 84.3 to 88.5 us, 0.73 to 0.76 PFLOP/s (a product of 8192^3 in
+// fp16 reaches 1.09), and 9.2 for the merge; the 8-bit kernel 84.9 and 9.5. Bound as that one: matrix units, vector units and LDS
 // are each busy about two fifths of the time, in two wavefronts a SIMD. Five ragged prompts of 90 to 1100 rows,
 // 14/2 heads of 64: 25.0 and 4.9 us, a tile's start before some eight steps. Without effect (a pass of two
 // layers 182.0 to 182.2, or 191.4 to 192.0): a higher priority for half of the wavefronts or for one phase of a
@@ -95,7 +95,8 @@ struct I4Stage {
   __device__ __forceinline__ void place_column(half_t* tile, uint32_t a, uint32_t a8, uint32_t b, uint32_t b8,
                                                       uint4_t n, half2_t low0, half2_t low1, int block, int quad,
                                                int d0) const {
-    const half2_t x = i4_values<P>(bits, a, a8, i4_half2(n[0]), low0), y = i4_values<P>(bits, b, b8, i4_half2(n[1]), low1);
+    const half2_t x = i4_values<P>(bits, a, a8, i4_half2(n[0]), low0);
+    const half2_t y = i4_values<P>(bits, b, b8, i4_half2(n[1]), low1);
     st<half4_t>(tile + I8Tile<D>::v_at(d0 + 2 * P, block, quad & 1) + 4 * (quad >> 1),
                 half4_t{x[0], x[1], y[0], y[1]});
   }

@@ -1,8 +1,9 @@
 // What the attentions over the quantised paged caches share on the host: how a batch is split between
 // the decode kernel and the prompt kernel, the workspace, the checks, the launches, and the merge of both
 // kernels' partials in one launch (two launches: 46.5 us a layer where one takes 43.5, 16 decode rows beside
-// 512 prompt rows on 3000 cached, 12/2 heads of 128, 4 bits). The formats' kernels come in as a class `Kernels` with decode<D>(args, cus, stream) and
-// prefill<D>(args, stream), and kSplitBlocks, the blocks of a split.
+// 512 prompt rows on 3000 cached, 12/2 heads of 128, 4 bits). The formats' kernels come in as a class
+// `Kernels` with decode<D>(args, cus, stream) and prefill<D>(args, stream), and kSplitBlocks, the blocks of a
+// split.
 #pragma once
 
 #include "prefill_int8.h"
@@ -224,7 +225,8 @@ static int quant_attention(const char* what, const QuantCall& c) {
   if (pl.small > 0) {
     a.num_seqs = pl.small, a.num_decode = c.num_decode;
     a.row_slots = pl.row_slots, a.max_splits = pl.max_splits, a.chunk_parts = pl.chunk_parts;
-    a.by_slots = I8Div::by(pl.row_slots), a.by_units = I8Div::by((int64_t)pl.small * c.kvh < 1 << 30 ? pl.small * c.kvh : 1);
+    a.by_slots = I8Div::by(pl.row_slots);
+    a.by_units = I8Div::by((int64_t)pl.small * c.kvh < 1 << 30 ? pl.small * c.kvh : 1);   // (not used above)
     a.part_o = reinterpret_cast<float*>(ws + pl.dec_o);
     a.part_ml = reinterpret_cast<float*>(ws + pl.dec_ml);
     rows = merge_rows(pl, c.num_decode, c.heads, c.kvh);
