@@ -286,8 +286,12 @@ def _run_own(s):
         return ops.kv_read_int4(cache.data, s["batch"]["used"])
     out = []
     if case["kind"] != "write":
+        # a pure-decode step's plan, shared by its layers
+        split_map = (ops.decode_split_map_int4(meta, h, kvh, d, s["batch"]["blocks"], s["q"].device)
+                     if case["chunks"] == 0 else None)
         for i in range(case["layers"]):
-            out.append(ops.paged_attention_int4(s["q"][i], *cache.layer(i), meta, s["scale"]))
+            out.append(ops.paged_attention_int4(s["q"][i], *cache.layer(i), meta, s["scale"],
+                                                split_map=split_map))
         return out
     for i in range(case["layers"]):
         if case["rope"]:
