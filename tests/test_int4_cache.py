@@ -343,3 +343,23 @@ def test_engine_on_the_cpu_with_a_4bit_cache():
     eng = GreedyEngine(model, 64, max_num_batched_tokens=24, max_model_len=256, kv_cache_dtype="int4")
     out = eng.generate(prompts, 6)
     assert isinstance(eng.kv, Int4KVCache) and eng.mixed_steps > 0 and [len(o) for o in out] == [6] * 3
+
+
+def test_a_step_asks_for_its_split_map():
+    """A decode step is written alike over each cache: its split map is asked for once and handed to every
+    layer's attention. This cache has none, and no other is taken."""
+    c = Case((4, 2, 16), [(20, 1), (300, 1)], num_decode=2, seed=70)
+    _, q, _, _, cache, meta = c.on("cpu")
+    layer = cache[0, 0], cache[0, 1]
+    want = R.paged_attention_int4(q, *layer, meta, c.scale)
+    for ops in (get_ops("reference"), get_ops("hip")):
+        split_map = ops.decode_split_map_int4(meta, c.H, c.KVH, c.D, c.NB, cache.device)
+        assert split_map is None
+        for other in ((torch.zeros(8, dtype=torch.int32), 32), torch.zeros(8), 0):
+            with pytest.raises(ValueError, match="split_map"):
+                ops.paged_attention_int4(q, *layer, meta, c.scale, split_map=other)
+            with pytest.raises(ValueError, match="split_map"):
+                ops.paged_attention_int4(q[:0], *layer, meta, c.scale, split_map=other)
+    assert torch.equal(R.paged_attention_int4(q, *layer, meta, c.scale, split_map=None), want)
+    with pytest.raises(ValueError, match="GPU"):             # (the map is no reason to refuse the call)
+        H.paged_attention_int4(q, *layer, meta, c.scale, split_map=None)

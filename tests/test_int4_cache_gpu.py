@@ -5,6 +5,7 @@ bound."""
 from __future__ import annotations
 
 import dataclasses
+import math
 
 import numpy as np
 import pytest
@@ -796,3 +797,57 @@ def test_engine_tokens_with_graphs_equal_eager():
         outs.append(eng.generate(prompts, 24))
         assert bool(sizes) == (eng.graph_steps > 0) and eng.mixed_steps > 0
     assert outs[0] == outs[1] == outs[2]
+
+
+def _small(case):
+    """A case of perf/more_operators.py with the same structure and fewer, shorter sequences."""
+    most = dict(layers=2, decodes=5, ctx_lo=200, ctx_hi=700, chunks=3, q_lo=90, q_hi=150, prefix_lo=100, prefix_hi=333)
+    return {k: min(v, most[k]) if k in most else v for k, v in case.items()}
+
+
+def _case_names():
+    from perf import more_operators
+    return [c["name"] for c in more_operators.listed()]
+
+
+@pytest.mark.parametrize("name", _case_names())
+def test_cases_as_a_program_calls_them(name, monkeypatch):
+    """The measured cases' calls (the split map of a decode step, its graph, layers with caches of their own,
+    the read-back) at small sizes, twice over the same state, against their results in 64 bits. Written
+    values are equal. A rotated q: a product and a fused product-sum in fp32, then fp16. Attention, with V
+    the largest value: a score is a sum of D products in fp32, off by e = (D + 8) 2^-24 scale |q| |k| and the
+    exponential's 2^-22, a weight by a factor within e^(+-2 e); a weight is rounded to fp16, by 2^-11 of it or
+    2^-25 of the largest; sums over n tokens as in oracle.int8_cache.paged_attention; the result rounds once."""
+    from perf import more_operators as cases
+
+    case = _small(next(c for c in cases.listed() if c["name"] == name))
+    monkeypatch.setattr(cases, "own", True)
+    state = cases.prepare(case, 7)
+    want = cases.exact(case, 7)
+    h, d = case["heads"], case["head_dim"]
+    assert ("graph" in state) == (case["chunks"] == 0 and case["kind"] != "read")
+    for _ in range(2):
+        out = cases.run(state)
+        torch.cuda.synchronize()
+        if case["kind"] == "read":
+            assert torch.equal(out.double(), want)
+            continue
+        if case["kind"] == "write":
+            assert torch.equal(out["cache"].double(), want["cache"])
+            assert len(out["q"]) == len(want["q"]) == (case["layers"] if case["rope"] else 0)
+            for i, (a, b) in enumerate(zip(out["q"], want["q"])):
+                x = state["q"][i].double().abs()
+                size = x + torch.cat([x[..., d // 2:], x[..., :d // 2]], -1)
+                assert ((a.double() - b).abs() <= 2.0 ** -11 * b.abs() + 2.0 ** -23 * size + 2.0 ** -25).all()
+            continue
+        n, u = state["batch"]["max_seq_len"], 2.0 ** -24
+        held = H.kv_read_int4(state["cache"].data, torch.arange(state["batch"]["blocks"], device=DEV)).double()
+        assert len(out) == len(want) == case["layers"]
+        for i, (a, b) in enumerate(zip(out, want)):
+            v = float(held[i, 1].abs().max())
+            reach = float(state["q"][i].double().norm(dim=-1).max() * held[i, 0].norm(dim=-1).max()) * state["scale"]
+            e = (d + 8) * u * reach + 2.0 ** -22
+            off = (math.expm1(2 * e) + 2.0 ** -11 + n * 2.0 ** -25 + (n / 32 + 16) * u
+                   + 8 * u * math.sqrt(n + 256)) * v
+            assert a.shape == b.shape == (state["q"].shape[1], h * d)
+            assert ((a.double() - b).abs() <= off + 2.0 ** -11 * (b.abs() + off) + 2.0 ** -25).all()

@@ -29,7 +29,7 @@ __all__ = ["kv_write", "paged_attention", "linear", "lm_head_int8", "logits_int8
            "gate_up_silu", "rope_kv_write_", "decode_kv_write_attention",
            "decode_rope_kv_write_attention", "kv_write_int8", "rope_kv_write_int8",
            "paged_attention_int8", "kv_write_int4", "rope_kv_write_int4", "kv_read_int4",
-           "paged_attention_int4"]
+           "decode_split_map_int4", "paged_attention_int4"]
 
 DEFAULT_PARTITION = 0            # v3 split size when the caller names none: 0 = own-length
 
@@ -1014,12 +1014,21 @@ def kv_read_int4(cache: torch.Tensor, blocks: torch.Tensor) -> torch.Tensor:
     return out
 
 
+def decode_split_map_int4(meta, H: int, KVH: int, D: int, num_blocks: int, device) -> None:
+    """decode_split_map for a step over a 4-bit cache: None. Its attention finds the splits from seq_lens
+    within each launch and merges them in one of its own, so there is nothing that a step's layers could
+    share. A step's program may ask for it and pass it on as over the fp16 cache."""
+    return None
+
+
 def paged_attention_int4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, meta,
-                         scale: float) -> torch.Tensor:
+                         scale: float, split_map: None = None) -> torch.Tensor:
     """paged_attention over a 4-bit cache (see kv_write_int4): q [T, H, D] -> [T, H*D], one row for each
     of the first num_decode sequences, the rows of query_start_loc for the others under the
     bottom-right causal mask. A row that sees a token of NaN is NaN; a row that sees no token is
-    zeros."""
+    zeros. split_map: what decode_split_map_int4 gives, None; a map of another cache's is refused."""
+    if split_map is not None:
+        raise ValueError("paged_attention_int4: split_map must be None (decode_split_map_int4)")
     T, H, D = q.shape
     if T == 0:
         return torch.empty(0, H * D, dtype=q.dtype, device=q.device)

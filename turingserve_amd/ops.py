@@ -21,7 +21,8 @@ def _reference() -> SimpleNamespace:
         attention_with_mask=r.attention_with_mask, kv_write_int8=r.kv_write_int8,
         rope_kv_write_int8=r.rope_kv_write_int8, paged_attention_int8=r.paged_attention_int8,
         kv_write_int4=r.kv_write_int4, rope_kv_write_int4=r.rope_kv_write_int4,
-        kv_read_int4=r.kv_read_int4, paged_attention_int4=r.paged_attention_int4)
+        kv_read_int4=r.kv_read_int4, paged_attention_int4=r.paged_attention_int4,
+        decode_split_map_int4=r.decode_split_map_int4)
 
 
 def _hip() -> SimpleNamespace:
@@ -53,6 +54,7 @@ def _hip() -> SimpleNamespace:
     ns.rope_kv_write_int4 = h.rope_kv_write_int4
     ns.kv_read_int4 = h.kv_read_int4
     ns.paged_attention_int4 = h.paged_attention_int4
+    ns.decode_split_map_int4 = h.decode_split_map_int4
     return ns
 
 

@@ -256,11 +256,18 @@ def _int4_values(cache: torch.Tensor, values: bool) -> torch.Tensor:
     return (x * steps.double()[..., None] + lows.double()[..., None]).flatten(-2).half()
 
 
+def decode_split_map_int4(meta, H: int, KVH: int, D: int, num_blocks: int, device) -> None:
+    """Twin: attention over a 4-bit cache has no split map."""
+    return None
+
+
 def paged_attention_int4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, meta,
-                         scale: float) -> torch.Tensor:
+                         scale: float, split_map: None = None) -> torch.Tensor:
     """Twin: the sequences' blocks as fp16 values, then causal attention over the tokens that the table
     holds (block ids outside the cache read block 0). Rows that see no token are zeros, rows that see a
-    token whose K is NaN are NaN."""
+    token whose K is NaN are NaN. split_map: None (decode_split_map_int4)."""
+    if split_map is not None:
+        raise ValueError("paged_attention_int4: split_map must be None (decode_split_map_int4)")
     T, H, D = q.shape
     NB, KVH = k_cache.shape[:2]
     out = torch.zeros(T, H * D, dtype=q.dtype, device=q.device)
