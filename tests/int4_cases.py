@@ -105,3 +105,24 @@ def near_the_rows(ops, device, heads):
                 bar = np.expm1(2 * d) * (w @ np.abs(vv)) + off[1]
                 at = slice(h * c.D, (h + 1) * c.D)
                 assert (np.abs(out[lo + i, at] - w @ vv) <= bar + lim[lo + i, at]).all()
+
+
+TINY = ["below half a step of fp16", "subnormal", "zeros", "negative zeros"]
+
+
+def tiny_rows(heads, kind):
+    """A case whose rows of qkv are next to nothing: one channel of 2^-24 in the second half of k, whose
+    rotation is the least number of its group and rounds to -0; multiples of 2^-24; zeros of both signs; of one."""
+    c = Case(heads, [(5, 1), (31, 1), (0, 40)], num_decode=2, seed=72)
+    rng = np.random.default_rng(73)
+    if kind == TINY[0]:
+        c.qkv[:] = 0
+        x = c.qkv.reshape(c.T, -1, c.D)
+        x[:, :, c.D // 2:] = (rng.random(x[:, :, c.D // 2:].shape) < 0.1) * np.float16(2.0 ** -24)
+    elif kind == TINY[1]:
+        c.qkv[:] = rng.integers(-40, 41, c.qkv.shape) * 2.0 ** -24
+    elif kind == TINY[2]:
+        c.qkv[:] = np.where(rng.random(c.qkv.shape) < 0.5, np.float16(0), np.float16(-0.0))
+    else:
+        c.qkv[:] = np.float16(-0.0)
+    return c

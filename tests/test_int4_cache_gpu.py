@@ -12,7 +12,7 @@ import pytest
 import torch
 
 from oracle import int4_cache as O
-from tests.int4_cases import HEADS, Case, near_the_rows
+from tests.int4_cases import HEADS, TINY, Case, near_the_rows, tiny_rows
 from turingserve_amd import get_ops
 from turingserve_amd import hip_ops as H
 from turingserve_amd.quant import Int4KVCache
@@ -851,3 +851,22 @@ def test_cases_as_a_program_calls_them(name, monkeypatch):
                    + 8 * u * math.sqrt(n + 256)) * v
             assert a.shape == b.shape == (state["q"].shape[1], h * d)
             assert ((a.double() - b).abs() <= off + 2.0 ** -11 * (b.abs() + off) + 2.0 ** -25).all()
+
+
+@pytest.mark.parametrize("heads", HEADS)
+@pytest.mark.parametrize("kind", TINY)
+def test_rope_write_of_tiny_rows(heads, kind):
+    """Byte for byte, rotated and as they are: a least number that is or rounds to -0 is 0, and so is the step of
+    a group of such."""
+    h, kvh, d = heads
+    c = tiny_rows(heads, kind)
+    qkv, _, _, _, cache, meta = c.on(DEV)
+    cos, sin = rope_tables(d, 1e6, 64, DEV)
+    H.rope_kv_write_int4(qkv, torch.from_numpy(c.pos).to(DEV), cos, sin, h, kvh, d, cache[0, 0], cache[0, 1],
+                         meta.slot_mapping)
+    _, kn, _ = c.split()
+    turned = O.rotate(kn, cos.cpu().numpy()[c.pos], sin.cpu().numpy()[c.pos])
+    assert_cache(cache, oracle_write(c, k=turned), f"{heads} {kind}")
+    _, _, k, v, cache, meta = c.on(DEV)
+    H.kv_write_int4(k, v, cache[0, 0], cache[0, 1], meta.slot_mapping)
+    assert_cache(cache, oracle_write(c), f"{heads} {kind} as they are")

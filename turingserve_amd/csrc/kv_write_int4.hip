@@ -115,7 +115,7 @@ __device__ __forceinline__ void i4_write_kv(const Int4WriteArgs& a) {
   if constexpr (LANES > 2) lo = fminf(lo, i8_lane<0x4e>(lo)), hi = fmaxf(hi, i8_lane<0x4e>(hi));   // 2 3 0 1
   const uint64_t lost = __ballot(bad), mine = PER == kWave ? ~0ull : ((1ull << PER % kWave) - 1)
                                                                        << (threadIdx.x % kWave / PER * PER);
-  half_t low = (half_t)(lo + 0.f);                         // (-0 as 0)
+  half_t low = (half_t)lo + (half_t)0.f;                   // (-0 as 0, also where a number rounds to it)
   const float span = fmaxf(hi - (float)low, 0.f) / 15.f;
   half_t step = (half_t)span;
   if ((float)step > span) step = __builtin_bit_cast(half_t, (uint16_t)(__builtin_bit_cast(uint16_t, step) - 1));
