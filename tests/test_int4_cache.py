@@ -11,7 +11,7 @@ import pytest
 import torch
 
 from oracle import int4_cache as O
-from tests.int4_cases import HEADS, Case, near_the_rows
+from tests.int4_cases import HEADS, TINY, Case, near_the_rows, tiny_rows
 from turingserve_amd import _native as N
 from turingserve_amd import get_ops
 from turingserve_amd import hip_ops as H
@@ -363,3 +363,22 @@ def test_a_step_asks_for_its_split_map():
     assert torch.equal(R.paged_attention_int4(q, *layer, meta, c.scale, split_map=None), want)
     with pytest.raises(ValueError, match="GPU"):             # (the map is no reason to refuse the call)
         H.paged_attention_int4(q, *layer, meta, c.scale, split_map=None)
+
+
+@pytest.mark.parametrize("heads", [(4, 2, 16), (6, 2, 32), (12, 2, 128)])
+@pytest.mark.parametrize("kind", TINY)
+def test_rope_twin_of_tiny_rows(heads, kind):
+    c = tiny_rows(heads, kind)
+    h, kvh, d = heads
+    qkv, _, _, _, cache, meta = c.on("cpu")
+    cos, sin = rope_tables(d, 1e6, 64, "cpu")
+    R.rope_kv_write_int4(qkv, torch.from_numpy(c.pos), cos, sin, h, kvh, d, cache[0, 0], cache[0, 1],
+                         meta.slot_mapping)
+    _, kn, vn = c.split()
+    turned = O.rotate(kn, cos.numpy()[c.pos], sin.numpy()[c.pos]).astype(np.float32)
+    if kind == TINY[0]:                                  # groups whose least number rounds to -0
+        least = turned.reshape(c.T, kvh, O.groups(d), -1).min(-1)
+        assert ((least < 0) & (least > -2.0 ** -25)).any()
+    want = c.cache
+    O.write(turned, vn, *want, c.slots)
+    assert np.array_equal(cache[0].numpy(), want)

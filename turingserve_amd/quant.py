@@ -91,7 +91,7 @@ def int4_quantise(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Te
     more than the largest value; code: rint((x - low) / step) within 0 .. 15, 0 where the step is 0."""
     x = x.unflatten(-1, (-1, min(x.shape[-1], INT4_GROUP)))
     lows = x.amin(-1).half() + 0.0                             # (-0 as 0)
-    span = (x.amax(-1) - lows.float()).clamp_min(0)
+    span = (x.amax(-1) - lows.float()).clamp_min(0) + 0.0      # (here too)
     span = span / torch.full_like(span, 15.0)
     steps = span.half()
     steps = (steps.view(torch.int16) - (steps.float() > span).to(torch.int16)).view(torch.float16)
