@@ -126,3 +126,68 @@ def tiny_rows(heads, kind):
     else:
         c.qkv[:] = np.float16(-0.0)
     return c
+
+
+def coherent_rows(heads):
+    """A case whose K decides its results: k_j = a_j u (1 + noise), v_j = a_j t (1 + noise) with u, t rows
+    of signs of a KV head and a_j between -1 and 1, q = +-(0.7 .. 1) r u with scale D r = 3. A score is about
+    +-3 a_j where a code moves it by a fifteenth, and a row's result +-0.6 t."""
+    c = Case(heads, [(0, 70), (0, 33)], seed=74)
+    rng = np.random.default_rng(75)
+    x = c.qkv.reshape(c.T, c.H + 2 * c.KVH, c.D)
+    signs = lambda: rng.choice([-1.0, 1.0], (c.KVH, c.D))
+    u, t, a = signs(), signs(), rng.uniform(-1, 1, (c.T, c.KVH, 1))
+    noise = lambda: 1 + 0.05 * rng.standard_normal((c.T, c.KVH, c.D))
+    g = c.H // c.KVH
+    size = rng.uniform(0.7, 1.0, (c.T, c.H, 1)) * rng.choice([-1, 1], (c.T, c.H, 1)) * 3 / (c.scale * c.D)
+    x[:, :c.H] = size * np.repeat(u, g, 0)
+    x[:, c.H:c.H + c.KVH] = a * u * noise()
+    x[:, c.H + c.KVH:] = a * t * noise()
+    return c
+
+
+def over_the_cache(ops, device, c, scale=None):
+    """(attention over the cache that the case's rows were written to, the cache)."""
+    _, q, k, v, cache, meta = c.on(device)
+    ops.kv_write_int4(k, v, cache[0, 0], cache[0, 1], meta.slot_mapping)
+    out = ops.paged_attention_int4(q, cache[0, 0], cache[0, 1], meta, c.scale if scale is None else scale)
+    return out.double().cpu().numpy(), cache[0].cpu().numpy()
+
+
+def over_the_rows(c, cache):
+    """(attention over the rows themselves in 64 bits, how far attention over their codes may be off).
+    A number x of a group whose span is 15 steps is off by e <= (1/2 + 2^-16) of one (15 * 2^-24 at least, by
+    which the end of a group of a subnormal step may be off) and 2^-11 |x| + 2^-25 (lows are exact: the rows
+    are fp16 numbers), a score by d_j = scale sum_i |q_i| e_ji, a weight, divided by the sum of all, by a factor within e^(+-(d_j + d)), d the largest d_j that the row
+    sees; as the weights add up to one, the result by sum_j w_j (e^(d_j + d) - 1) |v_j - out|, and by V's own
+    error at most. The operator's error over the codes (oracle.int4_cache) comes on top."""
+    _, lim = O.paged_attention(c.split()[0], cache[0], cache[1], c.tables, c.lens, c.starts, c.scale)
+    qn, kn, vn = (x.astype(np.float64) for x in c.split())
+
+    def error(x):
+        by = x.reshape(*x.shape[:2], O.groups(c.D), -1)
+        half = np.maximum((by.max(-1) - by.min(-1)) / 15 * (0.5 + 2.0 ** -16), 15 * 2.0 ** -24)
+        return np.repeat(half, c.D // O.groups(c.D), -1) + 2.0 ** -11 * np.abs(x) + 2.0 ** -25
+
+    ek, ev = error(kn), error(vn)
+    g = c.H // c.KVH
+    ref, bar = np.zeros((2, c.T, c.H, c.D))
+    for b, (_, n) in enumerate(c.items):
+        lo = int(c.starts[b])
+        for h in range(c.H):
+            for i in range(n):
+                at = slice(lo, lo + i + 1)
+                x, kk, vv = qn[lo + i, h], kn[at, h // g], vn[at, h // g]
+                s = kk @ x * c.scale
+                w = np.exp(s - s.max())
+                w /= w.sum()
+                d = ek[at, h // g] @ np.abs(x) * c.scale
+                ref[lo + i, h] = w @ vv
+                off = (w * np.expm1(d + d.max())) @ np.abs(vv - ref[lo + i, h])
+                bar[lo + i, h] = off + ev[at, h // g].max(0)
+    return ref.reshape(c.T, -1), bar.reshape(c.T, -1) + lim
+
+
+def outside(c, out, ref, bar):
+    """The (row, head)s with any result outside the bar."""
+    return (~(np.abs(out - ref) <= bar)).reshape(c.T, c.H, c.D).any(-1)

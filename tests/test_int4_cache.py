@@ -11,7 +11,8 @@ import pytest
 import torch
 
 from oracle import int4_cache as O
-from tests.int4_cases import HEADS, TINY, Case, near_the_rows, tiny_rows
+from tests.int4_cases import (HEADS, TINY, Case, coherent_rows, near_the_rows, outside, over_the_cache,
+                              over_the_rows, tiny_rows)
 from turingserve_amd import _native as N
 from turingserve_amd import get_ops
 from turingserve_amd import hip_ops as H
@@ -382,3 +383,18 @@ def test_rope_twin_of_tiny_rows(heads, kind):
     want = c.cache
     O.write(turned, vn, *want, c.slots)
     assert np.array_equal(cache[0].numpy(), want)
+
+
+@pytest.mark.parametrize("heads", HEADS)
+def test_attention_over_the_cache_is_that_over_coherent_rows(heads):
+    """Write and attention against the rows themselves, where the codes' error is small beside the result; and
+    what is no such attention does not pass: zeros, the negated or tripled result, one that ignores K, other
+    rows' results (of which those of the same sign may)."""
+    c = coherent_rows(heads)
+    out, cache = over_the_cache(R, "cpu", c)
+    ref, bar = over_the_rows(c, cache)
+    assert not outside(c, out, ref, bar).any()
+    flat, _ = over_the_cache(R, "cpu", c, scale=c.scale * 1e-6)
+    seen = np.concatenate([np.arange(n) for _, n in c.items]) >= 8
+    for wrong, part in ((out * 0, 0.9), (-out, 0.9), (3 * out, 0.9), (flat, 0.9), (np.roll(out, 7, 0), 0.25)):
+        assert outside(c, wrong, ref, bar)[seen].mean() > part

@@ -12,7 +12,8 @@ import pytest
 import torch
 
 from oracle import int4_cache as O
-from tests.int4_cases import HEADS, TINY, Case, near_the_rows, tiny_rows
+from tests.int4_cases import (HEADS, TINY, Case, coherent_rows, near_the_rows, outside, over_the_cache,
+                              over_the_rows, tiny_rows)
 from turingserve_amd import get_ops
 from turingserve_amd import hip_ops as H
 from turingserve_amd.quant import Int4KVCache
@@ -870,3 +871,11 @@ def test_rope_write_of_tiny_rows(heads, kind):
     _, _, k, v, cache, meta = c.on(DEV)
     H.kv_write_int4(k, v, cache[0, 0], cache[0, 1], meta.slot_mapping)
     assert_cache(cache, oracle_write(c), f"{heads} {kind} as they are")
+
+
+@pytest.mark.parametrize("heads", HEADS)
+def test_attention_over_the_cache_is_that_over_coherent_rows(heads):
+    c = coherent_rows(heads)
+    out, cache = over_the_cache(H, DEV, c)
+    ref, bar = over_the_rows(c, cache)
+    assert not outside(c, out, ref, bar).any()
