@@ -879,3 +879,51 @@ def test_attention_over_the_cache_is_that_over_coherent_rows(heads):
     out, cache = over_the_cache(H, DEV, c)
     ref, bar = over_the_rows(c, cache)
     assert not outside(c, out, ref, bar).any()
+
+
+def test_model_over_the_cache_is_the_fp16_model_over_what_it_holds():
+    """Each step through the model with a 4-bit cache, then through the same model over that cache read back
+    as fp16, its own new rows going to blocks behind it that no table names: both attend the same numbers, and
+    differ by fp16's roundings alone (bar 1e-2, a fifth at most of what the 4 bits themselves move the
+    logits by). Of every layer, the rows held are those that the fp16 model wrote, within half a step (and the
+    1e-2 of the activations)."""
+    from turingserve_amd.metadata import BatchItem, InputBuilder, SeqState
+    from turingserve_amd.qwen2 import Qwen2Config, Qwen2Model, random_weights
+
+    layers, blocks = 3, 40
+    cfg = Qwen2Config(256, 512, layers, 4, 2, 500, max_position_embeddings=512)
+    model = Qwen2Model(cfg, random_weights(cfg, DEV, seed=26, draw_on="cpu", init_std=0.06), get_ops("hip"), 512)
+    g = torch.Generator().manual_seed(27)
+    seqs = [SeqState(torch.randint(0, 500, (200,), generator=g).tolist(), list(range(1 + 13 * i, 14 + 13 * i)))
+            for i in range(3)]
+    kv, plain, builder = model.new_kv_cache(blocks, "int4"), model.new_kv_cache(blocks), InputBuilder(256, 8, 13, DEV)
+    pure_decode = model.pure_decode
+    mine, moved = [], []
+    for items in ([BatchItem(seqs[0], 0, seqs[0].token_ids[:50]), BatchItem(seqs[1], 0, seqs[1].token_ids[:33])],
+                  [BatchItem(seqs[0], 50, seqs[0].token_ids[50:51]), BatchItem(seqs[1], 33, seqs[1].token_ids[33:34]),
+                   BatchItem(seqs[2], 0, seqs[2].token_ids[:70])],
+                  [BatchItem(s, n, s.token_ids[n:n + 1]) for s, n in zip(seqs, (51, 34, 70))]):
+        inp = builder.build(items)
+        T, slots = inp.input_ids.shape[0], inp.meta.slot_mapping
+        logits = lambda cache, meta: model.compute_logits(model.forward(inp.input_ids, inp.positions, meta, cache),
+                                                          inp.sample_indices)
+        model.pure_decode = pure_decode
+        got = logits(kv, inp.meta)
+        mine.append(got), moved.append(logits(plain, inp.meta))
+        held = H.kv_read_int4(kv.data, torch.arange(blocks, device=DEV))
+        both = torch.cat([held, torch.zeros_like(held)[:, :, :-(-T // 16)]], dim=2)
+        model.pure_decode = lambda *_: False             # (attention reads its rows from the cache)
+        behind = torch.arange(T, device=DEV)
+        want = logits(both, dataclasses.replace(inp.meta, slot_mapping=16 * blocks + behind))
+        assert torch.equal(both[:, :, :blocks], held)
+        assert float((got - want).norm() / want.norm()) < 1e-2
+        wrote = both[:, :, blocks + behind // 16, :, behind % 16].double()                # [T, L, 2, KVH, D]
+        there = held[:, :, slots // 16, :, slots % 16].double()
+        rms = lambda x: x.square().mean((0, 3, 4)).sqrt()                                 # [L, 2]
+        for j in range(2):
+            steps = torch.from_numpy(O.unpack(kv.data[:, j].cpu().numpy(), cfg.head_dim, bool(j))[1].astype(np.float64))
+            step = rms(steps.to(DEV)[:, None, slots // 16, :, slots % 16].expand(-1, -1, 2, -1, -1))[:, j]
+            assert (rms(there - wrote)[:, j] <= 0.5 * step + 1e-2 * rms(wrote)[:, j]).all()
+            assert (0.5 * step < 0.25 * rms(wrote)[:, j]).all()
+    mine, moved = torch.cat(mine), torch.cat(moved)
+    assert float((mine - moved).norm() / moved.norm()) > 5e-2
