@@ -117,8 +117,8 @@ __device__ __forceinline__ I8Seq i8_seq(const Int8DecodeArgs& a, int b) {
   return s;
 }
 
-// Splits of a sequence's blocks: longer ones where several tiles of rows share them, so that its
-// partials stay those of one tile. (chunk_parts holds them, and row_slots the rows, within the host's
+// Splits of a sequence's blocks, of EACH blocks: longer ones where several tiles of rows share them, so that
+// its partials stay those of one tile. (chunk_parts holds them, and row_slots the rows, within the host's
 // bounds; past those there is one split.)
 template <int EACH = kI8SplitBlocks>
 __device__ __forceinline__ int i8_splits(const Int8DecodeArgs& a, const I8Seq& s, bool decode) {
@@ -126,7 +126,7 @@ __device__ __forceinline__ int i8_splits(const Int8DecodeArgs& a, const I8Seq& s
   if (decode) return i8_splits(nb, a.max_splits, EACH);
   if (rows > a.row_slots) return 1;
   const int tiles = s.n == 1 ? 1 : (rows + 15) / 16;
-  const int n = i8_splits(nb, min(a.max_splits, kI8MaxSplits / tiles), kI8SplitBlocks * tiles);
+  const int n = i8_splits(nb, min(a.max_splits, kI8MaxSplits / tiles), EACH * tiles);
   return n * rows > a.chunk_parts ? 1 : n;
 }
 
