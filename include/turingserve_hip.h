@@ -644,8 +644,8 @@ int ts_kv_read_int4(const void* cache, int32_t num_layers, int64_t num_blocks, i
  * the bottom-right causal mask) with K and V the fp16 numbers that the codes stand for. Products in fp16
  * with fp32 sums; scores, softmax statistics and outputs' sums are fp32. Before the P.V product a weight is
  * rounded to fp16, measured against (at most) the row's largest one: off by 2^-11 of itself, or 2^-25 of
- * that largest one where it is below 2^-14 of it. Rows that see no token are zeros; a row that sees a
- * token of NaN is NaN; tokens that it does not see have no say. A decode row's result does not depend
+ * that largest one where it is below 2^-14 of it; no rounding takes a result past 65504. Rows that see no
+ * token are zeros; a row that sees a token of NaN is NaN; tokens that it does not see have no say. A decode row's result does not depend
  * on the rest of the batch given max_seq_len. The host bounds shape the launch only: bounds below the
  * batch's real values are slower, not wrong. head_dims, heads, alignment, limits and the workspace as for
  * ts_paged_attention_int8. Rows of no sequence are not written.

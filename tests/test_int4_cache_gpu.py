@@ -927,3 +927,31 @@ def test_model_over_the_cache_is_the_fp16_model_over_what_it_holds():
             assert (0.5 * step < 0.25 * rms(wrote)[:, j]).all()
     mine, moved = torch.cat(mine), torch.cat(moved)
     assert float((mine - moved).norm() / moved.norm()) > 5e-2
+
+
+@pytest.mark.parametrize("heads", HEADS)
+def test_results_of_the_largest_values_are_finite(heads):
+    """V of 65504 in one half of the heads and -65504 in the other: a result is a mean of these, which no
+    rounding of a weight may take past the largest number. Every 32nd token has a score of 0, the others one
+    of log2(1/2 + 1.2 * 2^-12) in base 2: their weight is rounded up to 1/2 + 2^-11 for the product, not in the
+    sum, and the mean comes out 2^-11 too large. One piece, merged splits, the prompt kernel, cut tiles."""
+    c = Case(heads, [(n - 1, 1) for n in DECODE_LENS] + [(0, 90), (300, 40)], num_decode=len(DECODE_LENS), seed=76)
+    _, q, _, _, cache, meta = c.on(DEV)
+    n = 16 * c.NB
+    place = np.zeros(n, np.int64)                        # a slot's position
+    for b, length in enumerate(c.lens):
+        at = np.arange(length)
+        place[c.tables[b, at // 16].astype(np.int64) * 16 + at % 16] = at
+    k, v = torch.zeros(2, n, c.KVH, c.D, device=DEV).half()
+    k[torch.from_numpy(place % 32 > 0).to(DEV), :, 0] = -1
+    v[:, :c.KVH // 2], v[:, c.KVH // 2:] = 65504, -65504
+    H.kv_write_int4(k, v, cache[0, 0], cache[0, 1], torch.arange(n, device=DEV))
+    held = cache[0].cpu().numpy()
+    c.qkv[:] = 0
+    c.split()[0][..., 0] = 1
+    q = c.on(DEV)[1]
+    c.scale = -math.log(0.5 + 1.2 * 2.0 ** -12)
+    for bounds in (dict(), dict(max_seq_len=64), dict(max_prefill_seq_len=30000)):
+        out = attend(q, cache, dataclasses.replace(meta, **bounds), c.scale)
+        assert torch.isfinite(out).all(), bounds
+        assert_rows(out, c, f"{bounds}", cache=held)

@@ -7,6 +7,7 @@ namespace ts {
 
 struct Int4Kernels {
   static constexpr int kSplitBlocks = kI4SplitBlocks;
+  static constexpr bool kFinite = true;
 
   template <int D>
   static void decode(const Int8DecodeArgs& a, int cus, hipStream_t s) {

@@ -5,6 +5,7 @@ namespace ts {
 
 struct Int8Kernels {
   static constexpr int kSplitBlocks = kI8SplitBlocks;
+  static constexpr bool kFinite = false;                   // (a code times its scale may be any fp32 number)
 
   template <int D>
   static void decode(const Int8DecodeArgs& a, int cus, hipStream_t s) {

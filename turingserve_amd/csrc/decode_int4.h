@@ -314,7 +314,7 @@ __device__ __forceinline__ void i4_finish(const Int8DecodeArgs& a, const I8State
     if (splits == 1) {
       const float f = sum == 0.f ? 0.f : 1.f / sum;        // no visible key: zeros
       const int token = a.by_group(row0 + row), head = h * a.group + row0 + row - token * a.group;
-      ts::st<half4_t>(a.out + (int64_t)(q0 + token) * a.out_st + (int64_t)head * D + d, to_half4(o * f));
+      ts::st<half4_t>(a.out + (int64_t)(q0 + token) * a.out_st + (int64_t)head * D + d, i8_result<true>(o * f));
     } else {
       const int64_t at = i8_partial(a, b, h, row0 + row, splits) + split;
       ts::st<float4_t>(a.part_o + at * D + d, o);

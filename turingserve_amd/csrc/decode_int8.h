@@ -272,6 +272,18 @@ struct I8State {
   float4_t o[D / 16];
 };
 
+// A row's result in fp16. FINITE: V's values are fp16 numbers, and so is their mean in exact arithmetic; but
+// weights are rounded for the product and not in their sum, which moves a mean of 65504s by up to 2^-11 of
+// it, past the largest number. (NaN stays.)
+template <bool FINITE>
+__device__ __forceinline__ half4_t i8_result(float4_t o) {
+  if constexpr (FINITE) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = __builtin_elementwise_minimum(vmax(o[e], -65504.f), 65504.f);
+  }
+  return to_half4(o);
+}
+
 // What a block multiplies its scores by (scale * log2 e * ks), adds to them, and multiplies its weights
 // by in a row's sum (i8_value_factors).
 struct I8Factors {
@@ -522,7 +534,7 @@ __global__ void __launch_bounds__(kI8Threads, i8_decode_groups(D)) decode_int8_k
 // eight groups meeting in LDS, took twice as long at 2240 rows of a few splits: 10.5 us. One partial ahead
 // of the length and reductions by shuffles: 40.0 us a pass of four layers of one sequence of 6000 in 4 bits,
 // 38.4 so; sixteen ahead no less.)
-template <int D, int EACH = kI8SplitBlocks>
+template <int D, int EACH = kI8SplitBlocks, bool FINITE = false>
 __device__ __forceinline__ void i8_merge_row(const Int8DecodeArgs& a, int slot) {
   constexpr int PER_ROW = D / 4, GROUPS = kWave / PER_ROW;
   constexpr int N = 64 / GROUPS < 16 ? 64 / GROUPS : 16;   // partials of a lane at a time
@@ -577,7 +589,7 @@ __device__ __forceinline__ void i8_merge_row(const Int8DecodeArgs& a, int slot) 
   if (group > 0) return;
   const float inv = sum == 0.f ? 0.f : 1.f / sum;          // (nothing visible)
   const int token = a.by_group(r), head = h * a.group + r - token * a.group;
-  st<half4_t>(a.out + (int64_t)(seq.q0 + token) * a.out_st + (int64_t)head * D + d, to_half4(o * inv));
+  st<half4_t>(a.out + (int64_t)(seq.q0 + token) * a.out_st + (int64_t)head * D + d, i8_result<FINITE>(o * inv));
 }
 
 // The wavefront's row, of workgroup `group`.
@@ -585,9 +597,9 @@ __device__ __forceinline__ int i8_merge_slot(int group) {
   return group * kI8Waves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
 }
 
-template <int D, int EACH = kI8SplitBlocks>
+template <int D, int EACH = kI8SplitBlocks, bool FINITE = false>
 __global__ void __launch_bounds__(kI8Threads) decode_int8_merge_kernel(Int8DecodeArgs a) {
-  i8_merge_row<D, EACH>(a, i8_merge_slot(blockIdx.x));
+  i8_merge_row<D, EACH, FINITE>(a, i8_merge_slot(blockIdx.x));
 }
 
 }  // namespace ts

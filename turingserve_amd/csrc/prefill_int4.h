@@ -366,7 +366,7 @@ __device__ __forceinline__ void i4_piece(const Int8PrefillArgs& p, I4PrefillLds<
       if (D < 32 && d >= D) break;
       const float4_t x = float4_t{w.o[t][i], w.o[t][i + 1], w.o[t][i + 2], w.o[t][i + 3]} * f;
       if (whole)
-        st<half4_t>(dst + d, to_half4(x));
+        st<half4_t>(dst + d, i8_result<true>(x));
       else
         st<float4_t>(a.part_o + at * D + d, x);
     }

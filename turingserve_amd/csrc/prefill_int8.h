@@ -758,7 +758,7 @@ prefill_int8_kernel(Int8PrefillArgs p) {
 // 2048 rows on 4096 cached, 12/2 heads of 128: 9.5 us, 53 MB of partials; 10.5 when each workgroup
 // looked the tile up; 32 rows a workgroup are 1 to 2 us slower.)
 constexpr int kI8MergeRows = 16;
-template <int D, int ROWS>
+template <int D, int ROWS, bool FINITE = false>
 __device__ __forceinline__ void i8_merge_tile(const Int8PrefillArgs& p, int group) {
   constexpr int PER = 256 / (D / 4);                       // rows at a time
   constexpr int R = kI8MergeRows > PER ? kI8MergeRows / PER : 1, N = 4;   // rows of a thread, partials at a time
@@ -810,20 +810,20 @@ __device__ __forceinline__ void i8_merge_tile(const Int8PrefillArgs& p, int grou
     if (row >= j.rows) return;
     const float f = sum[r] == 0.f ? 0.f : 1.f / sum[r];
     const int token = a.by_group(row), head = j.h * a.group + row - token * a.group;
-    st<half4_t>(a.out + (int64_t)(j.q0 + token) * a.out_st + (int64_t)head * D + d, to_half4(o[r] * f));
+    st<half4_t>(a.out + (int64_t)(j.q0 + token) * a.out_st + (int64_t)head * D + d, i8_result<FINITE>(o[r] * f));
   }
 }
 
-template <int D, int ROWS>
+template <int D, int ROWS, bool FINITE = false>
 __global__ void __launch_bounds__(256) prefill_int8_merge_kernel(Int8PrefillArgs p) {
-  i8_merge_tile<D, ROWS>(p, blockIdx.x);
+  i8_merge_tile<D, ROWS, FINITE>(p, blockIdx.x);
 }
 
 // Both merges of a batch that needs both, the tiles' first: `tiles` workgroups of them.
-template <int D, int ROWS, int EACH>
+template <int D, int ROWS, int EACH, bool FINITE = false>
 __global__ void __launch_bounds__(256) int8_merge_kernel(Int8DecodeArgs a, Int8PrefillArgs p, int tiles) {
-  if ((int)blockIdx.x < tiles) return i8_merge_tile<D, ROWS>(p, blockIdx.x);
-  i8_merge_row<D, EACH>(a, i8_merge_slot((int)blockIdx.x - tiles));
+  if ((int)blockIdx.x < tiles) return i8_merge_tile<D, ROWS, FINITE>(p, blockIdx.x);
+  i8_merge_row<D, EACH, FINITE>(a, i8_merge_slot((int)blockIdx.x - tiles));
 }
 
 }  // namespace ts

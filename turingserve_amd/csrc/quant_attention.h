@@ -2,8 +2,8 @@
 // the decode kernel and the prompt kernel, the workspace, the checks, the launches, and the merge of both
 // kernels' partials in one launch (two launches: 46.5 us a layer where one takes 43.5, 16 decode rows beside
 // 512 prompt rows on 3000 cached, 12/2 heads of 128, 4 bits). The formats' kernels come in as a class
-// `Kernels` with decode<D>(args, cus, stream) and prefill<D>(args, stream), and kSplitBlocks, the blocks of a
-// split.
+// `Kernels` with decode<D>(args, cus, stream) and prefill<D>(args, stream), kSplitBlocks, the blocks of a
+// split, and kFinite, whether V's values are fp16 numbers (i8_result).
 #pragma once
 
 #include "prefill_int8.h"
@@ -141,16 +141,17 @@ static size_t quant_workspace_bytes(int num_seqs, int num_decode, int max_query_
 template <class Kernels, int D>
 static void quant_launch(const Int8DecodeArgs& a, int64_t rows, const Int8PrefillArgs& p, int cus, hipStream_t s) {
   constexpr int ROWS = 32 * i8_prefill_waves(D), EACH = Kernels::kSplitBlocks;
+  constexpr bool FINITE = Kernels::kFinite;
   const unsigned row_groups = rows > 0 && a.max_splits > 1 ? (unsigned)((rows + kI8Waves - 1) / kI8Waves) : 0;
   const unsigned tile_groups = p.groups > 1 ? (unsigned)(p.groups - 1) * (ROWS / kI8MergeRows) : 0;
   if (rows > 0) Kernels::template decode<D>(a, cus, s);
   if (p.groups > 0) Kernels::template prefill<D>(p, s);
   if (row_groups > 0 && tile_groups > 0)
-    int8_merge_kernel<D, ROWS, EACH><<<tile_groups + row_groups, 256, 0, s>>>(a, p, (int)tile_groups);
+    int8_merge_kernel<D, ROWS, EACH, FINITE><<<tile_groups + row_groups, 256, 0, s>>>(a, p, (int)tile_groups);
   else if (row_groups > 0)
-    decode_int8_merge_kernel<D, EACH><<<row_groups, kI8Threads, 0, s>>>(a);
+    decode_int8_merge_kernel<D, EACH, FINITE><<<row_groups, kI8Threads, 0, s>>>(a);
   else if (tile_groups > 0)
-    prefill_int8_merge_kernel<D, ROWS><<<tile_groups, 256, 0, s>>>(p);
+    prefill_int8_merge_kernel<D, ROWS, FINITE><<<tile_groups, 256, 0, s>>>(p);
 }
 
 template <class Kernels, bool SCALES>
