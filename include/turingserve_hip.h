@@ -604,15 +604,21 @@ int ts_paged_attention_int8(const void* q, int64_t q_stride_t, int64_t q_stride_
  * ts_kv_write_int4: for every token t with 0 <= s = slot_mapping[t] < 16 num_blocks, rows k[t] and v[t] go
  * to row s % 16 of block s / 16; other slots are skipped. Per KV head and group, in fp32 rounded to
  * nearest:
- *   low  = fp16(least value)
+ *   low  = fp16(least value), -0 as 0
  *   step = (largest value - low) / 15, 0 where that is negative, rounded towards zero to fp16
  *   code = rint((value - low) / step) within 0 .. 15, 0 where step is 0
- * so that a value is off by about half a step, and by a step and a few units in the last place of its
- * group's numbers at most at the group's upper end. A token whose K or V row of a head is not finite in
- * fp16 (|value| > 65504) is NaN in that head: codes and steps 0, lows NaN, K and V. What stood in a slot
- * has no say, and no other row is touched. No two tokens of a call may have the same slot (each would leave
- * parts of its row; no access leaves the cache). k / v rows fp16, 16-byte aligned; head_dim 16, 32, 64,
- * 128 or 256; tokens times heads below 2^30.
+ * so that a value is off by at most
+ *   half a step (and 2^-16 of one) where the step is a normal number; where it is subnormal or 0 (a span below
+ *   15 * 2^-14) half a step or 15 * 2^-24, the larger, since rounding it towards zero may cost the group's
+ *   upper end 15 units of 2^-24; a group of a span below 15 * 2^-24 is its low alone;
+ *   what it lies below low by, if that is more (k rotated in fp32 only: 2^-11 |low| or 2^-25 at most);
+ *   and the rounding of fp16(low + code * step) on top: 2^-11 of it or 2^-25, many steps in a group that is
+ *   narrow and far from zero.
+ * A token whose K or V row of a head is not finite in fp16 (|value| > 65504) is NaN in that head: codes
+ * and steps 0, lows NaN, K and V. What stood in a slot has no say, and no other row is touched. No two
+ * tokens of a call may have the same slot (each would leave parts of its row; no access leaves the
+ * cache). k / v rows fp16, 16-byte aligned; head_dim 16, 32, 64, 128 or 256; tokens times heads below
+ * 2^30.
  *
  * ts_rope_kv_write_int4: the same for the k and v heads of qkv [T, (H + 2 KVH) D], k rotated first
  * (rotate-half RoPE by the fp32 tables, computed in 64 bits and rounded to fp32), with the rotated q
@@ -644,11 +650,12 @@ int ts_kv_read_int4(const void* cache, int32_t num_layers, int64_t num_blocks, i
  * the bottom-right causal mask) with K and V the fp16 numbers that the codes stand for. Products in fp16
  * with fp32 sums; scores, softmax statistics and outputs' sums are fp32. Before the P.V product a weight is
  * rounded to fp16, measured against (at most) the row's largest one: off by 2^-11 of itself, or 2^-25 of
- * that largest one where it is below 2^-14 of it; no rounding takes a result past 65504. Rows that see no
- * token are zeros; a row that sees a token of NaN is NaN; tokens that it does not see have no say. A decode row's result does not depend
- * on the rest of the batch given max_seq_len. The host bounds shape the launch only: bounds below the
- * batch's real values are slower, not wrong. head_dims, heads, alignment, limits and the workspace as for
- * ts_paged_attention_int8. Rows of no sequence are not written.
+ * that largest one where it is below 2^-14 of it; no rounding takes a result past 65504. Rows that see
+ * no token are zeros; a row that sees a token of NaN is NaN; tokens that it does not see have no say. A
+ * decode row's result does not depend on the rest of the batch given max_seq_len. The host bounds shape
+ * the launch only: bounds below the batch's real values are slower, not wrong. head_dims, heads,
+ * alignment, limits and the workspace as for ts_paged_attention_int8. Rows of no sequence are not
+ * written.
  */
 size_t ts_paged_attention_int4_workspace_bytes(int32_t num_seqs, int32_t num_decode,
                                                int32_t max_query_len, int32_t max_seq_len,

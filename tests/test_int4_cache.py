@@ -17,7 +17,7 @@ from turingserve_amd import _native as N
 from turingserve_amd import get_ops
 from turingserve_amd import hip_ops as H
 from turingserve_amd import reference_ops as R
-from turingserve_amd.quant import Int4KVCache, int4_head_dim, int4_unit_bytes, int4_views
+from turingserve_amd.quant import Int4KVCache, int4_head_dim, int4_quantise, int4_unit_bytes, int4_views
 from turingserve_amd.qwen2 import rope_tables
 
 P = ctypes.c_void_p(256)                 # never dereferenced: the call fails validation first
@@ -398,3 +398,30 @@ def test_attention_over_the_cache_is_that_over_coherent_rows(heads):
     seen = np.concatenate([np.arange(n) for _, n in c.items]) >= 8
     for wrong, part in ((out * 0, 0.9), (-out, 0.9), (3 * out, 0.9), (flat, 0.9), (np.roll(out, 7, 0), 0.25)):
         assert outside(c, wrong, ref, bar)[seen].mean() > part
+
+
+@pytest.mark.parametrize("D", [16, 32, 128])
+def test_values_are_within_the_stated_bound(D):
+    """Of fp32 rows (a rotated k): half a step, 15 * 2^-24 where the step is subnormal or 0 (it is rounded
+    towards zero by up to 2^-24, the group's end by 15 of these; a normal one by 2^-10 of itself, which half
+    a step covers), or what a number lies below its group's low in fp16 by; then the value's own rounding."""
+    rng = np.random.default_rng(D)
+    rows = [rng.uniform(-1, 1, (40, D)) * size for size in (1e-7, 1e-6, 1e-5, 1e-3, 1.0, 300.0, 60000.0)]
+    rows += [rng.uniform(0, 1, (40, D)) * 10.0 ** rng.uniform(-6, 2, (40, 1)) + 10.0 ** rng.uniform(-4, 4, (40, 1))]
+    few = np.zeros((3, D))
+    few[0, 1], few[1, 1], few[2] = 14 * 2.0 ** -24, 29 * 2.0 ** -24, rng.uniform(1000.2, 1000.3, D)
+    x = np.concatenate(rows + [few]).astype(np.float32)
+    codes, steps, lows = int4_quantise(torch.from_numpy(x))
+    mine = O.quantise(x)
+    for a, b in zip(mine, (codes.flatten(-2), steps, lows)):
+        assert np.array_equal(a, b.numpy())
+    held, x = O.values_of(*mine).astype(np.float64), x.astype(np.float64)
+    wide = lambda n: np.repeat(n.astype(np.float64), D // O.groups(D), -1)
+    step, low = wide(mine[1]), wide(mine[2])
+    half = np.maximum(step * (0.5 + 2.0 ** -16), np.where(step < 2.0 ** -14, 15 * 2.0 ** -24, 0.0))
+    assert (low - x <= np.maximum(2.0 ** -11 * np.abs(low), 2.0 ** -25)).all()
+    off = np.abs(held - x)
+    assert (off <= np.maximum(half, low - x) + np.maximum(2.0 ** -11 * np.abs(held), 2.0 ** -25)).all()
+    # and no less: groups of a step of 0, of one of 2^-24, and of steps of 0.02 where fp16 has one number in 0.5
+    assert (off[-3:-1, 1] == 14 * 2.0 ** -24).all() and step[-3, 1] == 0 and step[-2, 1] == 2.0 ** -24
+    assert (off[-1] > 8 * step[-1]).any()

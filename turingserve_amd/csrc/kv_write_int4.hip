@@ -3,8 +3,10 @@
 //   low  = fp16(least value),  step = (largest value - low) / 15 in fp32, rounded towards zero to fp16,
 //   code = rint((value - low) / step) within 0 .. 15 (0 where step is 0),
 // fp32 throughout, divisions rounded correctly. The step is rounded towards zero so that no code stands for
-// more than the largest value (the nearest one could leave the fp16 range at 65504); that costs at most
-// 15 units in the step's last place, 0.015 of a step, where a code is off by half of one.
+// more than the largest value (the nearest one could leave the fp16 range at 65504); that costs the group's
+// upper end at most 15 units in the step's last place: 0.015 of a normal step (2^-14 or more), where a code is
+// off by half of one, and 15 * 2^-24 where the step is subnormal or 0, which may be all of a narrow group's
+// span.
 //
 // A thread holds an octet of a row of K or of V, those of a (token, KV head) side by side in a wavefront: a
 // group's extremes come over 4 neighbouring lanes, a rotation's partner from a second load, and whether
@@ -12,7 +14,8 @@
 //
 // 12/2 heads of 128 with RoPE: 64 appended rows 3.7 us (2.3 at least, a launch's chain slot and position ->
 // row and angles -> 64-bit products -> quotients), 2048 rows 6.5 us for 19.1 MB (2.9 TB/s, the same chain over
-// five workgroups a CU). With two octets of K and of V a thread, so that a rotation's pairs met in one, it
+// five workgroups a CU; a thread loads 64 bytes of angles for its 16 of a row, anew for each of a token's 14
+// rotated heads, and the other half of K a second time). With two octets of K and of V a thread, so that a rotation's pairs met in one, it
 // took 6.8 and 10.9: a fourth of the threads, each with four times the chain. The correctly rounded divisions
 // were most of the arithmetic; i4_word leaves all but the doubtful ones out.
 #include "int4_kv.h"
