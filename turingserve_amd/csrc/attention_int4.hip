@@ -13,12 +13,14 @@ struct Int4Kernels {
   static void decode(const Int8DecodeArgs& a, int cus, hipStream_t s) {
     // Every split of the batch, at most as many workgroups as the CUs hold; the rest go round. Where all that the
     // host's bound allows fit at once, each knows its split without the lengths. Us a pass of four layers of 12/2
-    // heads of 128, so and by the lookup: one sequence of 6000 tokens 34.5 / 38.4, four of 8000 to 32768 62.5 /
-    // 64.8, eight of 500 to 4000 36.5 / 40.4, eight of 500 under a bound of 32768 36.2 / 38.1. Beyond that those
-    // past a sequence's end take the others' places: 64 sequences of up to 4096 72 / 60. A second item's place is
-    // kept for up to 64 sequences, a lane each: those 64 58.4 where a new lookup makes them 60.5, 64 of 2000 to 8000
-    // of 8/8 heads of 64 (two layers) 123 / 131, 48 rows beside a chunk of 512 88.5 / 91. For up to 256, in LDS, it
-    // gained 3 % there and lost as much below.
+    // heads of 128 by events over replays, so and by the lookup: one sequence of 6000 tokens 34.5 / 38.4, four of
+    // 8000 to 32768 62.5 / 64.8, eight of 500 to 4000 36.5 / 40.4, eight of 500 under a bound of 32768 36.2 / 38.1.
+    // Beyond that those past a sequence's end take the others' places: 64 sequences of up to 4096 72 / 60. What the
+    // lookup found is kept for up to 64 sequences, a lane each, so that a workgroup need not look up again to find
+    // its next item or that there is none: those 64 (632 items in 1024 workgroups: none has a second) 58.4 where a
+    // new lookup makes them 60.5, 48 rows beside a chunk of 512 (952 items) 88.5 / 91, 64 of 2000 to 8000 of 8/8
+    // heads of 64 (two layers; several items a workgroup) 123 / 131. For up to 256, in LDS, it gained 3 % there and
+    // lost as much below.
     const int64_t most = a.num_seqs > a.num_decode ? INT32_MAX : (int64_t)a.num_decode * a.max_splits;
     const int64_t units = most * a.kvh * ((a.group + 15) / 16), cap = (int64_t)i4_decode_groups(D) * cus;
     if (a.group <= 16 && units <= cap)

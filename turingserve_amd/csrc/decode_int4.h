@@ -10,15 +10,22 @@
 // rounded to fp16, m being the row's running reference, which a new score moves only when it passes it
 // by 2^8; sums and accumulators are fp32.
 //
-// 64 sequences of 128 to 4096 tokens, 12/2 heads of 128: 11.0 us (9.5 at least) and 4.0 for the merge, 24 MB of cache
-// (4.9 us at a copy's 4.85 TB/s); one sequence of 6000: 5.1 (4.2) and 2.8 (2.3). The large ones are bound by the issue
-// of vector instructions, some 400 a pair of blocks at head_dim 128, half of them the widening, four
-// wavefronts a SIMD; the small ones by a workgroup's chain: length and table 1.2 us, first codes 0.75, two
-// pairs 1.8, the wavefronts' meeting and the partial 0.9, then the merge's launch. Twice the blocks a split
-// take 45.8 / 64.6 / 70.6 us a pass where these take 40.1 / 61.1 / 64.1 (one of 6000, those 64, four of 8000 to
-// 32768; before the splits were known ahead), half of them 50 / 68 / 78, eight wavefronts with twice the blocks
-// 45.6 / 66 / 72. Two 16-row tiles a workgroup, the codes widened once for both: 16 chunks of five rows 52
-// against 44, ahead only at chunks of 128 (57 / 64). The merge inside the launch, behind a map of the step's
+// 64 sequences of 128 to 4096 tokens, 12/2 heads of 128: 11.0 us (9.5 at least) and 4.0 for the merge, 24 MB of
+// cache (4.9 us at a copy's 4.85 TB/s); one sequence of 6000: 5.1 (4.2) and 2.8 (2.3). Neither memory nor an
+// issue port bounds the large ones: those 64 are 632 items (a split of a KV head) on 256 CUs, two or three a CU
+// where the mean is 2.5, and vector instructions, some 400 a pair of blocks at head_dim 128 and half of them
+// the widening, are issued in 42 % of a SIMD's cycles. An item's chain is much of what is left, and all of the
+// small ones: length and table 1.2 us, first codes 0.75, two pairs 1.8, the wavefronts' meeting and the partial
+// 0.9, then the merge's launch. Blocks a split, us a pass by events over replays, 16 / 32: one of 6000 (48
+// items, four layers) 34.2 / 40.6, those 64 58.7 / 68.0, four of 8000 to 32768 (440) 62.7 / 63.0, 24 of 200 to
+// 8192 over 14/2 heads of 64 (424, eight layers) 81.6 / 92.0; but 256 of 100 to 600 (800) 72.3 / 64.4, 48 rows
+// beside a chunk of 512 (952) 90.1 / 85.6, 128 of 500 to 4000 (1814) 111.6 / 97.2, 200 of 200 to 4000 over 14/2
+// heads of 64 (2180) 96.3 / 83.7, 32 of 500 to 16000 over 28/4 heads of 128 (2296, two layers) 57.9 / 53.3, 64
+// of 2000 to 8000 over 8/8 heads of 64 (8888, two layers) 121.9 / 106.7: 16 are ahead or level up to some 630
+// items, 32 from 800 on, by 5 to 14 %. The length is one for all batches. Earlier forms of the kernel, one of
+// 6000 / those 64 / four long ones: 8 blocks 50 / 68 / 78 where 16 took 40.1 / 61.1 / 64.1, eight wavefronts
+// with 32 45.6 / 66 / 72. Two 16-row tiles a workgroup, the codes widened once for both: 16 chunks of five rows
+// 52 against 44, ahead only at chunks of 128 (57 / 64). The merge inside the launch, behind a map of the step's
 // splits with counters: 48 to 56, 64 to 91 and 79 to 96, its loads past the caches and its code cold.
 #pragma once
 
@@ -28,7 +35,8 @@
 namespace ts {
 
 constexpr int kI4Waves = 4, kI4Threads = kI4Waves * kWave;
-constexpr int kI4SplitBlocks = 16;       // blocks of a split, as long as kI8MaxSplits suffice
+// Blocks of a split, as long as kI8MaxSplits suffice: the length that batches of few items want (above).
+constexpr int kI4SplitBlocks = 16;
 
 // One block's words of a lane (c, g): K of token c, channels (D / 4) g .. of D >= 64 (8 g .. of 32, 4 g ..
 // of 16); V of tokens 4 g + r, channels VW c .. VW c + VW - 1.
@@ -428,7 +436,8 @@ __global__ void __launch_bounds__(kI4Threads, i4_decode_groups(D)) decode_int4_d
 }
 
 // Every item of a batch, as many workgroups as the CUs hold, which go round. FEW: up to 64 sequences, of which
-// the next item's place and the ids of its blocks are at hand when one ends.
+// the next item's place and the ids of its blocks are at hand when one ends, or that there is none (what it
+// saves where a batch has fewer items than workgroups).
 template <int D, bool FEW>
 __global__ void __launch_bounds__(kI4Threads, i4_decode_groups(D)) decode_int4_kernel(Int8DecodeArgs a) {
   __shared__ __align__(16) I4DecodeLds<D> lds;
